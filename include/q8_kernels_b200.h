@@ -47,6 +47,10 @@ extern "C" {
 #define Q8K_DT_E4M3  3   /* float8_e4m3fn */
 #define Q8K_DT_I8    4
 
+/* ---- activations of the gated projection --------------------------------- */
+#define Q8K_ACT_SILU       1   /* g / (1 + exp(-g)) */
+#define Q8K_ACT_GELU_TANH  2   /* the tanh form of GELU, as in the linears */
+
 /* ---- device status word --------------------------------------------------
  * The tensor-core kernels (GEMM, attention) bound every mbarrier wait.  When a
  * wait gives up the kernel records  Q8K_STATUS_TIMEOUT | (site << 8)  in the
@@ -322,6 +326,56 @@ Q8K_API int q8k_linear(const void* x, int x_dtype, const void* w, int w_dtype, c
 Q8K_API int q8k_linear_static(const void* x, int x_dtype, const void* w, int w_dtype, const float* w_scales,
                               const float* bias, void* out, int out_dtype, int M, int N, int K,
                               int use_hadamard, int fuse_gelu, int* dev_status, void* stream);
+
+/* Layer norm over the last dim: y = (x - mean) / sqrt(var + eps) * weight + bias, var the mean square of x - mean; weight and bias
+ * fp32 [dim] or NULL.  x [rows, dim] with x_row_stride elements between rows, y dense; (x, y) types bf16/fp16/fp32 alike, bf16 -> e4m3,
+ * fp32 -> bf16 or fp16.  mean and rstd (fp32 [rows], may be NULL) are what the backward pass takes.  dim up to 16384, any
+ * alignment (rows of 16-byte alignment and a dim that is a multiple of 8 are faster).  No counterpart in the reference.        */
+Q8K_API int q8k_layer_norm(const void* x, int x_dtype, int64_t x_row_stride, const float* weight, const float* bias, void* y,
+                   int y_dtype, float* mean, float* rstd, int64_t rows, int dim, float eps, void* stream);
+/* Its gradients: dx (dense, x's type), dweight and dbias (fp32 [dim]), each NULL if it is not wanted; grad dense, of y's type (bf16 for
+ * an e4m3 output).  The two sums over rows need a workspace of q8k_layer_norm_backward_workspace_bytes (16-byte aligned); they are
+ * taken in a fixed order: the same bits in every call.  No counterpart in the reference.                                        */
+Q8K_API size_t q8k_layer_norm_backward_workspace_bytes(int64_t rows, int dim);
+Q8K_API int q8k_layer_norm_backward(const void* x, int x_dtype, int64_t x_row_stride, const void* grad, int grad_dtype,
+                            const float* mean, const float* rstd, const float* weight, void* dx, float* dweight, float* dbias,
+                            int64_t rows, int dim, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rotary embedding of queries and keys from positions, in one launch: q [batch, seq, q_heads, head_dim] and k likewise, each with
+ * {batch, token, head} strides in elements and dense channels; heads of 0 leave that tensor out.  Pair i of the first rotary_dim
+ * channels -- (2i, 2i + 1), or (i, i + rotary_dim / 2) with half_layout -- is turned by position * frequencies[i] radians
+ * (fp64 [rotary_dim / 2]; the product is formed in fp64) and scaled by amplitude; the other channels are copied.  positions: int32 or
+ * int64 at batch * position_batch_stride + token * position_token_stride, or NULL for 0 .. seq - 1.  dtype bf16, fp16 or fp32.  out may be
+ * the input itself.  backward: the angle negated, which is the gradient.  No counterpart in the reference.                       */
+Q8K_API int q8k_rotary(const void* q, const int64_t q_strides[3], void* q_out, const int64_t q_out_strides[3], int q_heads,
+               const void* k, const int64_t k_strides[3], void* k_out, const int64_t k_out_strides[3], int k_heads,
+               int dtype, const void* positions, int positions_int64, int64_t position_batch_stride,
+               int64_t position_token_stride, const double* frequencies, float amplitude, int batch, int seq, int head_dim,
+               int rotary_dim, int half_layout, int backward, void* stream);
+
+/* Gated projection: out = act(gate) * up in bf16 [M, F], where gate and up are the products of a [M, K] (int8, or e4m3 if !int8) with the
+ * first and the last F rows of w [2F, K], times a_scales[m] * w_scales[n], plus bias[n] (fp32 [2F] or NULL).  pre: NULL, or
+ * bf16 [M, 2, F] for gate and up, which the backward pass takes.  activation: Q8K_ACT_*.  F and K multiples of 16, pointers 16-byte
+ * aligned.  No counterpart in the reference.                                                                                    */
+Q8K_API int q8k_gated_mm(int int8, const void* a, const void* w, const float* bias, const float* a_scales, const float* w_scales,
+                 void* out, void* pre, int activation, int M, int F, int K, int* dev_status, void* stream);
+/* Its activation: rows of x (bf16 or e4m3), rotated (Hadamard, 1/sqrt(dim), rounded to x's type) or not, quantised per token to int8 or
+ * e4m3 as q8k_hadamard_quant and q8k_tokenwise_quant do it, but with the factor top * (1 / absmax) of two roundings in the place
+ * of top / absmax.  dim a multiple of 16.  No counterpart in the reference.                                                     */
+Q8K_API int q8k_gated_quant(const void* x, int x_dtype, int64_t x_row_stride, void* q, int q_dtype, float* scales, int64_t rows, int dim,
+                    int rotate, void* stream);
+/* Its backward pass up to the product with the weight: from grad bf16 [M, F] and pre, the row [grad * up * act'(gate) | grad * act(gate)]
+ * quantised per token to e4m3: q [M, 2F] and scales [M] as for q8k_gated_quant, from the fp32 values.  F a multiple of 16
+ * up to 16384.  No counterpart in the reference.                                                                                */
+Q8K_API int q8k_gated_backward_quant(const void* grad, const void* pre, void* q, float* scales, int activation, int M, int F,
+                             void* stream);
+
+/* The other operand of that product: w [2F, K] times w_scales[n], transposed and quantised to e4m3 with one scale per input channel:
+ * q [K, 2F] and scales [K].  The workspace has q8k_gated_weight_operand_workspace_bytes, 16-byte aligned.  No counterpart in the
+ * reference.                                                                                                                    */
+Q8K_API size_t q8k_gated_weight_operand_workspace_bytes(int F, int K);
+Q8K_API int q8k_gated_weight_operand(const void* w, int w_dtype, const float* w_scales, void* q, float* scales, int F, int K,
+                             void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -25,7 +25,8 @@ LIB_PATH = os.path.join(PKG_DIR, "libq8k_b200.so")
 HOST_PATH = os.path.join(PKG_DIR, "_host" + sysconfig.get_config_var("EXT_SUFFIX"))
 HOST_KEY = os.path.join(OBJ_DIR, os.path.basename(HOST_PATH) + ".key")     # what the extension was built against
 
-SOURCES = ["capi.cu", "rowwise.cu", "hadamard.cu", "gemm.cu", "gemm_pair.cu", "gemm_split.cu", "attention.cu"]
+SOURCES = ["capi.cu", "rowwise.cu", "hadamard.cu", "gemm.cu", "gemm_pair.cu", "gemm_split.cu", "attention.cu",
+           "layer_norm.cu", "rotary.cu", "gemm_gated.cu", "gated.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

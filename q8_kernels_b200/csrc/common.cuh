@@ -36,6 +36,12 @@ void set_error_detail(const char* fmt, ...);
         }                                                                          \
     } while (0)
 
+// q8k_tokenwise_quant / q8k_hadamard_quant under another name `op`, with the quantizer's factor in two steps (see quant_factor)
+int tokenwise_quant_as(const char* op, bool two_step, const void* x, int x_dtype, void* q, int q_dtype, float* scales, int64_t rows, int dim,
+                       int64_t x_row_stride, cudaStream_t st);
+int hadamard_quant_as(const char* op, bool two_step, const void* x, int x_dtype, void* q, int q_dtype, float* scales, int64_t rows, int dim,
+                      int64_t x_row_stride, float scale, cudaStream_t st);
+
 int gemm_num_sms();                          // SMs of the current device (148 if it cannot be asked)
 
 // Raise a kernel's dynamic shared memory limit, once per device (the call costs about 1 us, a launch 2.5).  The setting
@@ -96,6 +102,17 @@ inline int dtype_size(int dt) {
         case Q8K_DT_E4M3: case Q8K_DT_I8: return 1;
         default: return 0;
     }
+}
+
+// The factor that takes a row onto its 8-bit grid.  The quantizer of the linears rounds the quotient top / absmax once (TwoStep false);
+// the gated projection defines it as tensor code computes a scalar over a tensor, top * (1 / absmax), each rounded.  The two differ
+// in the last bit for some absmax, and a 16-bit value that lies exactly between two steps of the grid then falls on one side or
+// the other: the operator's definition has to say which.
+template <bool TwoStep> __device__ __forceinline__ float quant_factor(float top, float absmax) {
+    return TwoStep ? __fmul_rn(top, __frcp_rn(absmax)) : __fdiv_rn(top, absmax);
+}
+__device__ __forceinline__ float quant_factor(float top, float absmax, bool two_step) {
+    return two_step ? quant_factor<true>(top, absmax) : quant_factor<false>(top, absmax);
 }
 
 // ---------------------------------------------------------------- scalar conversions

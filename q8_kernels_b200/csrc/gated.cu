@@ -1,0 +1,291 @@
+// The gated projection around its GEMMs (gemm_gated.cu): the activation's quantizer, and the two operands of the backward product.
+//
+// Backward pass up to the product with the weight: out = act(gate) * up has the gradients
+//   dgate = dout * up * act'(gate),  dup = dout * act(gate)
+// which the FP8 GEMM takes as one row [dgate | dup] of 2F e4m3 values with one scale.  Bound by HBM: 2 bytes of dout and 4 of gate
+// and up are read per column, 2 bytes written; the 2F fp32 values of a row stay in registers between the absmax and the cast, so
+// nothing is rounded before it.
+
+#include <math.h>
+
+#include <type_traits>
+#include "common.cuh"
+
+namespace q8k {
+
+constexpr int kGatedItem = 8;
+constexpr int kGatedMaxF = 16384;
+
+// act(g) and its derivative, both from s = 1 / (1 + e^(-v)):  silu: v = g, act' = s (1 + g (1 - s));  tanh-GELU:
+// v = 2 sqrt(2/pi) (g + c g^3), act' = s + g s (1 - s) v'.  Where s (1 - s) is 0 the second term is, too, however large v' is.
+template <bool GELU> __device__ __forceinline__ void gated_act_grad(float g, float& act, float& grad) {
+    constexpr float kLog2e = 1.4426950408889634f, kA = 2.0f * 0.7978845608028654f, kB = kA * 0.044715f;
+    const float gg = g * g;
+    const float v = GELU ? g * fmaf(kB, gg, kA) : g;
+    float e, s;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-kLog2e * v));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(e + 1.0f));
+    act = g * s;
+    const float slope = s * (1.0f - s);
+    grad = slope == 0.f ? s : fmaf(g * slope, GELU ? fmaf(3.0f * kB, gg, kA) : 1.0f, s);
+}
+
+template <bool GELU, int ITEMS, int T>
+__global__ void __launch_bounds__(T)
+gated_backward_quant_kernel(const __nv_bfloat16* __restrict__ dout, const __nv_bfloat16* __restrict__ pre, uint8_t* __restrict__ q,
+                            float* __restrict__ scales, int F) {
+    __shared__ float red[T / 32];
+    pdl_wait();
+    pdl_release();
+    const int64_t row = blockIdx.x;
+    const __nv_bfloat16* dr = dout + row * F;
+    const __nv_bfloat16* pr = pre + row * 2 * F;
+    float dg[ITEMS][kGatedItem], du[ITEMS][kGatedItem];
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int e = (threadIdx.x + i * T) * kGatedItem;
+        if (e < F) {
+            float d[kGatedItem];
+            load_vec<__nv_bfloat16, kGatedItem>(dr + e, d);
+            load_vec<__nv_bfloat16, kGatedItem>(pr + e, dg[i]);
+            load_vec<__nv_bfloat16, kGatedItem>(pr + F + e, du[i]);
+#pragma unroll
+            for (int j = 0; j < kGatedItem; ++j) {
+                float act, grad;
+                gated_act_grad<GELU>(dg[i][j], act, grad);
+                dg[i][j] = d[j] * du[i][j] * grad;
+                du[i][j] = d[j] * act;
+                amax = fmaxf(amax, fmaxf(fabsf(dg[i][j]), fabsf(du[i][j])));
+            }
+        }
+    }
+    amax = warp_max(amax);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
+    __syncthreads();
+    amax = red[0];
+#pragma unroll
+    for (int w = 1; w < T / 32; ++w) amax = fmaxf(amax, red[w]);
+    const float scale = quant_factor<true>(448.0f, amax);      // the saturating cast below: see tokenwise_quant_kernel
+    const float mul = amax == 0.f ? 0.f : scale;
+    uint8_t* qr = q + row * 2 * F;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int e = (threadIdx.x + i * T) * kGatedItem;
+        if (e < F) {
+            union { uint2 v; uint16_t h[4]; } a, b;
+#pragma unroll
+            for (int j = 0; j < kGatedItem; j += 2) {
+                a.h[j / 2] = float2_to_e4m3x2_sat(__fmul_rn(dg[i][j], mul), __fmul_rn(dg[i][j + 1], mul));
+                b.h[j / 2] = float2_to_e4m3x2_sat(__fmul_rn(du[i][j], mul), __fmul_rn(du[i][j + 1], mul));
+            }
+            *reinterpret_cast<uint2*>(qr + e) = a.v;
+            *reinterpret_cast<uint2*>(qr + F + e) = b.v;
+        }
+    }
+    if (threadIdx.x == 0) scales[row] = __fdiv_rn(1.0f, scale);
+}
+
+template <bool GELU>
+static int launch_gated_backward(const void* dout, const void* pre, void* q, float* scales, int M, int F, cudaStream_t st) {
+    const int items = F / kGatedItem;
+#define Q8K_GB(ITEMS, T)                                                                                                      \
+    do {                                                                                                                      \
+        Q8K_CUDA_OK(launch_dependent(gated_backward_quant_kernel<GELU, ITEMS, T>, (unsigned)M, T, 0, st, 1, (const __nv_bfloat16*)dout, \
+                                     (const __nv_bfloat16*)pre, (uint8_t*)q, scales, F));                                     \
+        return Q8K_OK;                                                                                                        \
+    } while (0)
+    if (items <= 64) Q8K_GB(1, 64);
+    if (items <= 128) Q8K_GB(1, 128);
+    if (items <= 256) Q8K_GB(1, 256);
+    if (items <= 512) Q8K_GB(2, 256);
+    if (items <= 1024) Q8K_GB(4, 256);
+    Q8K_GB(4, 512);
+#undef Q8K_GB
+}
+
+// The weight operand of the backward product: w [N, K] (int8 or e4m3) times its row scales, transposed and quantised to e4m3 with one
+// scale per row of the result, i.e. per column of w.  Bound by HBM: w is read once and q written once; a column's absmax needs all
+// rows first, so there are two kernels, the second of which finds w in L2.
+//
+// Tiles of 128 columns, 16 per thread (one 16-byte load of a row), so a warp reads four rows of 128 bytes.
+constexpr int kWtCols = 128;
+constexpr int kWtMaxRows = 256;              // rows whose absmax one CTA takes
+constexpr int kWtRows = 128;                 // rows of a tile that is quantised and turned
+constexpr int kWtThreads = 256;
+
+template <typename Tw> __device__ __forceinline__ void wt_values(uint32_t w, float s, float (&v)[4]) {
+    if constexpr (std::is_same_v<Tw, int8_t>) {
+        // 2^23 + 128 + b has the byte b + 128 in its last bits: a permutation and an exact difference instead of a conversion,
+        // which runs at an eighth of their rate
+        const uint32_t u = w ^ 0x80808080u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = __fmul_rn(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7650 | j)) - 8388736.0f, s);
+    } else {
+        e4m3x4_to_float(w, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = __fmul_rn(v[j], s);
+    }
+}
+
+template <typename Tw>
+__global__ void __launch_bounds__(kWtThreads)
+gated_weight_absmax_kernel(const Tw* __restrict__ w, const float* __restrict__ row_scales, float* __restrict__ part, int N, int K) {
+    __shared__ float red[kWtThreads / 32][kWtCols];
+    pdl_wait();
+    pdl_release();
+    const int cg = threadIdx.x & 7, rl = threadIdx.x >> 3;     // column group, row within a step of 32
+    const int c0 = blockIdx.x * kWtCols + cg * 16;
+    const int r0 = blockIdx.y * kWtMaxRows;
+    float m[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) m[j] = 0.f;
+    if (c0 < K) {
+#pragma unroll
+        for (int i = 0; i < kWtMaxRows / 32; ++i) {
+            const int r = r0 + i * 32 + rl;
+            if (r < N) {
+                const uint4 x = *reinterpret_cast<const uint4*>(w + (int64_t)r * K + c0);
+                const float s = row_scales[r];
+                const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float v[4];
+                    wt_values<Tw>(xw[k], s, v);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) m[k * 4 + j] = fmaxf(m[k * 4 + j], fabsf(v[j]));
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {                             // over the four rows of a warp
+        m[j] = fmaxf(m[j], __shfl_xor_sync(0xffffffffu, m[j], 8));
+        m[j] = fmaxf(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
+        if ((threadIdx.x & 31) < 8) red[threadIdx.x >> 5][cg * 16 + j] = m[j];
+    }
+    __syncthreads();
+    const int c = blockIdx.x * kWtCols + threadIdx.x;
+    if (threadIdx.x < kWtCols && c < K) {
+        float a = red[0][threadIdx.x];
+#pragma unroll
+        for (int k = 1; k < kWtThreads / 32; ++k) a = fmaxf(a, red[k][threadIdx.x]);
+        part[(int64_t)blockIdx.y * K + c] = a;
+    }
+}
+
+template <typename Tw>
+__global__ void __launch_bounds__(kWtThreads)
+gated_weight_quant_kernel(const Tw* __restrict__ w, const float* __restrict__ row_scales, const float* __restrict__ part, int parts,
+                          uint8_t* __restrict__ q, float* __restrict__ scales, int N, int K) {
+    __shared__ float mul[kWtCols];
+    __shared__ __align__(16) uint32_t turned[kWtCols][kWtRows / 4];
+    pdl_wait();
+    pdl_release();
+    const int cb = blockIdx.x * kWtCols, r0 = blockIdx.y * kWtRows;
+    const int cg = threadIdx.x & 7, rg = threadIdx.x >> 3;     // 16 columns, four rows
+    uint4 x[4];
+    float s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {                              // N % 16 == 0: all four rows exist, or none
+        const bool in = cb + cg * 16 < K && r0 + rg * 4 < N;
+        x[i] = in ? *reinterpret_cast<const uint4*>(w + (int64_t)(r0 + rg * 4 + i) * K + cb + cg * 16) : make_uint4(0, 0, 0, 0);
+        s[i] = in ? row_scales[r0 + rg * 4 + i] : 0.f;
+    }
+    if (threadIdx.x < kWtCols && cb + (int)threadIdx.x < K) {
+        float a = 0.f;
+        for (int k = 0; k < parts; ++k) a = fmaxf(a, part[(int64_t)k * K + cb + threadIdx.x]);
+        const float f = quant_factor<true>(448.0f, a);
+        mul[threadIdx.x] = a == 0.f ? 0.f : f;                 // a column of zeros quantises to zeros
+        if (blockIdx.y == 0) scales[cb + threadIdx.x] = __fdiv_rn(1.0f, f);
+    }
+    __syncthreads();
+    if (cb + cg * 16 < K) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float v[4][4];                                     // [row][column]
+#pragma unroll
+            for (int i = 0; i < 4; ++i) wt_values<Tw>(k == 0 ? x[i].x : k == 1 ? x[i].y : k == 2 ? x[i].z : x[i].w, s[i], v[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = cg * 16 + k * 4 + j;
+                const float f = mul[c];
+                // saturating cast: see tokenwise_quant_kernel.  Row group rg of a column goes to word rg + 4 * (column group): the 32
+                // words that a warp stores lie in 32 banks, and four of a column stay together for the 16-byte reads below.
+                turned[c][(rg + 4 * cg) & 31] = (uint32_t)float2_to_e4m3x2_sat(__fmul_rn(v[0][j], f), __fmul_rn(v[1][j], f)) |
+                                                ((uint32_t)float2_to_e4m3x2_sat(__fmul_rn(v[2][j], f), __fmul_rn(v[3][j], f)) << 16);
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWtCols / 32; ++i) {
+        const int c = i * 32 + (threadIdx.x >> 3), part16 = threadIdx.x & 7;
+        const int n = r0 + part16 * 16;
+        if (cb + c < K && n < N)
+            *reinterpret_cast<uint4*>(q + (int64_t)(cb + c) * N + n) =
+                *reinterpret_cast<const uint4*>(&turned[c][(part16 * 4 + 4 * (c / 16)) & 31]);
+    }
+}
+
+template <typename Tw>
+static int launch_gated_weight(const void* w, const float* row_scales, void* q, float* scales, float* part, int N, int K, cudaStream_t st) {
+    const unsigned cols = (unsigned)((K + kWtCols - 1) / kWtCols);
+    const int parts = (N + kWtMaxRows - 1) / kWtMaxRows;
+    Q8K_CUDA_OK(launch_dependent(gated_weight_absmax_kernel<Tw>, dim3(cols, (unsigned)parts), kWtThreads, 0, st, 1, (const Tw*)w, row_scales,
+                                 part, N, K));
+    Q8K_CUDA_OK(launch_dependent(gated_weight_quant_kernel<Tw>, dim3(cols, (unsigned)((N + kWtRows - 1) / kWtRows)), kWtThreads, 0, st, 1,
+                                 (const Tw*)w, row_scales, part, parts, (uint8_t*)q, scales, N, K));
+    return Q8K_OK;
+}
+
+}  // namespace q8k
+
+extern "C" int q8k_gated_backward_quant(const void* grad, const void* pre, void* q, float* scales, int activation, int M, int F,
+                                        void* stream) {
+    using namespace q8k;
+    const char* op = "gated_backward_quant";
+    Q8K_REQUIRE(M >= 0 && F > 0 && F % 16 == 0, Q8K_ERR_INVALID_ARG, "%s: M=%d must not be negative and F=%d a multiple of 16", op, M, F);
+    Q8K_REQUIRE(F <= kGatedMaxF, Q8K_ERR_UNSUPPORTED, "%s: F=%d exceeds %d", op, F, kGatedMaxF);
+    Q8K_REQUIRE(activation == Q8K_ACT_SILU || activation == Q8K_ACT_GELU_TANH, Q8K_ERR_UNSUPPORTED, "%s: activation %d is unknown", op,
+                activation);
+    if (M == 0) return Q8K_OK;
+    Q8K_REQUIRE(grad && pre && q && scales && aligned16(grad) && aligned16(pre) && aligned16(q), Q8K_ERR_INVALID_ARG,
+                "%s: null or misaligned pointer", op);
+    cudaStream_t st = (cudaStream_t)stream;
+    return activation == Q8K_ACT_GELU_TANH ? launch_gated_backward<true>(grad, pre, q, scales, M, F, st)
+                                           : launch_gated_backward<false>(grad, pre, q, scales, M, F, st);
+}
+
+extern "C" size_t q8k_gated_weight_operand_workspace_bytes(int F, int K) {
+    if (F <= 0 || K <= 0) return 0;
+    return (2 * (size_t)F + q8k::kWtMaxRows - 1) / q8k::kWtMaxRows * (size_t)K * sizeof(float);
+}
+
+extern "C" int q8k_gated_weight_operand(const void* w, int w_dtype, const float* w_scales, void* q, float* scales, int F, int K,
+                                        void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace q8k;
+    const char* op = "gated_weight_operand";
+    Q8K_REQUIRE(F > 0 && K > 0 && F % 16 == 0 && K % 16 == 0, Q8K_ERR_INVALID_ARG, "%s: F=%d and K=%d must be positive multiples of 16", op,
+                F, K);
+    Q8K_REQUIRE(F <= 65535 * (kWtRows / 2), Q8K_ERR_TOO_LARGE, "%s: F=%d too large", op, F);
+    Q8K_REQUIRE(w && w_scales && q && scales && workspace && aligned16(w) && aligned16(q) && aligned16(workspace), Q8K_ERR_INVALID_ARG,
+                "%s: null or misaligned pointer", op);
+    const size_t need = q8k_gated_weight_operand_workspace_bytes(F, K);
+    Q8K_REQUIRE(workspace_bytes >= need, Q8K_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", op, workspace_bytes, need);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (w_dtype == Q8K_DT_I8) return launch_gated_weight<int8_t>(w, w_scales, q, scales, (float*)workspace, 2 * F, K, st);
+    if (w_dtype == Q8K_DT_E4M3) return launch_gated_weight<e4m3_t>(w, w_scales, q, scales, (float*)workspace, 2 * F, K, st);
+    set_error_detail("%s: weight dtype %d is not int8 or e4m3", op, w_dtype);
+    return Q8K_ERR_UNSUPPORTED;
+}
+
+extern "C" int q8k_gated_quant(const void* x, int x_dtype, int64_t x_row_stride, void* q, int q_dtype, float* scales, int64_t rows,
+                               int dim, int rotate, void* stream) {
+    using namespace q8k;
+    const char* op = "gated_quant";
+    Q8K_REQUIRE(x_dtype == Q8K_DT_BF16 || x_dtype == Q8K_DT_E4M3, Q8K_ERR_UNSUPPORTED, "%s: input dtype %d is not bf16 or e4m3", op, x_dtype);
+    cudaStream_t st = (cudaStream_t)stream;
+    return rotate ? hadamard_quant_as(op, true, x, x_dtype, q, q_dtype, scales, rows, dim, x_row_stride, 1.0f / sqrtf((float)dim), st)
+                  : tokenwise_quant_as(op, true, x, x_dtype, q, q_dtype, scales, rows, dim, x_row_stride, st);
+}

@@ -1,0 +1,410 @@
+// Gated 8-bit projection: gate and up projection, activation and product in one kernel,
+//   gate = (A . Wg^T) * (sa[m] * sg[n]) + bg[n],  up = (A . Wu^T) * (sa[m] * su[n]) + bu[n],  out = act(gate) * up   (bf16)
+// with Wg and Wu the first and the last F rows of one weight W [2F, K].  The backward pass needs gate and up: with SAVE they are stored
+// as well, rounded to bf16 as a projection's output would be; `out` is computed from the unrounded values.
+//
+// A pair of CTAs (cta_group::2) owns 256 rows and `bn` output columns, i.e. 2 bn columns of the product.  The MMA takes the first
+// half of its B rows from the even CTA and the second from the odd one: the even CTA loads rows of Wg, the odd one the same rows of
+// Wu, so columns [0, bn) of the accumulator are the gate and [bn, 2 bn) the up projection of the same output columns, in the TMEM
+// lanes of the same thread.  No weight has to be laid out anew, and neither projection's result leaves the SM.
+//
+// Roles, barriers and the bounded waits are those of the pair kernel (gemm_pair.cu): warp 0 TMA producer, warp 1 MMA issuer (even CTA)
+// and TMEM allocation, warps 2-9 epilogue; two accumulators, so that the epilogue of a tile runs under the products of
+// the next.
+
+#include "gemm_common.cuh"
+
+namespace q8k {
+
+constexpr int kGatedBN = 128;                // output columns of the widest tile: 256 columns of the product
+constexpr int kGatedTmemCols = 512;          // two accumulators of 256 columns
+
+template <bool SAVE>
+struct GatedSmemT {
+    static constexpr int kStages = SAVE ? 5 : 6;
+    static constexpr int kABytes = kGemmBM * kGemmBK;
+    static constexpr int kBBytes = kGatedBN * kGemmBK;
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    // output staging: per epilogue warp a ring of boxes of 32 rows x 64 bytes, one store each
+    static constexpr int kRing = SAVE ? 3 : 2;
+    static constexpr int kBoxBytes = 32 * 64;
+    static constexpr int kStoreOffset = kStages * kStageBytes;
+    static constexpr int kStoreBytes = (kGemmEpilogueThreads / 32) * kRing * kBoxBytes;
+    static constexpr int kBarOffset = kStoreOffset + kStoreBytes;
+    static constexpr int kNumBars = 2 * kStages + 4;
+    static constexpr int kTmemPtrOffset = kBarOffset + kNumBars * 8;
+    static constexpr int kAbortOffset = kTmemPtrOffset + 4;
+    static constexpr int kPriorOffset = kAbortOffset + 4;
+    static constexpr int kScaleOffset = (kPriorOffset + 4 + 15) & ~15;         // gate columns, then up columns
+    static constexpr int kBiasOffset = kScaleOffset + 2 * kGatedBN * 4;
+    static constexpr int kTotal = kBiasOffset + 2 * kGatedBN * 4;
+    static_assert(kTotal <= 227 * 1024, "gated GEMM shared memory");
+};
+
+struct GatedParams {
+    const float* a_scales;
+    const float* b_scales;                   // [2F]
+    const float* bias;                       // [2F] or null
+    int* status;
+    int M, F, K;
+    int bn;                                  // output columns of a tile: 32, 64, 96 or 128
+    int n_tiles, total_tiles;
+};
+
+// silu(g) = g / (1 + e^-g); tanh-GELU = g / (1 + e^(-2u)) with u = sqrt(2/pi) (g + 0.044715 g^3): no cancellation anywhere, a few fp32
+// ulps.  e^(-x) overflows to infinity for very negative x, and g / infinity is the right 0.
+template <bool GELU> __device__ __forceinline__ float gated_act(float g) {
+    constexpr float kLog2e = 1.4426950408889634f;
+    float t;
+    if constexpr (GELU) {
+        constexpr float kC0 = -2.0f * 0.7978845608028654f * kLog2e, kC1 = kC0 * 0.044715f;
+        t = g * fmaf(kC1, g * g, kC0);
+    } else {
+        t = -kLog2e * g;
+    }
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
+    return g * r;
+}
+
+template <bool INT8, bool GELU, bool SAVE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+gemm_8bit_gated_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
+                       const __grid_constant__ CUtensorMap tmap_out, const __grid_constant__ CUtensorMap tmap_pre, const GatedParams p) {
+    using L = GatedSmemT<SAVE>;
+    constexpr int STAGES = L::kStages;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t smem_base = ptx::smem_u32(smem);
+    if (smem_base & 1023u) {                                   // same offset in both CTAs: both leave
+        pdl_wait();
+        if (threadIdx.x == 0 && p.status != nullptr) atomicExch(p.status, Q8K_STATUS_TIMEOUT | (31 << 8));
+        return;
+    }
+    const uint32_t bar_base = smem_base + L::kBarOffset;
+    auto full_bar = [&](int s) { return bar_base + 8u * s; };
+    auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
+    auto tmem_full_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + a); };
+    auto tmem_empty_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + 2 + a); };
+    volatile uint32_t* tmem_ptr_smem = reinterpret_cast<volatile uint32_t*>(smem + L::kTmemPtrOffset);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kAbortOffset);
+    volatile int* prior_failure = reinterpret_cast<volatile int*>(smem + L::kPriorOffset);
+    float* scale_smem = reinterpret_cast<float*>(smem + L::kScaleOffset);
+    float* bias_smem = reinterpret_cast<float*>(smem + L::kBiasOffset);
+
+    const uint32_t rank = ptx::cluster_ctarank();              // 0: leader, gate rows; 1: up rows
+    const bool leader = rank == 0;
+    const int cluster_id = blockIdx.x >> 1;
+    const int num_clusters = gridDim.x >> 1;
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int k_iters = (p.K + kGemmBK - 1) / kGemmBK;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            ptx::mbar_init(full_bar(s), 2);                    // one arrive.expect_tx from each CTA's producer
+            ptx::mbar_init(empty_bar(s), 1);                   // one commit from the leader's MMA thread
+        }
+        for (int a = 0; a < 2; ++a) {
+            ptx::mbar_init(tmem_full_bar(a), 1);
+            ptx::mbar_init(tmem_empty_bar(a), 2 * (kGemmEpilogueThreads / 32));   // every epilogue warp of both CTAs
+        }
+        *abort_flag = 0;
+        ptx::fence_barrier_init();
+        ptx::fence_proxy_async_smem();
+        ptx::prefetch_tensormap(&tmap_a);
+        ptx::prefetch_tensormap(&tmap_w);
+        ptx::prefetch_tensormap(&tmap_out);
+        if (SAVE) ptx::prefetch_tensormap(&tmap_pre);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc_pair<kGatedTmemCols>(ptx::smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)));
+        ptx::tmem_relinquish_alloc_permit_pair();
+    }
+    pdl_wait();                                                // everything above overlaps the kernel before
+    // A launch that follows a failed one on the same status word does nothing; the leader decides for both CTAs.
+    if (threadIdx.x == 0 && leader) {
+        const int v = p.status != nullptr ? *reinterpret_cast<volatile int*>(p.status) : 0;
+        *prior_failure = v;
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(ptx::mapa_shared(smem_base + L::kPriorOffset, 1)), "r"(v)
+                     : "memory");
+    }
+    ptx::tcgen05_fence_before_sync();
+    __syncthreads();
+    ptx::cluster_sync_all();                                   // both CTAs' barriers exist before anyone signals across
+    ptx::tcgen05_fence_after_sync();
+    pdl_release();                                             // this CTA holds its TMEM: the next kernel may move in behind it
+    const bool skip = *prior_failure != 0;
+    const uint32_t tmem_base = *tmem_ptr_smem;
+
+    const uint32_t leader_full0 = ptx::mapa_shared(full_bar(0), 0);
+    auto leader_tmem_empty_bar = [&](int a) { return ptx::mapa_shared(tmem_empty_bar(a), 0); };
+
+    if (skip) {
+    } else if (warp == 0) {
+        // ------------------------------------------------ TMA producer (both CTAs)
+        if (ptx::elect_one()) {
+            int s = 0;
+            uint32_t ph = 1;                                   // empty_bar phase to wait for: the first round passes
+            bool ok = true;
+            const uint32_t bytes = L::kABytes + (uint32_t)p.bn * kGemmBK;
+            for (int tile = cluster_id; ok && tile < p.total_tiles; tile += num_clusters) {
+                const int a_row = tile / p.n_tiles * 2 * kGemmBM + (int)rank * kGemmBM;
+                // The gate's last tile may run on into the rows of the up projection, and that one's beyond the weight
+                // (zeros): columns from F on, which no store takes.
+                const int w_row = tile % p.n_tiles * p.bn + (int)rank * p.F;
+                for (int kb = 0; kb < k_iters; ++kb) {
+                    if (!ptx::mbar_wait(empty_bar(s), ph, abort_flag)) { ok = false; break; }
+                    const uint32_t fb = leader_full0 + 8u * s;
+                    ptx::mbar_arrive_expect_tx_cluster(fb, bytes);
+                    const uint32_t a_dst = smem_base + s * L::kStageBytes;
+                    ptx::tma_load_2d_pair(a_dst, &tmap_a, fb, kb * kGemmBK, a_row);
+                    ptx::tma_load_2d_pair(a_dst + L::kABytes, &tmap_w, fb, kb * kGemmBK, w_row);
+                    if (++s == STAGES) { s = 0; ph ^= 1u; }
+                }
+            }
+            if (!ok && p.status != nullptr) atomicExch(p.status, Q8K_STATUS_TIMEOUT | (28 << 8));
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------ MMA issuer (leader CTA only)
+        if (leader && ptx::elect_one()) {
+            int s = 0;
+            uint32_t ph = 0;
+            uint32_t tile_i = 0;
+            bool ok = true;
+            const uint32_t idesc = INT8 ? ptx::make_idesc_s8(2 * kGemmBM, 2 * p.bn) : ptx::make_idesc_e4m3(2 * kGemmBM, 2 * p.bn);
+            for (int tile = cluster_id; ok && tile < p.total_tiles; tile += num_clusters, ++tile_i) {
+                const uint32_t acc = tile_i & 1u;
+                const uint32_t acc_ph = (tile_i >> 1) & 1u;
+                if (!ptx::mbar_wait(tmem_empty_bar(acc), acc_ph ^ 1u, abort_flag)) { ok = false; break; }
+                ptx::tcgen05_fence_after_sync();
+                const uint32_t d_tmem = tmem_base + acc * (2 * kGatedBN);
+                for (int kb = 0; kb < k_iters; ++kb) {
+                    if (!ptx::mbar_wait(full_bar(s), ph, abort_flag)) { ok = false; break; }
+                    ptx::tcgen05_fence_after_sync();
+                    const uint32_t a_addr = smem_base + s * L::kStageBytes;
+                    const uint64_t a_desc = ptx::make_kmajor_desc(a_addr, 128);
+                    const uint64_t b_desc = ptx::make_kmajor_desc(a_addr + L::kABytes, 128);
+#pragma unroll
+                    for (int k = 0; k < kGemmBK / 32; ++k) {
+                        const uint32_t accumulate = (kb > 0 || k > 0) ? 1u : 0u;
+                        if constexpr (INT8) ptx::mma_i8_pair(d_tmem, a_desc + 2 * k, b_desc + 2 * k, idesc, accumulate);
+                        else ptx::mma_f8f6f4_pair(d_tmem, a_desc + 2 * k, b_desc + 2 * k, idesc, accumulate);
+                    }
+                    ptx::tcgen05_commit_both(empty_bar(s));    // the stage is reusable in both CTAs once these MMAs retire
+                    if (++s == STAGES) { s = 0; ph ^= 1u; }
+                }
+                if (ok) ptx::tcgen05_commit_both(tmem_full_bar(acc));
+            }
+            if (!ok && p.status != nullptr) atomicExch(p.status, Q8K_STATUS_TIMEOUT | (29 << 8));
+        }
+    } else {
+        // ------------------------------------------------ epilogue (warps 2..9) of this CTA's 128 rows
+        const int quarter = warp & 3;
+        const int half = (warp - 2) >> 2;
+        const int epi_tid = threadIdx.x - 64;
+        const uint32_t store_base = smem_base + L::kStoreOffset + (uint32_t)(warp - 2) * L::kRing * L::kBoxBytes;
+        const int chunks = p.bn / 32;
+        const int c_lo = half == 0 ? 0 : (chunks + 1) / 2;     // warps 2-5 take the first half of the chunks, 6-9 the rest
+        const int c_hi = half == 0 ? (chunks + 1) / 2 : chunks;
+        uint32_t tile_i = 0;
+        uint32_t box_i = 0;                                    // next box of this warp's ring
+        bool ok = true;
+        for (int tile = cluster_id; tile < p.total_tiles; tile += num_clusters, ++tile_i) {
+            const int row0 = tile / p.n_tiles * 2 * kGemmBM + (int)rank * kGemmBM + quarter * 32;
+            const int n0 = tile % p.n_tiles * p.bn;
+            const uint32_t acc = tile_i & 1u;
+            const uint32_t acc_ph = (tile_i >> 1) & 1u;
+
+            asm volatile("bar.sync 1, 256;" ::: "memory");     // the tile before has been read out of the arrays
+            for (int c = epi_tid; c < 2 * p.bn; c += kGemmEpilogueThreads) {
+                const bool up = c >= p.bn;
+                const int n = n0 + (up ? c - p.bn : c);
+                const bool in = n < p.F;
+                const int at = up ? p.F + n : n;
+                scale_smem[c] = in ? p.b_scales[at] : 0.f;
+                bias_smem[c] = in && p.bias != nullptr ? p.bias[at] : 0.f;
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+
+            const int row = row0 + lane;
+            const float sa = row < p.M ? p.a_scales[row] : 0.f;
+            const float2 sa2 = make_float2(sa, sa);
+            const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * (2 * kGatedBN);
+
+            if (ok) ok = ptx::mbar_wait(tmem_full_bar(acc), acc_ph, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) continue;
+            ptx::tcgen05_fence_after_sync();
+
+            // row `lane` of the box, 16-byte pieces swizzled as the tensor maps expect (SWIZZLE_64B: piece ^= (row >> 1) & 3)
+            const uint32_t sw = ((uint32_t)lane >> 1) & 3u;
+            auto store_chunk = [&](const CUtensorMap* map, const uint32_t (&w)[16], int x, int which_or_row, int row_or_zero) {
+                const uint32_t box = store_base + box_i * L::kBoxBytes;
+                if (++box_i == (uint32_t)L::kRing) box_i = 0;
+                if (lane == 0) ptx::bulk_wait_group_read<L::kRing - 1>();      // the store that last used this box has read it out
+                __syncwarp();
+                const uint32_t row_addr = box + (uint32_t)lane * 64u;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_addr + (((uint32_t)q ^ sw) << 4)),
+                                 "r"(w[4 * q]), "r"(w[4 * q + 1]), "r"(w[4 * q + 2]), "r"(w[4 * q + 3])
+                                 : "memory");
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::tma_store_3d(map, box, x, which_or_row, row_or_zero);
+                    ptx::bulk_commit_group();
+                }
+            };
+
+            for (int c = c_lo; c < c_hi; ++c) {                // (warp-uniform)
+                uint32_t rg[32], ru[32];
+                ptx::tmem_ld_32x32b_x32(t_row + c * 32, rg);
+                ptx::tmem_ld_32x32b_x32(t_row + p.bn + c * 32, ru);
+                ptx::tmem_wait_ld();
+                const int nc = n0 + c * 32;
+                if (nc >= p.F) continue;
+                uint32_t wo[16], wg[16], wu[16];
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) {
+                    const float2 g = epilogue_pair<INT8, false>(rg[j], rg[j + 1], sa2, scale_smem + c * 32 + j, bias_smem + c * 32 + j);
+                    const float2 u = epilogue_pair<INT8, false>(ru[j], ru[j + 1], sa2, scale_smem + p.bn + c * 32 + j,
+                                                                bias_smem + p.bn + c * 32 + j);
+                    const __nv_bfloat162 o = __floats2bfloat162_rn(gated_act<GELU>(g.x) * u.x, gated_act<GELU>(g.y) * u.y);
+                    wo[j / 2] = *reinterpret_cast<const uint32_t*>(&o);
+                    if constexpr (SAVE) {
+                        const __nv_bfloat162 g2 = __floats2bfloat162_rn(g.x, g.y), u2 = __floats2bfloat162_rn(u.x, u.y);
+                        wg[j / 2] = *reinterpret_cast<const uint32_t*>(&g2);
+                        wu[j / 2] = *reinterpret_cast<const uint32_t*>(&u2);
+                    }
+                }
+                store_chunk(&tmap_out, wo, nc * 2, row0, 0);
+                if constexpr (SAVE) {                          // [M, 2, F]: the gate's columns end at F, not in the up projection's
+                    store_chunk(&tmap_pre, wg, nc * 2, 0, row0);
+                    store_chunk(&tmap_pre, wu, nc * 2, 1, row0);
+                }
+            }
+            ptx::tcgen05_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_cluster(leader_tmem_empty_bar(acc));   // the leader's MMA thread waits for both CTAs
+        }
+        if (lane == 0) ptx::bulk_wait_group<0>();              // this warp's stores are performed before the CTA may exit
+        if (!ok && p.status != nullptr && epi_tid == 0) atomicExch(p.status, Q8K_STATUS_TIMEOUT | (30 << 8));
+    }
+
+    // ---------------------------------------------------- teardown: neither CTA may leave while the other can
+    // still read its shared memory, signal its barriers or write its TMEM
+    if (threadIdx.x == 0 && *abort_flag != 0) {
+        // A wait was abandoned: copies issued before that get time to land before the CTA gives its memory up.
+        const unsigned long long t0 = ptx::globaltimer_ns();
+        while (ptx::globaltimer_ns() - t0 < 50000ull) {}
+    }
+    ptx::tcgen05_fence_before_sync();
+    __syncthreads();
+    ptx::cluster_sync_all();
+    if (warp == 1) {
+        ptx::tcgen05_fence_after_sync();
+        ptx::tmem_dealloc_pair<kGatedTmemCols>(tmem_base);
+    }
+}
+
+// ------------------------------------------------------------------ host side
+template <bool INT8, bool GELU, bool SAVE>
+static int launch_gated_as(const CUtensorMap& ta, const CUtensorMap& tw, const CUtensorMap& to, const CUtensorMap& tp,
+                           const GatedParams& p, cudaStream_t st) {
+    using L = GatedSmemT<SAVE>;
+    auto kern = gemm_8bit_gated_kernel<INT8, GELU, SAVE>;
+    static std::atomic<uint64_t> smem_done{0};
+    if (int rc = allow_dynamic_smem((const void*)kern, L::kTotal, smem_done)) return rc;
+    static std::atomic<int> max_clusters{-1};                  // 2-CTA clusters that can be resident at once
+    int most = max_clusters.load(std::memory_order_relaxed);
+    if (most < 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2 * gemm_num_sms());
+        cfg.blockDim = dim3(kGemmThreads);
+        cfg.dynamicSmemBytes = L::kTotal;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&most, kern, &cfg) != cudaSuccess) { cudaGetLastError(); most = 0; }
+        max_clusters.store(most, std::memory_order_relaxed);
+    }
+    Q8K_REQUIRE(most >= 1, Q8K_ERR_UNSUPPORTED, "gated_mm: this device cannot run pairs of CTAs with %d bytes of shared memory", L::kTotal);
+    const int clusters = p.total_tiles < most ? p.total_tiles : most;
+    Q8K_CUDA_OK(launch_dependent(kern, 2 * clusters, kGemmThreads, L::kTotal, st, 1, ta, tw, to, tp, p));
+    return Q8K_OK;
+}
+
+// Columns of a tile: those with the shortest estimate of whole rounds of tiles times the time of one, 0.165 us per 128-byte slab of K for
+// the issuing threads or 0.31 us at 256 columns of the product, and 1.5 us for what a tile costs besides.
+static int gated_columns(int M, int F, int K, int clusters) {
+    const double slabs = (K + kGemmBK - 1) / kGemmBK;
+    double best = 1e30;
+    int bn = kGatedBN;
+    for (int c = kGatedBN; c >= 32; c -= 32) {
+        const double tiles = (double)((M + 2 * kGemmBM - 1) / (2 * kGemmBM)) * ((F + c - 1) / c);
+        const double rounds = (double)(int64_t)((tiles + clusters - 1) / clusters);
+        const double slab = 0.31 * c / kGatedBN > 0.165 ? 0.31 * c / kGatedBN : 0.165;
+        const double t = rounds * (slabs * slab + 1.5);
+        if (t < best) { best = t; bn = c; }
+    }
+    return bn;
+}
+
+}  // namespace q8k
+
+extern "C" int q8k_gated_mm(int int8, const void* a, const void* w, const float* bias, const float* a_scales, const float* w_scales,
+                            void* out, void* pre, int activation, int M, int F, int K, int* dev_status, void* stream) {
+    using namespace q8k;
+    const char* op = "gated_mm";
+    Q8K_REQUIRE(M >= 0 && F > 0 && K > 0, Q8K_ERR_INVALID_ARG, "%s: bad shape M=%d F=%d K=%d", op, M, F, K);
+    Q8K_REQUIRE(F % 16 == 0 && K % 16 == 0, Q8K_ERR_INVALID_ARG, "%s: F=%d and K=%d must be multiples of 16", op, F, K);
+    Q8K_REQUIRE(F <= 0x3fffffff && M <= 0x7fffffff - 2 * kGemmBM, Q8K_ERR_TOO_LARGE, "%s: M=%d or F=%d too large", op, M, F);
+    Q8K_REQUIRE(activation == Q8K_ACT_SILU || activation == Q8K_ACT_GELU_TANH, Q8K_ERR_UNSUPPORTED, "%s: activation %d is unknown", op,
+                activation);
+    if (M == 0) return Q8K_OK;
+    Q8K_REQUIRE(a && w && a_scales && w_scales && out, Q8K_ERR_INVALID_ARG, "%s: null pointer", op);
+    Q8K_REQUIRE(aligned16(a) && aligned16(w) && aligned16(out) && aligned16(pre), Q8K_ERR_INVALID_ARG,
+                "%s: a, w, out and pre must be 16-byte aligned", op);
+    GatedParams p = {a_scales, w_scales, bias, dev_status, M, F, K, 0, 0, 0};
+    p.bn = gated_columns(M, F, K, gemm_num_sms() / 2);
+    p.n_tiles = (F + p.bn - 1) / p.bn;
+    const int64_t total = (int64_t)((M + 2 * kGemmBM - 1) / (2 * kGemmBM)) * p.n_tiles;
+    Q8K_REQUIRE(total <= 0x7fffffffLL, Q8K_ERR_TOO_LARGE, "%s: too many tiles", op);
+    p.total_tiles = (int)total;
+    CUtensorMap ta, tw, to, tp;
+    {
+        const uint64_t dims[2] = {(uint64_t)K, (uint64_t)M};
+        const uint64_t strides[1] = {(uint64_t)K};
+        const uint32_t box[2] = {(uint32_t)kGemmBK, (uint32_t)kGemmBM};
+        if (int rc = make_byte_tensor_map(&ta, a, 2, dims, strides, box, 128, op)) return rc;
+    }
+    {
+        const uint64_t dims[2] = {(uint64_t)K, 2 * (uint64_t)F};
+        const uint64_t strides[1] = {(uint64_t)K};
+        const uint32_t box[2] = {(uint32_t)kGemmBK, (uint32_t)p.bn};
+        if (int rc = make_byte_tensor_map(&tw, w, 2, dims, strides, box, 128, op)) return rc;
+    }
+    {
+        const uint64_t dims[3] = {2 * (uint64_t)F, (uint64_t)M, 1};
+        const uint64_t strides[2] = {2 * (uint64_t)F, 2 * (uint64_t)F * (uint64_t)M};
+        const uint32_t box[3] = {64, 32, 1};
+        if (int rc = make_byte_tensor_map(&to, out, 3, dims, strides, box, 64, op)) return rc;
+    }
+    tp = to;
+    if (pre != nullptr) {
+        const uint64_t dims[3] = {2 * (uint64_t)F, 2, (uint64_t)M};
+        const uint64_t strides[2] = {2 * (uint64_t)F, 4 * (uint64_t)F};
+        const uint32_t box[3] = {64, 1, 32};
+        if (int rc = make_byte_tensor_map(&tp, pre, 3, dims, strides, box, 64, op)) return rc;
+    }
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool gelu = activation == Q8K_ACT_GELU_TANH;
+#define Q8K_GATED(I8, SV) (gelu ? launch_gated_as<I8, true, SV>(ta, tw, to, tp, p, st) : launch_gated_as<I8, false, SV>(ta, tw, to, tp, p, st))
+    if (pre != nullptr) return int8 ? Q8K_GATED(true, true) : Q8K_GATED(false, true);
+    return int8 ? Q8K_GATED(true, false) : Q8K_GATED(false, false);
+#undef Q8K_GATED
+}

@@ -96,7 +96,7 @@ __device__ __forceinline__ void store_quant(Tq* p, const float (&v)[N], float qs
 template <typename Tin, typename Tout, int LOG_G, Epilogue EPI>
 __global__ void __launch_bounds__(128)
 hadamard_small_kernel(const Tin* __restrict__ x, Tout* __restrict__ out, float* __restrict__ scales,
-                      int64_t rows, int dim, int64_t x_row_stride, float scale) {
+                      int64_t rows, int dim, int64_t x_row_stride, float scale, bool two_step) {
     constexpr int G = 1 << LOG_G;
     constexpr int ROWS_PER_CTA = 128 / G;
     const int lane = threadIdx.x & 31;
@@ -128,7 +128,7 @@ hadamard_small_kernel(const Tin* __restrict__ x, Tout* __restrict__ out, float* 
 #pragma unroll
         for (int m = 1; m < G; m <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, m));
         const float qmax = std::is_same_v<Tout, int8_t> ? 127.0f : 448.0f;
-        const float qscale = __fdiv_rn(qmax, amax);
+        const float qscale = quant_factor(qmax, amax, two_step);
         if (row_ok && e < dim) store_quant<Tout, 8>(out + row * (int64_t)dim + e, v, qscale, amax == 0.f);
         if (row_ok && sub == 0) scales[row] = __fdiv_rn(1.0f, qscale);
     }
@@ -275,7 +275,7 @@ template <typename Tin, typename Tout, int LOG_N, Epilogue EPI, bool NORM_MOD, b
 __global__ void __launch_bounds__(StreamGeo<Tin, LOG_N, NORM_MOD>::THREADS, StreamGeo<Tin, LOG_N, NORM_MOD>::CTAS)
 hadamard_stream_kernel(const Tin* __restrict__ x, Tout* __restrict__ out, float* __restrict__ scales, unsigned rows, int dim,
                        int64_t x_row_stride, float scale, const __nv_bfloat16* __restrict__ mod_scale,
-                       const __nv_bfloat16* __restrict__ mod_shift, unsigned rows_per_mod, unsigned blocks_per_mod) {
+                       const __nv_bfloat16* __restrict__ mod_shift, unsigned rows_per_mod, unsigned blocks_per_mod, bool two_step) {
     constexpr bool DEQ = std::is_same_v<Tin, int8_t>;
     static_assert(!DEQ || EPI == Epilogue::Cast, "int8 rows are only transformed, not quantised again");
     using Geo = StreamGeo<Tin, LOG_N, NORM_MOD>;
@@ -555,7 +555,7 @@ hadamard_stream_kernel(const Tin* __restrict__ x, Tout* __restrict__ out, float*
                 for (int k = 1; k < T / 32; ++k) amax = fmaxf(amax, red_max[k]);
             }
             const float qmax = std::is_same_v<Tout, int8_t> ? 127.0f : 448.0f;
-            const float qscale = __fdiv_rn(qmax, amax);
+            const float qscale = quant_factor(qmax, amax, two_step);
             if (row_ok && t == 0) scales[row] = __fdiv_rn(1.0f, qscale);
             const float qmul = amax == 0.f ? 0.f : qscale;     // an all-zero row quantises to zeros (0 * 0, not 0 * inf)
             const float2 q2 = make_float2(qmul, qmul);
@@ -615,7 +615,7 @@ hadamard_stream_kernel(const Tin* __restrict__ x, Tout* __restrict__ out, float*
 
 template <typename Tin, typename Tout, int LOG_N, Epilogue EPI, bool NORM_MOD>
 static int launch_stream(const Tin* x, Tout* out, float* scales, int64_t rows, int dim, int64_t stride, float scale,
-                         const __nv_bfloat16* ms, const __nv_bfloat16* mh, int64_t rows_per_mod, cudaStream_t st) {
+                         const __nv_bfloat16* ms, const __nv_bfloat16* mh, int64_t rows_per_mod, cudaStream_t st, bool two_step = false) {
     using Geo = StreamGeo<Tin, LOG_N, NORM_MOD>;
     const bool full = dim == Geo::N;
     auto kern = full ? hadamard_stream_kernel<Tin, Tout, LOG_N, EPI, NORM_MOD, true>
@@ -640,14 +640,14 @@ static int launch_stream(const Tin* x, Tout* out, float* scales, int64_t rows, i
     // rows (1 x 1 x 2048: 3.2 us, 3.4 with one unit).
     const int units = NORM_MOD && need == 1 && groups > slots ? (int)((group_rows + Geo::RPU - 1) / Geo::RPU) : Geo::UNITS;
     Q8K_CUDA_OK(launch_dependent(kern, (unsigned)(blocks * groups), units * Geo::UNIT, Geo::smem(units), st, 1, x, out, scales, (unsigned)rows,
-                                 dim, stride, scale, ms, mh, (unsigned)group_rows, (unsigned)blocks));
+                                 dim, stride, scale, ms, mh, (unsigned)group_rows, (unsigned)blocks, two_step));
     return Q8K_OK;
 }
 
 // ------------------------------------------------------------------ dispatch
 template <typename Tin, typename Tout, Epilogue EPI>
 static int launch_hadamard(const void* x, void* out, float* scales, int64_t rows, int dim,
-                           int64_t stride, float scale, cudaStream_t st, const char* op) {
+                           int64_t stride, float scale, cudaStream_t st, const char* op, bool two_step = false) {
     int log_n = 3;
     while ((1 << log_n) < dim) ++log_n;
     const Tin* xi = (const Tin*)x;
@@ -656,11 +656,11 @@ static int launch_hadamard(const void* x, void* out, float* scales, int64_t rows
         const int log_g = log_n - 3;
         const int rows_per_cta = 128 >> log_g;
         const unsigned grid = (unsigned)((rows + rows_per_cta - 1) / rows_per_cta);
-#define Q8K_HS(LG) case LG: hadamard_small_kernel<Tin, Tout, LG, EPI><<<grid, 128, 0, st>>>(xi, o, scales, rows, dim, stride, scale); break
+#define Q8K_HS(LG) case LG: hadamard_small_kernel<Tin, Tout, LG, EPI><<<grid, 128, 0, st>>>(xi, o, scales, rows, dim, stride, scale, two_step); break
         switch (log_g) { Q8K_HS(0); Q8K_HS(1); Q8K_HS(2); Q8K_HS(3); Q8K_HS(4); Q8K_HS(5); }
 #undef Q8K_HS
     } else {
-#define Q8K_HS(LN) case LN: return launch_stream<Tin, Tout, LN, EPI, false>(xi, o, scales, rows, dim, stride, scale, nullptr, nullptr, 1, st)
+#define Q8K_HS(LN) case LN: return launch_stream<Tin, Tout, LN, EPI, false>(xi, o, scales, rows, dim, stride, scale, nullptr, nullptr, 1, st, two_step)
         switch (log_n) {
             Q8K_HS(9); Q8K_HS(10); Q8K_HS(11); Q8K_HS(12); Q8K_HS(13); Q8K_HS(14);
             default: set_error_detail("%s: dim %d exceeds 16384", op, dim); return Q8K_ERR_UNSUPPORTED;
@@ -744,20 +744,27 @@ extern "C" int q8k_dequant_hadamard(const void* x, const float* row_scales, void
     return Q8K_ERR_UNSUPPORTED;
 }
 
-extern "C" int q8k_hadamard_quant(const void* x, int x_dtype, void* q, int q_dtype, float* scales,
-                                  int64_t rows, int dim, int64_t x_row_stride, float scale, void* stream) {
-    const char* op = "hadamard_quant";
+namespace q8k {
+int hadamard_quant_as(const char* op, bool two_step, const void* x, int x_dtype, void* q, int q_dtype, float* scales, int64_t rows, int dim,
+                      int64_t x_row_stride, float scale, cudaStream_t st) {
     if (int rc = check_hadamard_args(op, x, x_dtype, q, rows, dim, x_row_stride)) return rc;
     if (rows == 0) return Q8K_OK;
     Q8K_REQUIRE(scales != nullptr, Q8K_ERR_INVALID_ARG, "%s: null scales pointer", op);
-    cudaStream_t st = (cudaStream_t)stream;
     constexpr Epilogue Q = Epilogue::Quant;
-    if (x_dtype == Q8K_DT_BF16 && q_dtype == Q8K_DT_I8)   return launch_hadamard<__nv_bfloat16, int8_t, Q>(x, q, scales, rows, dim, x_row_stride, scale, st, op);
-    if (x_dtype == Q8K_DT_BF16 && q_dtype == Q8K_DT_E4M3) return launch_hadamard<__nv_bfloat16, e4m3_t, Q>(x, q, scales, rows, dim, x_row_stride, scale, st, op);
-    if (x_dtype == Q8K_DT_E4M3 && q_dtype == Q8K_DT_I8)   return launch_hadamard<e4m3_t, int8_t, Q>(x, q, scales, rows, dim, x_row_stride, scale, st, op);
-    if (x_dtype == Q8K_DT_E4M3 && q_dtype == Q8K_DT_E4M3) return launch_hadamard<e4m3_t, e4m3_t, Q>(x, q, scales, rows, dim, x_row_stride, scale, st, op);
+#define Q8K_HQ(TIN, TOUT) return launch_hadamard<TIN, TOUT, Q>(x, q, scales, rows, dim, x_row_stride, scale, st, op, two_step)
+    if (x_dtype == Q8K_DT_BF16 && q_dtype == Q8K_DT_I8)   Q8K_HQ(__nv_bfloat16, int8_t);
+    if (x_dtype == Q8K_DT_BF16 && q_dtype == Q8K_DT_E4M3) Q8K_HQ(__nv_bfloat16, e4m3_t);
+    if (x_dtype == Q8K_DT_E4M3 && q_dtype == Q8K_DT_I8)   Q8K_HQ(e4m3_t, int8_t);
+    if (x_dtype == Q8K_DT_E4M3 && q_dtype == Q8K_DT_E4M3) Q8K_HQ(e4m3_t, e4m3_t);
+#undef Q8K_HQ
     set_error_detail("%s: quantised dtype %d is not int8 or e4m3", op, q_dtype);
     return Q8K_ERR_UNSUPPORTED;
+}
+}  // namespace q8k
+
+extern "C" int q8k_hadamard_quant(const void* x, int x_dtype, void* q, int q_dtype, float* scales,
+                                  int64_t rows, int dim, int64_t x_row_stride, float scale, void* stream) {
+    return hadamard_quant_as("hadamard_quant", false, x, x_dtype, q, q_dtype, scales, rows, dim, x_row_stride, scale, (cudaStream_t)stream);
 }
 
 extern "C" int q8k_norm_modulate_quant(const void* x, const void* mod_scale, const void* mod_shift, void* q, int q_dtype,

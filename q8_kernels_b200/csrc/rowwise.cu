@@ -55,7 +55,7 @@ __device__ __forceinline__ float block_reduce_sum(float v, float* smem) {
 template <typename Tin, typename Tout, int ITEMS, int T>
 __global__ void __launch_bounds__(T)
 tokenwise_quant_kernel(const Tin* __restrict__ x, Tout* __restrict__ q, float* __restrict__ scales,
-                       int dim, int64_t x_row_stride) {
+                       int dim, int64_t x_row_stride, bool two_step) {
     __shared__ float red[32];
     pdl_wait();
     pdl_release();
@@ -78,7 +78,7 @@ tokenwise_quant_kernel(const Tin* __restrict__ x, Tout* __restrict__ q, float* _
 
     constexpr bool kInt8 = sizeof(Tout) == 1 && !__is_same(Tout, e4m3_t);
     const float qmax = kInt8 ? 127.0f : 448.0f;
-    const float scale = __fdiv_rn(qmax, amax);            // +inf for an all-zero row
+    const float scale = quant_factor(qmax, amax, two_step);   // +inf for an all-zero row
     const bool zero_row = amax == 0.f;
 
 #pragma unroll
@@ -437,12 +437,12 @@ rms_norm_backward_kernel(const Ty* __restrict__ y, const float* __restrict__ rrm
 
 // ------------------------------------------------------------------ launch helpers
 template <typename Tin, typename Tout>
-static int launch_quant(const void* x, void* q, float* scales, int64_t rows, int dim,
+static int launch_quant(const char* op, bool two_step, const void* x, void* q, float* scales, int64_t rows, int dim,
                         int64_t stride, cudaStream_t st) {
     const int items = dim / kItem;
 #define Q8K_Q_LAUNCH(ITEMS, T)                                                                  \
     Q8K_CUDA_OK(launch_dependent(tokenwise_quant_kernel<Tin, Tout, ITEMS, T>, (unsigned)rows, T, 0, st, 1,     \
-                                 (const Tin*)x, (Tout*)q, scales, dim, stride))
+                                 (const Tin*)x, (Tout*)q, scales, dim, stride, two_step))
     if (items <= 32)        Q8K_Q_LAUNCH(1, 32);
     else if (items <= 128)  Q8K_Q_LAUNCH(1, 128);
     else if (items <= 256)  Q8K_Q_LAUNCH(2, 128);
@@ -450,7 +450,7 @@ static int launch_quant(const void* x, void* q, float* scales, int64_t rows, int
     else if (items <= 1024) Q8K_Q_LAUNCH(4, 256);
     else if (items <= 2048) Q8K_Q_LAUNCH(8, 256);
     else if (items <= 4096) Q8K_Q_LAUNCH(8, 512);
-    else { set_error_detail("tokenwise_quant: dim %d exceeds 32768", dim); return Q8K_ERR_UNSUPPORTED; }
+    else { set_error_detail("%s: dim %d exceeds 32768", op, dim); return Q8K_ERR_UNSUPPORTED; }
 #undef Q8K_Q_LAUNCH
     Q8K_CUDA_OK(cudaGetLastError());
     return Q8K_OK;
@@ -487,20 +487,20 @@ static int check_rows_dim(const char* op, int64_t rows, int dim, int multiple) {
 
 using namespace q8k;
 
-extern "C" int q8k_tokenwise_quant(const void* x, int x_dtype, void* q, int q_dtype, float* scales,
-                                   int64_t rows, int dim, int64_t x_row_stride, void* stream) {
-    if (int rc = check_rows_dim("tokenwise_quant", rows, dim, 16)) return rc;
+namespace q8k {
+int tokenwise_quant_as(const char* op, bool two_step, const void* x, int x_dtype, void* q, int q_dtype, float* scales, int64_t rows, int dim,
+                       int64_t x_row_stride, cudaStream_t st) {
+    if (int rc = check_rows_dim(op, rows, dim, 16)) return rc;
     if (rows == 0) return Q8K_OK;
-    Q8K_REQUIRE(x && q && scales, Q8K_ERR_INVALID_ARG, "tokenwise_quant: null pointer");
-    Q8K_REQUIRE(aligned16(x) && aligned16(q), Q8K_ERR_INVALID_ARG, "tokenwise_quant: x and q must be 16-byte aligned");
+    Q8K_REQUIRE(x && q && scales, Q8K_ERR_INVALID_ARG, "%s: null pointer", op);
+    Q8K_REQUIRE(aligned16(x) && aligned16(q), Q8K_ERR_INVALID_ARG, "%s: x and q must be 16-byte aligned", op);
     Q8K_REQUIRE(x_row_stride >= dim && (x_row_stride * dtype_size(x_dtype)) % 16 == 0, Q8K_ERR_INVALID_ARG,
-                "tokenwise_quant: row stride %lld must be >= dim and a multiple of 16 bytes", (long long)x_row_stride);
+                "%s: row stride %lld must be >= dim and a multiple of 16 bytes", op, (long long)x_row_stride);
     Q8K_REQUIRE(q_dtype == Q8K_DT_I8 || q_dtype == Q8K_DT_E4M3, Q8K_ERR_UNSUPPORTED,
-                "tokenwise_quant: output dtype %d is not int8 or e4m3", q_dtype);
-    cudaStream_t st = (cudaStream_t)stream;
+                "%s: output dtype %d is not int8 or e4m3", op, q_dtype);
 #define Q8K_QD(TIN)                                                                              \
-    return q_dtype == Q8K_DT_I8 ? launch_quant<TIN, int8_t>(x, q, scales, rows, dim, x_row_stride, st) \
-                                : launch_quant<TIN, e4m3_t>(x, q, scales, rows, dim, x_row_stride, st)
+    return q_dtype == Q8K_DT_I8 ? launch_quant<TIN, int8_t>(op, two_step, x, q, scales, rows, dim, x_row_stride, st) \
+                                : launch_quant<TIN, e4m3_t>(op, two_step, x, q, scales, rows, dim, x_row_stride, st)
     switch (x_dtype) {
         case Q8K_DT_F32:  Q8K_QD(float);
         case Q8K_DT_F16:  Q8K_QD(__half);
@@ -509,8 +509,14 @@ extern "C" int q8k_tokenwise_quant(const void* x, int x_dtype, void* q, int q_dt
         default: break;
     }
 #undef Q8K_QD
-    set_error_detail("tokenwise_quant: input dtype %d not supported", x_dtype);
+    set_error_detail("%s: input dtype %d not supported", op, x_dtype);
     return Q8K_ERR_UNSUPPORTED;
+}
+}  // namespace q8k
+
+extern "C" int q8k_tokenwise_quant(const void* x, int x_dtype, void* q, int q_dtype, float* scales,
+                                   int64_t rows, int dim, int64_t x_row_stride, void* stream) {
+    return tokenwise_quant_as("tokenwise_quant", false, x, x_dtype, q, q_dtype, scales, rows, dim, x_row_stride, (cudaStream_t)stream);
 }
 
 extern "C" int q8k_transpose_quant(const void* x, int x_dtype, const float* row_scales, void* q, float* scales, int N, int K,

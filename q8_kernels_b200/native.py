@@ -720,3 +720,197 @@ def linear(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: Optio
            ptr(out), dt(out_type), M, N, K, int(bool(use_hadamard)), int(bool(fuse_gelu)), ptr(ws), ws.numel(),
            ptr(_lib.status_word(dev)))
     return out
+
+
+# ---------------------------------------------------------------- ops without a counterpart in the reference's modules
+
+def _strided_rows(x: torch.Tensor):
+    """(tensor, rows, dim, row stride) of [..., dim] for a kernel that takes rows at any alignment."""
+    dim = x.shape[-1]
+    if x.is_contiguous():
+        return x, x.numel() // dim, dim, dim
+    x2 = x.reshape(-1, dim)
+    if dim > 1 and x2.stride(1) != 1:
+        x2 = x2.contiguous()
+    return x2, x2.shape[0], dim, x2.stride(0) if x2.shape[0] > 1 else dim
+
+
+def _norm_vector(t: Optional[torch.Tensor], dim: int, name: str) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or tuple(t.shape) != (dim,):
+        raise Q8KernelError(f"layer_norm: {name} must be float32 [{dim}], not {t.dtype} {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float,
+               out_type: Optional[torch.dtype] = None, stats: bool = False) -> List[Optional[torch.Tensor]]:
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dim.  Returns ``[y, mean, rstd]``, the two fp32 vectors of shape
+    x.shape[:-1] only with ``stats`` (else None)."""
+    dev = require_cuda(x, weight, bias)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise Q8KernelError(f"layer_norm: x of shape {tuple(x.shape)} has no rows to normalise")
+    out_type = x.dtype if out_type is None else out_type
+    x2, rows, dim, stride = _strided_rows(x)
+    weight, bias = _norm_vector(weight, dim, "weight"), _norm_vector(bias, dim, "bias")
+    y = torch.empty(x.shape, dtype=out_type, device=dev)
+    mean, rstd = ([torch.empty(x.shape[:-1], dtype=torch.float32, device=dev) for _ in range(2)] if stats else (None, None))
+    launch(dev, "layer_norm", lib.q8k_layer_norm, ptr(x2), dt(x.dtype), stride, ptr(weight), ptr(bias), ptr(y), dt(out_type), ptr(mean),
+           ptr(rstd), rows, dim, float(eps))
+    return [y, mean, rstd]
+
+
+def layer_norm_backward(x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, grad: torch.Tensor,
+                        weight: Optional[torch.Tensor] = None, need_dx: bool = True, need_dweight: bool = False,
+                        need_dbias: bool = False) -> List[Optional[torch.Tensor]]:
+    """``[dx, dweight, dbias]`` of layer_norm from its input, the statistics that it returned and the output's gradient (x's type; bf16
+    or fp16 too for an fp32 x); None for what is not needed."""
+    dev = require_cuda(x, mean, rstd, grad, weight)
+    if x.dim() < 1 or x.shape[-1] == 0 or grad.shape != x.shape:
+        raise Q8KernelError(f"layer_norm_backward: gradient {tuple(grad.shape)} of an input {tuple(x.shape)}")
+    for t in (mean, rstd):
+        if t.dtype != torch.float32 or t.shape != x.shape[:-1]:
+            raise Q8KernelError("layer_norm_backward: mean and rstd must be those of layer_norm")
+    x2, rows, dim, stride = _strided_rows(x)
+    grad, mean, rstd = grad.contiguous(), mean.contiguous(), rstd.contiguous()
+    weight = _norm_vector(weight, dim, "weight")
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_dx else None
+    dw, db = (torch.empty(dim, dtype=torch.float32, device=dev) if need else None for need in (need_dweight, need_dbias))
+    work = None
+    if need_dweight or need_dbias:
+        work = torch.empty(lib.q8k_layer_norm_backward_workspace_bytes(rows, dim), dtype=torch.uint8, device=dev)
+    launch(dev, "layer_norm_backward", lib.q8k_layer_norm_backward, ptr(x2), dt(x.dtype), stride, ptr(grad), dt(grad.dtype), ptr(mean),
+           ptr(rstd), ptr(weight), ptr(dx), ptr(dw), ptr(db), rows, dim, ptr(work), 0 if work is None else work.numel())
+    return [dx, dw, db]
+
+
+_Strides = ctypes.c_int64 * 3
+
+
+def rotary(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: Optional[torch.Tensor], frequencies: torch.Tensor,
+           amplitude: float = 1.0, half: bool = True, backward: bool = False) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """q and k ([B,S,H,D] or [S,H,D], either may be None) with the first ``2 * len(frequencies)`` channels of each head turned by
+    ``position * frequency`` (``backward``: by the negative angle) and scaled by ``amplitude``: see functional.rotary."""
+    x = q if q is not None else k
+    if x is None:
+        raise Q8KernelError("rotary: neither q nor k")
+    dev = require_cuda(q, k, positions, frequencies)
+    if x.dim() not in (3, 4):
+        raise Q8KernelError(f"rotary: q and k must be [B,S,H,D] or [S,H,D], not {tuple(x.shape)}")
+    if q is not None and k is not None and (k.dtype != q.dtype or k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2]
+                                            or k.shape[-1] != q.shape[-1]):
+        raise Q8KernelError(f"rotary: q {q.dtype} {tuple(q.shape)} and k {k.dtype} {tuple(k.shape)} do not go together")
+    batch, seq = (1, x.shape[0]) if x.dim() == 3 else x.shape[:2]
+    dim = x.shape[-1]
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1:
+        raise Q8KernelError(f"rotary: frequencies must be float64 [rotary_dim / 2], not {frequencies.dtype} {tuple(frequencies.shape)}")
+    frequencies = frequencies.contiguous()
+    wide, pos_batch, pos_token = 0, 0, 0
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise Q8KernelError(f"rotary: positions must be int32 or int64, not {positions.dtype}")
+        if tuple(positions.shape) not in ((seq,), (1, seq), (batch, seq)):
+            raise Q8KernelError(f"rotary: positions {tuple(positions.shape)} for a batch of {batch} sequences of {seq}")
+        wide = int(positions.dtype == torch.int64)
+        pos_token = positions.stride(-1)
+        pos_batch = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
+
+    def tensor(t):
+        if t is None:
+            return None, None, None, (None, None, None, None, 0)
+        if dim > 1 and t.stride(-1) != 1:
+            t = t.contiguous()
+        out = torch.empty(t.shape, dtype=t.dtype, device=dev)
+        s, o = ((0,) * (t.dim() == 3) + a.stride()[:-1] for a in (t, out))
+        return t, out, None, (ptr(t), _Strides(*s), ptr(out), _Strides(*o), t.shape[-2])
+
+    q_in, q_out, _, q_args = tensor(q)                       # (the inputs stay alive until the launch)
+    k_in, k_out, _, k_args = tensor(k)
+    launch(dev, "rotary", lib.q8k_rotary, *q_args, *k_args, dt(x.dtype), ptr(positions), wide, pos_batch, pos_token, ptr(frequencies),
+           float(amplitude), batch, seq, dim, 2 * frequencies.numel(), int(half), int(backward))
+    return q_out, k_out
+
+
+ACTIVATIONS = {"silu": 1, "gelu_tanh": 2}
+GATED_TRAINING_MAX = 16384                                   # columns of a row that the backward pass keeps in registers
+
+
+def gated_check(a, w, bias, a_scales, w_scales, act, op="gated_mm", training=False) -> Tuple[torch.device, int]:
+    """What every call of the gated projection has to fulfil; returns the device and F."""
+    dev = require_cuda(a, w, bias, a_scales, w_scales)
+    if act not in ACTIVATIONS:
+        raise Q8KernelError(f"{op}: activation {act!r} is not one of {', '.join(ACTIVATIONS)}")
+    if w.dim() != 2 or w.shape[0] % 32 or w.shape[0] == 0:
+        raise Q8KernelError(f"{op}: the weight must be [2F, K] with F a multiple of 16, not {tuple(w.shape)}")
+    if a.dim() < 1 or a.shape[-1] != w.shape[1]:
+        raise Q8KernelError(f"{op}: activation {tuple(a.shape)} and weight {tuple(w.shape)} do not go together")
+    f = w.shape[0] // 2
+    for name, t, n in (("bias", bias, 2 * f), ("weight scales", w_scales, 2 * f), ("activation scales", a_scales, None)):
+        if t is not None and (t.dtype != torch.float32 or (t.numel() != n if n is not None else t.shape != a.shape[:-1])):
+            raise Q8KernelError(f"{op}: {name} of type {t.dtype} and shape {tuple(t.shape)} do not fit")
+    if training and f > GATED_TRAINING_MAX:
+        raise Q8KernelError(f"{op}: F={f} exceeds {GATED_TRAINING_MAX}, the most that the backward pass takes")
+    return dev, f
+
+
+def gated_mm(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a_scales: torch.Tensor, w_scales: torch.Tensor,
+             act: str = "silu", save: bool = False) -> List[Optional[torch.Tensor]]:
+    """``act(gate) * up`` (bf16 [...,F]) of the products of ``a`` [...,K] with the first and last F rows of ``w`` [2F,K], both int8 or both
+    e4m3.  Returns ``[out, pre]``, pre = bf16 [...,2,F] holding gate and up with ``save``, else None."""
+    if a.dtype != w.dtype or a.dtype not in (torch.int8, E4M3):
+        raise Q8KernelError(f"gated_mm: {a.dtype} activation and {w.dtype} weight must be both int8 or both float8_e4m3fn")
+    dev, f = gated_check(a, w, bias, a_scales, w_scales, act)
+    a, w, a_scales, w_scales = a.contiguous(), w.contiguous(), a_scales.contiguous(), w_scales.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    out = torch.empty(a.shape[:-1] + (f,), dtype=torch.bfloat16, device=dev)
+    pre = torch.empty(a.shape[:-1] + (2, f), dtype=torch.bfloat16, device=dev) if save else None
+    k = a.shape[-1]
+    launch(dev, "gated_mm", lib.q8k_gated_mm, int(a.dtype == torch.int8), ptr(a), ptr(w), ptr(bias), ptr(a_scales), ptr(w_scales), ptr(out),
+           ptr(pre), ACTIVATIONS[act], out.numel() // f, f, k, ptr(_lib.status_word(dev)))
+    return [out, pre]
+
+
+def gated_quant(x: torch.Tensor, rotate: bool, out_type: torch.dtype) -> List[torch.Tensor]:
+    """The activation of the gated projection: x [...,K] (bf16 or e4m3) rotated (``rotate``: Hadamard, 1/sqrt(K), rounded to x's type) and
+    quantised per token to int8 or e4m3.  Returns ``[q, scales]``.  As hadamard_quant / tokenwise_quant, but the row's factor is
+    ``top * (1 / absmax)``, two roundings, where those take ``top / absmax``."""
+    dev = require_cuda(x)
+    x2, rows, dim, stride = _rows(x)
+    q = torch.empty(x.shape, dtype=out_type, device=dev)
+    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    launch(dev, "gated_quant", lib.q8k_gated_quant, ptr(x2), dt(x.dtype), stride, ptr(q), dt(out_type), ptr(scales), rows, dim, int(rotate))
+    return [q, scales]
+
+
+def gated_weight_operand(w: torch.Tensor, w_scales: torch.Tensor) -> List[torch.Tensor]:
+    """``w * w_scales[:, None]`` ([2F,K], int8 or e4m3) transposed and quantised to e4m3 per input channel, the weight operand of the backward
+    product.  Returns ``[q, scales]``: e4m3 [K,2F] and fp32 [K]."""
+    dev = require_cuda(w, w_scales)
+    if w.dim() != 2 or w.shape[0] % 32 or w_scales.dtype != torch.float32 or w_scales.numel() != w.shape[0]:
+        raise Q8KernelError("gated_weight_operand: the weight must be [2F,K], F a multiple of 16, with float32 scales [2F]")
+    n, k = w.shape
+    w, w_scales = w.contiguous(), w_scales.contiguous()
+    q = torch.empty((k, n), dtype=E4M3, device=dev)
+    scales = torch.empty((k,), dtype=torch.float32, device=dev)
+    work = torch.empty(lib.q8k_gated_weight_operand_workspace_bytes(n // 2, k), dtype=torch.uint8, device=dev)
+    launch(dev, "gated_weight_operand", lib.q8k_gated_weight_operand, ptr(w), dt(w.dtype), ptr(w_scales), ptr(q), ptr(scales), n // 2, k,
+           ptr(work), work.numel())
+    return [q, scales]
+
+
+def gated_backward_quant(grad: torch.Tensor, pre: torch.Tensor, act: str = "silu") -> List[torch.Tensor]:
+    """``[grad * up * act'(gate) | grad * act(gate)]`` quantised per token to e4m3, from the output's gradient (bf16 [...,F]) and the
+    ``pre`` of gated_mm.  Returns ``[q, scales]``: e4m3 [...,2F] and fp32 [...]."""
+    dev = require_cuda(grad, pre)
+    if act not in ACTIVATIONS:
+        raise Q8KernelError(f"gated_backward_quant: activation {act!r} is not one of {', '.join(ACTIVATIONS)}")
+    if grad.dtype != torch.bfloat16 or pre.dtype != torch.bfloat16 or grad.dim() < 1 \
+            or tuple(pre.shape) != tuple(grad.shape[:-1]) + (2, grad.shape[-1]):
+        raise Q8KernelError("gated_backward_quant: the gradient must be bfloat16 [...,F] and pre bfloat16 [...,2,F]")
+    f = grad.shape[-1]
+    grad, pre = grad.contiguous(), pre.contiguous()
+    q = torch.empty(grad.shape[:-1] + (2 * f,), dtype=E4M3, device=dev)
+    scales = torch.empty(grad.shape[:-1], dtype=torch.float32, device=dev)
+    launch(dev, "gated_backward_quant", lib.q8k_gated_backward_quant, ptr(grad), ptr(pre), ptr(q), ptr(scales), ACTIVATIONS[act],
+           scales.numel(), f)
+    return [q, scales]
