@@ -19,10 +19,15 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
 
 #include <cmath>
+#include <optional>
+#include <stdexcept>
+#include <string>
 
 #include "../../include/q8_kernels_b200.h"
 
@@ -658,6 +663,366 @@ PyObject* qk_norm_rope_prep_pair(PyObject*, PyObject* const* args, Py_ssize_t n)
     FAST_END
 }
 
+// ---------------------------------------------------------------- layer norm, rotary positions, gated projection
+// These are differentiable: where an input has a gradient the call leaves a node of torch's C++ autograd behind, whose backward pass
+// launches without the interpreter.  (A Python autograd.Function costs some 60 us of host time for one forward and backward pass, the
+// kernels of a short call 10.)  What the functions of the same name in functional/ do with tensors that these do not take is the same.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
+int type_code(Dt t) { return t == Dt::Half ? Q8K_DT_F16 : dt_code(t); }      // (the ops above leave fp16 to their Python bodies)
+
+// An argument that may be missing.  (apply() does not take undefined tensors; the inputs that it numbers are those that are there.)
+using Maybe = std::optional<at::Tensor>;
+Maybe maybe(const at::Tensor* t) { return t == nullptr ? Maybe() : Maybe(*t); }
+at::Tensor value(const Maybe& t) { return t.has_value() ? *t : at::Tensor(); }
+
+struct Refused { int rc; const char* op; };                    // a launch's error on its way to Q8KernelError
+
+void must(int rc, const char* op) {
+    if (rc != Q8K_OK) throw Refused{rc, op};
+}
+// In a backward pass, which autograd runs: its error becomes a RuntimeError.
+void must_backward(int rc, const char* op) {
+    if (rc != Q8K_OK) throw std::runtime_error(std::string(op) + ": " + q8k_error_string(rc) + ": " + q8k_last_error_detail());
+}
+template <typename F> PyObject* answer(F&& f) {                // f() -> PyObject*, with Refused turned into the Python error
+    try {
+        return f();
+    } catch (const Refused& e) {
+        if (launched(e.rc, e.op)) Py_RETURN_NONE;
+        return nullptr;
+    }
+}
+void* stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+at::Tensor empty_like_dtype(at::IntArrayRef shape, const at::Tensor& like, Dt type) {
+    return at::empty(shape, at::TensorOptions().dtype(type).device(like.device()));
+}
+float* out_f(at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+const at::Tensor* defined(const at::Tensor& t) { return t.defined() ? &t : nullptr; }
+bool wants_grad(const at::Tensor* t) { return t != nullptr && t->requires_grad(); }
+
+// Gradients that cannot be differentiated again say so when that is tried, as once_differentiable does in Python.
+variable_list once_only(variable_list&& grads, const variable_list& incoming) {
+    bool graph = false;
+    for (const Variable& g : incoming) graph = graph || (g.defined() && g.requires_grad());
+    if (!c10::GradMode::is_enabled() || !graph) return std::move(grads);
+    for (Variable& g : grads)
+        if (g.defined()) g = g.detach().set_requires_grad(true);
+    auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that is differentiable once",
+                                                                 (int)grads.size());
+    return error->apply(std::move(grads));
+}
+
+// ---- layer_norm(x, weight | None, bias | None, eps, out_type)
+struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
+    static Variable run(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b, double eps, Dt out, at::Tensor* mean, at::Tensor* rstd) {
+        const int dim = (int)x.size(-1);
+        at::Tensor y = empty_like_dtype(x.sizes(), x, out);
+        if (mean != nullptr) {
+            *mean = empty_like_dtype(lead(x), x, Dt::Float);
+            *rstd = empty_like_dtype(lead(x), x, Dt::Float);
+        }
+        must(q8k_layer_norm(x.const_data_ptr(), type_code(x.scalar_type()), dim, fptr(defined(w)), fptr(defined(b)), y.data_ptr(), type_code(out),
+                            mean != nullptr ? mean->data_ptr<float>() : nullptr, rstd != nullptr ? rstd->data_ptr<float>() : nullptr,
+                            x.numel() / dim, dim, (float)eps, stream_of(x)), "layer_norm");
+        return y;
+    }
+    static Variable forward(AutogradContext* ctx, const Variable& x, const Maybe& w, const Maybe& b, double eps, int64_t out) {
+        at::Tensor mean, rstd;
+        Variable y = run(x, value(w), value(b), eps, (Dt)out, &mean, &rstd);
+        ctx->save_for_backward({x, value(w), mean, rstd});
+        ctx->saved_data["bias"] = b.has_value();
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        variable_list result(5);
+        if (!grads[0].defined()) return result;
+        {
+            at::NoGradGuard no_grad;
+            const at::Tensor &x = saved[0], &w = saved[1], &mean = saved[2], &rstd = saved[3];
+            at::Tensor g = grads[0];
+            if (g.scalar_type() == Dt::Float8_e4m3fn) g = g.to(Dt::BFloat16);       // exact
+            g = g.contiguous();
+            const int dim = (int)x.size(-1);
+            const int64_t rows = x.numel() / dim;
+            at::Tensor dx, dw, db, work;
+            if (ctx->needs_input_grad(0)) dx = empty_like_dtype(x.sizes(), x, x.scalar_type());
+            const bool has_w = w.defined();
+            if (has_w && ctx->needs_input_grad(1)) dw = empty_like_dtype({dim}, x, Dt::Float);
+            if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(1 + has_w)) db = empty_like_dtype({dim}, x, Dt::Float);
+            int64_t bytes = 0;
+            if (dw.defined() || db.defined()) {
+                bytes = (int64_t)q8k_layer_norm_backward_workspace_bytes(rows, dim);
+                work = empty_like_dtype({bytes}, x, Dt::Byte);
+            }
+            must_backward(q8k_layer_norm_backward(x.const_data_ptr(), type_code(x.scalar_type()), dim, g.const_data_ptr(),
+                                                  type_code(g.scalar_type()), mean.const_data_ptr<float>(), rstd.const_data_ptr<float>(),
+                                                  fptr(defined(w)), dx.defined() ? dx.data_ptr() : nullptr, out_f(dw), out_f(db), rows, dim,
+                                                  work.defined() ? work.data_ptr() : nullptr, (size_t)bytes, stream_of(x)),
+                          "layer_norm_backward");
+            result[0] = dx;
+            result[1] = dw;
+            result[2] = db;
+        }
+        return once_only(std::move(result), grads);
+    }
+};
+
+PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    FAST_BEGIN
+    Call c(args, n, 5);
+    const at::Tensor* x = c.tensor(0);
+    const at::Tensor* w = c.optional(1, Dt::Float);
+    const at::Tensor* b = c.optional(2, Dt::Float);
+    const float eps = c.real(3);
+    OR_NONE(c);
+    const Dt in = x->scalar_type(), out = c.dtype(4, in);
+    c.need(has_rows(x) && x->size(-1) <= 16384 && int_sized(x->numel() / x->size(-1)) &&
+           ((in == out && (in == Dt::Float || in == Dt::Half || in == Dt::BFloat16)) || (in == Dt::BFloat16 && out == Dt::Float8_e4m3fn) ||
+            (in == Dt::Float && (out == Dt::BFloat16 || out == Dt::Half))));
+    OR_NONE(c);
+    for (const at::Tensor* v : {w, b}) c.need(v == nullptr || (v->dim() == 1 && v->size(0) == x->size(-1)));
+    OR_NONE(c);
+    return answer([&]() -> PyObject* {
+        at::Tensor y;
+        {
+            WithoutGil unlocked;
+            if (c10::GradMode::is_enabled() && (x->requires_grad() || wants_grad(w) || wants_grad(b)))
+                y = LayerNormNode::apply(*x, maybe(w), maybe(b), (double)eps, (int64_t)out);
+            else
+                y = LayerNormNode::run(*x, value(maybe(w)), value(maybe(b)), eps, out, nullptr, nullptr);
+        }
+        return wrap(std::move(y));
+    });
+    FAST_END
+}
+
+// ---- rotary(q, k | None, positions | None, frequencies, amplitude, half)
+struct RotaryNode : torch::autograd::Function<RotaryNode> {
+    // q and k of [batch, seq, heads, dim], or without the batch; either may be undefined
+    static variable_list run(const at::Tensor& q, const at::Tensor& k, const at::Tensor& pos, const at::Tensor& freq, double amplitude, bool half,
+                             bool backward, int& rc) {
+        const at::Tensor& x = q.defined() ? q : k;
+        const int64_t d = x.dim(), batch = d == 4 ? x.size(0) : 1, seq = x.size(d - 3), dim = x.size(d - 1);
+        variable_list out(2);
+        int64_t stride[2][2][3] = {};
+        const at::Tensor* in[2] = {&q, &k};
+        for (int i = 0; i < 2; ++i) {
+            if (!in[i]->defined()) continue;
+            out[i] = empty_like_dtype(in[i]->sizes(), x, x.scalar_type());
+            for (int j = 0; j < 2; ++j) {
+                const at::Tensor& t = j == 0 ? *in[i] : out[i];
+                stride[i][j][0] = d == 4 ? t.stride(0) : 0;
+                stride[i][j][1] = t.stride(d - 3);
+                stride[i][j][2] = t.stride(d - 2);
+            }
+        }
+        const int64_t pb = pos.defined() && pos.dim() == 2 && pos.size(0) > 1 ? pos.stride(0) : 0;
+        const int64_t pt = pos.defined() ? pos.stride(-1) : 0;
+        auto heads = [&](const at::Tensor& t) { return t.defined() ? (int)t.size(d - 2) : 0; };
+        rc = q8k_rotary(cptr(defined(q)), stride[0][0], out[0].defined() ? out[0].data_ptr() : nullptr, stride[0][1], heads(q), cptr(defined(k)),
+                        stride[1][0], out[1].defined() ? out[1].data_ptr() : nullptr, stride[1][1], heads(k), type_code(x.scalar_type()),
+                        cptr(defined(pos)), pos.defined() && pos.scalar_type() == Dt::Long, pb, pt, freq.const_data_ptr<double>(),
+                        (float)amplitude, (int)batch, (int)seq, (int)dim, (int)(2 * freq.numel()), half, backward, stream_of(x));
+        return out;
+    }
+    static variable_list forward(AutogradContext* ctx, const Variable& q, const Maybe& k, const Maybe& pos, const Variable& freq,
+                                 double amplitude, bool half) {
+        int rc = 0;
+        variable_list out = run(q, value(k), value(pos), freq, amplitude, half, false, rc);
+        must(rc, "rotary");
+        ctx->save_for_backward({value(pos), freq});
+        ctx->saved_data["amplitude"] = amplitude;
+        ctx->saved_data["half"] = half;
+        ctx->set_materialize_grads(false);
+        if (!k.has_value()) out.pop_back();
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        variable_list result(6);
+        {
+            at::NoGradGuard no_grad;
+            at::Tensor g[2];
+            for (size_t i = 0; i < grads.size(); ++i) {
+                if (!grads[i].defined() || !ctx->needs_input_grad(i)) continue;
+                g[i] = grads[i].stride(-1) == 1 ? grads[i] : grads[i].contiguous();
+            }
+            if (!g[0].defined() && !g[1].defined()) return result;
+            int rc = 0;
+            variable_list d = run(g[0], g[1], saved[0], saved[1], ctx->saved_data["amplitude"].toDouble(), ctx->saved_data["half"].toBool(),
+                                  true, rc);
+            must_backward(rc, "rotary");
+            result[0] = d[0];
+            result[1] = d[1];
+        }
+        return once_only(std::move(result), grads);
+    }
+};
+
+PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    FAST_BEGIN
+    Call c(args, n, 6);
+    const at::Tensor* q = c.tensor(0, true);
+    const at::Tensor* k = c.ok && args[1] != Py_None ? c.tensor(1, true) : nullptr;
+    const at::Tensor* pos = c.ok && args[2] != Py_None ? c.tensor(2, true) : nullptr;
+    const at::Tensor* freq = c.tensor(3, Dt::Double);
+    const float amplitude = c.real(4);
+    const bool half = c.flag(5);
+    OR_NONE(c);
+    const Dt t = q->scalar_type();
+    const int64_t d = q->dim();
+    c.need((t == Dt::BFloat16 || t == Dt::Half || t == Dt::Float) && (d == 3 || d == 4) && q->stride(-1) == 1 && freq->dim() == 1);
+    OR_NONE(c);
+    const int64_t batch = d == 4 ? q->size(0) : 1, seq = q->size(d - 3), dim = q->size(-1);
+    c.need(int_sized(batch) && int_sized(seq) && dim <= 4096 && freq->numel() >= 1 && 2 * freq->numel() <= dim && q->size(d - 2) <= 65536);
+    if (k != nullptr) {
+        c.need(k->scalar_type() == t && k->dim() == d && k->stride(-1) == 1 && k->size(-1) == dim && k->size(d - 3) == seq &&
+               (d == 3 || k->size(0) == batch) && k->size(d - 2) <= 65536);
+    }
+    if (pos != nullptr) {
+        c.need((pos->scalar_type() == Dt::Long || pos->scalar_type() == Dt::Int) && (pos->dim() == 1 || pos->dim() == 2) &&
+               pos->size(-1) == seq && (pos->dim() == 1 || pos->size(0) == 1 || pos->size(0) == batch));
+    }
+    OR_NONE(c);
+    c.need((q->size(d - 2) + (k != nullptr ? k->size(d - 2) : 0)) * dim <= (1 << 24));
+    OR_NONE(c);
+    return answer([&]() -> PyObject* {
+        variable_list out;
+        {
+            WithoutGil unlocked;
+            if (c10::GradMode::is_enabled() && (q->requires_grad() || wants_grad(k))) {
+                out = RotaryNode::apply(*q, maybe(k), maybe(pos), *freq, (double)amplitude, half);
+            } else {
+                int rc = 0;
+                out = RotaryNode::run(*q, value(maybe(k)), value(maybe(pos)), *freq, amplitude, half, false, rc);
+                must(rc, "rotary");
+            }
+        }
+        PyObject* r = PyTuple_New(2);
+        if (r == nullptr) return nullptr;
+        PyTuple_SET_ITEM(r, 0, wrap(std::move(out[0])));
+        if (k != nullptr) {
+            PyTuple_SET_ITEM(r, 1, wrap(std::move(out[1])));
+        } else {
+            Py_INCREF(Py_None);
+            PyTuple_SET_ITEM(r, 1, Py_None);
+        }
+        return r;
+    });
+    FAST_END
+}
+
+// ---- gated_linear(a, b, bias | None, scale_b, activation code, int8, rotate)
+struct GatedNode : torch::autograd::Function<GatedNode> {
+    static at::Tensor run(const at::Tensor& a, const at::Tensor& b, const at::Tensor& bias, const at::Tensor& scale, int act, bool int8, bool rotate,
+                          at::Tensor* pre) {
+        const int64_t k = b.size(1), f = b.size(0) / 2, m = a.numel() / k;
+        at::DimVector shape(lead(a).begin(), lead(a).end());
+        // the quantised rows and, behind them, their scales: scratch of this call
+        const int64_t q_bytes = (m * k + 255) / 256 * 256;
+        at::Tensor q = empty_like_dtype({q_bytes + 4 * m}, a, Dt::Byte);
+        float* qs = reinterpret_cast<float*>(static_cast<uint8_t*>(q.data_ptr()) + q_bytes);
+        shape.push_back(f);
+        at::Tensor out = empty_like_dtype(shape, a, Dt::BFloat16);
+        if (pre != nullptr) {
+            shape.back() = 2;
+            shape.push_back(f);
+            *pre = empty_like_dtype(shape, a, Dt::BFloat16);
+        }
+        void* st = stream_of(a);
+        must(q8k_gated_quant(a.const_data_ptr(), type_code(a.scalar_type()), k, q.data_ptr(), int8 ? Q8K_DT_I8 : Q8K_DT_E4M3, qs, m, (int)k, rotate,
+                             st), "gated_quant");
+        must(q8k_gated_mm(int8, q.const_data_ptr(), b.const_data_ptr(), fptr(defined(bias)), qs, scale.const_data_ptr<float>(), out.data_ptr(),
+                          pre != nullptr ? pre->data_ptr() : nullptr, act, (int)m, (int)f, (int)k, g_status[a.device().index()]->data_ptr<int>(),
+                          st), "gated_mm");
+        return out;
+    }
+    static Variable forward(AutogradContext* ctx, const Variable& a, const Variable& b, const Maybe& bias, const Variable& scale, int64_t act,
+                            bool int8, bool rotate) {
+        at::Tensor pre;
+        Variable out = run(a, b, value(bias), scale, (int)act, int8, rotate, &pre);
+        ctx->save_for_backward({pre, b, scale});
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["rotate"] = rotate;
+        ctx->saved_data["type"] = (int64_t)a.scalar_type();
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        variable_list result(7);
+        if (!grads[0].defined()) return result;
+        {
+            at::NoGradGuard no_grad;
+            const at::Tensor &pre = saved[0], &b = saved[1], &scale = saved[2];
+            const at::Tensor g = grads[0].to(Dt::BFloat16).contiguous();
+            const int64_t k = b.size(1), n = b.size(0), f = n / 2, m = g.numel() / f;
+            at::DimVector shape(lead(g).begin(), lead(g).end());
+            shape.push_back(k);
+            at::Tensor dx = empty_like_dtype(shape, g, Dt::BFloat16);
+            if (m > 0) {
+                void* st = stream_of(g);
+                int* word = g_status[g.device().index()]->data_ptr<int>();
+                auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+                const int64_t work_bytes = up((int64_t)q8k_gated_weight_operand_workspace_bytes((int)f, (int)k));
+                // one scratch: gradient rows and scales, weight operand and scales, its workspace, the product before the rotation
+                const bool rotate = ctx->saved_data["rotate"].toBool();
+                const int64_t at_gs = up(m * n), at_w = at_gs + up(4 * m), at_ws = at_w + up(k * n), at_work = at_ws + up(4 * k),
+                              at_y = at_work + work_bytes, end = at_y + (rotate ? 2 * m * k : 0);
+                at::Tensor scratch = empty_like_dtype({end}, g, Dt::Byte);
+                uint8_t* s = static_cast<uint8_t*>(scratch.data_ptr());
+                float *gs = reinterpret_cast<float*>(s + at_gs), *ws = reinterpret_cast<float*>(s + at_ws);
+                must_backward(q8k_gated_backward_quant(g.const_data_ptr(), pre.const_data_ptr(), s, gs, (int)ctx->saved_data["act"].toInt(), (int)m,
+                                                       (int)f, st), "gated_backward_quant");
+                must_backward(q8k_gated_weight_operand(b.const_data_ptr(), type_code(b.scalar_type()), scale.const_data_ptr<float>(), s + at_w, ws,
+                                                       (int)f, (int)k, s + at_work, (size_t)work_bytes, st), "gated_weight_operand");
+                void* y = rotate ? static_cast<void*>(s + at_y) : dx.data_ptr();
+                must_backward(q8k_fp8_mm(s, s + at_w, nullptr, gs, ws, y, Q8K_DT_BF16, 1, 1, (int)m, (int)k, (int)n, 0, word, st), "fp8_mm");
+                if (rotate)
+                    must_backward(q8k_fast_hadamard_transform(y, Q8K_DT_BF16, dx.data_ptr(), Q8K_DT_BF16, m, (int)k, k,
+                                                              (float)(1.0 / std::sqrt((double)k)), st), "fast_hadamard_transform");
+            }
+            result[0] = dx.to((Dt)ctx->saved_data["type"].toInt());
+        }
+        return once_only(std::move(result), grads);
+    }
+};
+
+PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    FAST_BEGIN
+    Call c(args, n, 7);
+    const at::Tensor* a = c.tensor(0);
+    const at::Tensor* b = c.tensor(1);
+    const at::Tensor* bias = c.optional(2, Dt::Float);
+    const at::Tensor* scale = c.tensor(3, Dt::Float);
+    const long act = c.integer(4);
+    const bool int8 = c.flag(5), rotate = c.flag(6);
+    OR_NONE(c);
+    c.need((act == Q8K_ACT_SILU || act == Q8K_ACT_GELU_TANH) && (a->scalar_type() == Dt::BFloat16 || (int8 && a->scalar_type() == Dt::Float8_e4m3fn)) && has_rows(a) &&
+           b->scalar_type() == (int8 ? Dt::Char : Dt::Float8_e4m3fn) && b->dim() == 2 && b->size(1) == a->size(-1));
+    OR_NONE(c);
+    const int64_t k = b->size(1), nn = b->size(0), m = a->numel() / k;
+    const bool training = c10::GradMode::is_enabled() && a->requires_grad();
+    c.need(nn > 0 && nn % 32 == 0 && nn <= 0x3fffffff && k % 16 == 0 && k <= 16384 && m <= 0x7fffff00 && scale->numel() == nn &&
+           (bias == nullptr || bias->numel() == nn) && !(training && nn > 2 * 16384));
+    c.status();
+    OR_NONE(c);
+    return answer([&]() -> PyObject* {
+        at::Tensor out;
+        {
+            WithoutGil unlocked;
+            out = training ? GatedNode::apply(*a, *b, maybe(bias), *scale, (int64_t)act, int8, rotate)
+                           : GatedNode::run(*a, *b, value(maybe(bias)), *scale, (int)act, int8, rotate, nullptr);
+        }
+        return wrap(std::move(out));
+    });
+    FAST_END
+}
+
 // ---------------------------------------------------------------- module
 PyObject* set_check(PyObject*, PyObject* f) {
     Py_INCREF(f);
@@ -686,7 +1051,7 @@ PyMethodDef methods[] = {
     FAST(tokenwise_quant), FAST(hadamard_quant), FAST(fast_hadamard_transform), FAST(norm_modulate_quant), FAST(transpose_quant),
     FAST(dequant_hadamard), FAST(rms_norm), FAST(rms_norm_backward), FAST(rope), FAST(rope_backward), FAST(mm),
     FAST(mm_gate_residual), FAST(linear), FAST(flash_attention), FAST(attention_prep_rows), FAST(qk_norm_rope_prep),
-    FAST(kv_prep), FAST(qk_norm_rope_prep_pair),
+    FAST(kv_prep), FAST(qk_norm_rope_prep_pair), FAST(layer_norm), FAST(rotary), FAST(gated_linear),
     {"set_check", set_check, METH_O, nullptr}, {"set_status_word", set_status_word, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

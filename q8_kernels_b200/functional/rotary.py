@@ -6,6 +6,7 @@ from typing import Optional, Tuple
 import torch
 from torch.autograd.function import once_differentiable
 
+from .. import _host
 from ..native import Q8KernelError
 from ..native import rotary as _rotary
 
@@ -88,6 +89,10 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional
     2i with 2i + 1 ("interleaved").  Differentiable in q and k."""
     if layout not in LAYOUTS:
         raise Q8KernelError(f"apply_rotary: layout {layout!r} is not one of {', '.join(LAYOUTS)}")
+    amplitude, half = float(amplitude), layout == "half"
+    fast = _host.rotary(q, k, positions, frequencies, amplitude, half)
+    if fast is not None:
+        return fast
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return Rotary.apply(q, k, positions, frequencies, float(amplitude), layout == "half")
-    return _rotary(q, k, positions, frequencies, float(amplitude), layout == "half", False)
+        return Rotary.apply(q, k, positions, frequencies, amplitude, half)
+    return _rotary(q, k, positions, frequencies, amplitude, half, False)
