@@ -2,14 +2,19 @@
 //   z = (x - mean) * rstd,  rstd = 1 / sqrt(mean((x - mean)^2) + eps),  y = z * w + b
 //   dx = rstd * (g w - mean(g w) - z mean(g w z)),  dw = sum_rows g z,  db = sum_rows g
 //
-// Both passes are bound by HBM: the forward reads x and writes y, the backward reads x and g and writes dx.  A row lives in the
-// registers of T threads between its reductions and its output, so each element is read once.  The variance is taken from
-// the differences to the mean (a second sum over the registers, not E[x^2] - mean^2, which loses all digits of a row whose mean is
-// large against its spread).  Sums, statistics and the gradients of w and b are fp32.
+// Both passes are bound by HBM: the forward reads x and writes y, the backward reads x and g and writes dx.  Groups of T threads walk
+// over rows, T so that a thread has 16 elements of a row, with w, b and the sums of dw and db in registers for all of them; G groups
+// make a CTA.  A row has to be complete before its first output, so what keeps HBM busy are the next rows: they come by cp.async into
+// a ring of S - 1 rows ahead in shared memory, where bytes on their way cost no registers.  What every thread does once a row (the
+// exchange of the sums, addresses) is some 70 instructions: with 8 elements a thread they held the forward pass at 0.6 of the copy
+// rate (24576 x 2048 bf16), whatever the number of rows on their way; arithmetic is on packed pairs for the same reason.
 //
-// Columns of a thread: VEC (dim a multiple of 8, all rows 16-byte aligned): items of 8 consecutive elements, 16- or 32-byte
-// accesses.  Otherwise single elements T apart: a warp then reads 32 consecutive elements, and the columns of a thread are the same
-// in every row, wherever the rows start, which the sums over rows need.
+// The variance is taken from the differences to the mean, not E[x^2] - mean^2, which loses all digits of a row whose mean is large
+// against its spread.  Sums, statistics and the gradients of w and b are fp32.
+//
+// Columns of a thread: VEC (dim a multiple of 8, all rows 16-byte aligned): items of 8 consecutive elements, which the thread copies
+// and reads back itself, with no barrier.  Otherwise single elements T apart, the same in every row wherever the rows start (which the
+// sums over rows need): the group copies the row in the 16-byte pieces of memory that it lies in, and reads elements after a barrier.
 
 #include <type_traits>
 #include "common.cuh"
@@ -23,230 +28,468 @@ constexpr int kLnMaxDim = 16384;
 template <int T, bool VEC> __device__ __forceinline__ int ln_col(int t, int i, int j) {
     return VEC ? (t + i * T) * kLnItem + j : t + (i * kLnItem + j) * T;
 }
+template <int T, bool VEC> __device__ __forceinline__ bool ln_has(int t, int i, int j, int dim) {
+    return ln_col<T, VEC>(t, i, VEC ? 0 : j) < dim;
+}
+
+// An item as four packed pairs; columns that do not exist read as 0.
+struct LnItem { float2 v[kLnItem / 2]; };
 
 template <typename E, int T, bool VEC>
-__device__ __forceinline__ void ln_load(const E* __restrict__ row, int dim, int t, int i, float (&v)[kLnItem]) {
+__device__ __forceinline__ LnItem ln_load(const E* row, int dim, int t, int i) {
+    LnItem r;
+    float v[kLnItem];
     if constexpr (VEC) {
-        if (ln_col<T, VEC>(t, i, 0) < dim) load_vec<E, kLnItem>(row + ln_col<T, VEC>(t, i, 0), v);
+        if (ln_has<T, VEC>(t, i, 0, dim)) load_vec<E, kLnItem>(row + ln_col<T, VEC>(t, i, 0), v);
         else {
 #pragma unroll
             for (int j = 0; j < kLnItem; ++j) v[j] = 0.f;
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < kLnItem; ++j) v[j] = ln_col<T, VEC>(t, i, j) < dim ? to_float<E>(row[ln_col<T, VEC>(t, i, j)]) : 0.f;
+        for (int j = 0; j < kLnItem; ++j) v[j] = ln_has<T, VEC>(t, i, j, dim) ? to_float<E>(row[ln_col<T, VEC>(t, i, j)]) : 0.f;
     }
+#pragma unroll
+    for (int k = 0; k < kLnItem / 2; ++k) r.v[k] = make_float2(v[2 * k], v[2 * k + 1]);
+    return r;
 }
 
 template <typename E, int T, bool VEC>
-__device__ __forceinline__ void ln_store(E* __restrict__ row, int dim, int t, int i, const float (&v)[kLnItem]) {
+__device__ __forceinline__ void ln_store(E* row, int dim, int t, int i, const LnItem& r) {
+    float v[kLnItem];
+#pragma unroll
+    for (int k = 0; k < kLnItem / 2; ++k) { v[2 * k] = r.v[k].x; v[2 * k + 1] = r.v[k].y; }
     if constexpr (VEC) {
-        if (ln_col<T, VEC>(t, i, 0) < dim) store_vec<E, kLnItem>(row + ln_col<T, VEC>(t, i, 0), v);
+        if (ln_has<T, VEC>(t, i, 0, dim)) store_vec<E, kLnItem>(row + ln_col<T, VEC>(t, i, 0), v);
     } else {
 #pragma unroll
         for (int j = 0; j < kLnItem; ++j)
-            if (ln_col<T, VEC>(t, i, j) < dim) row[ln_col<T, VEC>(t, i, j)] = from_float<E>(v[j]);
+            if (ln_has<T, VEC>(t, i, j, dim)) row[ln_col<T, VEC>(t, i, j)] = from_float<E>(v[j]);
     }
 }
+__device__ __forceinline__ float2 pair_of(float v) { return make_float2(v, v); }
 
-// Sums of N values over the T threads of a row, the same in each of them.  `red` is the row group's own shared memory
-// (N * T / 32 floats); a barrier stands before its reuse.
-template <int T, int N>
-__device__ __forceinline__ void ln_row_sum(float (&v)[N], float* red) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = warp_sum(v[k]);
-    if constexpr (T > 32) {
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        if (lane == 0) {
-#pragma unroll
-            for (int k = 0; k < N; ++k) red[warp * N + k] = v[k];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            v[k] = red[k];
-#pragma unroll
-            for (int w = 1; w < T / 32; ++w) v[k] += red[w * N + k];
-        }
-        __syncthreads();
-    }
+// Barrier of the T threads of one row group: its own named barrier where a CTA has several.
+template <int T, int G> __device__ __forceinline__ void ln_group_sync(int group) {
+    if constexpr (T <= 32) __syncwarp();
+    else if constexpr (G == 1) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(T) : "memory");
 }
 
-// G rows per CTA, T threads each (G > 1 only with T = 32, where a row needs no barrier).
-template <typename Tx, typename Ty, int ITEMS, int T, int G, bool VEC>
-__global__ void __launch_bounds__(T * G)
-layer_norm_kernel(const Tx* __restrict__ x, int64_t x_stride, const float* __restrict__ w, const float* __restrict__ b,
-                  Ty* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows, int dim, float eps) {
-    static_assert(G == 1 || T == 32, "row groups of more than a warp would need barriers of their own");
-    __shared__ float red[T / 32];
-    const int t = G > 1 ? threadIdx.x & 31 : threadIdx.x;
-    const int64_t row = (int64_t)blockIdx.x * G + (G > 1 ? threadIdx.x >> 5 : 0);
-    pdl_wait();
-    pdl_release();
-    if (G > 1 && row >= rows) return;
-    const Tx* xr = x + row * x_stride;
-    float v[ITEMS][kLnItem];
-    float s[1] = {0.f};
+// Sum over the first WARPS (at most 32) lanes, in every lane of that power-of-two block.
+template <int WARPS> __device__ __forceinline__ float ln_lane_sum(float v) {
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        ln_load<Tx, T, VEC>(xr, dim, t, i, v[i]);
+    for (int o = WARPS / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+__device__ __forceinline__ void ln_copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void ln_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void ln_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Start the copy of a row into its slot of the ring.  [lo, hi) are the addresses of the tensor's first and behind its last element: a
+// piece that reaches beyond them is copied by the element.
+template <typename E, int ITEMS, int T, bool VEC>
+__device__ __forceinline__ void ln_fetch(const E* row, int dim, int t, char* slot, const char* lo, const char* hi) {
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(slot);
+    if constexpr (VEC) {
 #pragma unroll
-        for (int j = 0; j < kLnItem; ++j) s[0] += v[i][j];
-    }
-    ln_row_sum<T>(s, red);
-    const float inv = 1.0f / (float)dim;
-    const float mean = s[0] * inv;
-    s[0] = 0.f;
+        for (int i = 0; i < ITEMS; ++i) {
+            const int c = ln_col<T, VEC>(t, i, 0);
+            if (c < dim) {
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-#pragma unroll
-        for (int j = 0; j < kLnItem; ++j) {
-            if (ln_col<T, VEC>(t, i, VEC ? 0 : j) < dim) {
-                const float d = v[i][j] - mean;
-                s[0] = fmaf(d, d, s[0]);
+                for (int k = 0; k < (int)(kLnItem * sizeof(E) / 16); ++k)
+                    ln_copy16(dst + c * (int)sizeof(E) + 16 * k, reinterpret_cast<const char*>(row + c) + 16 * k);
+            }
+        }
+    } else {
+        const char* first = reinterpret_cast<const char*>(row);
+        const char* from = first - (reinterpret_cast<uintptr_t>(first) & 15);
+        const int bytes = (int)(first - from) + dim * (int)sizeof(E);
+        for (int k = t * 16; k < bytes; k += T * 16) {
+            const char* p = from + k;
+            if (p >= lo && p + 16 <= hi) {
+                ln_copy16(dst + k, p);
+            } else {
+                for (int e = 0; e < 16; e += (int)sizeof(E))
+                    if (p + e >= first && p + e < first + (int64_t)dim * (int)sizeof(E))
+                        *reinterpret_cast<E*>(slot + k + e) = *reinterpret_cast<const E*>(p + e);
             }
         }
     }
-    ln_row_sum<T>(s, red);
-    const float rstd = 1.0f / sqrtf(fmaf(s[0], inv, eps));
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        float wv[kLnItem], bv[kLnItem], o[kLnItem];
-        if (w != nullptr) ln_load<float, T, VEC>(w, dim, t, i, wv);
-        if (b != nullptr) ln_load<float, T, VEC>(b, dim, t, i, bv);
-#pragma unroll
-        for (int j = 0; j < kLnItem; ++j) {
-            o[j] = (v[i][j] - mean) * rstd;
-            if (w != nullptr) o[j] = b != nullptr ? fmaf(o[j], wv[j], bv[j]) : o[j] * wv[j];
-            else if (b != nullptr) o[j] += bv[j];
-        }
-        ln_store<Ty, T, VEC>(y + row * (int64_t)dim, dim, t, i, o);
-    }
-    if (t == 0) {
-        if (mean_out != nullptr) mean_out[row] = mean;
-        if (rstd_out != nullptr) rstd_out[row] = rstd;
-    }
+}
+// Where the row's first element lies in its slot.
+template <typename E, bool VEC> __device__ __forceinline__ const E* ln_slot_row(const char* slot, const E* row) {
+    return reinterpret_cast<const E*>(slot + (VEC ? 0 : reinterpret_cast<uintptr_t>(row) & 15));
 }
 
-// A CTA walks over rows and keeps its columns' sums of g z and g in registers; they go to part[group][2][dim] at the end and
-// layer_norm_wgrad_kernel adds the groups up in a fixed order: no atomics, the same bits in every run.
-template <typename Tx, typename Tg, int ITEMS, int T, int G, bool VEC, bool WGRAD>
-__global__ void __launch_bounds__(T * G)
+// Threads of a CTA, CTAs an SM holds by registers, rows of the ring: as many as the SM's 227 KB leave for all of them, up to four.
+template <int I, int T, int G> struct LnLayout { static constexpr int items = I, threads = T, rows = G, cta = T * G; };
+// keep: what a thread needs twice stays in registers (w, b and the row's values); else it is read again, from L1 or from the ring, so
+// that two rows of more than 8192 columns fit an SM at a time (forward), or one with the sums of dw and db (backward).  The ring has
+// two rows then, which leaves L1 the room for w and b: with all that fit they came from L2, twice the bytes of the row itself.
+template <typename L> struct LnForward {
+    static constexpr bool keep = L::items <= 2;
+    static constexpr int ctas = L::cta <= 256 ? 3 : keep ? 1 : 2;
+};
+template <typename L> struct LnBackward {
+    static constexpr bool keep = L::items <= 2;
+    static constexpr int ctas = L::cta <= 256 ? 2 : 1;
+};
+template <typename L, int CTAS, int BYTES> struct LnRing {
+    static constexpr int row = L::rows * (L::threads * L::items * kLnItem * BYTES + 64);
+    static constexpr int fit = 224 * 1024 / CTAS / row;
+    static constexpr int most = L::items <= 2 ? 4 : 2;
+    static constexpr int slots = fit > most ? most : fit < 1 ? 1 : fit;
+};
+
+// Mean and variance in one exchange between warps: each warp takes the mean of its own elements and the squares of their
+// differences to that (shuffles), and with n_w elements, sum s_w and squares q_w the row has
+//   mean = sum s_w / n,  n var = sum (q_w + n_w (s_w / n_w - mean)^2),
+// all terms positive.
+template <typename Tx, typename Ty, typename L, bool VEC>
+__global__ void __launch_bounds__(L::cta, LnForward<L>::ctas)
+layer_norm_kernel(const Tx* __restrict__ x, int64_t x_stride, const float* __restrict__ w, const float* __restrict__ b,
+                  Ty* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows, int dim, float eps,
+                  int slot_bytes) {
+    constexpr int ITEMS = L::items, T = L::threads, G = L::rows, WARPS = T / 32;
+    constexpr int S = LnRing<L, LnForward<L>::ctas, sizeof(Tx)>::slots;
+    constexpr bool KEEP = LnForward<L>::keep;
+    extern __shared__ __align__(16) char ln_smem[];
+    __shared__ float2 red[2][G][WARPS];
+    const int group = threadIdx.x / T, t = threadIdx.x % T;
+    char* ring = ln_smem + group * S * slot_bytes;
+    const int64_t step = (int64_t)gridDim.x * G;
+    const int64_t row0 = (int64_t)blockIdx.x * G + group;
+    const char* lo = reinterpret_cast<const char*>(x);
+    const char* hi = reinterpret_cast<const char*>(x + (rows - 1) * x_stride + dim);
+    auto fetch = [&](int64_t row, int slot) {
+        if (row < rows) ln_fetch<Tx, ITEMS, T, VEC>(x + row * x_stride, dim, t, ring + slot * slot_bytes, lo, hi);
+        ln_commit();
+    };
+    auto weight = [&](int i) {
+        LnItem r;
+#pragma unroll
+        for (int k = 0; k < kLnItem / 2; ++k) r.v[k] = pair_of(1.f);
+        return w != nullptr ? ln_load<float, T, VEC>(w, dim, t, i) : r;
+    };
+    auto bias = [&](int i) {
+        LnItem r;
+#pragma unroll
+        for (int k = 0; k < kLnItem / 2; ++k) r.v[k] = pair_of(0.f);
+        return b != nullptr ? ln_load<float, T, VEC>(b, dim, t, i) : r;
+    };
+    pdl_wait();
+    pdl_release();
+#pragma unroll
+    for (int k = 0; k < S - 1; ++k) fetch(row0 + k * step, k);
+    LnItem wv[KEEP ? ITEMS : 1], bv[KEEP ? ITEMS : 1];
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) { wv[i] = weight(i); bv[i] = bias(i); }
+    }
+    // elements of a warp: those of its threads (VEC: runs of 8 each, 256 from (warp * 32 + i * T) * 8 on; else 32 from warp * 32 on, T apart)
+    auto count = [&](int wp) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            if constexpr (VEC) {
+                n += max(0, min(32 * kLnItem, dim - (wp * 32 + i * T) * kLnItem));
+            } else {
+#pragma unroll
+                for (int j = 0; j < kLnItem; ++j) n += max(0, min(32, dim - wp * 32 - (i * kLnItem + j) * T));
+            }
+        }
+        return (float)n;
+    };
+    const float inv = 1.0f / (float)dim;
+    const float own_inv = 1.0f / fmaxf(1.f, count(t >> 5));
+    const float lane_n = count((t & 31) % WARPS), lane_inv = 1.0f / fmaxf(1.f, lane_n);
+    int slot = 0, turn = 0;
+    for (int64_t row = row0; row < rows; row += step, turn ^= 1) {
+        if constexpr (S == 1) {
+            if (!VEC) ln_group_sync<T, G>(group);              // the row before has been read
+            fetch(row, 0);
+            ln_wait<0>();
+        } else {
+            ln_wait<S - 2>();
+        }
+        if (!VEC) ln_group_sync<T, G>(group);                  // everyone's pieces have landed; the slot before has been read
+        const Tx* xr = ln_slot_row<Tx, VEC>(ring + slot * slot_bytes, x + row * x_stride);
+        LnItem v[KEEP ? ITEMS : 1];
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) v[i] = ln_load<Tx, T, VEC>(xr, dim, t, i);
+        }
+        auto value = [&](int i) -> const LnItem& {             // (a slot is not refilled before the next row)
+            if constexpr (!KEEP) v[0] = ln_load<Tx, T, VEC>(xr, dim, t, i);
+            return v[KEEP ? i : 0];
+        };
+        if constexpr (S > 1) fetch(row + (S - 1) * step, slot == 0 ? S - 1 : slot - 1);
+        if (++slot == S) slot = 0;
+        float2 s2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const LnItem& x8 = value(i);
+#pragma unroll
+            for (int k = 0; k < kLnItem / 2; ++k) s2 = fadd2(s2, x8.v[k]);
+        }
+        const float s = warp_sum(s2.x + s2.y);
+        float mean = s * (WARPS == 1 ? inv : own_inv);
+        float2 q2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            if (!VEC || ln_has<T, VEC>(t, i, 0, dim)) {
+                const LnItem& x8 = value(i);
+#pragma unroll
+                for (int k = 0; k < kLnItem / 2; ++k) {
+                    float2 d = fsub2(x8.v[k], pair_of(mean));
+                    if constexpr (!VEC) {
+                        if (!ln_has<T, VEC>(t, i, 2 * k, dim)) d.x = 0.f;
+                        if (!ln_has<T, VEC>(t, i, 2 * k + 1, dim)) d.y = 0.f;
+                    }
+                    q2 = ffma2(d, d, q2);
+                }
+            }
+        }
+        float q = warp_sum(q2.x + q2.y);
+        if constexpr (WARPS > 1) {
+            if ((t & 31) == 0) red[turn][group][t >> 5] = make_float2(s, q);
+            ln_group_sync<T, G>(group);                        // (two buffers: the one before is not written until the next barrier)
+            const float2 p = red[turn][group][(t & 31) % WARPS];          // lane k, k + WARPS, ... take warp k's part
+            mean = ln_lane_sum<WARPS>(p.x) * inv;
+            const float d = fmaf(p.x, lane_inv, -mean);        // (a warp without elements has lane_n = 0)
+            q = ln_lane_sum<WARPS>(fmaf(lane_n * d, d, p.y));
+        }
+        const float rstd = rsqrtf(fmaf(q, inv, eps));
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            if (!KEEP) { wv[0] = weight(i); bv[0] = bias(i); }
+            const LnItem& x8 = value(i);
+            LnItem o;
+#pragma unroll
+            for (int k = 0; k < kLnItem / 2; ++k)
+                o.v[k] = ffma2(fmul2(fsub2(x8.v[k], pair_of(mean)), pair_of(rstd)), wv[KEEP ? i : 0].v[k], bv[KEEP ? i : 0].v[k]);
+            ln_store<Ty, T, VEC>(y + row * (int64_t)dim, dim, t, i, o);
+        }
+        if (t == 0) {
+            if (mean_out != nullptr) mean_out[row] = mean;
+            if (rstd_out != nullptr) rstd_out[row] = rstd;
+        }
+    }
+    ln_wait<0>();                                              // (the copies behind the last row were empty)
+}
+
+// The groups of a CTA add their sums of g z and g in shared memory at the end, and part[CTA][2][dim] is summed over the CTAs by
+// layer_norm_wgrad_kernel: fixed orders, no atomics, the same bits in every run.
+template <typename Tx, typename Tg, typename L, bool VEC, bool WGRAD>
+__global__ void __launch_bounds__(L::cta, LnBackward<L>::ctas)
 layer_norm_backward_kernel(const Tx* __restrict__ x, int64_t x_stride, const Tg* __restrict__ g, const float* __restrict__ mean,
                            const float* __restrict__ rstd, const float* __restrict__ w, Tx* __restrict__ dx, float* __restrict__ part,
-                           int64_t rows, int dim) {
-    static_assert(G == 1 || T == 32, "row groups of more than a warp would need barriers of their own");
-    __shared__ float red[2 * (T / 32)];
-    const int t = G > 1 ? threadIdx.x & 31 : threadIdx.x;
-    const int64_t group = (int64_t)blockIdx.x * G + (G > 1 ? threadIdx.x >> 5 : 0);
+                           int64_t rows, int dim, int x_slot_bytes, int g_slot_bytes) {
+    constexpr int ITEMS = L::items, T = L::threads, G = L::rows, WARPS = T / 32;
+    constexpr int S = LnRing<L, LnBackward<L>::ctas, sizeof(Tx) + sizeof(Tg)>::slots;
+    constexpr bool KEEP = LnBackward<L>::keep;
+    extern __shared__ __align__(16) char ln_smem[];
+    __shared__ float2 red[2][G][WARPS];
+    const int group = threadIdx.x / T, t = threadIdx.x % T;
+    char* x_ring = ln_smem + group * S * (x_slot_bytes + g_slot_bytes);
+    char* g_ring = x_ring + S * x_slot_bytes;
+    const int64_t step = (int64_t)gridDim.x * G;
+    const int64_t row0 = (int64_t)blockIdx.x * G + group;
+    const char* x_lo = reinterpret_cast<const char*>(x);
+    const char* x_hi = reinterpret_cast<const char*>(x + (rows - 1) * x_stride + dim);
+    const char* g_lo = reinterpret_cast<const char*>(g);
+    const char* g_hi = reinterpret_cast<const char*>(g + rows * dim);
+    auto fetch = [&](int64_t row, int slot) {
+        if (row < rows) {
+            ln_fetch<Tx, ITEMS, T, VEC>(x + row * x_stride, dim, t, x_ring + slot * x_slot_bytes, x_lo, x_hi);
+            ln_fetch<Tg, ITEMS, T, VEC>(g + row * (int64_t)dim, dim, t, g_ring + slot * g_slot_bytes, g_lo, g_hi);
+        }
+        ln_commit();
+    };
+    auto weight = [&](int i) {
+        LnItem r;
+#pragma unroll
+        for (int k = 0; k < kLnItem / 2; ++k) r.v[k] = pair_of(1.f);
+        return w != nullptr ? ln_load<float, T, VEC>(w, dim, t, i) : r;
+    };
     pdl_wait();
     pdl_release();
-    float dw[WGRAD ? ITEMS : 1][kLnItem], db[WGRAD ? ITEMS : 1][kLnItem];
-    if constexpr (WGRAD) {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
+    for (int k = 0; k < S - 1; ++k) fetch(row0 + k * step, k);
+    float m_next = 0.f, r_next = 0.f;
+    if (row0 < rows) { m_next = mean[row0]; r_next = rstd[row0]; }
+    LnItem wv[KEEP ? ITEMS : 1];
+    LnItem dw[WGRAD ? ITEMS : 1], db[WGRAD ? ITEMS : 1];
 #pragma unroll
-            for (int j = 0; j < kLnItem; ++j) dw[i][j] = db[i][j] = 0.f;
+    for (int i = 0; i < ITEMS; ++i) {
+        if constexpr (WGRAD) {
+#pragma unroll
+            for (int k = 0; k < kLnItem / 2; ++k) dw[i].v[k] = db[i].v[k] = make_float2(0.f, 0.f);
+        }
+        if constexpr (KEEP) wv[i] = weight(i);
     }
     const float inv = 1.0f / (float)dim;
-    for (int64_t row = group; row < rows; row += (int64_t)gridDim.x * G) {
-        float z[ITEMS][kLnItem], gv[ITEMS][kLnItem];
-        const float m = mean[row], r = rstd[row];
-        float s[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            ln_load<Tx, T, VEC>(x + row * x_stride, dim, t, i, z[i]);
-            ln_load<Tg, T, VEC>(g + row * (int64_t)dim, dim, t, i, gv[i]);
+    int slot = 0, turn = 0;
+    for (int64_t row = row0; row < rows; row += step, turn ^= 1) {
+        if constexpr (S == 1) {
+            if (!VEC) ln_group_sync<T, G>(group);              // the row before has been read
+            fetch(row, 0);
+            ln_wait<0>();
+        } else {
+            ln_wait<S - 2>();
         }
+        if (!VEC) ln_group_sync<T, G>(group);                  // everyone's pieces have landed; the slot before has been read
+        const Tx* xr = ln_slot_row<Tx, VEC>(x_ring + slot * x_slot_bytes, x + row * x_stride);
+        const Tg* gr = ln_slot_row<Tg, VEC>(g_ring + slot * g_slot_bytes, g + row * (int64_t)dim);
+        const float m = m_next, r = r_next;
+        if (row + step < rows) { m_next = mean[row + step]; r_next = rstd[row + step]; }
+        // z = x r - m r, one rounding more than (x - m) r would have only where x and m cancel: the difference is taken first
+        auto normalised = [&](int i) {
+            LnItem z = ln_load<Tx, T, VEC>(xr, dim, t, i);
+#pragma unroll
+            for (int k = 0; k < kLnItem / 2; ++k) z.v[k] = fmul2(fsub2(z.v[k], pair_of(m)), pair_of(r));
+            return z;
+        };
+        LnItem z[KEEP ? ITEMS : 1], gw[KEEP ? ITEMS : 1];
+        float2 s0 = make_float2(0.f, 0.f), s1 = s0;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            float wv[kLnItem];
-            if (w != nullptr) ln_load<float, T, VEC>(w, dim, t, i, wv);
+            const int at = KEEP ? i : 0;
+            z[at] = normalised(i);
+            gw[at] = ln_load<Tg, T, VEC>(gr, dim, t, i);
+            if (!KEEP) wv[0] = weight(i);
 #pragma unroll
-            for (int j = 0; j < kLnItem; ++j) {                // columns that do not exist have g = 0: they add nothing
-                z[i][j] = (z[i][j] - m) * r;
+            for (int k = 0; k < kLnItem / 2; ++k) {            // columns that do not exist have g = 0: they add nothing
                 if constexpr (WGRAD) {
-                    dw[i][j] = fmaf(gv[i][j], z[i][j], dw[i][j]);
-                    db[i][j] += gv[i][j];
+                    dw[i].v[k] = ffma2(gw[at].v[k], z[at].v[k], dw[i].v[k]);
+                    db[i].v[k] = fadd2(db[i].v[k], gw[at].v[k]);
                 }
-                if (w != nullptr) gv[i][j] *= wv[j];
-                s[0] += gv[i][j];
-                s[1] = fmaf(gv[i][j], z[i][j], s[1]);
+                gw[at].v[k] = fmul2(gw[at].v[k], wv[at].v[k]);
+                s0 = fadd2(s0, gw[at].v[k]);
+                s1 = ffma2(gw[at].v[k], z[at].v[k], s1);
             }
         }
+        if constexpr (S > 1) fetch(row + (S - 1) * step, slot == 0 ? S - 1 : slot - 1);
+        if (++slot == S) slot = 0;
         if (dx == nullptr) continue;                           // only the sums over rows are wanted
-        ln_row_sum<T>(s, red);
-        const float a = s[0] * inv, c = s[1] * inv;
+        float a = warp_sum(s0.x + s0.y), c = warp_sum(s1.x + s1.y);
+        if constexpr (WARPS > 1) {
+            if ((t & 31) == 0) red[turn][group][t >> 5] = make_float2(a, c);
+            ln_group_sync<T, G>(group);                        // (two buffers: the one before is not written until the next barrier)
+            const float2 p = red[turn][group][(t & 31) % WARPS];
+            a = ln_lane_sum<WARPS>(p.x);
+            c = ln_lane_sum<WARPS>(p.y);
+        }
+        a *= inv;
+        c *= inv;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            float o[kLnItem];
+            const int at = KEEP ? i : 0;
+            if (!KEEP) {                                       // the slot is not refilled before the next row
+                z[0] = normalised(i);
+                gw[0] = ln_load<Tg, T, VEC>(gr, dim, t, i);
+                wv[0] = weight(i);
 #pragma unroll
-            for (int j = 0; j < kLnItem; ++j) o[j] = r * (gv[i][j] - fmaf(z[i][j], c, a));
+                for (int k = 0; k < kLnItem / 2; ++k) gw[0].v[k] = fmul2(gw[0].v[k], wv[0].v[k]);
+            }
+            LnItem o;
+#pragma unroll
+            for (int k = 0; k < kLnItem / 2; ++k)
+                o.v[k] = fmul2(fsub2(gw[at].v[k], ffma2(z[at].v[k], pair_of(c), pair_of(a))), pair_of(r));
             ln_store<Tx, T, VEC>(dx + row * (int64_t)dim, dim, t, i, o);
         }
     }
+    ln_wait<0>();                                              // (the copies behind the last row were empty)
     if constexpr (WGRAD) {
-        float* p = part + group * 2 * (int64_t)dim;
+        float* p = part + (int64_t)blockIdx.x * 2 * dim;
+        if constexpr (G == 1) {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            ln_store<float, T, VEC>(p, dim, t, i, dw[i]);
-            ln_store<float, T, VEC>(p + dim, dim, t, i, db[i]);
+            for (int i = 0; i < ITEMS; ++i) {
+                ln_store<float, T, VEC>(p, dim, t, i, dw[i]);
+                ln_store<float, T, VEC>(p + dim, dim, t, i, db[i]);
+            }
+        } else {
+            constexpr int W = T * kLnItem * ITEMS;             // columns of the layout, at least dim
+            float* sums = reinterpret_cast<float*>(ln_smem);   // in the ring's place
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                ln_store<float, T, VEC>(sums + group * 2 * W, W, t, i, dw[i]);
+                ln_store<float, T, VEC>(sums + group * 2 * W + W, W, t, i, db[i]);
+            }
+            __syncthreads();
+            for (int k = threadIdx.x; k < 2 * W; k += T * G) {
+                const int which = k / W, c = k - which * W;
+                if (c < dim) {
+                    float s = sums[k];
+#pragma unroll
+                    for (int o = 1; o < G; ++o) s += sums[o * 2 * W + k];
+                    p[which * dim + c] = s;
+                }
+            }
         }
     }
 }
 
-// dw[c] = sum over groups of part[group][0][c], db[c] likewise of part[group][1][c]: a CTA takes 32 of the 2 * dim columns, warp k the
-// groups k, k + 8, ..., and the eight sums are added in shared memory.
-constexpr int kLnSumWarps = 8;
+// dw[c] = sum over CTAs of part[CTA][0][c], db[c] likewise of part[CTA][1][c]: a CTA takes 32 of the 2 * dim columns, warp k the parts
+// k, k + 32, ..., and the 32 sums are added by shuffles.
+constexpr int kLnSumWarps = 32;
 __global__ void __launch_bounds__(32 * kLnSumWarps)
-layer_norm_wgrad_kernel(const float* __restrict__ part, int groups, float* __restrict__ dw, float* __restrict__ db, int dim) {
-    __shared__ float sums[kLnSumWarps][32];
+layer_norm_wgrad_kernel(const float* __restrict__ part, int parts, float* __restrict__ dw, float* __restrict__ db, int dim) {
+    __shared__ float sums[kLnSumWarps][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;
-    const bool in = c < 2 * (int64_t)dim;
     pdl_wait();
     pdl_release();
     float s = 0.f;
-    if (in) {
-#pragma unroll 8
-        for (int k = warp; k < groups; k += kLnSumWarps) s += part[k * 2 * (int64_t)dim + c];
+    if (c < 2 * (int64_t)dim) {
+#pragma unroll 10
+        for (int k = warp; k < parts; k += kLnSumWarps) s += part[k * 2 * (int64_t)dim + c];
     }
     sums[warp][lane] = s;
     __syncthreads();
-    if (warp == 0 && in) {
-        s = sums[0][lane];
-#pragma unroll
-        for (int k = 1; k < kLnSumWarps; ++k) s += sums[k][lane];
-        float* out = c < dim ? dw : db;
-        if (out != nullptr) out[c < dim ? c : c - dim] = s;
+    s = warp_sum(sums[lane][warp]);                            // column `warp` of the 32
+    const int64_t cw = (int64_t)blockIdx.x * 32 + warp;
+    if (lane == 0 && cw < 2 * (int64_t)dim) {
+        float* out = cw < dim ? dw : db;
+        if (out != nullptr) out[cw < dim ? cw : cw - dim] = s;
     }
 }
 
 // ------------------------------------------------------------------ host side
-// Calls f(items, threads per row, rows per CTA) with the row's layout as integral constants.
 template <typename F> static int ln_layout(int dim, F&& f) {
     const int items = (dim + kLnItem - 1) / kLnItem;
-#define Q8K_LN(I, T, G) return f(std::integral_constant<int, I>(), std::integral_constant<int, T>(), std::integral_constant<int, G>())
-    if (items <= 32) Q8K_LN(1, 32, 4);
-    if (items <= 128) Q8K_LN(1, 128, 1);
-    if (items <= 256) Q8K_LN(1, 256, 1);
-    if (items <= 512) Q8K_LN(2, 256, 1);
-    if (items <= 1024) Q8K_LN(4, 256, 1);
-    Q8K_LN(4, 512, 1);
-#undef Q8K_LN
+    if (items <= 32) return f(LnLayout<1, 32, 8>());
+    if (items <= 64) return f(LnLayout<2, 32, 8>());
+    if (items <= 128) return f(LnLayout<2, 64, 4>());
+    if (items <= 256) return f(LnLayout<2, 128, 2>());
+    if (items <= 512) return f(LnLayout<2, 256, 1>());
+    if (items <= 1024) return f(LnLayout<2, 512, 1>());
+    return f(LnLayout<4, 512, 1>());
 }
 
-// Row groups of a backward pass that sums over rows: as many CTAs as the device holds, or one row each.
-static int ln_groups(int64_t rows, int dim) {
-    int groups = 0;
-    ln_layout(dim, [&](auto, auto t, auto g) {
-        const int64_t ctas = (int64_t)gemm_num_sms() * (1024 / (t.value * g.value));
-        const int64_t need = (rows + g.value - 1) / g.value;
-        groups = (int)(need < ctas ? need : ctas) * g.value;
-        return 0;
+// CTAs of a pass: as many as the device holds, or what the rows need.  With sums over rows a CTA leaves 8 dim bytes of them behind,
+// as much as two to four rows are, so it should have four rows a group, unless that leaves SMs idle (1001 x 1537 fp16, backward:
+// 10.5 us with a CTA for every row group).
+template <bool BACKWARD> static int ln_ctas(int64_t rows, int dim, bool sums) {
+    return ln_layout(dim, [&](auto l) {
+        using L = decltype(l);
+        const int64_t most = (int64_t)gemm_num_sms() * (BACKWARD ? LnBackward<L>::ctas : LnForward<L>::ctas);
+        int64_t need = (rows + L::rows - 1) / L::rows;
+        if (sums && need > gemm_num_sms()) {
+            const int64_t fewer = (need + 3) / 4;
+            need = fewer > gemm_num_sms() ? fewer : gemm_num_sms();
+        }
+        return (int)(need < most ? need : most);
     });
-    return groups;
 }
+
+// Bytes of a row in the ring.
+static int ln_slot(int dim, int size, bool vec) { return (dim * size + 15) / 16 * 16 + (vec ? 0 : 16); }
 
 static int check_ln(const char* op, int64_t rows, int dim, int64_t x_stride) {
     Q8K_REQUIRE(rows >= 0 && rows <= 0x7fffffffLL, Q8K_ERR_INVALID_ARG, "%s: rows %lld out of range", op, (long long)rows);
@@ -261,32 +504,61 @@ static bool ln_aligned(const void* p, int dtype) {
     return size > 0 && reinterpret_cast<uintptr_t>(p) % size == 0;
 }
 
+template <typename Tx, typename Ty, typename L, bool VEC>
+static int launch_ln_as(const void* x, int64_t x_stride, const float* w, const float* b, void* y, float* mean, float* rstd, int64_t rows,
+                        int dim, float eps, cudaStream_t st) {
+    auto kern = layer_norm_kernel<Tx, Ty, L, VEC>;
+    using Ring = LnRing<L, LnForward<L>::ctas, sizeof(Tx)>;
+    constexpr int S = Ring::slots, most = S * Ring::row;
+    const int slot = ln_slot(dim, sizeof(Tx), VEC);
+    if (most > 40 * 1024) {
+        static std::atomic<uint64_t> smem_done{0};
+        if (int rc = allow_dynamic_smem((const void*)kern, most, smem_done)) return rc;
+    }
+    Q8K_CUDA_OK(launch_dependent(kern, (unsigned)ln_ctas<false>(rows, dim, false), L::cta, L::rows * S * slot, st, 1, (const Tx*)x, x_stride,
+                                 w, b, (Ty*)y, mean, rstd, rows, dim, eps, slot));
+    return Q8K_OK;
+}
+
 template <typename Tx, typename Ty>
 static int launch_ln(const void* x, int64_t x_stride, const float* w, const float* b, void* y, float* mean, float* rstd, int64_t rows,
                      int dim, float eps, bool vec, cudaStream_t st) {
-    return ln_layout(dim, [&](auto i, auto t, auto g) {
-        constexpr int I = decltype(i)::value, T = decltype(t)::value, G = decltype(g)::value;
-        auto kern = vec ? layer_norm_kernel<Tx, Ty, I, T, G, true> : layer_norm_kernel<Tx, Ty, I, T, G, false>;
-        Q8K_CUDA_OK(launch_dependent(kern, (unsigned)((rows + G - 1) / G), T * G, 0, st, 1, (const Tx*)x, x_stride, w, b, (Ty*)y, mean,
-                                     rstd, rows, dim, eps));
-        return Q8K_OK;
+    return ln_layout(dim, [&](auto l) {
+        using L = decltype(l);
+        return vec ? launch_ln_as<Tx, Ty, L, true>(x, x_stride, w, b, y, mean, rstd, rows, dim, eps, st)
+                   : launch_ln_as<Tx, Ty, L, false>(x, x_stride, w, b, y, mean, rstd, rows, dim, eps, st);
     });
+}
+
+template <typename Tx, typename Tg, typename L, bool VEC, bool WGRAD>
+static int launch_ln_backward_as(const void* x, int64_t x_stride, const void* g, const float* mean, const float* rstd, const float* w, void* dx,
+                                 float* part, int64_t rows, int dim, cudaStream_t st) {
+    auto kern = layer_norm_backward_kernel<Tx, Tg, L, VEC, WGRAD>;
+    using Ring = LnRing<L, LnBackward<L>::ctas, sizeof(Tx) + sizeof(Tg)>;
+    constexpr int S = Ring::slots;
+    constexpr int sums = WGRAD && L::rows > 1 ? L::cta * 2 * L::items * kLnItem * (int)sizeof(float) : 0;
+    constexpr int most = S * Ring::row > sums ? S * Ring::row : sums;
+    static_assert(most <= 226 * 1024, "layer norm ring");
+    const int x_slot = ln_slot(dim, sizeof(Tx), VEC), g_slot = ln_slot(dim, sizeof(Tg), VEC);
+    if (most > 40 * 1024) {
+        static std::atomic<uint64_t> smem_done{0};
+        if (int rc = allow_dynamic_smem((const void*)kern, most, smem_done)) return rc;
+    }
+    const int bytes = L::rows * S * (x_slot + g_slot);
+    Q8K_CUDA_OK(launch_dependent(kern, (unsigned)ln_ctas<true>(rows, dim, WGRAD), L::cta, bytes > sums ? bytes : sums, st, 1, (const Tx*)x,
+                                 x_stride, (const Tg*)g, mean, rstd, w, (Tx*)dx, part, rows, dim, x_slot, g_slot));
+    return Q8K_OK;
 }
 
 template <typename Tx, typename Tg>
 static int launch_ln_backward(const void* x, int64_t x_stride, const void* g, const float* mean, const float* rstd, const float* w,
                               void* dx, float* part, int64_t rows, int dim, bool vec, cudaStream_t st) {
-    return ln_layout(dim, [&](auto i, auto t, auto gr) {
-        constexpr int I = decltype(i)::value, T = decltype(t)::value, G = decltype(gr)::value;
-        // without sums over rows nothing is gained by a CTA that takes more than its G rows
-        const unsigned grid = part != nullptr ? (unsigned)(ln_groups(rows, dim) / G) : (unsigned)((rows + G - 1) / G);
-        auto kern = part != nullptr ? (vec ? layer_norm_backward_kernel<Tx, Tg, I, T, G, true, true>
-                                           : layer_norm_backward_kernel<Tx, Tg, I, T, G, false, true>)
-                                    : (vec ? layer_norm_backward_kernel<Tx, Tg, I, T, G, true, false>
-                                           : layer_norm_backward_kernel<Tx, Tg, I, T, G, false, false>);
-        Q8K_CUDA_OK(launch_dependent(kern, grid, T * G, 0, st, 1, (const Tx*)x, x_stride, (const Tg*)g, mean, rstd, w, (Tx*)dx, part,
-                                     rows, dim));
-        return Q8K_OK;
+    return ln_layout(dim, [&](auto l) {
+        using L = decltype(l);
+        if (part != nullptr) return vec ? launch_ln_backward_as<Tx, Tg, L, true, true>(x, x_stride, g, mean, rstd, w, dx, part, rows, dim, st)
+                                        : launch_ln_backward_as<Tx, Tg, L, false, true>(x, x_stride, g, mean, rstd, w, dx, part, rows, dim, st);
+        return vec ? launch_ln_backward_as<Tx, Tg, L, true, false>(x, x_stride, g, mean, rstd, w, dx, part, rows, dim, st)
+                   : launch_ln_backward_as<Tx, Tg, L, false, false>(x, x_stride, g, mean, rstd, w, dx, part, rows, dim, st);
     });
 }
 
@@ -321,7 +593,7 @@ extern "C" int q8k_layer_norm(const void* x, int x_dtype, int64_t x_row_stride, 
 
 extern "C" size_t q8k_layer_norm_backward_workspace_bytes(int64_t rows, int dim) {
     if (rows <= 0 || dim <= 0 || dim > kLnMaxDim) return 0;
-    return (size_t)ln_groups(rows, dim) * 2 * (size_t)dim * sizeof(float);
+    return (size_t)ln_ctas<true>(rows, dim, true) * 2 * (size_t)dim * sizeof(float);
 }
 
 extern "C" int q8k_layer_norm_backward(const void* x, int x_dtype, int64_t x_row_stride, const void* grad, int grad_dtype,
@@ -363,6 +635,6 @@ extern "C" int q8k_layer_norm_backward(const void* x, int x_dtype, int64_t x_row
 #undef Q8K_LN_BWD
     if (rc != Q8K_OK || !sums) return rc;
     Q8K_CUDA_OK(launch_dependent(layer_norm_wgrad_kernel, (unsigned)((2 * (int64_t)dim + 31) / 32), 32 * kLnSumWarps, 0, st, 1, part,
-                                 ln_groups(rows, dim), dweight, dbias, dim));
+                                 ln_ctas<true>(rows, dim, true), dweight, dbias, dim));
     return Q8K_OK;
 }
