@@ -106,7 +106,9 @@ static int launch_gated_backward(const void* dout, const void* pre, void* q, flo
 
 // The weight operand of the backward product: w [N, K] (int8 or e4m3) times its row scales, transposed and quantised to e4m3 with one
 // scale per row of the result, i.e. per column of w.  Bound by HBM: w is read once and q written once; a column's absmax needs all
-// rows first, so there are two kernels, the second of which finds w in L2.
+// rows first, so there are two passes, the second of which finds w in L2, with a small kernel between them that makes the columns'
+// factors of the partial maxima (taken by each CTA of the second pass for itself, 64 dependent loads, they were most of its time:
+// 16384 x 2048 int8 40.9 us).
 //
 // Tiles of 128 columns, 16 per thread (one 16-byte load of a row), so a warp reads four rows of 128 bytes.
 constexpr int kWtCols = 128;
@@ -174,14 +176,39 @@ gated_weight_absmax_kernel(const Tw* __restrict__ w, const float* __restrict__ r
     }
 }
 
-template <typename Tw>
-__global__ void __launch_bounds__(kWtThreads)
-gated_weight_quant_kernel(const Tw* __restrict__ w, const float* __restrict__ row_scales, const float* __restrict__ part, int parts,
-                          uint8_t* __restrict__ q, float* __restrict__ scales, int N, int K) {
-    __shared__ float mul[kWtCols];
-    __shared__ __align__(16) uint32_t turned[kWtCols][kWtRows / 4];
+// factors[c] = 448 * (1 / absmax of column c) (0 for a column of zeros), scales[c] = 1 / that: 32 columns a CTA.
+constexpr int kWtFactorWarps = 8;
+__global__ void __launch_bounds__(32 * kWtFactorWarps)
+gated_weight_factor_kernel(const float* __restrict__ part, int parts, float* __restrict__ factors, float* __restrict__ scales, int K) {
+    __shared__ float red[kWtFactorWarps][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + lane;
     pdl_wait();
     pdl_release();
+    float a = 0.f;
+    if (c < K) {
+#pragma unroll 8
+        for (int k = warp; k < parts; k += kWtFactorWarps) a = fmaxf(a, part[(int64_t)k * K + c]);
+    }
+    red[warp][lane] = a;
+    __syncthreads();
+    if (warp == 0 && c < K) {
+#pragma unroll
+        for (int k = 1; k < kWtFactorWarps; ++k) a = fmaxf(a, red[k][lane]);
+        const float f = quant_factor<true>(448.0f, a);
+        factors[c] = a == 0.f ? 0.f : f;                       // a column of zeros quantises to zeros
+        scales[c] = __fdiv_rn(1.0f, f);
+    }
+}
+
+// The kernels before this one on the stream read w and let it start only once they had waited for its writer, so w may be loaded
+// before the wait.
+template <typename Tw>
+__global__ void __launch_bounds__(kWtThreads)
+gated_weight_quant_kernel(const Tw* __restrict__ w, const float* __restrict__ row_scales, const float* __restrict__ factors,
+                          uint8_t* __restrict__ q, int N, int K) {
+    __shared__ float mul[kWtCols];
+    __shared__ __align__(16) uint32_t turned[kWtCols][kWtRows / 4];
     const int cb = blockIdx.x * kWtCols, r0 = blockIdx.y * kWtRows;
     const int cg = threadIdx.x & 7, rg = threadIdx.x >> 3;     // 16 columns, four rows
     uint4 x[4];
@@ -192,13 +219,9 @@ gated_weight_quant_kernel(const Tw* __restrict__ w, const float* __restrict__ ro
         x[i] = in ? *reinterpret_cast<const uint4*>(w + (int64_t)(r0 + rg * 4 + i) * K + cb + cg * 16) : make_uint4(0, 0, 0, 0);
         s[i] = in ? row_scales[r0 + rg * 4 + i] : 0.f;
     }
-    if (threadIdx.x < kWtCols && cb + (int)threadIdx.x < K) {
-        float a = 0.f;
-        for (int k = 0; k < parts; ++k) a = fmaxf(a, part[(int64_t)k * K + cb + threadIdx.x]);
-        const float f = quant_factor<true>(448.0f, a);
-        mul[threadIdx.x] = a == 0.f ? 0.f : f;                 // a column of zeros quantises to zeros
-        if (blockIdx.y == 0) scales[cb + threadIdx.x] = __fdiv_rn(1.0f, f);
-    }
+    pdl_wait();
+    pdl_release();
+    if (threadIdx.x < kWtCols && cb + (int)threadIdx.x < K) mul[threadIdx.x] = factors[cb + threadIdx.x];
     __syncthreads();
     if (cb + cg * 16 < K) {
 #pragma unroll
@@ -234,8 +257,11 @@ static int launch_gated_weight(const void* w, const float* row_scales, void* q, 
     const int parts = (N + kWtMaxRows - 1) / kWtMaxRows;
     Q8K_CUDA_OK(launch_dependent(gated_weight_absmax_kernel<Tw>, dim3(cols, (unsigned)parts), kWtThreads, 0, st, 1, (const Tw*)w, row_scales,
                                  part, N, K));
+    float* factors = part + (int64_t)parts * K;
+    Q8K_CUDA_OK(launch_dependent(gated_weight_factor_kernel, dim3((unsigned)((K + 31) / 32)), 32 * kWtFactorWarps, 0, st, 1, part, parts, factors,
+                                 scales, K));
     Q8K_CUDA_OK(launch_dependent(gated_weight_quant_kernel<Tw>, dim3(cols, (unsigned)((N + kWtRows - 1) / kWtRows)), kWtThreads, 0, st, 1,
-                                 (const Tw*)w, row_scales, part, parts, (uint8_t*)q, scales, N, K));
+                                 (const Tw*)w, row_scales, factors, (uint8_t*)q, N, K));
     return Q8K_OK;
 }
 
@@ -259,7 +285,7 @@ extern "C" int q8k_gated_backward_quant(const void* grad, const void* pre, void*
 
 extern "C" size_t q8k_gated_weight_operand_workspace_bytes(int F, int K) {
     if (F <= 0 || K <= 0) return 0;
-    return (2 * (size_t)F + q8k::kWtMaxRows - 1) / q8k::kWtMaxRows * (size_t)K * sizeof(float);
+    return ((2 * (size_t)F + q8k::kWtMaxRows - 1) / q8k::kWtMaxRows + 1) * (size_t)K * sizeof(float);   // partial maxima, factors
 }
 
 extern "C" int q8k_gated_weight_operand(const void* w, int w_dtype, const float* w_scales, void* q, float* scales, int F, int K,
