@@ -112,21 +112,27 @@ static int launch_gated_backward(const void* dout, const void* pre, void* q, flo
 //
 // Tiles of 128 columns, 16 per thread (one 16-byte load of a row), so a warp reads four rows of 128 bytes.
 constexpr int kWtCols = 128;
-constexpr int kWtMaxRows = 256;              // rows whose absmax one CTA takes
+constexpr int kWtMaxRows = 512;              // rows whose absmax one CTA takes
 constexpr int kWtRows = 128;                 // rows of a tile that is quantised and turned
 constexpr int kWtThreads = 256;
 
-template <typename Tw> __device__ __forceinline__ void wt_values(uint32_t w, float s, float (&v)[4]) {
+// Four elements times their row's scale, as packed pairs of columns: both passes are bound by instruction issue.
+template <typename Tw> __device__ __forceinline__ void wt_values(uint32_t w, float s, float2 (&v)[2]) {
     if constexpr (std::is_same_v<Tw, int8_t>) {
         // 2^23 + 128 + b has the byte b + 128 in its last bits: a permutation and an exact difference instead of a conversion,
         // which runs at an eighth of their rate
         const uint32_t u = w ^ 0x80808080u;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = __fmul_rn(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7650 | j)) - 8388736.0f, s);
+        for (int j = 0; j < 2; ++j) {
+            const float2 f = make_float2(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7650 | (2 * j))),
+                                         __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7650 | (2 * j + 1))));
+            v[j] = fmul2(fsub2(f, make_float2(8388736.0f, 8388736.0f)), make_float2(s, s));
+        }
     } else {
-        e4m3x4_to_float(w, v);
+        float f[4];
+        e4m3x4_to_float(w, f);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = __fmul_rn(v[j], s);
+        for (int j = 0; j < 2; ++j) v[j] = fmul2(make_float2(f[2 * j], f[2 * j + 1]), make_float2(s, s));
     }
 }
 
@@ -143,19 +149,28 @@ gated_weight_absmax_kernel(const Tw* __restrict__ w, const float* __restrict__ r
 #pragma unroll
     for (int j = 0; j < 16; ++j) m[j] = 0.f;
     if (c0 < K) {
+        // two rows at a time into one maximum of three operands; rows beyond N (a multiple of 16, so not pairs of them) have scale 0
+#pragma unroll 4
+        for (int i = 0; i < kWtMaxRows / 64; ++i) {
+            const int r = r0 + i * 64 + rl * 2;
+            const bool in = r < N;
+            uint32_t xw[2][4];
+            float s[2];
 #pragma unroll
-        for (int i = 0; i < kWtMaxRows / 32; ++i) {
-            const int r = r0 + i * 32 + rl;
-            if (r < N) {
-                const uint4 x = *reinterpret_cast<const uint4*>(w + (int64_t)r * K + c0);
-                const float s = row_scales[r];
-                const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
+            for (int h = 0; h < 2; ++h) {
+                const uint4 x = in ? *reinterpret_cast<const uint4*>(w + (int64_t)(r + h) * K + c0) : make_uint4(0, 0, 0, 0);
+                s[h] = in ? row_scales[r + h] : 0.f;
+                xw[h][0] = x.x; xw[h][1] = x.y; xw[h][2] = x.z; xw[h][3] = x.w;
+            }
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float v[4];
-                    wt_values<Tw>(xw[k], s, v);
+            for (int k = 0; k < 4; ++k) {
+                float2 u[2], v[2];
+                wt_values<Tw>(xw[0][k], s[0], u);
+                wt_values<Tw>(xw[1][k], s[1], v);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) m[k * 4 + j] = fmaxf(m[k * 4 + j], fabsf(v[j]));
+                for (int j = 0; j < 2; ++j) {
+                    asm("max.f32 %0, %0, %1, %2;" : "+f"(m[k * 4 + 2 * j]) : "f"(fabsf(u[j].x)), "f"(fabsf(v[j].x)));
+                    asm("max.f32 %0, %0, %1, %2;" : "+f"(m[k * 4 + 2 * j + 1]) : "f"(fabsf(u[j].y)), "f"(fabsf(v[j].y)));
                 }
             }
         }
@@ -207,7 +222,7 @@ template <typename Tw>
 __global__ void __launch_bounds__(kWtThreads)
 gated_weight_quant_kernel(const Tw* __restrict__ w, const float* __restrict__ row_scales, const float* __restrict__ factors,
                           uint8_t* __restrict__ q, int N, int K) {
-    __shared__ float mul[kWtCols];
+    __shared__ __align__(16) float mul[kWtCols];
     __shared__ __align__(16) uint32_t turned[kWtCols][kWtRows / 4];
     const int cb = blockIdx.x * kWtCols, r0 = blockIdx.y * kWtRows;
     const int cg = threadIdx.x & 7, rg = threadIdx.x >> 3;     // 16 columns, four rows
@@ -226,17 +241,22 @@ gated_weight_quant_kernel(const Tw* __restrict__ w, const float* __restrict__ ro
     if (cb + cg * 16 < K) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            float v[4][4];                                     // [row][column]
+            float2 v[4][2];                                    // [row][pair of columns]
+            const int c = cg * 16 + k * 4;
+            const float4 f = *reinterpret_cast<const float4*>(mul + c);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) wt_values<Tw>(k == 0 ? x[i].x : k == 1 ? x[i].y : k == 2 ? x[i].z : x[i].w, s[i], v[i]);
+            for (int i = 0; i < 4; ++i) {
+                wt_values<Tw>(k == 0 ? x[i].x : k == 1 ? x[i].y : k == 2 ? x[i].z : x[i].w, s[i], v[i]);
+                v[i][0] = fmul2(v[i][0], make_float2(f.x, f.y));
+                v[i][1] = fmul2(v[i][1], make_float2(f.z, f.w));
+            }
+            // saturating cast: see tokenwise_quant_kernel.  Row group rg of a column goes to word rg + 4 * (column group): the 32
+            // words that a warp stores lie in 32 banks, and four of a column stay together for the 16-byte reads below.
+            const int at = (rg + 4 * cg) & 31;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int c = cg * 16 + k * 4 + j;
-                const float f = mul[c];
-                // saturating cast: see tokenwise_quant_kernel.  Row group rg of a column goes to word rg + 4 * (column group): the 32
-                // words that a warp stores lie in 32 banks, and four of a column stay together for the 16-byte reads below.
-                turned[c][(rg + 4 * cg) & 31] = (uint32_t)float2_to_e4m3x2_sat(__fmul_rn(v[0][j], f), __fmul_rn(v[1][j], f)) |
-                                                ((uint32_t)float2_to_e4m3x2_sat(__fmul_rn(v[2][j], f), __fmul_rn(v[3][j], f)) << 16);
+            for (int j = 0; j < 2; ++j) {
+                turned[c + 2 * j][at] = (uint32_t)float2_to_e4m3x2_sat(v[0][j].x, v[1][j].x) | ((uint32_t)float2_to_e4m3x2_sat(v[2][j].x, v[3][j].x) << 16);
+                turned[c + 2 * j + 1][at] = (uint32_t)float2_to_e4m3x2_sat(v[0][j].y, v[1][j].y) | ((uint32_t)float2_to_e4m3x2_sat(v[2][j].y, v[3][j].y) << 16);
             }
         }
     }
