@@ -5,11 +5,18 @@
 // same kernel with the angle negated.
 //
 // Bound by HBM: every element of q and k is read and written once, in one launch, and no table is read.  The angles are
-// computed here, once per token and pair, and shared by all heads through shared memory.  A position of a million radians has
+// computed here, once per token and pair, and shared by the heads through shared memory.  A position of a million radians has
 // no correct digit in fp32 after its reduction, so position * freq / (2 pi) is formed in fp64, the whole turns are dropped there, and
 // sine and cosine are taken of the rest, at most half a turn, in fp32.
+//
+// What is left to save are instructions: at the copy rate an SM has some 15 for an element.  So a thread takes the same channels of
+// up to eight heads of one token: its cosines and sines come from shared memory once, and its addresses advance by the head's stride.
+// CTAs of 128 threads, eight an SM: the chain from position to sine of one hides behind the stores of another, and the last ones to
+// finish are short.  Measured (bf16, CUDA graphs): 6144 tokens x 64 heads x 64 interleaved 17.5 us (0.88 of the copy rate), 16384 x 40 x
+// 128 half 61.8 us (0.83).  Tried: six CTAs without spills (17.9, 64.3), one head's loads at a time (19.8, 65.2), a thread for one
+// unit with the next token's elements on their way meanwhile (30.9, 103).
 
-#include <math_constants.h>
+#include <type_traits>
 #include "common.cuh"
 
 namespace q8k {
@@ -32,107 +39,137 @@ struct RotaryParams {
     int seq, head_dim, rotary_dim, half;     // half: layout
 };
 
-constexpr int kRotaryThreads = 256;
 constexpr int kRotaryMaxDim = 4096;
+constexpr int kRotaryThreads = 128;
+constexpr int kRotaryHeads = 8;              // heads of a thread, where there are threads for the others
 
-// V channels at a time where everything is 16-byte aligned (VEC), one pair at a time otherwise.  A CTA takes `tpc` consecutive tokens.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kRotaryThreads)
-rotary_kernel(const __grid_constant__ RotaryParams p, int tpc) {
-    extern __shared__ float2 turns[];                          // [tpc][rotary_dim / 2] cosine, sine
-    constexpr int V = VEC ? 16 / sizeof(T) : 1;
+// How a CTA's threads are laid out over its tokens: unit_lanes threads for the units of a head, head_lanes for the heads.
+struct RotaryLanes { int units, unit_lanes, head_lanes, tokens; };
+
+template <int BYTES> struct RotaryRaw;
+template <> struct RotaryRaw<2>  { using type = uint16_t; };
+template <> struct RotaryRaw<4>  { using type = uint32_t; };
+template <> struct RotaryRaw<8>  { using type = uint2; };
+template <> struct RotaryRaw<16> { using type = uint4; };
+
+// V channels at a time, all accesses aligned to them.  TWO: a pair's channels lie apart (half layout, or V = 1), so a unit is V pairs in
+// two runs of V channels; otherwise V / 2 pairs in one.  PART: there are channels behind the rotated ones, whose units copy one or two
+// runs.
+template <typename T, int V, bool TWO, bool PART>
+__global__ void __launch_bounds__(kRotaryThreads, TWO && PART ? 6 : 8)
+rotary_kernel(const __grid_constant__ RotaryParams p, const RotaryLanes l) {
+    constexpr int PAIRS = TWO ? V : V / 2;
+    constexpr int AHEAD = TWO ? 2 : 4;                         // heads whose loads are on their way together
+    using Raw = typename RotaryRaw<V * sizeof(T)>::type;
+    union Elems { Raw r; T e[V]; };
+    extern __shared__ float2 turns[];                          // [tokens][rotary_dim / 2] cosine, sine
     const int half_dim = p.rotary_dim / 2;
-    const int64_t token0 = (int64_t)blockIdx.x * tpc;
-    const int nt = (int)(p.tokens - token0 < tpc ? p.tokens - token0 : tpc);
+    const int per_token = l.unit_lanes * l.head_lanes;
+    const int tl = threadIdx.x / per_token, rest = threadIdx.x - tl * per_token;
+    const unsigned token = blockIdx.x * (unsigned)l.tokens + (unsigned)tl;
+    const unsigned batch = token / (unsigned)p.seq, s = token - batch * (unsigned)p.seq;
+    const bool here = tl < l.tokens && token < (unsigned)p.tokens;
     pdl_wait();
     pdl_release();
 
-    for (int i = threadIdx.x; i < nt * half_dim; i += kRotaryThreads) {
-        const int tl = i / half_dim, pair = i - tl * half_dim;
-        const int64_t token = token0 + tl;
-        const int64_t batch = token / p.seq, s = token - batch * p.seq;
+    if (here) {                                                // a token's threads make its angles
         int64_t pos = s;
         if (p.positions != nullptr) {
             const int64_t at = batch * p.pos_batch + s * p.pos_token;
             pos = p.positions64 ? static_cast<const int64_t*>(p.positions)[at] : (int64_t)static_cast<const int32_t*>(p.positions)[at];
         }
-        const double t = (double)pos * (p.freq[pair] * 0.15915494309189535);   // 1 / (2 pi)
-        float sn, cs;
-        sincospif(2.0f * (float)(t - rint(t)), &sn, &cs);
-        turns[i] = make_float2(cs * p.amplitude, sn * p.amplitude * p.sign);
+        for (int i = rest; i < half_dim; i += per_token) {
+            const double t = (double)pos * (p.freq[i] * 0.15915494309189535);  // 1 / (2 pi)
+            float sn, cs;
+            sincospif(2.0f * (float)(t - rint(t)), &sn, &cs);
+            turns[tl * half_dim + i] = make_float2(cs * p.amplitude, sn * p.amplitude * p.sign);
+        }
     }
     __syncthreads();
+    if (!here) return;
 
-    // units of a head: in the half layout V pairs (two runs of V channels), in the interleaved one V / 2 pairs (one run;
-    // VEC = false: the pair); then the channels behind the rotated ones, V at a time
-    const int rot_units = p.half || !VEC ? half_dim / V : p.rotary_dim / V;
-    const int units = rot_units + (p.head_dim - p.rotary_dim) / V;
-    const int heads = p.q.heads + p.k.heads;
-    const int per_token = heads * units;
-    for (int i = threadIdx.x; i < nt * per_token; i += kRotaryThreads) {
-        const int tl = i / per_token;
-        const int r = i - tl * per_token;
-        const int h = r / units, u = r - h * units;
-        const int64_t token = token0 + tl;
-        const int64_t batch = token / p.seq, s = token - batch * p.seq;
-        const bool is_q = h < p.q.heads;
-        const RotaryTensor& a = is_q ? p.q : p.k;
-        const int hl = is_q ? h : h - p.q.heads;
-        const T* in = static_cast<const T*>(a.in) + batch * a.in_batch + s * a.in_token + hl * a.in_head;
-        T* out = static_cast<T*>(a.out) + batch * a.out_batch + s * a.out_token + hl * a.out_head;
-        const float2* cs = turns + tl * half_dim;
-        if (u >= rot_units) {
-            const int c = p.rotary_dim + (u - rot_units) * V;
-            if constexpr (VEC) *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<const uint4*>(in + c);
-            else out[c] = in[c];
-        } else if constexpr (!VEC) {
-            const int c0 = p.half ? u : 2 * u, c1 = p.half ? u + half_dim : 2 * u + 1;
-            const float x = to_float<T>(in[c0]), y = to_float<T>(in[c1]);
-            out[c0] = from_float<T>(x * cs[u].x - y * cs[u].y);
-            out[c1] = from_float<T>(y * cs[u].x + x * cs[u].y);
-        } else if (p.half) {
-            const int c = u * V;
-            float x[V], y[V], ox[V], oy[V];
-            load_vec<T, V>(in + c, x);
-            load_vec<T, V>(in + c + half_dim, y);
+    const int h0 = rest / l.unit_lanes;
+    const int rot_units = half_dim / PAIRS;
+    for (int u = rest - h0 * l.unit_lanes; u < l.units; u += l.unit_lanes) {
+        const bool copy = PART && u >= rot_units;
+        const int c = copy ? p.rotary_dim + (u - rot_units) * (TWO ? 2 * V : V) : V == 1 && !p.half ? 2 * u : u * V;
+        const int next = copy ? V : p.half ? half_dim : 1;     // from a unit's first run to its second
+        const bool second = TWO && (!copy || c + V < p.head_dim);
+        float2 w[PAIRS];
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float2 w = cs[c + j];
-                ox[j] = x[j] * w.x - y[j] * w.y;
-                oy[j] = y[j] * w.x + x[j] * w.y;
-            }
-            store_vec<T, V>(out + c, ox);
-            store_vec<T, V>(out + c + half_dim, oy);
-        } else {
-            const int c = u * V;
-            float x[V], o[V];
-            load_vec<T, V>(in + c, x);
+        for (int j = 0; j < PAIRS; ++j) w[j] = copy ? make_float2(1.f, 0.f) : turns[tl * half_dim + u * PAIRS + j];
+        auto walk = [&](const RotaryTensor& a, int h) {        // heads h, h + head_lanes, ... of q or k
+            const T* in = static_cast<const T*>(a.in) + batch * a.in_batch + s * a.in_token + h * a.in_head + c;
+            T* out = static_cast<T*>(a.out) + batch * a.out_batch + s * a.out_token + h * a.out_head + c;
+            const int64_t in_step = l.head_lanes * a.in_head, out_step = l.head_lanes * a.out_head;
+            while (h < a.heads) {
+                Elems x[AHEAD], y[AHEAD];
+                const int n = (a.heads - h + l.head_lanes - 1) / l.head_lanes;     // heads left
 #pragma unroll
-            for (int j = 0; j < V; j += 2) {
-                const float2 w = cs[(c + j) / 2];
-                o[j] = x[j] * w.x - x[j + 1] * w.y;
-                o[j + 1] = x[j + 1] * w.x + x[j] * w.y;
+                for (int k = 0; k < AHEAD; ++k) {
+                    if (k < n) {
+                        x[k].r = *reinterpret_cast<const Raw*>(in);
+                        if (second) y[k].r = *reinterpret_cast<const Raw*>(in + next);
+                        in += in_step;
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    if (k >= n) break;
+                    if (!copy) {
+#pragma unroll
+                        for (int j = 0; j < PAIRS; ++j) {
+                            T& a0 = x[k].e[TWO ? j : 2 * j];
+                            T& b0 = TWO ? y[k].e[j] : x[k].e[TWO ? 0 : 2 * j + 1];
+                            const float f = to_float<T>(a0), g = to_float<T>(b0);
+                            a0 = from_float<T>(f * w[j].x - g * w[j].y);
+                            b0 = from_float<T>(g * w[j].x + f * w[j].y);
+                        }
+                    }
+                    *reinterpret_cast<Raw*>(out) = x[k].r;
+                    if (second) *reinterpret_cast<Raw*>(out + next) = y[k].r;
+                    out += out_step;
+                }
+                h += AHEAD * l.head_lanes;
             }
-            store_vec<T, V>(out + c, o);
-        }
+        };
+        // heads of k go on where those of q end, so that every lane has as many
+        const int after = p.q.heads > h0 ? (p.q.heads - h0 + l.head_lanes - 1) / l.head_lanes * l.head_lanes + h0 : h0;
+        walk(p.q, h0);
+        walk(p.k, after - p.q.heads);
     }
 }
 
-template <typename T> static int launch_rotary(const RotaryParams& p, bool vec, cudaStream_t st) {
-    // tokens per CTA: about four units of work a thread, but no fewer CTAs than SMs
-    const int v = vec ? (int)(16 / sizeof(T)) : 1;
-    const int64_t per_token = (int64_t)(p.q.heads + p.k.heads) * (p.head_dim / v);
-    int64_t tpc = (4 * kRotaryThreads + per_token - 1) / per_token;
-    const int64_t spread = (p.tokens + gemm_num_sms() - 1) / gemm_num_sms();
-    if (tpc > spread) tpc = spread;
-    const int64_t room = 32 * 1024 / (4 * p.rotary_dim);      // shared memory: 4 bytes times rotary_dim per token, up to 32 KB
-    if (tpc > room) tpc = room;
-    if (tpc < 1) tpc = 1;
-    const int64_t grid = (p.tokens + tpc - 1) / tpc;
-    Q8K_REQUIRE(grid <= 0x7fffffffLL, Q8K_ERR_TOO_LARGE, "rotary: %lld tokens", (long long)p.tokens);
-    auto kern = vec ? rotary_kernel<T, true> : rotary_kernel<T, false>;
-    Q8K_CUDA_OK(launch_dependent(kern, (unsigned)grid, kRotaryThreads, (size_t)tpc * p.rotary_dim * 4, st, 1, p, (int)tpc));
+template <typename T, int V, bool TWO> static int launch_rotary_as(const RotaryParams& p, cudaStream_t st) {
+    const int heads = p.q.heads + p.k.heads;
+    RotaryLanes l;
+    constexpr int run = TWO ? 2 * V : V;
+    l.units = p.rotary_dim / 2 / (TWO ? V : V / 2) + (p.head_dim - p.rotary_dim + run - 1) / run;
+    l.unit_lanes = l.units < kRotaryThreads ? l.units : kRotaryThreads;
+    // kRotaryHeads heads a thread, fewer while there are SMs without a CTA; then as many tokens as threads are left for
+    const int rest = kRotaryThreads / l.unit_lanes;
+    int per_thread = kRotaryHeads;
+    auto lanes = [&](int n) { const int want = (heads + n - 1) / n; return want < rest ? want : rest; };
+    while (per_thread > 1 && (p.tokens + rest / lanes(per_thread) - 1) / (rest / lanes(per_thread)) < gemm_num_sms()) --per_thread;
+    l.head_lanes = lanes(per_thread);
+    l.tokens = rest / l.head_lanes;
+    const int room = 24 * 1024 / (4 * p.rotary_dim);           // shared memory: 4 bytes times rotary_dim per token, up to 24 KB
+    if (l.tokens > room) l.tokens = room;
+    const int64_t grid = (p.tokens + l.tokens - 1) / l.tokens;
+    const unsigned threads = (unsigned)((l.tokens * l.unit_lanes * l.head_lanes + 31) / 32 * 32);
+    auto kern = p.rotary_dim < p.head_dim ? rotary_kernel<T, V, TWO, true> : rotary_kernel<T, V, TWO, false>;
+    Q8K_CUDA_OK(launch_dependent(kern, (unsigned)grid, threads, (size_t)l.tokens * p.rotary_dim * 4, st, 1, p, l));
     return Q8K_OK;
+}
+
+// v: channels that all accesses are aligned to, a power of two
+template <typename T> static int launch_rotary(const RotaryParams& p, int v, cudaStream_t st) {
+    if constexpr (sizeof(T) == 2) {
+        if (v == 8) return p.half ? launch_rotary_as<T, 8, true>(p, st) : launch_rotary_as<T, 8, false>(p, st);
+    }
+    if (v >= 4) return p.half ? launch_rotary_as<T, 4, true>(p, st) : launch_rotary_as<T, 4, false>(p, st);
+    if (v >= 2) return p.half ? launch_rotary_as<T, 2, true>(p, st) : launch_rotary_as<T, 2, false>(p, st);
+    return launch_rotary_as<T, 1, true>(p, st);
 }
 
 }  // namespace q8k
@@ -159,9 +196,14 @@ extern "C" int q8k_rotary(const void* q, const int64_t q_strides[3], void* q_out
                 "%s: null or misaligned frequencies", op);
     Q8K_REQUIRE(reinterpret_cast<uintptr_t>(positions) % (positions_int64 ? 8 : 4) == 0, Q8K_ERR_INVALID_ARG,
                 "%s: misaligned positions", op);
+    Q8K_REQUIRE((int64_t)batch * seq <= 0x7fffffffLL, Q8K_ERR_TOO_LARGE, "%s: %lld tokens", op, (long long)batch * seq);
     RotaryParams p = {};
-    const int v = 16 / size;
-    bool vec = head_dim % v == 0 && rotary_dim % v == 0 && (!half_layout || (rotary_dim / 2) % v == 0);
+    // the widest access, up to 16 bytes, that divides the channels, strides and addresses of all four tensors
+    int v = 16 / size;
+    auto divides = [&](int64_t n) { while (n % v != 0) v /= 2; };
+    divides(head_dim);
+    divides(rotary_dim);
+    if (half_layout) divides(rotary_dim / 2);
     auto tensor = [&](RotaryTensor& t, const void* in, const int64_t* is, void* out, const int64_t* os, int heads) {
         t.heads = heads;
         if (heads == 0) return true;
@@ -171,9 +213,14 @@ extern "C" int q8k_rotary(const void* q, const int64_t q_strides[3], void* q_out
         t.in = in; t.out = out;
         t.in_batch = is[0]; t.in_token = is[1]; t.in_head = is[2];
         t.out_batch = os[0]; t.out_token = os[1]; t.out_head = os[2];
-        vec = vec && aligned16(in) && aligned16(out);
+        divides((int64_t)(reinterpret_cast<uintptr_t>(in) / size));
+        divides((int64_t)(reinterpret_cast<uintptr_t>(out) / size));
         const int64_t n[3] = {batch, seq, heads};              // a stride over one element does not matter
-        for (int i = 0; i < 3; ++i) vec = vec && (n[i] == 1 || (is[i] % v == 0 && os[i] % v == 0));
+        for (int i = 0; i < 3; ++i) {
+            if (n[i] == 1) continue;
+            divides(is[i]);
+            divides(os[i]);
+        }
         return true;
     };
     Q8K_REQUIRE(tensor(p.q, q, q_strides, q_out, q_out_strides, q_heads) && tensor(p.k, k, k_strides, k_out, k_out_strides, k_heads),
@@ -188,7 +235,7 @@ extern "C" int q8k_rotary(const void* q, const int64_t q_strides[3], void* q_out
     p.tokens = (int64_t)batch * seq;
     p.seq = seq; p.head_dim = head_dim; p.rotary_dim = rotary_dim; p.half = half_layout != 0;
     cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == Q8K_DT_BF16) return launch_rotary<__nv_bfloat16>(p, vec, st);
-    if (dtype == Q8K_DT_F16) return launch_rotary<__half>(p, vec, st);
-    return launch_rotary<float>(p, vec, st);
+    if (dtype == Q8K_DT_BF16) return launch_rotary<__nv_bfloat16>(p, v, st);
+    if (dtype == Q8K_DT_F16) return launch_rotary<__half>(p, v, st);
+    return launch_rotary<float>(p, v, st);
 }
