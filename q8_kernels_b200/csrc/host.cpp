@@ -665,8 +665,9 @@ PyObject* qk_norm_rope_prep_pair(PyObject*, PyObject* const* args, Py_ssize_t n)
 
 // ---------------------------------------------------------------- layer norm, rotary positions, gated projection
 // These are differentiable: where an input has a gradient the call leaves a node of torch's C++ autograd behind, whose backward pass
-// launches without the interpreter.  (A Python autograd.Function costs some 60 us of host time for one forward and backward pass, the
-// kernels of a short call 10.)  What the functions of the same name in functional/ do with tensors that these do not take is the same.
+// launches without the interpreter.  The underscore marks them: they answer for functions of functional/, not of native.py.  (A Python autograd.Function costs some 60 us of host time for one forward and backward pass, the
+// kernels of a short call 10.)  What functional.layer_norm.layer_norm, functional.rotary.apply_rotary and functional.gated do with tensors
+// that these do not take is the same.
 
 using torch::autograd::AutogradContext;
 using torch::autograd::Variable;
@@ -716,7 +717,7 @@ variable_list once_only(variable_list&& grads, const variable_list& incoming) {
     return error->apply(std::move(grads));
 }
 
-// ---- layer_norm(x, weight | None, bias | None, eps, out_type)
+// ---- _layer_norm(x, weight | None, bias | None, eps, out_type)
 struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     static Variable run(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b, double eps, Dt out, at::Tensor* mean, at::Tensor* rstd) {
         const int dim = (int)x.size(-1);
@@ -772,7 +773,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     }
 };
 
-PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+PyObject* _layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     FAST_BEGIN
     Call c(args, n, 5);
     const at::Tensor* x = c.tensor(0);
@@ -801,7 +802,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     FAST_END
 }
 
-// ---- rotary(q, k | None, positions | None, frequencies, amplitude, half)
+// ---- _rotary(q, k | None, positions | None, frequencies, amplitude, half)
 struct RotaryNode : torch::autograd::Function<RotaryNode> {
     // q and k of [batch, seq, heads, dim], or without the batch; either may be undefined
     static variable_list run(const at::Tensor& q, const at::Tensor& k, const at::Tensor& pos, const at::Tensor& freq, double amplitude, bool half,
@@ -864,7 +865,7 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
     }
 };
 
-PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+PyObject* _rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     FAST_BEGIN
     Call c(args, n, 6);
     const at::Tensor* q = c.tensor(0, true);
@@ -917,7 +918,7 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     FAST_END
 }
 
-// ---- gated_linear(a, b, bias | None, scale_b, activation code, int8, rotate)
+// ---- _gated_linear(a, b, bias | None, scale_b, activation code, int8, rotate)
 struct GatedNode : torch::autograd::Function<GatedNode> {
     static at::Tensor run(const at::Tensor& a, const at::Tensor& b, const at::Tensor& bias, const at::Tensor& scale, int act, bool int8, bool rotate,
                           at::Tensor* pre) {
@@ -992,7 +993,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
     }
 };
 
-PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+PyObject* _gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
     FAST_BEGIN
     Call c(args, n, 7);
     const at::Tensor* a = c.tensor(0);
@@ -1051,7 +1052,7 @@ PyMethodDef methods[] = {
     FAST(tokenwise_quant), FAST(hadamard_quant), FAST(fast_hadamard_transform), FAST(norm_modulate_quant), FAST(transpose_quant),
     FAST(dequant_hadamard), FAST(rms_norm), FAST(rms_norm_backward), FAST(rope), FAST(rope_backward), FAST(mm),
     FAST(mm_gate_residual), FAST(linear), FAST(flash_attention), FAST(attention_prep_rows), FAST(qk_norm_rope_prep),
-    FAST(kv_prep), FAST(qk_norm_rope_prep_pair), FAST(layer_norm), FAST(rotary), FAST(gated_linear),
+    FAST(kv_prep), FAST(qk_norm_rope_prep_pair), FAST(_layer_norm), FAST(_rotary), FAST(_gated_linear),
     {"set_check", set_check, METH_O, nullptr}, {"set_status_word", set_status_word, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

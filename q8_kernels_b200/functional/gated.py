@@ -49,7 +49,7 @@ class GatedLinearFunc(torch.autograd.Function):
 
 def _gated(op, a, b, bias, scale_a, scale_b, act, int8, rotate):
     if scale_a is None:
-        fast = native._host.gated_linear(a, b, bias, scale_b, native.ACTIVATIONS.get(act, 0), int8, rotate)
+        fast = native._host._gated_linear(a, b, bias, scale_b, native.ACTIVATIONS.get(act, 0), int8, rotate)
         if fast is not None:
             return fast
     weight_type = torch.int8 if int8 else E4M3

@@ -33,7 +33,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dim of x (bf16, fp16 or fp32; any leading dims and strides), with fp32
     ``weight`` and ``bias`` of that dim, at most 16384.  ``out_type``: x's type (default), e4m3 for bf16, or bf16 / fp16 for fp32.
     Statistics and sums are fp32; the gradients of weight and bias are fp32 and have the same bits in every run."""
-    fast = _host.layer_norm(x, weight, bias, eps, out_type)
+    fast = _host._layer_norm(x, weight, bias, eps, out_type)
     if fast is not None:
         return fast
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):

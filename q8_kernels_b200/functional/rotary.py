@@ -90,7 +90,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional
     if layout not in LAYOUTS:
         raise Q8KernelError(f"apply_rotary: layout {layout!r} is not one of {', '.join(LAYOUTS)}")
     amplitude, half = float(amplitude), layout == "half"
-    fast = _host.rotary(q, k, positions, frequencies, amplitude, half)
+    fast = _host._rotary(q, k, positions, frequencies, amplitude, half)
     if fast is not None:
         return fast
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):

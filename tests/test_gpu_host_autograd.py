@@ -33,7 +33,7 @@ def test_differentiable_ops_native_and_python_body(i):
 
     def run(native):
         leaf = x.clone().requires_grad_(True)
-        names = ("layer_norm", "rotary", "gated_linear")
+        names = ("_layer_norm", "_rotary", "_gated_linear")
         kept = {n: getattr(_host, n) for n in names}
         for n in names:
             def watch(*a, fn=kept[n]):
@@ -76,14 +76,14 @@ def test_differentiable_ops_leave_others_to_python():
     from q8_kernels_b200.functional.rotary import rotary_frequencies
     x = torch.zeros(4, 6, 2, 64, device="cuda", dtype=BF16)
     freq = rotary_frequencies(64)[0].cuda()
-    assert _host.layer_norm(x, None, None, 1e-5, None) is not None and _host.rotary(x, None, None, freq, 1.0, True) is not None
-    assert _host.layer_norm(x[..., ::2], None, None, 1e-5, None) is None and _host.layer_norm(x, None, None, 1e-5, torch.float16) is None
-    assert _host.layer_norm(x.cpu(), None, None, 1e-5, None) is None and _host.layer_norm(x, None, None, 1, None) is None
-    assert _host.rotary(x[..., ::2], None, None, freq[:16], 1.0, True) is None and _host.rotary(x, x.half(), None, freq, 1.0, True) is None
-    assert _host.rotary(x, None, None, freq.float(), 1.0, True) is None
-    assert torch.func.vmap(lambda t: torch.tensor(_host.layer_norm(t, None, None, 1e-5, None) is None))(x).all()
+    assert _host._layer_norm(x, None, None, 1e-5, None) is not None and _host._rotary(x, None, None, freq, 1.0, True) is not None
+    assert _host._layer_norm(x[..., ::2], None, None, 1e-5, None) is None and _host._layer_norm(x, None, None, 1e-5, torch.float16) is None
+    assert _host._layer_norm(x.cpu(), None, None, 1e-5, None) is None and _host._layer_norm(x, None, None, 1, None) is None
+    assert _host._rotary(x[..., ::2], None, None, freq[:16], 1.0, True) is None and _host._rotary(x, x.half(), None, freq, 1.0, True) is None
+    assert _host._rotary(x, None, None, freq.float(), 1.0, True) is None
+    assert torch.func.vmap(lambda t: torch.tensor(_host._layer_norm(t, None, None, 1e-5, None) is None))(x).all()
     w, s = torch.zeros(64, 64, dtype=torch.int8, device="cuda"), torch.zeros(64, device="cuda")
     a = x.view(-1, 64)
-    assert _host.gated_linear(a, w, None, s, 1, True, True) is not None
-    assert _host.gated_linear(a, w, None, s, 0, True, True) is None and _host.gated_linear(a, w, None, s, 1, False, True) is None
-    assert _host.gated_linear(a, w[:48], None, s[:48], 1, True, True) is None and _host.gated_linear(a, w, s[:3], s, 1, True, True) is None
+    assert _host._gated_linear(a, w, None, s, 1, True, True) is not None
+    assert _host._gated_linear(a, w, None, s, 0, True, True) is None and _host._gated_linear(a, w, None, s, 1, False, True) is None
+    assert _host._gated_linear(a, w[:48], None, s[:48], 1, True, True) is None and _host._gated_linear(a, w, s[:3], s, 1, True, True) is None

@@ -98,3 +98,12 @@ def test_cpu_tensors_are_refused():
         rotary.apply_rotary(x.view(1, 4, 1, 64), None, None, rotary_frequencies(64)[0])
     with pytest.raises(Q8KernelError):
         gated.q8_gated_linear(x, torch.zeros(64, 64, dtype=torch.int8), None, None, torch.zeros(64))
+
+
+def test_native_path_looks_at_no_argument_of_a_call_with_a_wrong_number_of_them():
+    from q8_kernels_b200 import _host
+    for name, n in {"_layer_norm": 5, "_rotary": 6, "_gated_linear": 7}.items():
+        for k in range(n + 3):
+            if k != n:
+                assert getattr(_host, name)(*[None] * k) is None
+        assert getattr(_host, name)(*[torch.zeros(4, 64)] * n) is None
