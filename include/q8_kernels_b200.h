@@ -359,6 +359,15 @@ Q8K_API int q8k_rotary(const void* q, const int64_t q_strides[3], void* q_out, c
  * aligned.  No counterpart in the reference.                                                                                    */
 Q8K_API int q8k_gated_mm(int int8, const void* a, const void* w, const float* bias, const float* a_scales, const float* w_scales,
                  void* out, void* pre, int activation, int M, int F, int K, int* dev_status, void* stream);
+/* Which tiles such a call runs on the current device (148 SMs assumed without one), for tests and tuning: plan = {1 if CTA pairs with 256
+ * rows, else 0 (128 rows a CTA), output columns of a tile}.  Launches nothing; no counterpart in the reference.                  */
+Q8K_API int q8k_gated_plan(int M, int F, int K, int plan[2]);
+/* q8k_gated_quant and q8k_gated_mm in one call: x dense [M, K] (bf16 or e4m3), w int8 or e4m3, over a workspace of
+ * q8k_gated_linear_workspace_bytes (256-byte aligned).  No counterpart in the reference.                                        */
+Q8K_API size_t q8k_gated_linear_workspace_bytes(int M, int K);
+Q8K_API int q8k_gated_linear(const void* x, int x_dtype, const void* w, int w_dtype, const float* w_scales, const float* bias, void* out,
+                     void* pre, int activation, int M, int F, int K, int rotate, void* workspace, size_t workspace_bytes,
+                     int* dev_status, void* stream);
 /* Its activation: rows of x (bf16 or e4m3), rotated (Hadamard, 1/sqrt(dim), rounded to x's type) or not, quantised per token to int8 or
  * e4m3 as q8k_hadamard_quant and q8k_tokenwise_quant do it, but with the factor top * (1 / absmax) of two roundings in the place
  * of top / absmax.  dim a multiple of 16.  No counterpart in the reference.                                                     */

@@ -90,6 +90,9 @@ SIGNATURES = {
     "q8k_rotary": (_c_int, [_c_ptr] * 4 + [_c_int] + [_c_ptr] * 4 + [_c_int, _c_int, _c_ptr, _c_int, _c_i64, _c_i64, _c_ptr, _c_f32]
                    + [_c_int] * 6 + [_c_ptr]),
     "q8k_gated_mm": (_c_int, [_c_int] + [_c_ptr] * 7 + [_c_int] * 4 + [_c_ptr, _c_ptr]),
+    "q8k_gated_plan": (_c_int, [_c_int] * 3 + [_c_ptr]),
+    "q8k_gated_linear_workspace_bytes": (_c_size, [_c_int, _c_int]),
+    "q8k_gated_linear": (_c_int, [_c_ptr, _c_int, _c_ptr, _c_int] + [_c_ptr] * 4 + [_c_int] * 5 + [_c_ptr, _c_size, _c_ptr, _c_ptr]),
     "q8k_gated_quant": (_c_int, [_c_ptr, _c_int, _c_i64, _c_ptr, _c_int, _c_ptr, _c_i64, _c_int, _c_int, _c_ptr]),
     "q8k_gated_weight_operand_workspace_bytes": (_c_size, [_c_int, _c_int]),
     "q8k_gated_weight_operand": (_c_int, [_c_ptr, _c_int] + [_c_ptr] * 3 + [_c_int, _c_int, _c_ptr, _c_size, _c_ptr]),

@@ -42,6 +42,11 @@ int tokenwise_quant_as(const char* op, bool two_step, const void* x, int x_dtype
 int hadamard_quant_as(const char* op, bool two_step, const void* x, int x_dtype, void* q, int q_dtype, float* scales, int64_t rows, int dim,
                       int64_t x_row_stride, float scale, cudaStream_t st);
 
+// q8k_gated_mm under another name.  weight_ready: the weight was complete when the kernel before this one began its work, so its loads
+// need not wait for that kernel.
+int gated_mm(const char* op, bool weight_ready, int int8, const void* a, const void* w, const float* bias, const float* a_scales,
+             const float* w_scales, void* out, void* pre, int activation, int M, int F, int K, int* dev_status, void* stream);
+
 int gemm_num_sms();                          // SMs of the current device (148 if it cannot be asked)
 
 // Raise a kernel's dynamic shared memory limit, once per device (the call costs about 1 us, a launch 2.5).  The setting

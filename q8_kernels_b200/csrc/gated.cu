@@ -335,3 +335,33 @@ extern "C" int q8k_gated_quant(const void* x, int x_dtype, int64_t x_row_stride,
     return rotate ? hadamard_quant_as(op, true, x, x_dtype, q, q_dtype, scales, rows, dim, x_row_stride, 1.0f / sqrtf((float)dim), st)
                   : tokenwise_quant_as(op, true, x, x_dtype, q, q_dtype, scales, rows, dim, x_row_stride, st);
 }
+
+extern "C" size_t q8k_gated_linear_workspace_bytes(int M, int K) {
+    if (M <= 0 || K <= 0) return 0;
+    return ((size_t)M * (size_t)K + 255) / 256 * 256 + (size_t)M * sizeof(float);
+}
+
+extern "C" int q8k_gated_linear(const void* x, int x_dtype, const void* w, int w_dtype, const float* w_scales, const float* bias, void* out,
+                                void* pre, int activation, int M, int F, int K, int rotate, void* workspace, size_t workspace_bytes,
+                                int* dev_status, void* stream) {
+    using namespace q8k;
+    const char* op = "gated_linear";
+    Q8K_REQUIRE(M >= 0 && F > 0 && K > 0 && F % 16 == 0 && K % 16 == 0, Q8K_ERR_INVALID_ARG,
+                "%s: M=%d must not be negative, F=%d and K=%d multiples of 16", op, M, F, K);
+    Q8K_REQUIRE(w_dtype == Q8K_DT_I8 || w_dtype == Q8K_DT_E4M3, Q8K_ERR_UNSUPPORTED, "%s: weight dtype %d is not int8 or e4m3", op, w_dtype);
+    Q8K_REQUIRE(x_dtype == Q8K_DT_BF16 || x_dtype == Q8K_DT_E4M3, Q8K_ERR_UNSUPPORTED, "%s: input dtype %d is not bf16 or e4m3", op, x_dtype);
+    Q8K_REQUIRE(activation == Q8K_ACT_SILU || activation == Q8K_ACT_GELU_TANH, Q8K_ERR_UNSUPPORTED, "%s: activation %d is unknown", op,
+                activation);
+    if (M == 0) return Q8K_OK;
+    Q8K_REQUIRE(x && w && w_scales && out && aligned16(w) && aligned16(out) && aligned16(pre), Q8K_ERR_INVALID_ARG,
+                "%s: null or misaligned pointer", op);
+    Q8K_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 256 == 0, Q8K_ERR_INVALID_ARG,
+                "%s: the workspace must be 256-byte aligned", op);
+    const size_t need = q8k_gated_linear_workspace_bytes(M, K);
+    Q8K_REQUIRE(workspace_bytes >= need, Q8K_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", op, workspace_bytes, need);
+    float* scales = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ((size_t)M * (size_t)K + 255) / 256 * 256);
+    if (int rc = q8k_gated_quant(x, x_dtype, K, workspace, w_dtype, scales, M, K, rotate, stream)) return rc;
+    // The quantizer waits for everything before it and only then lets its dependents start, or does so by ending: by the time the
+    // product may run, the weight is complete.
+    return gated_mm(op, true, w_dtype == Q8K_DT_I8, workspace, w, bias, scales, w_scales, out, pre, activation, M, F, K, dev_status, stream);
+}

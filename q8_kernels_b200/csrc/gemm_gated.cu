@@ -309,6 +309,220 @@ gemm_8bit_gated_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     }
 }
 
+// ------------------------------------------------------------------ few rows
+// With few rows the weight is all there is to move, and pair tiles leave half of the tensor cores' rows and, with 64 tiles for 8192
+// columns, a seventh of the SMs idle.  Here every CTA owns 128 rows x bn columns (bn a multiple of 8, chosen so that the tiles fill the
+// device once): the first bn rows of its B operand come from Wg, the last bn from Wu.  Of A only the rows that exist are loaded, into a
+// slot of their size, so that the ring holds most of a tile's weights at once; the MMA reads 128 rows from there all the same, which
+// brings whatever lies behind into accumulator rows that nobody looks at.
+//
+// With `early` the weight's first loads are issued before the wait for the kernel before this one, which quantises the activation.
+// The caller vouches that the weight was complete when that kernel began: it did not let this one start before its own wait.
+constexpr int kGatedFewMaxStages = 16;
+constexpr int kGatedFewMaxBN = 128;
+struct GatedFewTail {                        // behind the operand ring
+    static constexpr int kNumBars = 2 * kGatedFewMaxStages + 1;
+    static constexpr int kTmemPtrOffset = kNumBars * 8;
+    static constexpr int kAbortOffset = kTmemPtrOffset + 4;
+    static constexpr int kScaleOffset = (kAbortOffset + 4 + 15) & ~15;
+    static constexpr int kBiasOffset = kScaleOffset + 2 * kGatedFewMaxBN * 4;
+    static constexpr int kTotal = kBiasOffset + 2 * kGatedFewMaxBN * 4;
+};
+struct GatedFewParams {
+    const float* a_scales;
+    const float* b_scales;
+    const float* bias;
+    __nv_bfloat16* out;                      // [M, F]
+    __nv_bfloat16* pre;                      // [M, 2, F] or null
+    int* status;
+    int M, F, K;
+    int bn, n_tiles;
+    int stages, a_slot, stage_bytes, load_bytes;
+    int early;
+    uint32_t idesc;
+};
+
+template <int COLS> __device__ __forceinline__ void gated_few_tmem(bool alloc, uint32_t arg) {
+    if (alloc) ptx::tmem_alloc<COLS>(arg);
+    else ptx::tmem_dealloc<COLS>(arg);
+}
+__device__ __forceinline__ void gated_few_tmem_any(int bn, bool alloc, uint32_t arg) {   // whole warp, convergent
+    if (bn <= 16) gated_few_tmem<32>(alloc, arg);
+    else if (bn <= 32) gated_few_tmem<64>(alloc, arg);
+    else if (bn <= 64) gated_few_tmem<128>(alloc, arg);
+    else gated_few_tmem<256>(alloc, arg);
+}
+
+template <bool INT8, bool GELU>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+gemm_8bit_gated_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
+                           const __grid_constant__ GatedFewParams p) {
+    using L = GatedFewTail;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t smem_base = ptx::smem_u32(smem);
+    uint8_t* tail = smem + p.stages * p.stage_bytes;
+    const uint32_t bar_base = ptx::smem_u32(tail);
+    auto full_bar = [&](int s) { return bar_base + 8u * s; };
+    auto empty_bar = [&](int s) { return bar_base + 8u * (kGatedFewMaxStages + s); };
+    const uint32_t acc_bar = bar_base + 8u * (2 * kGatedFewMaxStages);
+    volatile uint32_t* tmem_ptr_smem = reinterpret_cast<volatile uint32_t*>(tail + L::kTmemPtrOffset);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + L::kAbortOffset);
+    float* scale_smem = reinterpret_cast<float*>(tail + L::kScaleOffset);
+    float* bias_smem = reinterpret_cast<float*>(tail + L::kBiasOffset);
+    __shared__ int prior_failure;
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int m0 = (int)(blockIdx.x / p.n_tiles) * kGemmBM;
+    const int n0 = (int)(blockIdx.x % p.n_tiles) * p.bn;
+    const int k_iters = (p.K + kGemmBK - 1) / kGemmBK;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; ++s) {
+            ptx::mbar_init(full_bar(s), 1);
+            ptx::mbar_init(empty_bar(s), 1);
+        }
+        ptx::mbar_init(acc_bar, 1);
+        *abort_flag = 0;
+        ptx::fence_barrier_init();
+        ptx::fence_proxy_async_smem();
+        ptx::prefetch_tensormap(&tmap_w);
+        ptx::prefetch_tensormap(&tmap_a);
+    }
+    if (warp == 1) {
+        gated_few_tmem_any(p.bn, true, ptx::smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)));
+        ptx::tmem_relinquish_alloc_permit();
+    }
+    ptx::tcgen05_fence_before_sync();
+    __syncthreads();
+    ptx::tcgen05_fence_after_sync();
+    const uint32_t tmem_base = *tmem_ptr_smem;
+    auto load_weight = [&](int s, int kb) {                    // (columns from F on: see gemm_8bit_gated_kernel; no store takes them)
+        const uint32_t dst = smem_base + s * p.stage_bytes + p.a_slot;
+        ptx::mbar_arrive_expect_tx(full_bar(s), (uint32_t)p.load_bytes);
+        ptx::tma_load_2d(dst, &tmap_w, full_bar(s), kb * kGemmBK, n0);
+        ptx::tma_load_2d(dst + p.bn * kGemmBK, &tmap_w, full_bar(s), kb * kGemmBK, p.F + n0);
+    };
+    const int ahead = p.early ? min(p.stages, k_iters) : 0;
+    if (warp == 0 && ahead > 0) {
+        if (ptx::elect_one()) {
+            for (int s = 0; s < ahead; ++s) load_weight(s, s);
+        }
+        __syncwarp();
+    }
+    pdl_wait();
+    if (threadIdx.x == 0) prior_failure = p.status != nullptr ? *reinterpret_cast<volatile int*>(p.status) : 0;
+    __syncthreads();
+    pdl_release();                                             // this CTA holds its TMEM: the next kernel may move in behind it
+    // A launch that follows a failed one on the same status word stores nothing (loads that are under way have to land).
+    bool ok = true;
+    const bool skip = prior_failure != 0;
+
+    const int quarter = warp & 3;
+    const int half = (warp - 2) >> 2;
+    if (warp == 0) {
+        if (ptx::elect_one()) {
+            int s = 0;
+            uint32_t ph = 1;                                   // empty_bar phase to wait for: the first round passes
+            for (int kb = 0; kb < k_iters; ++kb) {
+                if (kb >= ahead) {
+                    if (!ptx::mbar_wait(empty_bar(s), ph, abort_flag)) { ok = false; break; }
+                    load_weight(s, kb);
+                }
+                ptx::tma_load_2d(smem_base + s * p.stage_bytes, &tmap_a, full_bar(s), kb * kGemmBK, m0);
+                if (++s == p.stages) { s = 0; ph ^= 1u; }
+            }
+            if (!ok && p.status != nullptr) atomicExch(p.status, Q8K_STATUS_TIMEOUT | (32 << 8));
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (ptx::elect_one()) {
+            int s = 0;
+            uint32_t ph = 0;
+            for (int kb = 0; kb < k_iters; ++kb) {
+                if (!ptx::mbar_wait(full_bar(s), ph, abort_flag)) { ok = false; break; }
+                ptx::tcgen05_fence_after_sync();
+                const uint32_t a_addr = smem_base + s * p.stage_bytes;
+                const uint64_t a_desc = ptx::make_kmajor_desc(a_addr, 128);
+                const uint64_t b_desc = ptx::make_kmajor_desc(a_addr + p.a_slot, 128);
+#pragma unroll
+                for (int k = 0; k < kGemmBK / 32; ++k) {
+                    const uint32_t accumulate = (kb > 0 || k > 0) ? 1u : 0u;
+                    if constexpr (INT8) ptx::mma_i8(tmem_base, a_desc + 2 * k, b_desc + 2 * k, p.idesc, accumulate);
+                    else ptx::mma_f8f6f4(tmem_base, a_desc + 2 * k, b_desc + 2 * k, p.idesc, accumulate);
+                }
+                ptx::tcgen05_commit(empty_bar(s));
+                if (++s == p.stages) { s = 0; ph ^= 1u; }
+            }
+            if (ok) ptx::tcgen05_commit(acc_bar);
+            else if (p.status != nullptr) atomicExch(p.status, Q8K_STATUS_TIMEOUT | (33 << 8));
+        }
+        __syncwarp();
+    } else {
+        for (int c = (int)threadIdx.x - 64; c < 2 * p.bn; c += kGemmEpilogueThreads) {
+            const bool up = c >= p.bn;
+            const int n = n0 + (up ? c - p.bn : c);
+            const bool in = n < p.F;
+            const int at = up ? p.F + n : n;
+            scale_smem[c] = in ? p.b_scales[at] : 0.f;
+            bias_smem[c] = in && p.bias != nullptr ? p.bias[at] : 0.f;
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const int row = m0 + quarter * 32 + lane;
+        const bool row_ok = row < p.M && !skip;
+        const float sa = row < p.M ? p.a_scales[row] : 0.f;
+        const float2 sa2 = make_float2(sa, sa);
+        ok = ptx::mbar_wait(acc_bar, 0, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);                      // keep the warp convergent for tcgen05.ld
+        ptx::tcgen05_fence_after_sync();
+        if (!ok && p.status != nullptr && threadIdx.x == 64) atomicExch(p.status, Q8K_STATUS_TIMEOUT | (34 << 8));
+        if (ok && m0 + quarter * 32 < p.M) {                   // (warp-uniform)
+            const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16);
+            // groups of eight columns in turn: F % 16 == 0, so eight are all in or all out
+#pragma unroll 1
+            for (int c = half * 8; c < p.bn && n0 + c < p.F; c += 16) {
+                uint32_t rg[8], ru[8];
+                ptx::tmem_ld_32x32b_x8(t_row + c, rg);
+                ptx::tmem_ld_32x32b_x8(t_row + p.bn + c, ru);
+                ptx::tmem_wait_ld();
+                uint32_t wo[4], wg[4], wu[4];
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const float2 g = epilogue_pair<INT8, false>(rg[j], rg[j + 1], sa2, scale_smem + c + j, bias_smem + c + j);
+                    const float2 u = epilogue_pair<INT8, false>(ru[j], ru[j + 1], sa2, scale_smem + p.bn + c + j, bias_smem + p.bn + c + j);
+                    const __nv_bfloat162 o = __floats2bfloat162_rn(gated_act<GELU>(g.x) * u.x, gated_act<GELU>(g.y) * u.y);
+                    const __nv_bfloat162 g2 = __floats2bfloat162_rn(g.x, g.y), u2 = __floats2bfloat162_rn(u.x, u.y);
+                    wo[j / 2] = *reinterpret_cast<const uint32_t*>(&o);
+                    wg[j / 2] = *reinterpret_cast<const uint32_t*>(&g2);
+                    wu[j / 2] = *reinterpret_cast<const uint32_t*>(&u2);
+                }
+                if (row_ok) {
+                    *reinterpret_cast<uint4*>(p.out + (int64_t)row * p.F + n0 + c) = make_uint4(wo[0], wo[1], wo[2], wo[3]);
+                    if (p.pre != nullptr) {
+                        __nv_bfloat16* pr = p.pre + (int64_t)row * 2 * p.F + n0 + c;
+                        *reinterpret_cast<uint4*>(pr) = make_uint4(wg[0], wg[1], wg[2], wg[3]);
+                        *reinterpret_cast<uint4*>(pr + p.F) = make_uint4(wu[0], wu[1], wu[2], wu[3]);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+
+    if (threadIdx.x == 0 && *abort_flag != 0) {
+        // a wait was abandoned: give copies still in flight time to land before the CTA gives up its shared memory
+        const unsigned long long t0 = ptx::globaltimer_ns();
+        while (ptx::globaltimer_ns() - t0 < 50000ull) {}
+    }
+    ptx::tcgen05_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        ptx::tcgen05_fence_after_sync();
+        gated_few_tmem_any(p.bn, false, tmem_base);
+    }
+}
+
 // ------------------------------------------------------------------ host side
 template <bool INT8, bool GELU, bool SAVE>
 static int launch_gated_as(const CUtensorMap& ta, const CUtensorMap& tw, const CUtensorMap& to, const CUtensorMap& tp,
@@ -338,28 +552,75 @@ static int launch_gated_as(const CUtensorMap& ta, const CUtensorMap& tw, const C
     return Q8K_OK;
 }
 
-// Columns of a tile: those with the shortest estimate of whole rounds of tiles times the time of one, 0.165 us per 128-byte slab of K for
-// the issuing threads or 0.31 us at 256 columns of the product, and 1.5 us for what a tile costs besides.
-static int gated_columns(int M, int F, int K, int clusters) {
+// Which kernel and tiles: those with the shortest estimate.
+//   pair: whole rounds of tiles times 0.165 us per 128-byte slab of K for the issuing threads or 0.31 us at 256 columns of the
+//         product, and 1.5 us for what a tile costs besides
+struct GatedPlan { bool few; int bn; };
+static GatedPlan gated_plan(int M, int F, int K, int sms) {
     const double slabs = (K + kGemmBK - 1) / kGemmBK;
+    const int clusters = sms / 2;
     double best = 1e30;
-    int bn = kGatedBN;
+    GatedPlan plan = {false, kGatedBN};
     for (int c = kGatedBN; c >= 32; c -= 32) {
         const double tiles = (double)((M + 2 * kGemmBM - 1) / (2 * kGemmBM)) * ((F + c - 1) / c);
         const double rounds = (double)(int64_t)((tiles + clusters - 1) / clusters);
         const double slab = 0.31 * c / kGatedBN > 0.165 ? 0.31 * c / kGatedBN : 0.165;
         const double t = rounds * (slabs * slab + 1.5);
-        if (t < best) { best = t; bn = c; }
+        if (t < best) { best = t; plan.bn = c; }
     }
-    return bn;
+    if (M <= kGemmBM) {
+        plan.few = true;
+        plan.bn = (F + sms - 1) / sms;
+        plan.bn = (plan.bn + 7) / 8 * 8;
+        if (plan.bn < 16) plan.bn = 16;
+        if (plan.bn > kGatedFewMaxBN) plan.bn = kGatedFewMaxBN;
+    }
+    return plan;
 }
 
-}  // namespace q8k
+template <bool INT8, bool GELU>
+static int launch_gated_few(const void* a, const void* w, const GatedParams& g, void* out, void* pre, int bn, bool early, cudaStream_t st,
+                            const char* op) {
+    GatedFewParams p = {g.a_scales, g.b_scales, g.bias, (__nv_bfloat16*)out, (__nv_bfloat16*)pre, g.status, g.M, g.F, g.K};
+    const int a_rows = g.M >= kGemmBM ? kGemmBM : (g.M + 7) / 8 * 8;
+    p.bn = bn;
+    p.n_tiles = (g.F + bn - 1) / bn;
+    p.a_slot = a_rows * kGemmBK;
+    p.load_bytes = (a_rows + 2 * bn) * kGemmBK;
+    p.stage_bytes = (p.load_bytes + 1023) / 1024 * 1024;
+    const int k_iters = (g.K + kGemmBK - 1) / kGemmBK;
+    // the MMA of the last stage reads 16 KB from its slot of A on: the ring ends at least there
+    const int budget = 225 * 1024 - GatedFewTail::kTotal - kGemmBM * kGemmBK;
+    p.stages = budget / p.stage_bytes;
+    if (p.stages > kGatedFewMaxStages) p.stages = kGatedFewMaxStages;
+    if (p.stages > k_iters) p.stages = k_iters;
+    p.early = early ? 1 : 0;
+    p.idesc = INT8 ? ptx::make_idesc_s8(kGemmBM, 2 * bn) : ptx::make_idesc_e4m3(kGemmBM, 2 * bn);
+    CUtensorMap ta, tw;
+    {
+        const uint64_t dims[2] = {(uint64_t)g.K, (uint64_t)g.M};
+        const uint64_t strides[1] = {(uint64_t)g.K};
+        const uint32_t box[2] = {(uint32_t)kGemmBK, (uint32_t)a_rows};
+        if (int rc = make_byte_tensor_map(&ta, a, 2, dims, strides, box, 128, op)) return rc;
+    }
+    {
+        const uint64_t dims[2] = {(uint64_t)g.K, 2 * (uint64_t)g.F};
+        const uint64_t strides[1] = {(uint64_t)g.K};
+        const uint32_t box[2] = {(uint32_t)kGemmBK, (uint32_t)bn};
+        if (int rc = make_byte_tensor_map(&tw, w, 2, dims, strides, box, 128, op)) return rc;
+    }
+    auto kern = gemm_8bit_gated_few_kernel<INT8, GELU>;
+    static std::atomic<uint64_t> smem_done{0};
+    if (int rc = allow_dynamic_smem((const void*)kern, 226 * 1024, smem_done)) return rc;
+    const int smem = 1024 + p.stages * p.stage_bytes + GatedFewTail::kTotal + kGemmBM * kGemmBK;
+    const int64_t grid = (int64_t)((g.M + kGemmBM - 1) / kGemmBM) * p.n_tiles;
+    Q8K_REQUIRE(grid <= 0x7fffffffLL, Q8K_ERR_TOO_LARGE, "%s: too many tiles", op);
+    Q8K_CUDA_OK(launch_dependent(kern, (unsigned)grid, kGemmThreads, smem, st, 1, ta, tw, p));
+    return Q8K_OK;
+}
 
-extern "C" int q8k_gated_mm(int int8, const void* a, const void* w, const float* bias, const float* a_scales, const float* w_scales,
-                            void* out, void* pre, int activation, int M, int F, int K, int* dev_status, void* stream) {
-    using namespace q8k;
-    const char* op = "gated_mm";
+int gated_mm(const char* op, bool weight_ready, int int8, const void* a, const void* w, const float* bias, const float* a_scales,
+             const float* w_scales, void* out, void* pre, int activation, int M, int F, int K, int* dev_status, void* stream) {
     Q8K_REQUIRE(M >= 0 && F > 0 && K > 0, Q8K_ERR_INVALID_ARG, "%s: bad shape M=%d F=%d K=%d", op, M, F, K);
     Q8K_REQUIRE(F % 16 == 0 && K % 16 == 0, Q8K_ERR_INVALID_ARG, "%s: F=%d and K=%d must be multiples of 16", op, F, K);
     Q8K_REQUIRE(F <= 0x3fffffff && M <= 0x7fffffff - 2 * kGemmBM, Q8K_ERR_TOO_LARGE, "%s: M=%d or F=%d too large", op, M, F);
@@ -370,7 +631,16 @@ extern "C" int q8k_gated_mm(int int8, const void* a, const void* w, const float*
     Q8K_REQUIRE(aligned16(a) && aligned16(w) && aligned16(out) && aligned16(pre), Q8K_ERR_INVALID_ARG,
                 "%s: a, w, out and pre must be 16-byte aligned", op);
     GatedParams p = {a_scales, w_scales, bias, dev_status, M, F, K, 0, 0, 0};
-    p.bn = gated_columns(M, F, K, gemm_num_sms() / 2);
+    const GatedPlan plan = gated_plan(M, F, K, gemm_num_sms());
+    const bool gelu = activation == Q8K_ACT_GELU_TANH;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (plan.few) {
+        return int8 ? (gelu ? launch_gated_few<true, true>(a, w, p, out, pre, plan.bn, weight_ready, st, op)
+                            : launch_gated_few<true, false>(a, w, p, out, pre, plan.bn, weight_ready, st, op))
+                    : (gelu ? launch_gated_few<false, true>(a, w, p, out, pre, plan.bn, weight_ready, st, op)
+                            : launch_gated_few<false, false>(a, w, p, out, pre, plan.bn, weight_ready, st, op));
+    }
+    p.bn = plan.bn;
     p.n_tiles = (F + p.bn - 1) / p.bn;
     const int64_t total = (int64_t)((M + 2 * kGemmBM - 1) / (2 * kGemmBM)) * p.n_tiles;
     Q8K_REQUIRE(total <= 0x7fffffffLL, Q8K_ERR_TOO_LARGE, "%s: too many tiles", op);
@@ -401,10 +671,24 @@ extern "C" int q8k_gated_mm(int int8, const void* a, const void* w, const float*
         const uint32_t box[3] = {64, 1, 32};
         if (int rc = make_byte_tensor_map(&tp, pre, 3, dims, strides, box, 64, op)) return rc;
     }
-    cudaStream_t st = (cudaStream_t)stream;
-    const bool gelu = activation == Q8K_ACT_GELU_TANH;
 #define Q8K_GATED(I8, SV) (gelu ? launch_gated_as<I8, true, SV>(ta, tw, to, tp, p, st) : launch_gated_as<I8, false, SV>(ta, tw, to, tp, p, st))
     if (pre != nullptr) return int8 ? Q8K_GATED(true, true) : Q8K_GATED(false, true);
     return int8 ? Q8K_GATED(true, false) : Q8K_GATED(false, false);
 #undef Q8K_GATED
+}
+
+}  // namespace q8k
+
+extern "C" int q8k_gated_mm(int int8, const void* a, const void* w, const float* bias, const float* a_scales, const float* w_scales,
+                            void* out, void* pre, int activation, int M, int F, int K, int* dev_status, void* stream) {
+    return q8k::gated_mm("gated_mm", false, int8, a, w, bias, a_scales, w_scales, out, pre, activation, M, F, K, dev_status, stream);
+}
+
+extern "C" int q8k_gated_plan(int M, int F, int K, int plan[2]) {
+    using q8k::set_error_detail;
+    Q8K_REQUIRE(plan != nullptr && M > 0 && F > 0 && K > 0, Q8K_ERR_INVALID_ARG, "gated_plan: null plan or bad shape");
+    const q8k::GatedPlan p = q8k::gated_plan(M, F, K, q8k::gemm_num_sms());
+    plan[0] = p.few ? 0 : 1;
+    plan[1] = p.bn;
+    return Q8K_OK;
 }

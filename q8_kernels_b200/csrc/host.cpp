@@ -920,14 +920,12 @@ PyObject* _rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // ---- _gated_linear(a, b, bias | None, scale_b, activation code, int8, rotate)
 struct GatedNode : torch::autograd::Function<GatedNode> {
-    static at::Tensor run(const at::Tensor& a, const at::Tensor& b, const at::Tensor& bias, const at::Tensor& scale, int act, bool int8, bool rotate,
+    static at::Tensor run(const at::Tensor& a, const at::Tensor& b, const at::Tensor& bias, const at::Tensor& scale, int act, bool rotate,
                           at::Tensor* pre) {
         const int64_t k = b.size(1), f = b.size(0) / 2, m = a.numel() / k;
         at::DimVector shape(lead(a).begin(), lead(a).end());
-        // the quantised rows and, behind them, their scales: scratch of this call
-        const int64_t q_bytes = (m * k + 255) / 256 * 256;
-        at::Tensor q = empty_like_dtype({q_bytes + 4 * m}, a, Dt::Byte);
-        float* qs = reinterpret_cast<float*>(static_cast<uint8_t*>(q.data_ptr()) + q_bytes);
+        const int64_t bytes = (int64_t)q8k_gated_linear_workspace_bytes((int)m, (int)k);
+        at::Tensor work = empty_like_dtype({bytes}, a, Dt::Byte);
         shape.push_back(f);
         at::Tensor out = empty_like_dtype(shape, a, Dt::BFloat16);
         if (pre != nullptr) {
@@ -935,18 +933,16 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
             shape.push_back(f);
             *pre = empty_like_dtype(shape, a, Dt::BFloat16);
         }
-        void* st = stream_of(a);
-        must(q8k_gated_quant(a.const_data_ptr(), type_code(a.scalar_type()), k, q.data_ptr(), int8 ? Q8K_DT_I8 : Q8K_DT_E4M3, qs, m, (int)k, rotate,
-                             st), "gated_quant");
-        must(q8k_gated_mm(int8, q.const_data_ptr(), b.const_data_ptr(), fptr(defined(bias)), qs, scale.const_data_ptr<float>(), out.data_ptr(),
-                          pre != nullptr ? pre->data_ptr() : nullptr, act, (int)m, (int)f, (int)k, g_status[a.device().index()]->data_ptr<int>(),
-                          st), "gated_mm");
+        must(q8k_gated_linear(a.const_data_ptr(), type_code(a.scalar_type()), b.const_data_ptr(), type_code(b.scalar_type()),
+                              scale.const_data_ptr<float>(), fptr(defined(bias)), out.data_ptr(), pre != nullptr ? pre->data_ptr() : nullptr, act,
+                              (int)m, (int)f, (int)k, rotate, work.data_ptr(), (size_t)bytes, g_status[a.device().index()]->data_ptr<int>(),
+                              stream_of(a)), "gated_linear");
         return out;
     }
     static Variable forward(AutogradContext* ctx, const Variable& a, const Variable& b, const Maybe& bias, const Variable& scale, int64_t act,
-                            bool int8, bool rotate) {
+                            bool rotate) {
         at::Tensor pre;
-        Variable out = run(a, b, value(bias), scale, (int)act, int8, rotate, &pre);
+        Variable out = run(a, b, value(bias), scale, (int)act, rotate, &pre);
         ctx->save_for_backward({pre, b, scale});
         ctx->saved_data["act"] = act;
         ctx->saved_data["rotate"] = rotate;
@@ -955,7 +951,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
         const variable_list saved = ctx->get_saved_variables();
-        variable_list result(7);
+        variable_list result(6);
         if (!grads[0].defined()) return result;
         {
             at::NoGradGuard no_grad;
@@ -1016,8 +1012,8 @@ PyObject* _gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
         at::Tensor out;
         {
             WithoutGil unlocked;
-            out = training ? GatedNode::apply(*a, *b, maybe(bias), *scale, (int64_t)act, int8, rotate)
-                           : GatedNode::run(*a, *b, value(maybe(bias)), *scale, (int)act, int8, rotate, nullptr);
+            out = training ? GatedNode::apply(*a, *b, maybe(bias), *scale, (int64_t)act, rotate)
+                           : GatedNode::run(*a, *b, value(maybe(bias)), *scale, (int)act, rotate, nullptr);
         }
         return wrap(std::move(out));
     });
