@@ -552,9 +552,15 @@ static int launch_gated_as(const CUtensorMap& ta, const CUtensorMap& tw, const C
     return Q8K_OK;
 }
 
-// Which kernel and tiles: those with the shortest estimate.
-//   pair: whole rounds of tiles times 0.165 us per 128-byte slab of K for the issuing threads or 0.31 us at 256 columns of the
-//         product, and 1.5 us for what a tile costs besides
+// Which kernel and tiles: those with the shortest estimate (us).
+//   pair: 3.3, and for every round of tiles 1.5 and per 128-byte slab of K 0.165 for the issuing threads or 0.31 at 256 columns
+//         of the product
+//   few:  where its tiles fill the device at most once (or there are at most 128 rows): 3.3, the epilogue's 1.5e-4 bn^2, and the
+//         longer of the slabs, each 0.165 or its bytes at 140 GB/s of one SM's L2 port, and the weight at 5.5 TB/s
+// Measured, best tiles of either (pair against few, CUDA graphs, weights from HBM): M = 1, K = 2048, F = 8192 14.1 against 8.8;  M = 77,
+// K = 4096, F = 10240 23.5 against 16.9;  M = 128, K = 2048, F = 8192 11.7 against 9.5;  M = 129 11.8 against 12.4;  M = 512 16.4 against
+// 22.5;  K = F = 4096, M = 256 12.0 against 11.3, M = 384 15.7 against 13.6;  K = 2048, F = 5504, M = 300 13.4 against 12.0, M = 600 15.8
+// against 18.8;  K = 2048, F = 688, M = 1000 7.0 against 6.2;  K = 512, F = 1408, M = 1001 5.9 against 5.3, M = 2002 8.1 against 10.3.
 struct GatedPlan { bool few; int bn; };
 static GatedPlan gated_plan(int M, int F, int K, int sms) {
     const double slabs = (K + kGemmBK - 1) / kGemmBK;
@@ -565,15 +571,22 @@ static GatedPlan gated_plan(int M, int F, int K, int sms) {
         const double tiles = (double)((M + 2 * kGemmBM - 1) / (2 * kGemmBM)) * ((F + c - 1) / c);
         const double rounds = (double)(int64_t)((tiles + clusters - 1) / clusters);
         const double slab = 0.31 * c / kGatedBN > 0.165 ? 0.31 * c / kGatedBN : 0.165;
-        const double t = rounds * (slabs * slab + 1.5);
+        const double t = 3.3 + rounds * (slabs * slab + 1.5);
         if (t < best) { best = t; plan.bn = c; }
     }
-    if (M <= kGemmBM) {
+    // the narrowest tiles that fill the device once
+    const int64_t m_tiles = (M + kGemmBM - 1) / kGemmBM;
+    const int64_t per_row = sms / m_tiles;                     // tiles that 128 rows may have
+    int64_t bn = per_row == 0 ? kGatedFewMaxBN + 1 : ((F + per_row - 1) / per_row + 7) / 8 * 8;
+    if (bn < 16) bn = 16;
+    if (M <= kGemmBM && bn > kGatedFewMaxBN) bn = kGatedFewMaxBN;
+    if (bn > kGatedFewMaxBN) return plan;
+    const int a_rows = M >= kGemmBM ? kGemmBM : (M + 7) / 8 * 8;
+    const double bytes = (double)(a_rows + 2 * bn) * kGemmBK / 140e3;
+    const double stream = slabs * (bytes > 0.165 ? bytes : 0.165), weight = 2.0 * F * K / 5.5e6;
+    if (M <= kGemmBM || 3.3 + 1.5e-4 * bn * bn + (stream > weight ? stream : weight) < best) {
         plan.few = true;
-        plan.bn = (F + sms - 1) / sms;
-        plan.bn = (plan.bn + 7) / 8 * 8;
-        if (plan.bn < 16) plan.bn = 16;
-        if (plan.bn > kGatedFewMaxBN) plan.bn = kGatedFewMaxBN;
+        plan.bn = (int)bn;
     }
     return plan;
 }

@@ -107,3 +107,35 @@ def test_native_path_looks_at_no_argument_of_a_call_with_a_wrong_number_of_them(
             if k != n:
                 assert getattr(_host, name)(*[None] * k) is None
         assert getattr(_host, name)(*[torch.zeros(4, 64)] * n) is None
+
+
+def test_gated_plan():
+    """Rows of at most 128 take the 128-row tiles, many rows the pairs; tiles cover F and are of widths that the kernels take."""
+    import ctypes
+    lib = _lib.lib
+    plan = (ctypes.c_int * 2)()
+
+    def of(m, f, k):
+        assert lib.q8k_gated_plan(m, f, k, plan) == 0
+        return plan[0], plan[1]
+
+    for m in (1, 8, 77, 128, 129, 256, 257, 1000, 6144, 100000):
+        for f in (16, 48, 688, 1408, 5504, 8192, 10240, 16400, 40960):
+            for k in (16, 512, 2048, 8192):
+                pair, bn = of(m, f, k)
+                assert (bn % 32 == 0 and 32 <= bn <= 128) if pair else (bn % 8 == 0 and 16 <= bn <= 128)
+                assert not (m <= 128 and pair) and not (m >= 40000 and f >= 512 and not pair)
+                if not pair and m > 128:                        # one round of tiles
+                    assert -(-m // 128) * -(-f // bn) <= 148
+    assert of(1, 8192, 2048) == (0, 56) and of(6144, 8192, 2048) == (1, 128)
+    assert lib.q8k_gated_plan(0, 16, 16, plan) == -1 and lib.q8k_gated_plan(1, 16, 16, None) == -1
+    # the call that does both steps: its refusals
+    buf = (torch.zeros(4096, dtype=torch.uint8).data_ptr() + 255) // 256 * 256
+    need = lib.q8k_gated_linear_workspace_bytes(4, 64)
+    assert need >= 4 * 64 + 16 and lib.q8k_gated_linear_workspace_bytes(0, 64) == 0
+
+    def linear(x=buf, xt=_lib.DT_BF16, wt=_lib.DT_I8, act=1, m=4, f=32, k=64, work=buf, size=need):
+        return lib.q8k_gated_linear(x, xt, buf, wt, buf, None, buf, None, act, m, f, k, 1, work, size, None, None)
+
+    assert linear(x=None) == -1 and linear(xt=_lib.DT_F16) == -2 and linear(wt=_lib.DT_BF16) == -2 and linear(act=7) == -2 and linear(f=24) == -1
+    assert linear(k=40) == -1 and linear(work=None) == -1 and linear(work=buf + 16) == -1 and linear(size=need - 1) == -3 and linear(m=0) == 0
