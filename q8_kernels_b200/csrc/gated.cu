@@ -112,7 +112,7 @@ static int launch_gated_backward(const void* dout, const void* pre, void* q, flo
 //
 // Tiles of 128 columns, 16 per thread (one 16-byte load of a row), so a warp reads four rows of 128 bytes.
 constexpr int kWtCols = 128;
-constexpr int kWtMaxRows = 512;              // rows whose absmax one CTA takes
+constexpr int kWtMaxRows = 512;              // rows whose absmax one CTA takes, at most (multiples of 64)
 constexpr int kWtRows = 128;                 // rows of a tile that is quantised and turned
 constexpr int kWtThreads = 256;
 
@@ -138,13 +138,14 @@ template <typename Tw> __device__ __forceinline__ void wt_values(uint32_t w, flo
 
 template <typename Tw>
 __global__ void __launch_bounds__(kWtThreads)
-gated_weight_absmax_kernel(const Tw* __restrict__ w, const float* __restrict__ row_scales, float* __restrict__ part, int N, int K) {
+gated_weight_absmax_kernel(const Tw* __restrict__ w, const float* __restrict__ row_scales, float* __restrict__ part, int N, int K,
+                           int rows) {
     __shared__ float red[kWtThreads / 32][kWtCols];
     pdl_wait();
     pdl_release();
     const int cg = threadIdx.x & 7, rl = threadIdx.x >> 3;     // column group, row within a step of 32
     const int c0 = blockIdx.x * kWtCols + cg * 16;
-    const int r0 = blockIdx.y * kWtMaxRows;
+    const int r0 = blockIdx.y * rows, r_end = min(r0 + rows, N);
     float m[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) m[j] = 0.f;
@@ -153,7 +154,7 @@ gated_weight_absmax_kernel(const Tw* __restrict__ w, const float* __restrict__ r
 #pragma unroll 4
         for (int i = 0; i < kWtMaxRows / 64; ++i) {
             const int r = r0 + i * 64 + rl * 2;
-            const bool in = r < N;
+            const bool in = r < r_end;
             uint32_t xw[2][4];
             float s[2];
 #pragma unroll
@@ -236,14 +237,16 @@ gated_weight_quant_kernel(const Tw* __restrict__ w, const float* __restrict__ ro
     }
     pdl_wait();
     pdl_release();
-    if (threadIdx.x < kWtCols && cb + (int)threadIdx.x < K) mul[threadIdx.x] = factors[cb + threadIdx.x];
+    // column group g's k-th four factors lie at (8 k + g) * 4: the eight groups of a warp read 128 bytes in a row
+    if (threadIdx.x < kWtCols && cb + (int)threadIdx.x < K)
+        mul[(threadIdx.x & 15) / 4 * 32 + threadIdx.x / 16 * 4 + (threadIdx.x & 3)] = factors[cb + threadIdx.x];
     __syncthreads();
     if (cb + cg * 16 < K) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             float2 v[4][2];                                    // [row][pair of columns]
             const int c = cg * 16 + k * 4;
-            const float4 f = *reinterpret_cast<const float4*>(mul + c);
+            const float4 f = *reinterpret_cast<const float4*>(mul + k * 32 + cg * 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 wt_values<Tw>(k == 0 ? x[i].x : k == 1 ? x[i].y : k == 2 ? x[i].z : x[i].w, s[i], v[i]);
@@ -274,9 +277,13 @@ gated_weight_quant_kernel(const Tw* __restrict__ w, const float* __restrict__ ro
 template <typename Tw>
 static int launch_gated_weight(const void* w, const float* row_scales, void* q, float* scales, float* part, int N, int K, cudaStream_t st) {
     const unsigned cols = (unsigned)((K + kWtCols - 1) / kWtCols);
-    const int parts = (N + kWtMaxRows - 1) / kWtMaxRows;
+    // four CTAs an SM, all of one size: rows a CTA by that, in steps of 64
+    const unsigned want = (unsigned)(4 * gemm_num_sms()) / cols > 0 ? (unsigned)(4 * gemm_num_sms()) / cols : 1u;
+    int rows = (int)((N + want - 1) / want + 63) / 64 * 64;
+    if (rows > kWtMaxRows) rows = kWtMaxRows;
+    const int parts = (N + rows - 1) / rows;
     Q8K_CUDA_OK(launch_dependent(gated_weight_absmax_kernel<Tw>, dim3(cols, (unsigned)parts), kWtThreads, 0, st, 1, (const Tw*)w, row_scales,
-                                 part, N, K));
+                                 part, N, K, rows));
     float* factors = part + (int64_t)parts * K;
     Q8K_CUDA_OK(launch_dependent(gated_weight_factor_kernel, dim3((unsigned)((K + 31) / 32)), 32 * kWtFactorWarps, 0, st, 1, part, parts, factors,
                                  scales, K));
@@ -305,7 +312,7 @@ extern "C" int q8k_gated_backward_quant(const void* grad, const void* pre, void*
 
 extern "C" size_t q8k_gated_weight_operand_workspace_bytes(int F, int K) {
     if (F <= 0 || K <= 0) return 0;
-    return ((2 * (size_t)F + q8k::kWtMaxRows - 1) / q8k::kWtMaxRows + 1) * (size_t)K * sizeof(float);   // partial maxima, factors
+    return ((2 * (size_t)F + 63) / 64 + 1) * (size_t)K * sizeof(float);   // partial maxima of at least 64 rows, factors
 }
 
 extern "C" int q8k_gated_weight_operand(const void* w, int w_dtype, const float* w_scales, void* q, float* scales, int F, int K,
