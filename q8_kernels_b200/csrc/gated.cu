@@ -4,7 +4,8 @@
 //   dgate = dout * up * act'(gate),  dup = dout * act(gate)
 // which the FP8 GEMM takes as one row [dgate | dup] of 2F e4m3 values with one scale.  Bound by HBM: 2 bytes of dout and 4 of gate
 // and up are read per column, 2 bytes written; the 2F fp32 values of a row stay in registers between the absmax and the cast, so
-// nothing is rounded before it.
+// nothing is rounded before it.  CTAs walk over rows and have the next ones on their way to shared memory by cp.async, each thread
+// the pieces that it reads itself.
 
 #include <math.h>
 
@@ -16,91 +17,159 @@ namespace q8k {
 constexpr int kGatedItem = 8;
 constexpr int kGatedMaxF = 16384;
 
-// act(g) and its derivative, both from s = 1 / (1 + e^(-v)):  silu: v = g, act' = s (1 + g (1 - s));  tanh-GELU:
-// v = 2 sqrt(2/pi) (g + c g^3), act' = s + g s (1 - s) v'.  Where s (1 - s) is 0 the second term is, too, however large v' is.
-template <bool GELU> __device__ __forceinline__ void gated_act_grad(float g, float& act, float& grad) {
+// act(g) and its derivative of two adjacent columns, both from s = 1 / (1 + e^(-v)):  silu: v = g, act' = s + g s (1 - s);  tanh-GELU:
+// v = 2 sqrt(2/pi) (g + c g^3), act' = s + g s (1 - s) v'.  Where s (1 - s) is 0 the second term is, too, also where g^2 has overflowed.
+// Packed pairs: element by element the kernel issued 26 instructions a column, half of its slots.
+template <bool GELU> __device__ __forceinline__ void gated_act_grad(float2 g, float2& act, float2& grad) {
     constexpr float kLog2e = 1.4426950408889634f, kA = 2.0f * 0.7978845608028654f, kB = kA * 0.044715f;
-    const float gg = g * g;
-    const float v = GELU ? g * fmaf(kB, gg, kA) : g;
-    float e, s;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-kLog2e * v));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(e + 1.0f));
-    act = g * s;
-    const float slope = s * (1.0f - s);
-    grad = slope == 0.f ? s : fmaf(g * slope, GELU ? fmaf(3.0f * kB, gg, kA) : 1.0f, s);
+    auto pair = [](float v) { return make_float2(v, v); };
+    float2 gg, t;                                              // -v log2 e
+    if constexpr (GELU) {
+        gg = fmul2(g, g);
+        t = fmul2(g, ffma2(gg, pair(-kLog2e * kB), pair(-kLog2e * kA)));
+    } else {
+        t = fmul2(g, pair(-kLog2e));
+    }
+    float2 e, s;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+    e = fadd2(e, pair(1.0f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(e.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(e.y));
+    act = fmul2(g, s);
+    const float2 rest = fsub2(pair(1.0f), s);
+    float2 slope = fmul2(act, rest);                           // g s (1 - s)
+    if constexpr (GELU) {
+        const float2 dv = ffma2(gg, pair(3.0f * kB), pair(kA));
+        slope = fmul2(slope, dv);
+        slope.x = s.x == 0.f || rest.x == 0.f ? 0.f : slope.x;
+        slope.y = s.y == 0.f || rest.y == 0.f ? 0.f : slope.y;
+    }
+    grad = fadd2(s, slope);
 }
 
-template <bool GELU, int ITEMS, int T>
-__global__ void __launch_bounds__(T)
+__device__ __forceinline__ float2 bf16_pair(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+
+__device__ __forceinline__ void gated_copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// T threads of ITEMS groups of 8 columns, CTAS of them an SM, S rows in the ring (6 bytes a column each).
+template <int I, int TT, int C, int SS> struct GatedBackLayout { static constexpr int items = I, threads = TT, ctas = C, slots = SS; };
+
+template <bool GELU, typename L>
+__global__ void __launch_bounds__(L::threads, L::ctas)
 gated_backward_quant_kernel(const __nv_bfloat16* __restrict__ dout, const __nv_bfloat16* __restrict__ pre, uint8_t* __restrict__ q,
-                            float* __restrict__ scales, int F) {
-    __shared__ float red[T / 32];
+                            float* __restrict__ scales, int M, int F) {
+    constexpr int ITEMS = L::items, T = L::threads, S = L::slots;
+    extern __shared__ __align__(16) uint8_t gated_smem[];      // [S][dout | gate | up]
+    __shared__ float red[2][T / 32];
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(gated_smem);
+    const int slot_bytes = 6 * F;
+    auto fetch = [&](int row, int slot) {
+        if (row < M) {
+            const __nv_bfloat16* dr = dout + (int64_t)row * F;
+            const __nv_bfloat16* pr = pre + (int64_t)row * 2 * F;
+            const uint32_t dst = ring + slot * slot_bytes;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int e = (threadIdx.x + i * T) * kGatedItem;
+                if (e < F) {
+                    gated_copy16(dst + 2 * e, dr + e);
+                    gated_copy16(dst + 2 * F + 2 * e, pr + e);
+                    gated_copy16(dst + 4 * F + 2 * e, pr + F + e);
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     pdl_wait();
     pdl_release();
-    const int64_t row = blockIdx.x;
-    const __nv_bfloat16* dr = dout + row * F;
-    const __nv_bfloat16* pr = pre + row * 2 * F;
-    float dg[ITEMS][kGatedItem], du[ITEMS][kGatedItem];
-    float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        const int e = (threadIdx.x + i * T) * kGatedItem;
-        if (e < F) {
-            float d[kGatedItem];
-            load_vec<__nv_bfloat16, kGatedItem>(dr + e, d);
-            load_vec<__nv_bfloat16, kGatedItem>(pr + e, dg[i]);
-            load_vec<__nv_bfloat16, kGatedItem>(pr + F + e, du[i]);
+    for (int k = 0; k < S - 1; ++k) fetch(blockIdx.x + k * gridDim.x, k);
+    int slot = 0, turn = 0;
+    for (int row = blockIdx.x; row < M; row += gridDim.x, turn ^= 1) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+        const uint8_t* in = gated_smem + slot * slot_bytes;
+        float2 dg[ITEMS][kGatedItem / 2], du[ITEMS][kGatedItem / 2];
+        float amax = 0.f;
 #pragma unroll
-            for (int j = 0; j < kGatedItem; ++j) {
-                float act, grad;
-                gated_act_grad<GELU>(dg[i][j], act, grad);
-                dg[i][j] = d[j] * du[i][j] * grad;
-                du[i][j] = d[j] * act;
-                amax = fmaxf(amax, fmaxf(fabsf(dg[i][j]), fabsf(du[i][j])));
+        for (int i = 0; i < ITEMS; ++i) {
+            const int e = (threadIdx.x + i * T) * kGatedItem;
+            if (e < F) {
+                const uint4 d4 = *reinterpret_cast<const uint4*>(in + 2 * e);
+                const uint4 g4 = *reinterpret_cast<const uint4*>(in + 2 * F + 2 * e);
+                const uint4 u4 = *reinterpret_cast<const uint4*>(in + 4 * F + 2 * e);
+                const uint32_t dw[4] = {d4.x, d4.y, d4.z, d4.w}, gw[4] = {g4.x, g4.y, g4.z, g4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w};
+#pragma unroll
+                for (int k = 0; k < kGatedItem / 2; ++k) {
+                    const float2 d = bf16_pair(dw[k]);
+                    float2 act, grad;
+                    gated_act_grad<GELU>(bf16_pair(gw[k]), act, grad);
+                    dg[i][k] = fmul2(fmul2(d, bf16_pair(uw[k])), grad);
+                    du[i][k] = fmul2(d, act);
+                    asm("max.f32 %0, %0, %1, %2;" : "+f"(amax) : "f"(fabsf(dg[i][k].x)), "f"(fabsf(dg[i][k].y)));
+                    asm("max.f32 %0, %0, %1, %2;" : "+f"(amax) : "f"(fabsf(du[i][k].x)), "f"(fabsf(du[i][k].y)));
+                }
             }
         }
-    }
-    amax = warp_max(amax);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
-    __syncthreads();
-    amax = red[0];
+        fetch(row + (S - 1) * gridDim.x, slot == 0 ? S - 1 : slot - 1);       // into the slot that this thread read a row ago
+        if (++slot == S) slot = 0;
+        amax = warp_max(amax);
+        if ((threadIdx.x & 31) == 0) red[turn][threadIdx.x >> 5] = amax;
+        __syncthreads();                                       // (two arrays: the one before is not written until the next barrier)
+        amax = red[turn][0];
 #pragma unroll
-    for (int w = 1; w < T / 32; ++w) amax = fmaxf(amax, red[w]);
-    const float scale = quant_factor<true>(448.0f, amax);      // the saturating cast below: see tokenwise_quant_kernel
-    const float mul = amax == 0.f ? 0.f : scale;
-    uint8_t* qr = q + row * 2 * F;
+        for (int w = 1; w < T / 32; ++w) amax = fmaxf(amax, red[turn][w]);
+        const float scale = quant_factor<true>(448.0f, amax);  // the saturating cast below: see tokenwise_quant_kernel
+        const float mul = amax == 0.f ? 0.f : scale;
+        const float2 mul2 = make_float2(mul, mul);
+        uint8_t* qr = q + (int64_t)row * 2 * F;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        const int e = (threadIdx.x + i * T) * kGatedItem;
-        if (e < F) {
-            union { uint2 v; uint16_t h[4]; } a, b;
+        for (int i = 0; i < ITEMS; ++i) {
+            const int e = (threadIdx.x + i * T) * kGatedItem;
+            if (e < F) {
+                union { uint2 v; uint16_t h[4]; } a, b;
 #pragma unroll
-            for (int j = 0; j < kGatedItem; j += 2) {
-                a.h[j / 2] = float2_to_e4m3x2_sat(__fmul_rn(dg[i][j], mul), __fmul_rn(dg[i][j + 1], mul));
-                b.h[j / 2] = float2_to_e4m3x2_sat(__fmul_rn(du[i][j], mul), __fmul_rn(du[i][j + 1], mul));
+                for (int k = 0; k < kGatedItem / 2; ++k) {
+                    const float2 x = fmul2(dg[i][k], mul2), y = fmul2(du[i][k], mul2);
+                    a.h[k] = float2_to_e4m3x2_sat(x.x, x.y);
+                    b.h[k] = float2_to_e4m3x2_sat(y.x, y.y);
+                }
+                *reinterpret_cast<uint2*>(qr + e) = a.v;
+                *reinterpret_cast<uint2*>(qr + F + e) = b.v;
             }
-            *reinterpret_cast<uint2*>(qr + e) = a.v;
-            *reinterpret_cast<uint2*>(qr + F + e) = b.v;
         }
+        if (threadIdx.x == 0) scales[row] = __fdiv_rn(1.0f, scale);
     }
-    if (threadIdx.x == 0) scales[row] = __fdiv_rn(1.0f, scale);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");       // (the copies behind the last row were empty)
+}
+
+template <bool GELU, typename L>
+static int launch_gated_backward_as(const void* dout, const void* pre, void* q, float* scales, int M, int F, cudaStream_t st) {
+    auto kern = gated_backward_quant_kernel<GELU, L>;
+    constexpr int most = L::slots * 6 * L::items * L::threads * kGatedItem;
+    static_assert(most * L::ctas <= 224 * 1024, "gated backward ring");
+    if (most > 40 * 1024) {
+        static std::atomic<uint64_t> smem_done{0};
+        if (int rc = allow_dynamic_smem((const void*)kern, most, smem_done)) return rc;
+    }
+    const int ctas = gemm_num_sms() * L::ctas;
+    Q8K_CUDA_OK(launch_dependent(kern, (unsigned)(M < ctas ? M : ctas), L::threads, L::slots * 6 * F, st, 1, (const __nv_bfloat16*)dout,
+                                 (const __nv_bfloat16*)pre, (uint8_t*)q, scales, M, F));
+    return Q8K_OK;
 }
 
 template <bool GELU>
 static int launch_gated_backward(const void* dout, const void* pre, void* q, float* scales, int M, int F, cudaStream_t st) {
     const int items = F / kGatedItem;
-#define Q8K_GB(ITEMS, T)                                                                                                      \
-    do {                                                                                                                      \
-        Q8K_CUDA_OK(launch_dependent(gated_backward_quant_kernel<GELU, ITEMS, T>, (unsigned)M, T, 0, st, 1, (const __nv_bfloat16*)dout, \
-                                     (const __nv_bfloat16*)pre, (uint8_t*)q, scales, F));                                     \
-        return Q8K_OK;                                                                                                        \
-    } while (0)
-    if (items <= 64) Q8K_GB(1, 64);
-    if (items <= 128) Q8K_GB(1, 128);
-    if (items <= 256) Q8K_GB(1, 256);
-    if (items <= 512) Q8K_GB(2, 256);
-    if (items <= 1024) Q8K_GB(4, 256);
-    Q8K_GB(4, 512);
+#define Q8K_GB(...) return launch_gated_backward_as<GELU, GatedBackLayout<__VA_ARGS__>>(dout, pre, q, scales, M, F, st)
+    if (items <= 64) Q8K_GB(1, 64, 16, 4);
+    if (items <= 128) Q8K_GB(1, 128, 8, 4);
+    if (items <= 256) Q8K_GB(1, 256, 4, 4);
+    if (items <= 512) Q8K_GB(2, 256, 3, 3);
+    if (items <= 1024) Q8K_GB(4, 256, 2, 2);
+    Q8K_GB(4, 512, 1, 2);
 #undef Q8K_GB
 }
 
@@ -300,6 +369,7 @@ extern "C" int q8k_gated_backward_quant(const void* grad, const void* pre, void*
     const char* op = "gated_backward_quant";
     Q8K_REQUIRE(M >= 0 && F > 0 && F % 16 == 0, Q8K_ERR_INVALID_ARG, "%s: M=%d must not be negative and F=%d a multiple of 16", op, M, F);
     Q8K_REQUIRE(F <= kGatedMaxF, Q8K_ERR_UNSUPPORTED, "%s: F=%d exceeds %d", op, F, kGatedMaxF);
+    Q8K_REQUIRE(M <= 0x7fff0000, Q8K_ERR_TOO_LARGE, "%s: M=%d too large", op, M);
     Q8K_REQUIRE(activation == Q8K_ACT_SILU || activation == Q8K_ACT_GELU_TANH, Q8K_ERR_UNSUPPORTED, "%s: activation %d is unknown", op,
                 activation);
     if (M == 0) return Q8K_OK;
