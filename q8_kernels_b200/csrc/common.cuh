@@ -47,6 +47,11 @@ int hadamard_quant_as(const char* op, bool two_step, const void* x, int x_dtype,
 int gated_mm(const char* op, bool weight_ready, int int8, const void* a, const void* w, const float* bias, const float* a_scales,
              const float* w_scales, void* out, void* pre, int activation, int M, int F, int K, int* dev_status, void* stream);
 
+// The product of so few rows, as gated_fused_rows allows, that the kernel rotates and quantises them itself.
+bool gated_fused_rows(int M, int K);
+int gated_mm_fused(const char* op, bool int8, const void* x, bool rotate, const void* w, const float* bias, const float* w_scales, void* out,
+                   void* pre, int activation, int M, int F, int K, int* dev_status, void* stream);
+
 int gemm_num_sms();                          // SMs of the current device (148 if it cannot be asked)
 
 // Raise a kernel's dynamic shared memory limit, once per device (the call costs about 1 us, a launch 2.5).  The setting

@@ -436,6 +436,8 @@ extern "C" int q8k_gated_linear(const void* x, int x_dtype, const void* w, int w
                 "%s: the workspace must be 256-byte aligned", op);
     const size_t need = q8k_gated_linear_workspace_bytes(M, K);
     Q8K_REQUIRE(workspace_bytes >= need, Q8K_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", op, workspace_bytes, need);
+    if (x_dtype == Q8K_DT_BF16 && aligned16(x) && gated_fused_rows(M, K))
+        return gated_mm_fused(op, w_dtype == Q8K_DT_I8, x, rotate != 0, w, bias, w_scales, out, pre, activation, M, F, K, dev_status, stream);
     float* scales = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ((size_t)M * (size_t)K + 255) / 256 * 256);
     if (int rc = q8k_gated_quant(x, x_dtype, K, workspace, w_dtype, scales, M, K, rotate, stream)) return rc;
     // The quantizer waits for everything before it and only then lets its dependents start, or does so by ending: by the time the
