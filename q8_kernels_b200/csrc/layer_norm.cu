@@ -461,13 +461,14 @@ layer_norm_wgrad_kernel(const float* __restrict__ part, int parts, float* __rest
 }
 
 // ------------------------------------------------------------------ host side
-template <typename F> static int ln_layout(int dim, F&& f) {
+template <bool BACKWARD, typename F> static int ln_layout(int dim, F&& f) {
     const int items = (dim + kLnItem - 1) / kLnItem;
-    if (items <= 32) return f(LnLayout<1, 32, 8>());
-    if (items <= 64) return f(LnLayout<2, 32, 8>());
-    if (items <= 128) return f(LnLayout<2, 64, 4>());
-    if (items <= 256) return f(LnLayout<2, 128, 2>());
-    if (items <= 512) return f(LnLayout<2, 256, 1>());
+    constexpr int N = BACKWARD ? 2 : 1;      // CTAs of 512 threads leave half the sums behind that those of 256 do
+    if (items <= 32) return f(LnLayout<1, 32, 8 * N>());
+    if (items <= 64) return f(LnLayout<2, 32, 8 * N>());
+    if (items <= 128) return f(LnLayout<2, 64, 4 * N>());
+    if (items <= 256) return f(LnLayout<2, 128, 2 * N>());
+    if (items <= 512) return f(LnLayout<2, 256, N>());
     if (items <= 1024) return f(LnLayout<2, 512, 1>());
     return f(LnLayout<4, 512, 1>());
 }
@@ -476,7 +477,7 @@ template <typename F> static int ln_layout(int dim, F&& f) {
 // as much as two to four rows are, so it should have four rows a group, unless that leaves SMs idle (1001 x 1537 fp16, backward:
 // 10.5 us with a CTA for every row group).
 template <bool BACKWARD> static int ln_ctas(int64_t rows, int dim, bool sums) {
-    return ln_layout(dim, [&](auto l) {
+    return ln_layout<BACKWARD>(dim, [&](auto l) {
         using L = decltype(l);
         const int64_t most = (int64_t)gemm_num_sms() * (BACKWARD ? LnBackward<L>::ctas : LnForward<L>::ctas);
         int64_t need = (rows + L::rows - 1) / L::rows;
@@ -523,7 +524,7 @@ static int launch_ln_as(const void* x, int64_t x_stride, const float* w, const f
 template <typename Tx, typename Ty>
 static int launch_ln(const void* x, int64_t x_stride, const float* w, const float* b, void* y, float* mean, float* rstd, int64_t rows,
                      int dim, float eps, bool vec, cudaStream_t st) {
-    return ln_layout(dim, [&](auto l) {
+    return ln_layout<false>(dim, [&](auto l) {
         using L = decltype(l);
         return vec ? launch_ln_as<Tx, Ty, L, true>(x, x_stride, w, b, y, mean, rstd, rows, dim, eps, st)
                    : launch_ln_as<Tx, Ty, L, false>(x, x_stride, w, b, y, mean, rstd, rows, dim, eps, st);
@@ -553,7 +554,7 @@ static int launch_ln_backward_as(const void* x, int64_t x_stride, const void* g,
 template <typename Tx, typename Tg>
 static int launch_ln_backward(const void* x, int64_t x_stride, const void* g, const float* mean, const float* rstd, const float* w,
                               void* dx, float* part, int64_t rows, int dim, bool vec, cudaStream_t st) {
-    return ln_layout(dim, [&](auto l) {
+    return ln_layout<true>(dim, [&](auto l) {
         using L = decltype(l);
         if (part != nullptr) return vec ? launch_ln_backward_as<Tx, Tg, L, true, true>(x, x_stride, g, mean, rstd, w, dx, part, rows, dim, st)
                                         : launch_ln_backward_as<Tx, Tg, L, false, true>(x, x_stride, g, mean, rstd, w, dx, part, rows, dim, st);
