@@ -675,7 +675,7 @@ static int launch_gated_as(const CUtensorMap& ta, const CUtensorMap& tw, const C
         if (cudaOccupancyMaxActiveClusters(&most, kern, &cfg) != cudaSuccess) { cudaGetLastError(); most = 0; }
         max_clusters.store(most, std::memory_order_relaxed);
     }
-    Q8K_REQUIRE(most >= 1, Q8K_ERR_UNSUPPORTED, "gated_mm: this device cannot run pairs of CTAs with %d bytes of shared memory", L::kTotal);
+    if (most < 1) return Q8K_ERR_UNSUPPORTED;
     const int clusters = p.total_tiles < most ? p.total_tiles : most;
     Q8K_CUDA_OK(launch_dependent(kern, 2 * clusters, kGemmThreads, L::kTotal, st, 1, ta, tw, to, tp, p));
     return Q8K_OK;
@@ -814,12 +814,13 @@ int gated_mm(const char* op, bool weight_ready, int int8, const void* a, const v
     const GatedPlan plan = gated_plan(M, F, K, gemm_num_sms());
     const bool gelu = activation == Q8K_ACT_GELU_TANH;
     cudaStream_t st = (cudaStream_t)stream;
-    if (plan.few) {
-        return int8 ? (gelu ? launch_gated_few<true, true, false>(a, w, p, out, pre, plan.bn, weight_ready, nullptr, false, st, op)
-                            : launch_gated_few<true, false, false>(a, w, p, out, pre, plan.bn, weight_ready, nullptr, false, st, op))
-                    : (gelu ? launch_gated_few<false, true, false>(a, w, p, out, pre, plan.bn, weight_ready, nullptr, false, st, op)
-                            : launch_gated_few<false, false, false>(a, w, p, out, pre, plan.bn, weight_ready, nullptr, false, st, op));
-    }
+    auto few = [&](int bn) {
+        return int8 ? (gelu ? launch_gated_few<true, true, false>(a, w, p, out, pre, bn, weight_ready, nullptr, false, st, op)
+                            : launch_gated_few<true, false, false>(a, w, p, out, pre, bn, weight_ready, nullptr, false, st, op))
+                    : (gelu ? launch_gated_few<false, true, false>(a, w, p, out, pre, bn, weight_ready, nullptr, false, st, op)
+                            : launch_gated_few<false, false, false>(a, w, p, out, pre, bn, weight_ready, nullptr, false, st, op));
+    };
+    if (plan.few) return few(plan.bn);
     p.bn = plan.bn;
     p.n_tiles = (F + p.bn - 1) / p.bn;
     const int64_t total = (int64_t)((M + 2 * kGemmBM - 1) / (2 * kGemmBM)) * p.n_tiles;
@@ -852,9 +853,12 @@ int gated_mm(const char* op, bool weight_ready, int int8, const void* a, const v
         if (int rc = make_byte_tensor_map(&tp, pre, 3, dims, strides, box, 64, op)) return rc;
     }
 #define Q8K_GATED(I8, SV) (gelu ? launch_gated_as<I8, true, SV>(ta, tw, to, tp, p, st) : launch_gated_as<I8, false, SV>(ta, tw, to, tp, p, st))
-    if (pre != nullptr) return int8 ? Q8K_GATED(true, true) : Q8K_GATED(false, true);
-    return int8 ? Q8K_GATED(true, false) : Q8K_GATED(false, false);
+    int rc;
+    if (pre != nullptr) rc = int8 ? Q8K_GATED(true, true) : Q8K_GATED(false, true);
+    else rc = int8 ? Q8K_GATED(true, false) : Q8K_GATED(false, false);
 #undef Q8K_GATED
+    if (rc != Q8K_ERR_UNSUPPORTED) return rc;
+    return few(F < kGatedFewMaxBN ? (F + 7) / 8 * 8 : kGatedFewMaxBN);         // the device cannot co-schedule the pairs
 }
 
 }  // namespace q8k

@@ -802,7 +802,8 @@ PyObject* _layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     FAST_END
 }
 
-// ---- _rotary(q, k | None, positions | None, frequencies, amplitude, half)
+// ---- _rotary(q, k | None, positions | None, frequencies, amplitude, half): frequencies as float64, or their bits as int64, which is how
+// RotaryEmbedding holds them (a view as float64 would cost as much as the launch)
 struct RotaryNode : torch::autograd::Function<RotaryNode> {
     // q and k of [batch, seq, heads, dim], or without the batch; either may be undefined
     static variable_list run(const at::Tensor& q, const at::Tensor& k, const at::Tensor& pos, const at::Tensor& freq, double amplitude, bool half,
@@ -827,7 +828,7 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
         auto heads = [&](const at::Tensor& t) { return t.defined() ? (int)t.size(d - 2) : 0; };
         rc = q8k_rotary(cptr(defined(q)), stride[0][0], out[0].defined() ? out[0].data_ptr() : nullptr, stride[0][1], heads(q), cptr(defined(k)),
                         stride[1][0], out[1].defined() ? out[1].data_ptr() : nullptr, stride[1][1], heads(k), type_code(x.scalar_type()),
-                        cptr(defined(pos)), pos.defined() && pos.scalar_type() == Dt::Long, pb, pt, freq.const_data_ptr<double>(),
+                        cptr(defined(pos)), pos.defined() && pos.scalar_type() == Dt::Long, pb, pt, static_cast<const double*>(freq.const_data_ptr()),
                         (float)amplitude, (int)batch, (int)seq, (int)dim, (int)(2 * freq.numel()), half, backward, stream_of(x));
         return out;
     }
@@ -871,13 +872,13 @@ PyObject* _rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor* q = c.tensor(0, true);
     const at::Tensor* k = c.ok && args[1] != Py_None ? c.tensor(1, true) : nullptr;
     const at::Tensor* pos = c.ok && args[2] != Py_None ? c.tensor(2, true) : nullptr;
-    const at::Tensor* freq = c.tensor(3, Dt::Double);
+    const at::Tensor* freq = c.tensor(3);
     const float amplitude = c.real(4);
     const bool half = c.flag(5);
     OR_NONE(c);
     const Dt t = q->scalar_type();
     const int64_t d = q->dim();
-    c.need((t == Dt::BFloat16 || t == Dt::Half || t == Dt::Float) && (d == 3 || d == 4) && q->stride(-1) == 1 && freq->dim() == 1);
+    c.need((freq->scalar_type() == Dt::Double || freq->scalar_type() == Dt::Long) && (t == Dt::BFloat16 || t == Dt::Half || t == Dt::Float) && (d == 3 || d == 4) && q->stride(-1) == 1 && freq->dim() == 1);
     OR_NONE(c);
     const int64_t batch = d == 4 ? q->size(0) : 1, seq = q->size(d - 3), dim = q->size(-1);
     c.need(int_sized(batch) && int_sized(seq) && dim <= 4096 && freq->numel() >= 1 && 2 * freq->numel() <= dim && q->size(d - 2) <= 65536);
@@ -956,7 +957,8 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
         {
             at::NoGradGuard no_grad;
             const at::Tensor &pre = saved[0], &b = saved[1], &scale = saved[2];
-            const at::Tensor g = grads[0].to(Dt::BFloat16).contiguous();
+            at::Tensor g = grads[0].to(Dt::BFloat16).contiguous();
+            if (reinterpret_cast<uintptr_t>(g.const_data_ptr()) % 16 != 0) g = g.clone();
             const int64_t k = b.size(1), n = b.size(0), f = n / 2, m = g.numel() / f;
             at::DimVector shape(lead(g).begin(), lead(g).end());
             shape.push_back(k);
@@ -999,7 +1001,8 @@ PyObject* _gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const long act = c.integer(4);
     const bool int8 = c.flag(5), rotate = c.flag(6);
     OR_NONE(c);
-    c.need((act == Q8K_ACT_SILU || act == Q8K_ACT_GELU_TANH) && (a->scalar_type() == Dt::BFloat16 || (int8 && a->scalar_type() == Dt::Float8_e4m3fn)) && has_rows(a) &&
+    auto aligned = [](const at::Tensor* t) { return reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 == 0; };
+    c.need(aligned(a) && aligned(b) && (act == Q8K_ACT_SILU || act == Q8K_ACT_GELU_TANH) && (a->scalar_type() == Dt::BFloat16 || (int8 && a->scalar_type() == Dt::Float8_e4m3fn)) && has_rows(a) &&
            b->scalar_type() == (int8 ? Dt::Char : Dt::Float8_e4m3fn) && b->dim() == 2 && b->size(1) == a->size(-1));
     OR_NONE(c);
     const int64_t k = b->size(1), nn = b->size(0), m = a->numel() / k;

@@ -45,7 +45,11 @@ class GatedLinear(nn.Module):
 
     @classmethod
     def from_linears(cls, gate: nn.Linear, up: nn.Linear, act: str = "silu", linear: str = "int8", use_hadamard: bool = True):
-        """Quantises the two 16-bit projections of a checkpoint, as Q8Linear / FP8Linear.from_linear do."""
+        """Quantises the two 16-bit projections of a checkpoint, as Q8Linear / FP8Linear.from_linear do.  With the rotation (int8 always)
+        their input must have a power of two of channels: only that many the Hadamard matrix leaves the products as they are."""
+        if (linear == "int8" or use_hadamard) and gate.in_features & (gate.in_features - 1):
+            raise ValueError(f"{gate.in_features} input channels are no power of two, which the rotation needs: use linear='fp8' with "
+                             "use_hadamard=False")
         if gate.weight.shape != up.weight.shape or (gate.bias is None) != (up.bias is None):
             raise ValueError("the gate and the up projection must have the same shape and both a bias or none")
         layer = cls(gate.in_features, gate.out_features, act, gate.bias is not None, linear, use_hadamard, gate.weight.device)

@@ -3,7 +3,7 @@ import torch
 import torch.nn as nn
 
 from .activations import GELU, GatedLinear
-from .linear import make_linear
+from .linear import FP8Linear, Q8Linear, make_linear
 
 
 class FeedForward(nn.Module):
@@ -19,13 +19,25 @@ class FeedForward(nn.Module):
 
 class GatedFeedForward(nn.Module):
     """``proj_down(act(gate(x)) * up(x))``, gate and up projection, activation and product in one kernel.  ``inner_dim`` columns between the
-    projections, a multiple of 16.  Trains as its linears do: the activation has a gradient.  No counterpart in the reference."""
+    projections, a multiple of 16.  ``linear="int8"`` rotates both activations, so both widths have to be powers of two; "fp8" rotates
+    the first if its width is one, and not the second, where FP8Linear has no gradient with a rotation.  Trains as its linears do: the
+    activation has a gradient.  No counterpart in the reference."""
 
     def __init__(self, dim: int, inner_dim: int, act: str = "silu", bias: bool = True, linear: str = "int8"):
         super().__init__()
         self.inner_dim = inner_dim
-        self.gate_up = GatedLinear(dim, inner_dim, act, bias=bias, linear=linear)
-        self.proj_down = make_linear(linear, inner_dim, dim, bias=bias)
+        if linear == "int8" and (dim & (dim - 1) or inner_dim & (inner_dim - 1)):
+            raise ValueError(f"int8 linears rotate their activations: {dim} and {inner_dim} have to be powers of two")
+        self.gate_up = GatedLinear(dim, inner_dim, act, bias=bias, linear=linear, use_hadamard=dim & (dim - 1) == 0)
+        self.proj_down = Q8Linear(inner_dim, dim, bias) if linear == "int8" else FP8Linear(inner_dim, dim, bias)
 
     def forward(self, x, out_dtype=torch.bfloat16):
         return self.proj_down(self.gate_up(x), out_dtype=out_dtype)
+
+    @classmethod
+    def from_linears(cls, gate: nn.Linear, up: nn.Linear, down: nn.Linear, act: str = "silu", linear: str = "int8"):
+        """Quantises the three 16-bit projections of a checkpoint."""
+        layer = cls(gate.in_features, gate.out_features, act, gate.bias is not None, linear)
+        layer.gate_up = GatedLinear.from_linears(gate, up, act, linear, layer.gate_up.use_hadamard)
+        layer.proj_down = Q8Linear.from_linear(down) if linear == "int8" else FP8Linear.from_linear(down)
+        return layer

@@ -4,6 +4,7 @@ from typing import Optional
 import torch
 import torch.nn as nn
 
+from .. import _host
 from .. import functional as Q8F
 from ..native import Q8KernelError
 
@@ -21,7 +22,7 @@ class RotaryEmbedding(nn.Module):
         frequencies, self.amplitude = Q8F.rotary.rotary_frequencies(rotary_dim, base, scaling)
         if rotary_dim > head_dim:
             raise Q8KernelError(f"RotaryEmbedding: rotary_dim {rotary_dim} exceeds the head dim {head_dim}")
-        self.head_dim, self.rotary_dim, self.layout = head_dim, rotary_dim, layout
+        self.head_dim, self.rotary_dim, self.layout, self._half = head_dim, rotary_dim, layout, layout == "half"
         # held as the bits of the 64-bit values: a module that is cast to another floating type must not round them
         self.register_buffer("_frequency_bits", frequencies.view(torch.int64).to(device), persistent=False)
 
@@ -32,4 +33,7 @@ class RotaryEmbedding(nn.Module):
     def forward(self, q, k=None, positions=None):
         if q.shape[-1] != self.head_dim:
             raise Q8KernelError(f"RotaryEmbedding: heads of {q.shape[-1]} channels, {self.head_dim} expected")
+        fast = _host._rotary(q, k, positions, self._frequency_bits, self.amplitude, self._half)
+        if fast is not None:
+            return fast
         return Q8F.rotary.apply_rotary(q, k, positions, self.frequencies, self.amplitude, self.layout)

@@ -724,6 +724,11 @@ def linear(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: Optio
 
 # ---------------------------------------------------------------- ops without a counterpart in the reference's modules
 
+def _aligned(x: torch.Tensor) -> torch.Tensor:
+    """x, or a copy of a dense x that does not begin on the 16 bytes that the gated projection's kernels need."""
+    return x.clone() if x.is_contiguous() and x.data_ptr() % 16 else x
+
+
 def _strided_rows(x: torch.Tensor):
     """(tensor, rows, dim, row stride) of [..., dim] for a kernel that takes rows at any alignment."""
     dim = x.shape[-1]
@@ -860,7 +865,7 @@ def gated_mm(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a_s
     if a.dtype != w.dtype or a.dtype not in (torch.int8, E4M3):
         raise Q8KernelError(f"gated_mm: {a.dtype} activation and {w.dtype} weight must be both int8 or both float8_e4m3fn")
     dev, f = gated_check(a, w, bias, a_scales, w_scales, act)
-    a, w, a_scales, w_scales = a.contiguous(), w.contiguous(), a_scales.contiguous(), w_scales.contiguous()
+    a, w, a_scales, w_scales = _aligned(a.contiguous()), _aligned(w.contiguous()), a_scales.contiguous(), w_scales.contiguous()
     bias = None if bias is None else bias.contiguous()
     out = torch.empty(a.shape[:-1] + (f,), dtype=torch.bfloat16, device=dev)
     pre = torch.empty(a.shape[:-1] + (2, f), dtype=torch.bfloat16, device=dev) if save else None
@@ -875,7 +880,7 @@ def gated_quant(x: torch.Tensor, rotate: bool, out_type: torch.dtype) -> List[to
     quantised per token to int8 or e4m3.  Returns ``[q, scales]``.  As hadamard_quant / tokenwise_quant, but the row's factor is
     ``top * (1 / absmax)``, two roundings, where those take ``top / absmax``."""
     dev = require_cuda(x)
-    x2, rows, dim, stride = _rows(x)
+    x2, rows, dim, stride = _rows(_aligned(x))
     q = torch.empty(x.shape, dtype=out_type, device=dev)
     scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
     launch(dev, "gated_quant", lib.q8k_gated_quant, ptr(x2), dt(x.dtype), stride, ptr(q), dt(out_type), ptr(scales), rows, dim, int(rotate))
@@ -889,7 +894,7 @@ def gated_weight_operand(w: torch.Tensor, w_scales: torch.Tensor) -> List[torch.
     if w.dim() != 2 or w.shape[0] % 32 or w_scales.dtype != torch.float32 or w_scales.numel() != w.shape[0]:
         raise Q8KernelError("gated_weight_operand: the weight must be [2F,K], F a multiple of 16, with float32 scales [2F]")
     n, k = w.shape
-    w, w_scales = w.contiguous(), w_scales.contiguous()
+    w, w_scales = _aligned(w.contiguous()), w_scales.contiguous()
     q = torch.empty((k, n), dtype=E4M3, device=dev)
     scales = torch.empty((k,), dtype=torch.float32, device=dev)
     work = torch.empty(lib.q8k_gated_weight_operand_workspace_bytes(n // 2, k), dtype=torch.uint8, device=dev)
@@ -908,7 +913,7 @@ def gated_backward_quant(grad: torch.Tensor, pre: torch.Tensor, act: str = "silu
             or tuple(pre.shape) != tuple(grad.shape[:-1]) + (2, grad.shape[-1]):
         raise Q8KernelError("gated_backward_quant: the gradient must be bfloat16 [...,F] and pre bfloat16 [...,2,F]")
     f = grad.shape[-1]
-    grad, pre = grad.contiguous(), pre.contiguous()
+    grad, pre = _aligned(grad.contiguous()), _aligned(pre.contiguous())
     q = torch.empty(grad.shape[:-1] + (2 * f,), dtype=E4M3, device=dev)
     scales = torch.empty(grad.shape[:-1], dtype=torch.float32, device=dev)
     launch(dev, "gated_backward_quant", lib.q8k_gated_backward_quant, ptr(grad), ptr(pre), ptr(q), ptr(scales), ACTIVATIONS[act],

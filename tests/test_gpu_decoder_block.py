@@ -8,7 +8,7 @@ BF16 = torch.bfloat16
 
 
 class Block(torch.nn.Module):
-    def __init__(self, dim=512, inner=1360, linear="int8"):
+    def __init__(self, dim=512, inner=1024, linear="int8"):
         super().__init__()
         from q8_kernels_b200.modules import GatedFeedForward, LayerNorm, RotaryEmbedding
         from q8_kernels_b200.modules.linear import make_linear
@@ -39,8 +39,8 @@ def filled(block, seed=0):
         if hasattr(m, "scales"):
             n, k = m.weight.shape
             w = (torch.randn(n, k, generator=g, device="cuda") * k ** -0.5).to(BF16)
-            p = 1 << (k - 1).bit_length()
-            m.weight.data, m.scales.data = native.hadamard_quant(w, k ** -0.5, m.weight.dtype)
+            p = k if getattr(m, "use_hadamard", True) else 0     # a rotated weight, or as it is
+            m.weight.data, m.scales.data = native.hadamard_quant(w, k ** -0.5, m.weight.dtype) if p else native.tokenwise_quant(w, m.weight.dtype)
             m.bias.data = 0.1 * torch.randn(n, generator=g, device="cuda")
             wide[name] = (m.weight.double() * m.scales.double().unsqueeze(1), m.bias.double(), p)
     for m in (block.norm1, block.norm2):
@@ -50,6 +50,8 @@ def filled(block, seed=0):
 
 
 def rotated(x, p):
+    if not p:
+        return x
     d = x.shape[-1]
     h = torch.ones(1, 1, dtype=torch.float64, device=x.device)
     while h.shape[0] < p:
@@ -87,7 +89,7 @@ def test_block(linear):
     """Rounding errors of a normalised row, each relative to its tensor: int8 rows of rotated, i.e. normal, values have steps of 4 sigma / 127,
     1 % rms; e4m3 rows at most 2^-4, 2.6 % rms; q, k, v and the probabilities e4m3.  Eight of them one after the other, added up
     as squares, in a sum with the residual: 8 % with e4m3 everywhere."""
-    block = Block(linear=linear)
+    block = Block(inner=1024 if linear == "int8" else 1360, linear=linear)
     wide = filled(block)
     x = torch.randn(2, 77, 512, device="cuda").to(BF16)
     positions = torch.stack([torch.arange(77, device="cuda"), torch.arange(77, device="cuda") + 900])

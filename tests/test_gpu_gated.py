@@ -273,31 +273,80 @@ def test_captured_and_on_another_stream():
     assert all(torch.equal(bits(a), bits(b)) for a, b in zip(out, fresh))
 
 
-@pytest.mark.parametrize("linear", ["int8", "fp8"])
-def test_modules(linear):
-    from q8_kernels_b200.functional import gated
+@pytest.mark.parametrize("linear,dim,inner", [("int8", 512, 256), ("fp8", 512, 256), ("fp8", 528, 272)])
+def test_modules(linear, dim, inner):
     from q8_kernels_b200.modules import GatedFeedForward, GatedLinear, FP8Linear, Q8Linear
-    gate, up = (torch.nn.Linear(512, 272).cuda().to(BF16) for _ in range(2))
-    m = GatedLinear.from_linears(gate, up, "gelu_tanh", linear)
-    assert set(m.state_dict()) == {"weight", "bias", "scales"} and m.weight.shape == (544, 512)
-    kind = Q8Linear if linear == "int8" else FP8Linear
-    one = kind.from_linear(gate) if linear == "int8" else kind.from_linear(gate, use_hadamard=True)
-    assert torch.equal(bits(m.weight.data[:272]), bits(one.weight.data)) and torch.equal(m.scales[:272], one.scales)
-    x = torch.randn(3, 40, 512, device="cuda").to(BF16)
-    # 8 bits of weights and activations: int8 rows of N(0,1) have steps of about 1 / 30 (0.3 / 30 rms of the value), e4m3 2^-4 at most
+    gate, up = (torch.nn.Linear(dim, inner).cuda().to(BF16) for _ in range(2))
+    down = torch.nn.Linear(inner, dim).cuda().to(BF16)
+    rotate = dim == 512
+    m = GatedLinear.from_linears(gate, up, "gelu_tanh", linear, rotate)
+    assert set(m.state_dict()) == {"weight", "bias", "scales"} and m.weight.shape == (2 * inner, dim)
+    one = Q8Linear.from_linear(gate) if linear == "int8" else FP8Linear.from_linear(gate, use_hadamard=rotate)
+    assert torch.equal(bits(m.weight.data[:inner]), bits(one.weight.data)) and torch.equal(m.scales[:inner], one.scales)
+    x = torch.randn(3, 40, dim, device="cuda").to(BF16)
+    # 8 bits of weights and activations: int8 rows of N(0,1) have steps of 4 sigma / 127, 1 % rms, e4m3 2.6 %; of both operands of gate and
+    # up, of the product and the last weight: at most six of them as squares, and as much again for the sums' cancellation
+    bound = 12 ** 0.5 * (0.01 if linear == "int8" else 0.026)
     ref = torch.nn.functional.gelu(gate(x).float(), approximate="tanh") * up(x).float()
     y = m(x)
-    assert ((y.float() - ref).norm() / ref.norm()).item() <= (0.05 if linear == "int8" else 4 * 2.0 ** -4)
-    ff = GatedFeedForward(512, 272, "gelu_tanh", linear=linear).cuda()
-    ff.gate_up.load_state_dict(m.state_dict())
-    down = torch.nn.Linear(272, 512).cuda().to(BF16)
-    ff.proj_down = kind.from_linear(down) if linear == "int8" else kind.from_linear(down, use_hadamard=False)
+    assert ((y.float() - ref).norm() / ref.norm()).item() <= bound
+    ff = GatedFeedForward.from_linears(gate, up, down, "gelu_tanh", linear)
     assert torch.equal(bits(ff(x)), bits(ff.proj_down(y, out_dtype=BF16)))
+    whole = ref @ down.weight.float().T + down.bias.float()
+    assert ((ff(x).view_as(whole).float() - whole).norm() / (whole - down.bias.float()).norm()).item() <= bound
+    other = GatedFeedForward(dim, inner, "gelu_tanh", linear=linear).cuda()
+    other.load_state_dict(ff.state_dict())
+    assert torch.equal(bits(other(x)), bits(ff(x)))
     x.requires_grad_(True)
     assert torch.autograd.grad(ff(x).float().sum(), [x])[0].shape == x.shape
-    for bad in (dict(act="relu"), dict(linear="int4")):
+
+
+def test_modules_refuse():
+    from q8_kernels_b200.modules import GatedFeedForward, GatedLinear
+    for bad in (lambda: GatedLinear(64, 64, act="relu"), lambda: GatedLinear(64, 64, linear="int4"), lambda: GatedFeedForward(64, 96),
+                lambda: GatedFeedForward(96, 64),
+                lambda: GatedLinear.from_linears(*(torch.nn.Linear(96, 64).cuda().to(BF16) for _ in range(2)), "silu", "int8"),
+                lambda: GatedLinear.from_linears(torch.nn.Linear(64, 64).cuda().to(BF16), torch.nn.Linear(64, 32).cuda().to(BF16))):
         with pytest.raises(ValueError):
-            GatedLinear(64, 64, **bad)
+            bad()
+
+
+def test_misaligned_tensors():
+    """Dense tensors that begin off the 16 bytes of the kernels' accesses."""
+    from q8_kernels_b200 import native
+    from q8_kernels_b200.functional import gated
+    for m in (5, 40):
+        x, w, ws, bias = inputs(m, 512, 64, I8, 8)
+
+        def off(t):
+            o = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape)
+            return o.copy_(t)
+
+        want = gated.q8_gated_linear(x, w, bias, None, ws)
+        leaf = off(x).requires_grad_(True)
+        y = gated.q8_gated_linear(leaf, off(w), off(bias), None, off(ws))
+        assert torch.equal(bits(y), bits(want))
+        q, qs = native.gated_quant(x, True, I8)
+        assert torch.equal(bits(gated.q8_gated_linear(off(q), off(w), bias, off(qs), ws)), bits(want))
+        y = gated.q8_gated_linear(leaf, w, bias, None, ws)
+        g = torch.randn(m, 64, device="cuda").to(BF16)
+        assert torch.equal(bits(torch.autograd.grad(y, [leaf], off(g), retain_graph=True)[0]), bits(torch.autograd.grad(y, [leaf], g)[0]))
+
+
+def test_under_checkpointing():
+    from torch.utils.checkpoint import checkpoint
+    from q8_kernels_b200.functional import gated, layer_norm
+    x, w, ws, bias = inputs(33, 512, 64, I8, 10)
+    nw = torch.ones(512, device="cuda", requires_grad=True)
+    x.requires_grad_(True)
+    g = torch.randn(33, 64, device="cuda").to(BF16)
+
+    def f(a):
+        return gated.q8_gated_linear(layer_norm.layer_norm(a, nw), w, bias, None, ws)
+
+    plain = torch.autograd.grad(f(x), [x, nw], g)
+    again = torch.autograd.grad(checkpoint(f, x, use_reentrant=False), [x, nw], g)
+    assert all(torch.equal(bits(a), bits(b)) for a, b in zip(plain, again))
 
 
 def test_refusals():
