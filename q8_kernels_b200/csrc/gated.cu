@@ -5,7 +5,7 @@
 // which the FP8 GEMM takes as one row [dgate | dup] of 2F e4m3 values with one scale.  Bound by HBM: 2 bytes of dout and 4 of gate
 // and up are read per column, 2 bytes written; the 2F fp32 values of a row stay in registers between the absmax and the cast, so
 // nothing is rounded before it.  CTAs walk over rows and have the next ones on their way to shared memory by cp.async, each thread
-// the pieces that it reads itself.
+// the pieces that it reads itself: 6144 x 8192 66 us, 0.93 of the copy rate (85 with a CTA for every row).
 
 #include <math.h>
 
@@ -177,7 +177,7 @@ static int launch_gated_backward(const void* dout, const void* pre, void* q, flo
 // scale per row of the result, i.e. per column of w.  Bound by HBM: w is read once and q written once; a column's absmax needs all
 // rows first, so there are two passes, the second of which finds w in L2, with a small kernel between them that makes the columns'
 // factors of the partial maxima (taken by each CTA of the second pass for itself, 64 dependent loads, they were most of its time:
-// 16384 x 2048 int8 40.9 us).
+// 16384 x 2048 int8 40.9 us).  Now 22.5 us, where w once in and q once out are 10.
 //
 // Tiles of 128 columns, 16 per thread (one 16-byte load of a row), so a warp reads four rows of 128 bytes.
 constexpr int kWtCols = 128;

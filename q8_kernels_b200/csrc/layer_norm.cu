@@ -7,7 +7,8 @@
 // make a CTA.  A row has to be complete before its first output, so what keeps HBM busy are the next rows: they come by cp.async into
 // a ring of S - 1 rows ahead in shared memory, where bytes on their way cost no registers.  What every thread does once a row (the
 // exchange of the sums, addresses) is some 70 instructions: with 8 elements a thread they held the forward pass at 0.6 of the copy
-// rate (24576 x 2048 bf16), whatever the number of rows on their way; arithmetic is on packed pairs for the same reason.
+// rate (24576 x 2048 bf16), whatever the number of rows on their way; arithmetic is on packed pairs for the same reason.  Now forward
+// 36.6 us (0.84 of the copy rate), backward with dw and db 54.9 (0.84), issue slots 64 % busy in both.
 //
 // The variance is taken from the differences to the mean, not E[x^2] - mean^2, which loses all digits of a row whose mean is large
 // against its spread.  Sums, statistics and the gradients of w and b are fp32.

@@ -5,7 +5,8 @@ The weight ``b`` [2F, K] holds the gate's rows first and the up projection's beh
 quantised as ``q8_linear`` and ``fp8_linear`` do it, but for the last bit of a row's factor (see native.gated_quant); where the bits of those
 are wanted, quantise with them and pass ``scale_a``.  As there, weights are frozen and the activation is what has a gradient: the
 gradient of [gate | up] is quantised per token and the de-quantised weight per input channel to e4m3, the FP8 GEMM
-multiplies them, and the result is rotated back where the forward pass rotated.
+multiplies them, and the result is rotated back where the forward pass rotated.  Both the product and the rotated result are rounded to
+bf16, as in q8_linear's backward pass: the transform takes 16-bit rows, and half a bf16 step is far below the e4m3 steps before it.
 """
 from typing import Optional
 
