@@ -665,9 +665,9 @@ PyObject* qk_norm_rope_prep_pair(PyObject*, PyObject* const* args, Py_ssize_t n)
 
 // ---------------------------------------------------------------- layer norm, rotary positions, gated projection
 // These are differentiable: where an input has a gradient the call leaves a node of torch's C++ autograd behind, whose backward pass
-// launches without the interpreter.  The underscore marks them: they answer for functions of functional/, not of native.py.  (A Python autograd.Function costs some 60 us of host time for one forward and backward pass, the
+// launches without the interpreter.  (A Python autograd.Function costs some 60 us of host time for one forward and backward pass, the
 // kernels of a short call 10.)  What functional.layer_norm.layer_norm, functional.rotary.apply_rotary and functional.gated do with tensors
-// that these do not take is the same.
+// that these do not take is the same.  The underscore marks them: they answer for functions of functional/, not of native.py.
 
 using torch::autograd::AutogradContext;
 using torch::autograd::Variable;
@@ -878,7 +878,8 @@ PyObject* _rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     OR_NONE(c);
     const Dt t = q->scalar_type();
     const int64_t d = q->dim();
-    c.need((freq->scalar_type() == Dt::Double || freq->scalar_type() == Dt::Long) && (t == Dt::BFloat16 || t == Dt::Half || t == Dt::Float) && (d == 3 || d == 4) && q->stride(-1) == 1 && freq->dim() == 1);
+    c.need((freq->scalar_type() == Dt::Double || freq->scalar_type() == Dt::Long) && (t == Dt::BFloat16 || t == Dt::Half || t == Dt::Float) &&
+           (d == 3 || d == 4) && q->stride(-1) == 1 && freq->dim() == 1);
     OR_NONE(c);
     const int64_t batch = d == 4 ? q->size(0) : 1, seq = q->size(d - 3), dim = q->size(-1);
     c.need(int_sized(batch) && int_sized(seq) && dim <= 4096 && freq->numel() >= 1 && 2 * freq->numel() <= dim && q->size(d - 2) <= 65536);
@@ -1002,8 +1003,8 @@ PyObject* _gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const bool int8 = c.flag(5), rotate = c.flag(6);
     OR_NONE(c);
     auto aligned = [](const at::Tensor* t) { return reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 == 0; };
-    c.need(aligned(a) && aligned(b) && (act == Q8K_ACT_SILU || act == Q8K_ACT_GELU_TANH) && (a->scalar_type() == Dt::BFloat16 || (int8 && a->scalar_type() == Dt::Float8_e4m3fn)) && has_rows(a) &&
-           b->scalar_type() == (int8 ? Dt::Char : Dt::Float8_e4m3fn) && b->dim() == 2 && b->size(1) == a->size(-1));
+    c.need(aligned(a) && aligned(b) && (act == Q8K_ACT_SILU || act == Q8K_ACT_GELU_TANH) &&
+           (a->scalar_type() == Dt::BFloat16 || (int8 && a->scalar_type() == Dt::Float8_e4m3fn)) && has_rows(a) && b->scalar_type() == (int8 ? Dt::Char : Dt::Float8_e4m3fn) && b->dim() == 2 && b->size(1) == a->size(-1));
     OR_NONE(c);
     const int64_t k = b->size(1), nn = b->size(0), m = a->numel() / k;
     const bool training = c10::GradMode::is_enabled() && a->requires_grad();

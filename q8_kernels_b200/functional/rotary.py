@@ -89,6 +89,8 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional
     2i with 2i + 1 ("interleaved").  Differentiable in q and k."""
     if layout not in LAYOUTS:
         raise Q8KernelError(f"apply_rotary: layout {layout!r} is not one of {', '.join(LAYOUTS)}")
+    if frequencies.dtype != torch.float64:                       # (_host takes int64 as the bits that RotaryEmbedding holds)
+        raise Q8KernelError(f"apply_rotary: frequencies must be float64 [rotary_dim / 2], not {frequencies.dtype}")
     amplitude, half = float(amplitude), layout == "half"
     fast = _host._rotary(q, k, positions, frequencies, amplitude, half)
     if fast is not None:

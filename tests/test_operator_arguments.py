@@ -139,3 +139,11 @@ def test_gated_plan():
 
     assert linear(x=None) == -1 and linear(xt=_lib.DT_F16) == -2 and linear(wt=_lib.DT_BF16) == -2 and linear(act=7) == -2 and linear(f=24) == -1
     assert linear(k=40) == -1 and linear(work=None) == -1 and linear(work=buf + 16) == -1 and linear(size=need - 1) == -3 and linear(m=0) == 0
+
+
+def test_whole_numbers_are_no_frequencies():
+    from q8_kernels_b200.functional import rotary
+    x = torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16)
+    for freq in (torch.ones(32, dtype=torch.int64), torch.ones(32)):
+        with pytest.raises(Q8KernelError, match="float64"):
+            rotary.apply_rotary(x, None, None, freq)
