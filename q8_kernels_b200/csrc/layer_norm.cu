@@ -3,12 +3,13 @@
 //   dx = rstd * (g w - mean(g w) - z mean(g w z)),  dw = sum_rows g z,  db = sum_rows g
 //
 // Both passes are bound by HBM: the forward reads x and writes y, the backward reads x and g and writes dx.  Groups of T threads walk
-// over rows, T so that a thread has 16 elements of a row, with w, b and the sums of dw and db in registers for all of them; G groups
-// make a CTA.  A row has to be complete before its first output, so what keeps HBM busy are the next rows: they come by cp.async into
-// a ring of S - 1 rows ahead in shared memory, where bytes on their way cost no registers.  What every thread does once a row (the
-// exchange of the sums, addresses) is some 70 instructions: with 8 elements a thread they held the forward pass at 0.6 of the copy
-// rate (24576 x 2048 bf16), whatever the number of rows on their way; arithmetic is on packed pairs for the same reason.  Now forward
-// 36.6 us (0.84 of the copy rate), backward with dw and db 54.9 (0.84), issue slots 64 % busy in both.
+// over rows, with w, b and the sums of dw and db in registers; G groups make a CTA.  A row has to be complete before its first output,
+// so what keeps HBM busy are the next rows: they come by cp.async into a ring of S - 1 rows ahead in shared memory, where bytes on
+// their way cost no registers.  What every thread does once a row (the exchange of the sums, addresses) is some 150 instructions, the
+// rest 5 to 8 an element, so a thread has many elements of a row: 24 or 32, which few warps with many registers each allow; arithmetic
+// is on packed pairs for the same reason.  24576 x 2048 bf16: forward 33.1 us (0.93 of the copy rate; with 16 elements a thread 36.5,
+// with 64, w and b from L1, 46 to 51), backward 47.0 (0.98), with dw and db 54.8;  16384 x 1536 16.8, 25.0, 33.4 (16 elements: 22.6,
+// 28.3, 38.3);  8192 x 1537 18.0, 19.7, 28.4 (20.2, 21.9, 29.8): single elements cost twice the instructions.
 //
 // The variance is taken from the differences to the mean, not E[x^2] - mean^2, which loses all digits of a row whose mean is large
 // against its spread.  Sums, statistics and the gradients of w and b are fp32.
@@ -128,21 +129,21 @@ template <typename E, bool VEC> __device__ __forceinline__ const E* ln_slot_row(
 
 // Threads of a CTA, CTAs an SM holds by registers, rows of the ring: as many as the SM's 227 KB leave for all of them, up to four.
 template <int I, int T, int G> struct LnLayout { static constexpr int items = I, threads = T, rows = G, cta = T * G; };
-// keep: what a thread needs twice stays in registers (w, b and the row's values); else it is read again, from L1 or from the ring, so
-// that two rows of more than 8192 columns fit an SM at a time (forward), or one with the sums of dw and db (backward).  The ring has
-// two rows then, which leaves L1 the room for w and b: with all that fit they came from L2, twice the bytes of the row itself.
+// keep: w and b (backward: also z and g w) stay in registers; else, for rows of more than 8192 columns, they are read again, from L1 or
+// from the ring, so that two such rows fit an SM at a time (forward), or one with the sums of dw and db (backward).  The ring has two
+// rows then, which leaves L1 the room for w and b: with all that fit they came from L2, twice the bytes of the row itself.
 template <typename L> struct LnForward {
-    static constexpr bool keep = L::items <= 2;
-    static constexpr int ctas = L::cta <= 256 ? 3 : keep ? 1 : 2;
+    static constexpr bool keep = L::items <= 4;                // w and b in registers
+    static constexpr int ctas = L::cta == 128 ? (L::items == 4 ? 3 : 4) : L::cta > 256 ? 1 : L::items <= 2 ? 3 : 2;
 };
 template <typename L> struct LnBackward {
-    static constexpr bool keep = L::items <= 2;
-    static constexpr int ctas = L::cta <= 256 ? 2 : 1;
+    static constexpr bool keep = L::items <= 2 || L::cta <= 256;
+    static constexpr int ctas = L::cta == 128 ? (L::items == 4 ? 3 : 4) : L::cta <= 256 && L::items <= 2 ? 2 : 1;
 };
 template <typename L, int CTAS, int BYTES> struct LnRing {
     static constexpr int row = L::rows * (L::threads * L::items * kLnItem * BYTES + 64);
     static constexpr int fit = 224 * 1024 / CTAS / row;
-    static constexpr int most = L::items <= 2 ? 4 : 2;
+    static constexpr int most = L::items <= 2 || (L::cta <= 256 && L::items <= 4) ? 4 : 2;
     static constexpr int slots = fit > most ? most : fit < 1 ? 1 : fit;
 };
 
@@ -219,23 +220,16 @@ layer_norm_kernel(const Tx* __restrict__ x, int64_t x_stride, const float* __res
         }
         if (!VEC) ln_group_sync<T, G>(group);                  // everyone's pieces have landed; the slot before has been read
         const Tx* xr = ln_slot_row<Tx, VEC>(ring + slot * slot_bytes, x + row * x_stride);
-        LnItem v[KEEP ? ITEMS : 1];
-        if constexpr (KEEP) {
+        LnItem v[ITEMS];
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i) v[i] = ln_load<Tx, T, VEC>(xr, dim, t, i);
-        }
-        auto value = [&](int i) -> const LnItem& {             // (a slot is not refilled before the next row)
-            if constexpr (!KEEP) v[0] = ln_load<Tx, T, VEC>(xr, dim, t, i);
-            return v[KEEP ? i : 0];
-        };
+        for (int i = 0; i < ITEMS; ++i) v[i] = ln_load<Tx, T, VEC>(xr, dim, t, i);
         if constexpr (S > 1) fetch(row + (S - 1) * step, slot == 0 ? S - 1 : slot - 1);
         if (++slot == S) slot = 0;
         float2 s2 = make_float2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            const LnItem& x8 = value(i);
 #pragma unroll
-            for (int k = 0; k < kLnItem / 2; ++k) s2 = fadd2(s2, x8.v[k]);
+            for (int k = 0; k < kLnItem / 2; ++k) s2 = fadd2(s2, v[i].v[k]);
         }
         const float s = warp_sum(s2.x + s2.y);
         float mean = s * (WARPS == 1 ? inv : own_inv);
@@ -243,10 +237,9 @@ layer_norm_kernel(const Tx* __restrict__ x, int64_t x_stride, const float* __res
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             if (!VEC || ln_has<T, VEC>(t, i, 0, dim)) {
-                const LnItem& x8 = value(i);
 #pragma unroll
                 for (int k = 0; k < kLnItem / 2; ++k) {
-                    float2 d = fsub2(x8.v[k], pair_of(mean));
+                    float2 d = fsub2(v[i].v[k], pair_of(mean));
                     if constexpr (!VEC) {
                         if (!ln_has<T, VEC>(t, i, 2 * k, dim)) d.x = 0.f;
                         if (!ln_has<T, VEC>(t, i, 2 * k + 1, dim)) d.y = 0.f;
@@ -268,11 +261,10 @@ layer_norm_kernel(const Tx* __restrict__ x, int64_t x_stride, const float* __res
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             if (!KEEP) { wv[0] = weight(i); bv[0] = bias(i); }
-            const LnItem& x8 = value(i);
             LnItem o;
 #pragma unroll
             for (int k = 0; k < kLnItem / 2; ++k)
-                o.v[k] = ffma2(fmul2(fsub2(x8.v[k], pair_of(mean)), pair_of(rstd)), wv[KEEP ? i : 0].v[k], bv[KEEP ? i : 0].v[k]);
+                o.v[k] = ffma2(fmul2(fsub2(v[i].v[k], pair_of(mean)), pair_of(rstd)), wv[KEEP ? i : 0].v[k], bv[KEEP ? i : 0].v[k]);
             ln_store<Ty, T, VEC>(y + row * (int64_t)dim, dim, t, i, o);
         }
         if (t == 0) {
@@ -462,32 +454,51 @@ layer_norm_wgrad_kernel(const float* __restrict__ part, int parts, float* __rest
 }
 
 // ------------------------------------------------------------------ host side
-template <bool BACKWARD, typename F> static int ln_layout(int dim, F&& f) {
+// Layouts.  fp32 rows have twice the bytes for the same instructions, and above 768 columns 16 elements a thread do better with them
+// (6144 x 2048: forward 17.7 us against 20.4 with 32, backward 24.7 against 29.7).
+enum : int { kLnForward, kLnDx, kLnSums };   // backward pass without and with dw and db
+template <int PASS, bool FP32, typename F> static int ln_layout(int dim, F&& f) {
     const int items = (dim + kLnItem - 1) / kLnItem;
-    constexpr int N = BACKWARD ? 2 : 1;      // CTAs of 512 threads leave half the sums behind that those of 256 do
-    if (items <= 32) return f(LnLayout<1, 32, 8 * N>());
-    if (items <= 64) return f(LnLayout<2, 32, 8 * N>());
-    if (items <= 128) return f(LnLayout<2, 64, 4 * N>());
-    if (items <= 256) return f(LnLayout<2, 128, 2 * N>());
-    if (items <= 512) return f(LnLayout<2, 256, N>());
-    if (items <= 1024) return f(LnLayout<2, 512, 1>());
-    return f(LnLayout<4, 512, 1>());
+    constexpr int B = PASS == kLnForward ? 1 : 2;
+    constexpr int S = PASS == kLnSums ? 2 : 1;                 // CTAs of twice the size leave half the sums behind
+    if (items <= 32) return f(LnLayout<1, 32, 8 * B>());
+    if (items <= 64) return f(LnLayout<2, 32, 8 * B>());
+    if (items <= 96) return f(LnLayout<3, 32, 4 * S>());
+    if constexpr (FP32) {
+        if (items <= 128) return f(LnLayout<2, 64, 4 * B>());
+        if (items <= 256) return f(LnLayout<2, 128, 2 * B>());
+        if (items <= 512) return f(LnLayout<2, 256, B>());
+    } else {
+        if (items <= 128) return f(LnLayout<4, 32, 4 * S>());
+        if (items <= 192) return f(LnLayout<3, 64, 2 * S>());
+        if (items <= 256) return f(LnLayout<4, 64, 2 * S>());
+        if (items <= 384) return f(LnLayout<3, 128, S>());
+        if (items <= 512) return f(LnLayout<4, 128, S>());
+    }
+    if constexpr (PASS == kLnForward) {
+        if (items <= 768) return f(LnLayout<3, 256, 1>());
+        if (items <= 1024) return f(LnLayout<2, 512, 1>());
+        return f(LnLayout<8, 256, 1>());
+    } else {
+        if (items <= 1024) return f(LnLayout<2, 512, 1>());
+        return f(LnLayout<4, 512, 1>());
+    }
 }
 
 // CTAs of a pass: as many as the device holds, or what the rows need.  With sums over rows a CTA leaves 8 dim bytes of them behind,
 // as much as two to four rows are, so it should have four rows a group, unless that leaves SMs idle (1001 x 1537 fp16, backward:
 // 10.5 us with a CTA for every row group).
-template <bool BACKWARD> static int ln_ctas(int64_t rows, int dim, bool sums) {
-    return ln_layout<BACKWARD>(dim, [&](auto l) {
-        using L = decltype(l);
-        const int64_t most = (int64_t)gemm_num_sms() * (BACKWARD ? LnBackward<L>::ctas : LnForward<L>::ctas);
-        int64_t need = (rows + L::rows - 1) / L::rows;
-        if (sums && need > gemm_num_sms()) {
-            const int64_t fewer = (need + 3) / 4;
-            need = fewer > gemm_num_sms() ? fewer : gemm_num_sms();
-        }
-        return (int)(need < most ? need : most);
-    });
+template <typename L> static int ln_grid(int64_t rows, int ctas, bool sums) {
+    const int64_t most = (int64_t)gemm_num_sms() * ctas;
+    int64_t need = (rows + L::rows - 1) / L::rows;
+    if (sums && need > gemm_num_sms()) {
+        const int64_t fewer = (need + 3) / 4;
+        need = fewer > gemm_num_sms() ? fewer : gemm_num_sms();
+    }
+    return (int)(need < most ? need : most);
+}
+template <bool FP32> static int ln_sums_ctas(int64_t rows, int dim) {
+    return ln_layout<kLnSums, FP32>(dim, [&](auto l) { return ln_grid<decltype(l)>(rows, LnBackward<decltype(l)>::ctas, true); });
 }
 
 // Bytes of a row in the ring.
@@ -517,7 +528,7 @@ static int launch_ln_as(const void* x, int64_t x_stride, const float* w, const f
         static std::atomic<uint64_t> smem_done{0};
         if (int rc = allow_dynamic_smem((const void*)kern, most, smem_done)) return rc;
     }
-    Q8K_CUDA_OK(launch_dependent(kern, (unsigned)ln_ctas<false>(rows, dim, false), L::cta, L::rows * S * slot, st, 1, (const Tx*)x, x_stride,
+    Q8K_CUDA_OK(launch_dependent(kern, (unsigned)ln_grid<L>(rows, LnForward<L>::ctas, false), L::cta, L::rows * S * slot, st, 1, (const Tx*)x, x_stride,
                                  w, b, (Ty*)y, mean, rstd, rows, dim, eps, slot));
     return Q8K_OK;
 }
@@ -525,11 +536,12 @@ static int launch_ln_as(const void* x, int64_t x_stride, const float* w, const f
 template <typename Tx, typename Ty>
 static int launch_ln(const void* x, int64_t x_stride, const float* w, const float* b, void* y, float* mean, float* rstd, int64_t rows,
                      int dim, float eps, bool vec, cudaStream_t st) {
-    return ln_layout<false>(dim, [&](auto l) {
+    auto launch = [&](auto l) {
         using L = decltype(l);
         return vec ? launch_ln_as<Tx, Ty, L, true>(x, x_stride, w, b, y, mean, rstd, rows, dim, eps, st)
                    : launch_ln_as<Tx, Ty, L, false>(x, x_stride, w, b, y, mean, rstd, rows, dim, eps, st);
-    });
+    };
+    return ln_layout<kLnForward, sizeof(Tx) == 4>(dim, launch);
 }
 
 template <typename Tx, typename Tg, typename L, bool VEC, bool WGRAD>
@@ -547,7 +559,7 @@ static int launch_ln_backward_as(const void* x, int64_t x_stride, const void* g,
         if (int rc = allow_dynamic_smem((const void*)kern, most, smem_done)) return rc;
     }
     const int bytes = L::rows * S * (x_slot + g_slot);
-    Q8K_CUDA_OK(launch_dependent(kern, (unsigned)ln_ctas<true>(rows, dim, WGRAD), L::cta, bytes > sums ? bytes : sums, st, 1, (const Tx*)x,
+    Q8K_CUDA_OK(launch_dependent(kern, (unsigned)ln_grid<L>(rows, LnBackward<L>::ctas, WGRAD), L::cta, bytes > sums ? bytes : sums, st, 1, (const Tx*)x,
                                  x_stride, (const Tg*)g, mean, rstd, w, (Tx*)dx, part, rows, dim, x_slot, g_slot));
     return Q8K_OK;
 }
@@ -555,10 +567,14 @@ static int launch_ln_backward_as(const void* x, int64_t x_stride, const void* g,
 template <typename Tx, typename Tg>
 static int launch_ln_backward(const void* x, int64_t x_stride, const void* g, const float* mean, const float* rstd, const float* w,
                               void* dx, float* part, int64_t rows, int dim, bool vec, cudaStream_t st) {
-    return ln_layout<true>(dim, [&](auto l) {
+    if (part != nullptr)
+        return ln_layout<kLnSums, sizeof(Tx) == 4>(dim, [&](auto l) {
+            using L = decltype(l);
+            return vec ? launch_ln_backward_as<Tx, Tg, L, true, true>(x, x_stride, g, mean, rstd, w, dx, part, rows, dim, st)
+                       : launch_ln_backward_as<Tx, Tg, L, false, true>(x, x_stride, g, mean, rstd, w, dx, part, rows, dim, st);
+        });
+    return ln_layout<kLnDx, sizeof(Tx) == 4>(dim, [&](auto l) {
         using L = decltype(l);
-        if (part != nullptr) return vec ? launch_ln_backward_as<Tx, Tg, L, true, true>(x, x_stride, g, mean, rstd, w, dx, part, rows, dim, st)
-                                        : launch_ln_backward_as<Tx, Tg, L, false, true>(x, x_stride, g, mean, rstd, w, dx, part, rows, dim, st);
         return vec ? launch_ln_backward_as<Tx, Tg, L, true, false>(x, x_stride, g, mean, rstd, w, dx, part, rows, dim, st)
                    : launch_ln_backward_as<Tx, Tg, L, false, false>(x, x_stride, g, mean, rstd, w, dx, part, rows, dim, st);
     });
@@ -595,7 +611,8 @@ extern "C" int q8k_layer_norm(const void* x, int x_dtype, int64_t x_row_stride, 
 
 extern "C" size_t q8k_layer_norm_backward_workspace_bytes(int64_t rows, int dim) {
     if (rows <= 0 || dim <= 0 || dim > kLnMaxDim) return 0;
-    return (size_t)ln_ctas<true>(rows, dim, true) * 2 * (size_t)dim * sizeof(float);
+    const int a = ln_sums_ctas<false>(rows, dim), b = ln_sums_ctas<true>(rows, dim);       // whatever x's type
+    return (size_t)(a > b ? a : b) * 2 * (size_t)dim * sizeof(float);
 }
 
 extern "C" int q8k_layer_norm_backward(const void* x, int x_dtype, int64_t x_row_stride, const void* grad, int grad_dtype,
@@ -637,6 +654,6 @@ extern "C" int q8k_layer_norm_backward(const void* x, int x_dtype, int64_t x_row
 #undef Q8K_LN_BWD
     if (rc != Q8K_OK || !sums) return rc;
     Q8K_CUDA_OK(launch_dependent(layer_norm_wgrad_kernel, (unsigned)((2 * (int64_t)dim + 31) / 32), 32 * kLnSumWarps, 0, st, 1, part,
-                                 ln_ctas<true>(rows, dim, true), dweight, dbias, dim));
+                                 x_dtype == Q8K_DT_F32 ? ln_sums_ctas<true>(rows, dim) : ln_sums_ctas<false>(rows, dim), dweight, dbias, dim));
     return Q8K_OK;
 }
