@@ -137,13 +137,13 @@ template <typename L> struct LnForward {
     static constexpr int ctas = L::cta == 128 ? (L::items == 4 ? 3 : 4) : L::cta > 256 ? 1 : L::items <= 2 ? 3 : 2;
 };
 template <typename L> struct LnBackward {
-    static constexpr bool keep = L::items <= 2 || L::cta <= 256;
+    static constexpr bool keep = L::items <= 2 || L::cta <= 384;
     static constexpr int ctas = L::cta == 128 ? (L::items == 4 ? 3 : 4) : L::cta <= 256 && L::items <= 2 ? 2 : 1;
 };
 template <typename L, int CTAS, int BYTES> struct LnRing {
     static constexpr int row = L::rows * (L::threads * L::items * kLnItem * BYTES + 64);
     static constexpr int fit = 224 * 1024 / CTAS / row;
-    static constexpr int most = L::items <= 2 || (L::cta <= 256 && L::items <= 4) ? 4 : 2;
+    static constexpr int most = L::items <= 2 || (L::cta <= 384 && L::items <= 4) ? 4 : 2;
     static constexpr int slots = fit > most ? most : fit < 1 ? 1 : fit;
 };
 
@@ -463,7 +463,7 @@ template <int PASS, bool FP32, typename F> static int ln_layout(int dim, F&& f) 
     constexpr int S = PASS == kLnSums ? 2 : 1;                 // CTAs of twice the size leave half the sums behind
     if (items <= 32) return f(LnLayout<1, 32, 8 * B>());
     if (items <= 64) return f(LnLayout<2, 32, 8 * B>());
-    if (items <= 96) return f(LnLayout<3, 32, 4 * S>());
+    if (items <= 96) return f(LnLayout<3, 32, PASS == kLnSums ? 12 : 4>());
     if constexpr (FP32) {
         if (items <= 128) return f(LnLayout<2, 64, 4 * B>());
         if (items <= 256) return f(LnLayout<2, 128, 2 * B>());
