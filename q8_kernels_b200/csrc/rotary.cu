@@ -11,10 +11,10 @@
 //
 // What is left to save are instructions: at the copy rate an SM has some 15 for an element.  So a thread takes the same channels of
 // up to eight heads of one token: its cosines and sines come from shared memory once, and its addresses advance by the head's stride.
-// CTAs of 128 threads, eight an SM: the chain from position to sine of one hides behind the stores of another, and the last ones to
-// finish are short.  Measured (bf16, CUDA graphs): 6144 tokens x 64 heads x 64 interleaved 17.5 us (0.88 of the copy rate), 16384 x 40 x
-// 128 half 61.8 us (0.83).  Tried: six CTAs without spills (17.9, 64.3), one head's loads at a time (19.8, 65.2), a thread for one
-// unit with the next token's elements on their way meanwhile (30.9, 103).
+// CTAs of 128 threads, eight an SM: the chain from position to sine hides behind the first loads and behind other CTAs' stores, and the
+// last ones to finish are short.  Measured (bf16, CUDA graphs): 6144 tokens x 64 heads x 64 interleaved 16.3 us (0.94 of the copy rate),
+// 16384 x 40 x 128 half 55.5 us (0.93).  Tried, when these took 17.5 and 61.6: six CTAs without spills (17.9, 64.3), one head's loads at a
+// time (19.8, 65.2), a thread for one unit with the next token's elements on their way meanwhile (30.9, 103).
 
 #include <type_traits>
 #include "common.cuh"
@@ -72,6 +72,34 @@ rotary_kernel(const __grid_constant__ RotaryParams p, const RotaryLanes l) {
     pdl_wait();
     pdl_release();
 
+    const int h0 = rest / l.unit_lanes;
+    const int rot_units = half_dim / PAIRS;
+    using Batch = Elems[AHEAD];
+    auto fetch = [](Batch& x, Batch& y, const T*& in, int64_t step, int n, int next, bool second) {
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            if (k < n) {
+                x[k].r = *reinterpret_cast<const Raw*>(in);
+                if (second) y[k].r = *reinterpret_cast<const Raw*>(in + next);
+                in += step;
+            }
+        }
+    };
+    auto left = [&](const RotaryTensor& a, int h) { return (a.heads - h + l.head_lanes - 1) / l.head_lanes; };
+    auto start_of = [&](const RotaryTensor& a, int h, int c) {
+        return static_cast<const T*>(a.in) + batch * a.in_batch + s * a.in_token + h * a.in_head + c;
+    };
+    // The first heads of q are on their way while the angles are made: 61.6 -> 55.5 and 17.5 -> 16.3 us; 6144 x 64 x 128 with 64 channels
+    // rotated 41.9 -> 36.5 half, 41.1 -> 33.1 interleaved.  (Behind: 6164 tokens, 6 heads of 192 in 4-byte accesses 12.4 -> 13.4.)
+    const int u0 = rest - h0 * l.unit_lanes;
+    Batch x, y;
+    const bool early = here && u0 < l.units && h0 < p.q.heads;
+    if (early) {
+        const bool copy = TWO && PART && u0 >= rot_units;
+        const int c = V == 1 && !p.half ? 2 * u0 : copy ? 2 * u0 * V : u0 * V;
+        const T* in = start_of(p.q, h0, c);
+        fetch(x, y, in, l.head_lanes * p.q.in_head, left(p.q, h0), copy ? V : p.half ? half_dim : 1, TWO && (!copy || c + V < p.head_dim));
+    }
     if (here) {                                                // a token's threads make its angles
         int64_t pos = s;
         if (p.positions != nullptr) {
@@ -88,31 +116,23 @@ rotary_kernel(const __grid_constant__ RotaryParams p, const RotaryLanes l) {
     __syncthreads();
     if (!here) return;
 
-    const int h0 = rest / l.unit_lanes;
-    const int rot_units = half_dim / PAIRS;
-    for (int u = rest - h0 * l.unit_lanes; u < l.units; u += l.unit_lanes) {
+    for (int u = u0; u < l.units; u += l.unit_lanes) {
         const bool copy = PART && u >= rot_units;
-        const int c = copy ? p.rotary_dim + (u - rot_units) * (TWO ? 2 * V : V) : V == 1 && !p.half ? 2 * u : u * V;
+        const int c = TWO && copy ? 2 * u * V : V == 1 && !p.half ? 2 * u : u * V;
         const int next = copy ? V : p.half ? half_dim : 1;     // from a unit's first run to its second
         const bool second = TWO && (!copy || c + V < p.head_dim);
         float2 w[PAIRS];
 #pragma unroll
         for (int j = 0; j < PAIRS; ++j) w[j] = copy ? make_float2(1.f, 0.f) : turns[tl * half_dim + u * PAIRS + j];
-        auto walk = [&](const RotaryTensor& a, int h) {        // heads h, h + head_lanes, ... of q or k
-            const T* in = static_cast<const T*>(a.in) + batch * a.in_batch + s * a.in_token + h * a.in_head + c;
+        auto walk = [&](const RotaryTensor& a, int h, bool there) {      // heads h, h + head_lanes, ... of q or k
+            const T* in = start_of(a, h, c);
             T* out = static_cast<T*>(a.out) + batch * a.out_batch + s * a.out_token + h * a.out_head + c;
             const int64_t in_step = l.head_lanes * a.in_head, out_step = l.head_lanes * a.out_head;
             while (h < a.heads) {
-                Elems x[AHEAD], y[AHEAD];
-                const int n = (a.heads - h + l.head_lanes - 1) / l.head_lanes;     // heads left
-#pragma unroll
-                for (int k = 0; k < AHEAD; ++k) {
-                    if (k < n) {
-                        x[k].r = *reinterpret_cast<const Raw*>(in);
-                        if (second) y[k].r = *reinterpret_cast<const Raw*>(in + next);
-                        in += in_step;
-                    }
-                }
+                const int n = left(a, h);                      // heads left
+                if (there) in += AHEAD * in_step;
+                else fetch(x, y, in, in_step, n, next, second);
+                there = false;
 #pragma unroll
                 for (int k = 0; k < AHEAD; ++k) {
                     if (k >= n) break;
@@ -135,8 +155,8 @@ rotary_kernel(const __grid_constant__ RotaryParams p, const RotaryLanes l) {
         };
         // heads of k go on where those of q end, so that every lane has as many
         const int after = p.q.heads > h0 ? (p.q.heads - h0 + l.head_lanes - 1) / l.head_lanes * l.head_lanes + h0 : h0;
-        walk(p.q, h0);
-        walk(p.k, after - p.q.heads);
+        walk(p.q, h0, early && u == u0);
+        walk(p.k, after - p.q.heads, false);
     }
 }
 
