@@ -252,3 +252,18 @@ def test_refusals():
                 lambda: layer_norm(torch.zeros(2, 16400, device="cuda")), lambda: layer_norm(x[:, :0]), lambda: layer_norm(x, w.view(1, 64), b)):
         with pytest.raises(Q8KernelError):
             bad()
+
+
+@pytest.mark.parametrize("r,d", [(20000, 40), (20000, 500), (12000, 760), (12000, 777), (12000, 1000), (8000, 1500), (8000, 1537), (6000, 2040),
+                                 (4000, 3000), (4000, 4000), (1500, 5000), (1500, 5001), (1200, 8000), (1200, 10240)])
+@pytest.mark.parametrize("t", [BF16, F32])
+def test_more_rows_than_the_ring_holds(r, d, t):
+    """Every group of threads comes by each slot of its ring again."""
+    from q8_kernels_b200 import native
+    x, w, b, g = rows(r, d, t, seed=r + d, offset=2.0)
+    y, mean, rstd = native.layer_norm(x, w, b, 1e-5, None, True)
+    check_forward(y, x, w, b, 1e-5)
+    g = g.to(t)
+    check_backward(native.layer_norm_backward(x, mean, rstd, g, w, True, True, True), x, w, g, 1e-5)
+    dx = native.layer_norm_backward(x, mean, rstd, g, w, True, False, False)[0]
+    check_backward([dx, None, None], x, w, g, 1e-5)
