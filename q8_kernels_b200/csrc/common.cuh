@@ -271,6 +271,19 @@ __device__ __forceinline__ float warp_max(float v) {
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
+// The larger value, or NaN if either is: the maximum of the gated projection's quantizer, whose rows with NaN get NaN as their scale.  (The
+// quantizer of the linears leaves NaN out, as fmaxf does.)
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_of(float a, float b, bool nan) { return nan ? max_nan(a, b) : fmaxf(a, b); }
+__device__ __forceinline__ float warp_max_nan(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
 // sm_100 packed fp32 pairs: one issue slot does two lanes of FMA-pipe work, each lane rounded as
 // the scalar instruction would be.
 __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {

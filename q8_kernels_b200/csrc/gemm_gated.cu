@@ -364,7 +364,7 @@ __device__ __forceinline__ int gated_buf(int e) { return e + (e >> 3); }
 
 // The quantised activation of up to eight rows, into the operand layout of the MMA (rows of 128 bytes, 16-byte pieces XOR the row), by the
 // 256 epilogue threads.  The same values and bits as q8k_gated_quant: butterflies in fp32, stride 1 first, then the scale, the
-// rounding to bf16 and the row's grid.
+// rounding to bf16 and the row's grid.  A row with NaN has NaN as its maximum and scale: int8 bytes could not hold it.
 template <bool INT8>
 __device__ __forceinline__ void gated_quant_rows(const GatedFewParams& p, uint8_t* smem, float* a_scales, float* red, int k_iters) {
     const int threads = kGemmEpilogueThreads / p.groups;       // 64, 128 or 256
@@ -419,7 +419,7 @@ __device__ __forceinline__ void gated_quant_rows(const GatedFewParams& p, uint8_
                     for (int j = 0; j < 8; ++j) {
                         if (last) {
                             v[j] = __bfloat162float(__float2bfloat16_rn(__fmul_rn(v[j], p.scale)));
-                            if (e[j] < p.K) amax = fmaxf(amax, fabsf(v[j]));
+                            if (e[j] < p.K) amax = max_nan(amax, fabsf(v[j]));
                         }
                         buf[gated_buf(e[j])] = v[j];
                     }
@@ -430,13 +430,13 @@ __device__ __forceinline__ void gated_quant_rows(const GatedFewParams& p, uint8_
                 float v[8];
                 load_vec<__nv_bfloat16, 8>(xr + b * 8, v);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[j]));
+                for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[j]));
             }
         }
-        amax = warp_max(amax);
+        amax = warp_max_nan(amax);
         if ((tid & 31) == 0) red[tid >> 5] = amax;
         sync();
-        for (int k = 0; k < threads / 32; ++k) amax = fmaxf(amax, red[group * (threads / 32) + k]);
+        for (int k = 0; k < threads / 32; ++k) amax = max_nan(amax, red[group * (threads / 32) + k]);
         const float f = quant_factor<true>(INT8 ? 127.0f : 448.0f, amax);
         const float mul = amax == 0.f ? 0.f : f;
         if (t == 0) a_scales[row] = __fdiv_rn(1.0f, f);

@@ -123,10 +123,10 @@ hadamard_small_kernel(const Tin* __restrict__ x, Tout* __restrict__ out, float* 
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             v[j] = round_through<Tin>(__fmul_rn(v[j], scale));
-            if (e + j < dim) amax = fmaxf(amax, fabsf(v[j]));
+            if (e + j < dim) amax = max_of(amax, fabsf(v[j]), two_step);
         }
 #pragma unroll
-        for (int m = 1; m < G; m <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, m));
+        for (int m = 1; m < G; m <<= 1) amax = max_of(amax, __shfl_xor_sync(0xffffffffu, amax, m), two_step);
         const float qmax = std::is_same_v<Tout, int8_t> ? 127.0f : 448.0f;
         const float qscale = quant_factor(qmax, amax, two_step);
         if (row_ok && e < dim) store_quant<Tout, 8>(out + row * (int64_t)dim + e, v, qscale, amax == 0.f);
@@ -503,7 +503,8 @@ hadamard_stream_kernel(const Tin* __restrict__ x, Tout* __restrict__ out, float*
             }
         } else {
             // Round to the input dtype (what the unfused chain stores) and take the row's absmax: of the fp32 values, rounded
-            // afterwards (bf16), or of the e4m3 bytes widened to fp16 pairs (exact).  NaNs do not count, as with fmaxf.
+            // afterwards (bf16), or of the e4m3 bytes widened to fp16 pairs (exact).  A NaN is the maximum (two_step), or does not
+            // count, as with fmaxf: then the maximum of a thread that has one is taken again without it.
             uint32_t pk[V / (IN8 ? 4 : 2)];
             float amax;
             if constexpr (IN8) {
@@ -523,12 +524,22 @@ hadamard_stream_kernel(const Tin* __restrict__ x, Tout* __restrict__ out, float*
                             for (int g = 0; g < 4; ++g) {
                                 const uint32_t ww = g < 2 ? w.x : w.y;
                                 const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(g & 1 ? ww >> 16 : ww & 0xffffu), __NV_E4M3);
-                                if (in_row((f + 2 * g) / C)) m2 = __hmax2(m2, __habs2(__half2(h)));
+                                if (in_row((f + 2 * g) / C)) m2 = __hmax2_nan(m2, __habs2(__half2(h)));
                             }
                         }
                     }
                 }
-                amax = fmaxf(__low2float(m2), __high2float(m2));
+                amax = max_nan(__low2float(m2), __high2float(m2));
+                if (!two_step && amax != amax) {
+                    m2 = __floats2half2_rn(0.f, 0.f);
+#pragma unroll
+                    for (int f = 0; f < V; f += 2) {
+                        const uint32_t ww = pk[f / 4];
+                        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(f & 2 ? ww >> 16 : ww & 0xffffu), __NV_E4M3);
+                        if (any_in_row(f / C / SKIP * SKIP) && in_row(f / C)) m2 = __hmax2(m2, __habs2(__half2(h)));
+                    }
+                    amax = fmaxf(__low2float(m2), __high2float(m2));
+                }
             } else {
                 float mx[2] = {0.f, 0.f};
 #pragma unroll
@@ -539,20 +550,28 @@ hadamard_stream_kernel(const Tin* __restrict__ x, Tout* __restrict__ out, float*
                             const __nv_bfloat162 w = __floats2bfloat162_rn(v[f], v[f + 1]);
                             pk[f / 2] = *reinterpret_cast<const uint32_t*>(&w);
                             float& m = mx[(f / 2) & 1];
-                            if (in_row(f / C)) asm("max.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(v[f])), "f"(fabsf(v[f + 1])));
+                            if (in_row(f / C)) asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(v[f])), "f"(fabsf(v[f + 1])));
                         }
                     }
                 }
-                amax = __bfloat162float(__float2bfloat16_rn(fmaxf(mx[0], mx[1])));   // rounding keeps the order
+                amax = __bfloat162float(__float2bfloat16_rn(max_nan(mx[0], mx[1])));   // rounding keeps the order
+                if (!two_step && amax != amax) {
+                    amax = 0.f;
+#pragma unroll
+                    for (int f = 0; f < V; f += 2) {
+                        if (any_in_row(f / C / SKIP * SKIP) && in_row(f / C))
+                            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(pk[f / 2] << 16)), fabsf(__uint_as_float(pk[f / 2] & 0xffff0000u))));
+                    }
+                }
             }
 #pragma unroll
-            for (int m = 1; m < (T < 32 ? T : 32); m <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, m));
+            for (int m = 1; m < (T < 32 ? T : 32); m <<= 1) amax = max_of(amax, __shfl_xor_sync(0xffffffffu, amax, m), two_step);
             if constexpr (T > 32) {
                 if ((threadIdx.x & 31) == 0) red_max[threadIdx.x >> 5] = amax;
                 __syncthreads();
                 amax = red_max[0];
 #pragma unroll
-                for (int k = 1; k < T / 32; ++k) amax = fmaxf(amax, red_max[k]);
+                for (int k = 1; k < T / 32; ++k) amax = max_of(amax, red_max[k], two_step);
             }
             const float qmax = std::is_same_v<Tout, int8_t> ? 127.0f : 448.0f;
             const float qscale = quant_factor(qmax, amax, two_step);

@@ -18,15 +18,15 @@ namespace q8k {
 constexpr int kItem = 8;
 
 template <int T>
-__device__ __forceinline__ float block_reduce_max(float v, float* smem) {
-    v = warp_max(v);
+__device__ __forceinline__ float block_reduce_max(float v, float* smem, bool nan) {
+    v = nan ? warp_max_nan(v) : warp_max(v);
     if constexpr (T > 32) {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
         if (lane == 0) smem[warp] = v;
         __syncthreads();
         float r = smem[0];
 #pragma unroll
-        for (int w = 1; w < T / 32; ++w) r = fmaxf(r, smem[w]);
+        for (int w = 1; w < T / 32; ++w) r = max_of(r, smem[w], nan);
         __syncthreads();
         v = r;
     }
@@ -71,10 +71,20 @@ tokenwise_quant_kernel(const Tin* __restrict__ x, Tout* __restrict__ q, float* _
         if (e < dim) {
             load_vec<Tin, kItem>(xr + e, v[i]);
 #pragma unroll
-            for (int j = 0; j < kItem; ++j) amax = fmaxf(amax, fabsf(v[i][j]));
+            for (int j = 0; j < kItem; ++j) amax = max_nan(amax, fabsf(v[i][j]));
         }
     }
-    amax = block_reduce_max<T>(amax, red);
+    if (!two_step && amax != amax) {                          // NaN does not count (max_nan: the gated projection's)
+        amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            if ((threadIdx.x + i * T) * kItem < dim) {
+#pragma unroll
+                for (int j = 0; j < kItem; ++j) amax = fmaxf(amax, fabsf(v[i][j]));
+            }
+        }
+    }
+    amax = block_reduce_max<T>(amax, red, two_step);
 
     constexpr bool kInt8 = sizeof(Tout) == 1 && !__is_same(Tout, e4m3_t);
     const float qmax = kInt8 ? 127.0f : 448.0f;

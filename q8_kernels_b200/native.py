@@ -878,7 +878,8 @@ def gated_mm(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a_s
 def gated_quant(x: torch.Tensor, rotate: bool, out_type: torch.dtype) -> List[torch.Tensor]:
     """The activation of the gated projection: x [...,K] (bf16 or e4m3) rotated (``rotate``: Hadamard, 1/sqrt(K), rounded to x's type) and
     quantised per token to int8 or e4m3.  Returns ``[q, scales]``.  As hadamard_quant / tokenwise_quant, but the row's factor is
-    ``top * (1 / absmax)``, two roundings, where those take ``top / absmax``."""
+    ``top * (1 / absmax)``, two roundings, where those take ``top / absmax``, and a row with NaN has NaN as its scale, where those leave NaN
+    out of the maximum (an int8 row would lose it)."""
     dev = require_cuda(x)
     x2, rows, dim, stride = _rows(_aligned(x))
     q = torch.empty(x.shape, dtype=out_type, device=dev)
