@@ -370,7 +370,8 @@ Q8K_API int q8k_gated_linear(const void* x, int x_dtype, const void* w, int w_dt
                      int* dev_status, void* stream);
 /* Its activation: rows of x (bf16 or e4m3), rotated (Hadamard, 1/sqrt(dim), rounded to x's type) or not, quantised per token to int8 or
  * e4m3 as q8k_hadamard_quant and q8k_tokenwise_quant do it, but with the factor top * (1 / absmax) of two roundings in the place
- * of top / absmax; a row with NaN has NaN as its scale.  dim a multiple of 16.  No counterpart in the reference.               */
+ * of top / absmax; a row with NaN has NaN as its scale, and one whose absmax is below top / FLT_MAX the factor
+ * FLT_MAX.  dim a multiple of 16.  No counterpart in the reference.                                                             */
 Q8K_API int q8k_gated_quant(const void* x, int x_dtype, int64_t x_row_stride, void* q, int q_dtype, float* scales, int64_t rows, int dim,
                     int rotate, void* stream);
 /* Its backward pass up to the product with the weight: from grad bf16 [M, F] and pre, the row [grad * up * act'(gate) | grad * act(gate)]

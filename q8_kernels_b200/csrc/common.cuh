@@ -118,8 +118,13 @@ inline int dtype_size(int dt) {
 // the gated projection defines it as tensor code computes a scalar over a tensor, top * (1 / absmax), each rounded.  The two differ
 // in the last bit for some absmax, and a 16-bit value that lies exactly between two steps of the grid then falls on one side or
 // the other: the operator's definition has to say which.
+// Below top / FLT_MAX (1.3e-36) there is no such factor; an infinite one would make NaN of the row's zeros.  The gated projection
+// takes FLT_MAX there, which leaves such rows fewer steps and loses nothing that 1 / FLT_MAX can hold; only a row of zeros has an infinite factor
+// (scale 0), and its zeros are not multiplied.
 template <bool TwoStep> __device__ __forceinline__ float quant_factor(float top, float absmax) {
-    return TwoStep ? __fmul_rn(top, __frcp_rn(absmax)) : __fdiv_rn(top, absmax);
+    if constexpr (!TwoStep) return __fdiv_rn(top, absmax);
+    const float f = __fmul_rn(top, __frcp_rn(absmax));
+    return absmax > 0.f && f > 3.402823466e38f ? 3.402823466e38f : f;
 }
 __device__ __forceinline__ float quant_factor(float top, float absmax, bool two_step) {
     return two_step ? quant_factor<true>(top, absmax) : quant_factor<false>(top, absmax);
