@@ -346,7 +346,8 @@ Q8K_API int q8k_layer_norm_backward(const void* x, int x_dtype, int64_t x_row_st
  * channels -- (2i, 2i + 1), or (i, i + rotary_dim / 2) with half_layout -- is turned by position * frequencies[i] radians
  * (fp64 [rotary_dim / 2]; the product is formed in fp64) and scaled by amplitude; the other channels are copied.  positions: int32 or
  * int64 at batch * position_batch_stride + token * position_token_stride, or NULL for 0 .. seq - 1.  dtype bf16, fp16 or fp32.  out may be
- * the input itself.  backward: the angle negated, which is the gradient.  No counterpart in the reference.                       */
+ * the input itself, with the same strides and no two heads that overlap; beyond that inputs and outputs must not share memory.  backward:
+ * the angle negated, which is the gradient.  No counterpart in the reference.                                                    */
 Q8K_API int q8k_rotary(const void* q, const int64_t q_strides[3], void* q_out, const int64_t q_out_strides[3], int q_heads,
                const void* k, const int64_t k_strides[3], void* k_out, const int64_t k_out_strides[3], int k_heads,
                int dtype, const void* positions, int positions_int64, int64_t position_batch_stride,

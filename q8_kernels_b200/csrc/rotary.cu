@@ -192,6 +192,26 @@ template <typename T> static int launch_rotary(const RotaryParams& p, int v, cud
     return launch_rotary_as<T, 1, true>(p, st);
 }
 
+// Whether a tensor may be rotated in its own place: one layout, whose heads do not overlap.  Every element is then read and written by
+// one thread; with shared elements a thread would load what another has rotated already.
+static bool rotary_in_place(const int64_t* in, const int64_t* out, const int64_t (&count)[3], int64_t head_dim) {
+    int64_t extent = head_dim;
+    int order[3], n = 0;
+    for (int i = 0; i < 3; ++i) {
+        if (count[i] == 1) continue;                           // a stride over one element does not matter
+        if (in[i] != out[i]) return false;
+        int at = n++;
+        for (; at > 0 && in[order[at - 1]] > in[i]; --at) order[at] = order[at - 1];
+        order[at] = i;
+    }
+    for (int k = 0; k < n; ++k) {                              // from the innermost out: each step beyond all that lies inside it
+        const int64_t step = in[order[k]];
+        if (step < extent) return false;
+        extent += step * (count[order[k]] - 1);
+    }
+    return true;
+}
+
 }  // namespace q8k
 
 using namespace q8k;
@@ -212,6 +232,13 @@ extern "C" int q8k_rotary(const void* q, const int64_t q_strides[3], void* q_out
     Q8K_REQUIRE(dtype == Q8K_DT_F32 || dtype == Q8K_DT_F16 || dtype == Q8K_DT_BF16, Q8K_ERR_UNSUPPORTED,
                 "%s: dtype %d is not float32, float16 or bfloat16", op, dtype);
     if (batch == 0 || seq == 0 || q_heads + k_heads == 0) return Q8K_OK;
+    for (int i = 0; i < 2; ++i) {
+        const void *in = i ? k : q, *out = i ? k_out : q_out;
+        const int64_t *is = i ? k_strides : q_strides, *os = i ? k_out_strides : q_out_strides;
+        const int64_t count[3] = {batch, seq, i ? k_heads : q_heads};
+        Q8K_REQUIRE(count[2] == 0 || in == nullptr || in != out || is == nullptr || os == nullptr || rotary_in_place(is, os, count, head_dim),
+                    Q8K_ERR_INVALID_ARG, "%s: in place, %s needs the input's strides and heads that do not overlap", op, i ? "k" : "q");
+    }
     Q8K_REQUIRE(frequencies != nullptr && reinterpret_cast<uintptr_t>(frequencies) % 8 == 0, Q8K_ERR_INVALID_ARG,
                 "%s: null or misaligned frequencies", op);
     Q8K_REQUIRE(reinterpret_cast<uintptr_t>(positions) % (positions_int64 ? 8 : 4) == 0, Q8K_ERR_INVALID_ARG,

@@ -822,15 +822,15 @@ def rotary(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: Opti
 
     def tensor(t):
         if t is None:
-            return None, None, None, (None, None, None, None, 0)
+            return None, None, (None, None, None, None, 0)
         if dim > 1 and t.stride(-1) != 1:
             t = t.contiguous()
         out = torch.empty(t.shape, dtype=t.dtype, device=dev)
         s, o = ((0,) * (t.dim() == 3) + a.stride()[:-1] for a in (t, out))
-        return t, out, None, (ptr(t), _Strides(*s), ptr(out), _Strides(*o), t.shape[-2])
+        return t, out, (ptr(t), _Strides(*s), ptr(out), _Strides(*o), t.shape[-2])
 
-    q_in, q_out, _, q_args = tensor(q)                       # (the inputs stay alive until the launch)
-    k_in, k_out, _, k_args = tensor(k)
+    q_in, q_out, q_args = tensor(q)                          # (the inputs stay alive until the launch)
+    k_in, k_out, k_args = tensor(k)
     launch(dev, "rotary", lib.q8k_rotary, *q_args, *k_args, dt(x.dtype), ptr(positions), wide, pos_batch, pos_token, ptr(frequencies),
            float(amplitude), batch, seq, dim, 2 * frequencies.numel(), int(half), int(backward))
     return q_out, k_out
