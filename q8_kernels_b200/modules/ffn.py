@@ -21,7 +21,8 @@ class GatedFeedForward(nn.Module):
     """``proj_down(act(gate(x)) * up(x))``, gate and up projection, activation and product in one kernel.  ``inner_dim`` columns between the
     projections, a multiple of 16.  ``linear="int8"`` rotates both activations, so both widths have to be powers of two; "fp8" rotates
     the first if its width is one, and not the second, where FP8Linear has no gradient with a rotation.  Trains as its linears do: the
-    activation has a gradient.  No counterpart in the reference."""
+    activation has a gradient.  The output has x's leading dims, whatever they are (the linears alone return [1, M, N] for [M, K]).
+    No counterpart in the reference."""
 
     def __init__(self, dim: int, inner_dim: int, act: str = "silu", bias: bool = True, linear: str = "int8"):
         super().__init__()
@@ -32,7 +33,13 @@ class GatedFeedForward(nn.Module):
         self.proj_down = Q8Linear(inner_dim, dim, bias) if linear == "int8" else FP8Linear(inner_dim, dim, bias)
 
     def forward(self, x, out_dtype=torch.bfloat16):
-        return self.proj_down(self.gate_up(x), out_dtype=out_dtype)
+        h = self.gate_up(x)
+        dim = self.proj_down.out_features
+        if h.numel() == 0:                                   # the linears' backward pass does not take a tensor without rows
+            return h[..., :1].expand(*h.shape[:-1], dim).to(out_dtype)
+        if h.dim() not in (2, 3):
+            h = h.reshape(-1, self.inner_dim)
+        return self.proj_down(h, out_dtype=out_dtype).reshape(*x.shape[:-1], dim)
 
     @classmethod
     def from_linears(cls, gate: nn.Linear, up: nn.Linear, down: nn.Linear, act: str = "silu", linear: str = "int8"):
