@@ -704,6 +704,8 @@ at::Tensor empty_like_dtype(at::IntArrayRef shape, const at::Tensor& like, Dt ty
 float* out_f(at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 const at::Tensor* defined(const at::Tensor& t) { return t.defined() ? &t : nullptr; }
 bool wants_grad(const at::Tensor* t) { return t != nullptr && t->requires_grad(); }
+// Carries a forward-mode derivative (there is one level of them), which the Python bodies refuse.
+bool has_tangent(const at::Tensor* t) { return t != nullptr && t->_fw_grad(0).defined(); }
 
 // Gradients that cannot be differentiated again say so when that is tried, as once_differentiable does in Python.
 variable_list once_only(variable_list&& grads, const variable_list& incoming) {
@@ -787,6 +789,7 @@ PyObject* _layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
             (in == Dt::Float && (out == Dt::BFloat16 || out == Dt::Half))));
     OR_NONE(c);
     for (const at::Tensor* v : {w, b}) c.need(v == nullptr || (v->dim() == 1 && v->size(0) == x->size(-1)));
+    c.need(!has_tangent(x) && !has_tangent(w) && !has_tangent(b));
     OR_NONE(c);
     return answer([&]() -> PyObject* {
         at::Tensor y;
@@ -892,7 +895,7 @@ PyObject* _rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
                pos->size(-1) == seq && (pos->dim() == 1 || pos->size(0) == 1 || pos->size(0) == batch));
     }
     OR_NONE(c);
-    c.need((q->size(d - 2) + (k != nullptr ? k->size(d - 2) : 0)) * dim <= (1 << 24));
+    c.need((q->size(d - 2) + (k != nullptr ? k->size(d - 2) : 0)) * dim <= (1 << 24) && !has_tangent(q) && !has_tangent(k));
     OR_NONE(c);
     return answer([&]() -> PyObject* {
         variable_list out;
@@ -1009,7 +1012,7 @@ PyObject* _gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t k = b->size(1), nn = b->size(0), m = a->numel() / k;
     const bool training = c10::GradMode::is_enabled() && a->requires_grad();
     c.need(nn > 0 && nn % 32 == 0 && nn <= 0x3fffffff && k % 16 == 0 && k <= 16384 && m <= 0x7fffff00 && scale->numel() == nn &&
-           (bias == nullptr || bias->numel() == nn) && !(training && nn > 2 * 16384));
+           (bias == nullptr || bias->numel() == nn) && !(training && nn > 2 * 16384) && !has_tangent(a));
     c.status();
     OR_NONE(c);
     return answer([&]() -> PyObject* {

@@ -5,7 +5,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _host
-from ..native import E4M3, layer_norm_backward
+from ..native import E4M3, layer_norm_backward, refuse_tangents
 from ..native import layer_norm as _layer_norm
 
 
@@ -36,6 +36,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     fast = _host._layer_norm(x, weight, bias, eps, out_type)
     if fast is not None:
         return fast
+    refuse_tangents("layer_norm", x, weight, bias)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return LayerNorm8bit.apply(x, weight, bias, eps, out_type)
     return _layer_norm(x, weight, bias, eps, out_type, False)[0]

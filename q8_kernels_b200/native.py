@@ -724,6 +724,12 @@ def linear(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: Optio
 
 # ---------------------------------------------------------------- ops without a counterpart in the reference's modules
 
+def refuse_tangents(op: str, *tensors: Optional[torch.Tensor]) -> None:
+    """The differentiable ops have no forward-mode derivative: an input that carries one is refused, as its output would have lost it."""
+    if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise Q8KernelError(f"{op}: forward-mode derivatives are not supported")
+
+
 def _aligned(x: torch.Tensor) -> torch.Tensor:
     """x, or a copy of a dense x that does not begin on the 16 bytes that the gated projection's kernels need."""
     return x.clone() if x.is_contiguous() and x.data_ptr() % 16 else x
