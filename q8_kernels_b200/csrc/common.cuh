@@ -36,10 +36,13 @@ void set_error_detail(const char* fmt, ...);
         }                                                                          \
     } while (0)
 
-// q8k_tokenwise_quant / q8k_hadamard_quant under another name `op`, with the quantizer's factor in two steps (see quant_factor)
-int tokenwise_quant_as(const char* op, bool two_step, const void* x, int x_dtype, void* q, int q_dtype, float* scales, int64_t rows, int dim,
+// q8k_tokenwise_quant / q8k_hadamard_quant under another name `op`; GATED: with the gated projection's factor and maximum (see quant_factor,
+// max_nan)
+template <bool GATED>
+int tokenwise_quant_as(const char* op, const void* x, int x_dtype, void* q, int q_dtype, float* scales, int64_t rows, int dim,
                        int64_t x_row_stride, cudaStream_t st);
-int hadamard_quant_as(const char* op, bool two_step, const void* x, int x_dtype, void* q, int q_dtype, float* scales, int64_t rows, int dim,
+template <bool GATED>
+int hadamard_quant_as(const char* op, const void* x, int x_dtype, void* q, int q_dtype, float* scales, int64_t rows, int dim,
                       int64_t x_row_stride, float scale, cudaStream_t st);
 
 // q8k_gated_mm under another name.  weight_ready: the weight was complete when the kernel before this one began its work, so its loads
@@ -125,9 +128,6 @@ template <bool TwoStep> __device__ __forceinline__ float quant_factor(float top,
     if constexpr (!TwoStep) return __fdiv_rn(top, absmax);
     const float f = __fmul_rn(top, __frcp_rn(absmax));
     return absmax > 0.f && f > 3.402823466e38f ? 3.402823466e38f : f;
-}
-__device__ __forceinline__ float quant_factor(float top, float absmax, bool two_step) {
-    return two_step ? quant_factor<true>(top, absmax) : quant_factor<false>(top, absmax);
 }
 
 // ---------------------------------------------------------------- scalar conversions
@@ -271,11 +271,6 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&in)[N
     }
 }
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
 // The larger value, or NaN if either is: the maximum of the gated projection's quantizer, whose rows with NaN get NaN as their scale.  (The
 // quantizer of the linears leaves NaN out, as fmaxf does.)
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -283,10 +278,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-__device__ __forceinline__ float max_of(float a, float b, bool nan) { return nan ? max_nan(a, b) : fmaxf(a, b); }
-__device__ __forceinline__ float warp_max_nan(float v) {
+template <bool Nan> __device__ __forceinline__ float max_of(float a, float b) { return Nan ? max_nan(a, b) : fmaxf(a, b); }
+template <bool Nan = false> __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    for (int o = 16; o > 0; o >>= 1) v = max_of<Nan>(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
 // sm_100 packed fp32 pairs: one issue slot does two lanes of FMA-pipe work, each lane rounded as

@@ -409,8 +409,8 @@ extern "C" int q8k_gated_quant(const void* x, int x_dtype, int64_t x_row_stride,
     const char* op = "gated_quant";
     Q8K_REQUIRE(x_dtype == Q8K_DT_BF16 || x_dtype == Q8K_DT_E4M3, Q8K_ERR_UNSUPPORTED, "%s: input dtype %d is not bf16 or e4m3", op, x_dtype);
     cudaStream_t st = (cudaStream_t)stream;
-    return rotate ? hadamard_quant_as(op, true, x, x_dtype, q, q_dtype, scales, rows, dim, x_row_stride, 1.0f / sqrtf((float)dim), st)
-                  : tokenwise_quant_as(op, true, x, x_dtype, q, q_dtype, scales, rows, dim, x_row_stride, st);
+    return rotate ? hadamard_quant_as<true>(op, x, x_dtype, q, q_dtype, scales, rows, dim, x_row_stride, 1.0f / sqrtf((float)dim), st)
+                  : tokenwise_quant_as<true>(op, x, x_dtype, q, q_dtype, scales, rows, dim, x_row_stride, st);
 }
 
 extern "C" size_t q8k_gated_linear_workspace_bytes(int M, int K) {

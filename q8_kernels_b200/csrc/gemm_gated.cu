@@ -433,7 +433,7 @@ __device__ __forceinline__ void gated_quant_rows(const GatedFewParams& p, uint8_
                 for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[j]));
             }
         }
-        amax = warp_max_nan(amax);
+        amax = warp_max<true>(amax);
         if ((tid & 31) == 0) red[tid >> 5] = amax;
         sync();
         for (int k = 0; k < threads / 32; ++k) amax = max_nan(amax, red[group * (threads / 32) + k]);

@@ -92,11 +92,11 @@ __device__ __forceinline__ void store_quant(Tq* p, const float (&v)[N], float qs
 
 // ------------------------------------------------------------------ small rows
 // LOG_G = log2(lanes per row).  Tout is the cast output type (Cast) or the
-// quantised type (Quant: int8_t or e4m3_t).
-template <typename Tin, typename Tout, int LOG_G, Epilogue EPI>
+// quantised type (Quant: int8_t or e4m3_t).  GATED: the quantizer has the gated projection's factor and maximum (quant_factor, max_nan).
+template <typename Tin, typename Tout, int LOG_G, Epilogue EPI, bool GATED>
 __global__ void __launch_bounds__(128)
 hadamard_small_kernel(const Tin* __restrict__ x, Tout* __restrict__ out, float* __restrict__ scales,
-                      int64_t rows, int dim, int64_t x_row_stride, float scale, bool two_step) {
+                      int64_t rows, int dim, int64_t x_row_stride, float scale) {
     constexpr int G = 1 << LOG_G;
     constexpr int ROWS_PER_CTA = 128 / G;
     const int lane = threadIdx.x & 31;
@@ -123,13 +123,14 @@ hadamard_small_kernel(const Tin* __restrict__ x, Tout* __restrict__ out, float* 
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             v[j] = round_through<Tin>(__fmul_rn(v[j], scale));
-            if (e + j < dim) amax = max_of(amax, fabsf(v[j]), two_step);
+            if (e + j < dim) amax = max_of<GATED>(amax, fabsf(v[j]));
         }
 #pragma unroll
-        for (int m = 1; m < G; m <<= 1) amax = max_of(amax, __shfl_xor_sync(0xffffffffu, amax, m), two_step);
+        for (int m = 1; m < G; m <<= 1) amax = max_of<GATED>(amax, __shfl_xor_sync(0xffffffffu, amax, m));
         const float qmax = std::is_same_v<Tout, int8_t> ? 127.0f : 448.0f;
-        const float qscale = quant_factor(qmax, amax, two_step);
-        if (row_ok && e < dim) store_quant<Tout, 8>(out + row * (int64_t)dim + e, v, qscale, amax == 0.f);
+        const float qscale = quant_factor<GATED>(qmax, amax);
+        if (row_ok && e < dim)
+            store_quant<Tout, 8>(out + row * (int64_t)dim + e, v, GATED && amax == 0.f ? 0.f : qscale, !GATED && amax == 0.f);
         if (row_ok && sub == 0) scales[row] = __fdiv_rn(1.0f, qscale);
     }
 }
@@ -208,7 +209,7 @@ __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wai
 // where s, h are the per-batch modulation rows (bf16 [rows / rows_per_mod, dim]).  A CTA stays inside one batch entry
 // and keeps its two modulation rows in shared memory.
 // int8 rows (Cast only) are dequantised on the way in: v = bf16(q * scales[row]), the weight of a backward pass.
-// FULL: dim is the power of two itself, so no element of a row needs a bounds test.
+// FULL: dim is the power of two itself, so no element of a row needs a bounds test.  GATED: as in the small kernel.
 
 // Raw staging: position of the 16-byte chunk c (row order) of a row whose threads own CPT chunks each, such
 // that eight consecutive threads reading their k-th chunk touch eight different bank groups.
@@ -271,11 +272,11 @@ struct StreamGeo {
     static constexpr int CTAS = BY_SMEM < BY_REGS ? BY_SMEM : BY_REGS;
 };
 
-template <typename Tin, typename Tout, int LOG_N, Epilogue EPI, bool NORM_MOD, bool FULL>
+template <typename Tin, typename Tout, int LOG_N, Epilogue EPI, bool NORM_MOD, bool FULL, bool GATED>
 __global__ void __launch_bounds__(StreamGeo<Tin, LOG_N, NORM_MOD>::THREADS, StreamGeo<Tin, LOG_N, NORM_MOD>::CTAS)
 hadamard_stream_kernel(const Tin* __restrict__ x, Tout* __restrict__ out, float* __restrict__ scales, unsigned rows, int dim,
                        int64_t x_row_stride, float scale, const __nv_bfloat16* __restrict__ mod_scale,
-                       const __nv_bfloat16* __restrict__ mod_shift, unsigned rows_per_mod, unsigned blocks_per_mod, bool two_step) {
+                       const __nv_bfloat16* __restrict__ mod_shift, unsigned rows_per_mod, unsigned blocks_per_mod) {
     constexpr bool DEQ = std::is_same_v<Tin, int8_t>;
     static_assert(!DEQ || EPI == Epilogue::Cast, "int8 rows are only transformed, not quantised again");
     using Geo = StreamGeo<Tin, LOG_N, NORM_MOD>;
@@ -503,8 +504,8 @@ hadamard_stream_kernel(const Tin* __restrict__ x, Tout* __restrict__ out, float*
             }
         } else {
             // Round to the input dtype (what the unfused chain stores) and take the row's absmax: of the fp32 values, rounded
-            // afterwards (bf16), or of the e4m3 bytes widened to fp16 pairs (exact).  A NaN is the maximum (two_step), or does not
-            // count, as with fmaxf: then the maximum of a thread that has one is taken again without it.
+            // afterwards (bf16), or of the e4m3 bytes widened to fp16 pairs (exact).  NaNs do not count, as with fmaxf, or are the maximum
+            // (GATED).
             uint32_t pk[V / (IN8 ? 4 : 2)];
             float amax;
             if constexpr (IN8) {
@@ -524,22 +525,12 @@ hadamard_stream_kernel(const Tin* __restrict__ x, Tout* __restrict__ out, float*
                             for (int g = 0; g < 4; ++g) {
                                 const uint32_t ww = g < 2 ? w.x : w.y;
                                 const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(g & 1 ? ww >> 16 : ww & 0xffffu), __NV_E4M3);
-                                if (in_row((f + 2 * g) / C)) m2 = __hmax2_nan(m2, __habs2(__half2(h)));
+                                if (in_row((f + 2 * g) / C)) m2 = GATED ? __hmax2_nan(m2, __habs2(__half2(h))) : __hmax2(m2, __habs2(__half2(h)));
                             }
                         }
                     }
                 }
-                amax = max_nan(__low2float(m2), __high2float(m2));
-                if (!two_step && amax != amax) {
-                    m2 = __floats2half2_rn(0.f, 0.f);
-#pragma unroll
-                    for (int f = 0; f < V; f += 2) {
-                        const uint32_t ww = pk[f / 4];
-                        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(f & 2 ? ww >> 16 : ww & 0xffffu), __NV_E4M3);
-                        if (any_in_row(f / C / SKIP * SKIP) && in_row(f / C)) m2 = __hmax2(m2, __habs2(__half2(h)));
-                    }
-                    amax = fmaxf(__low2float(m2), __high2float(m2));
-                }
+                amax = max_of<GATED>(__low2float(m2), __high2float(m2));
             } else {
                 float mx[2] = {0.f, 0.f};
 #pragma unroll
@@ -550,31 +541,26 @@ hadamard_stream_kernel(const Tin* __restrict__ x, Tout* __restrict__ out, float*
                             const __nv_bfloat162 w = __floats2bfloat162_rn(v[f], v[f + 1]);
                             pk[f / 2] = *reinterpret_cast<const uint32_t*>(&w);
                             float& m = mx[(f / 2) & 1];
-                            if (in_row(f / C)) asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(v[f])), "f"(fabsf(v[f + 1])));
+                            if (in_row(f / C)) {
+                                if constexpr (GATED) asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(v[f])), "f"(fabsf(v[f + 1])));
+                                else asm("max.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(v[f])), "f"(fabsf(v[f + 1])));
+                            }
                         }
                     }
                 }
-                amax = __bfloat162float(__float2bfloat16_rn(max_nan(mx[0], mx[1])));   // rounding keeps the order
-                if (!two_step && amax != amax) {
-                    amax = 0.f;
-#pragma unroll
-                    for (int f = 0; f < V; f += 2) {
-                        if (any_in_row(f / C / SKIP * SKIP) && in_row(f / C))
-                            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(pk[f / 2] << 16)), fabsf(__uint_as_float(pk[f / 2] & 0xffff0000u))));
-                    }
-                }
+                amax = __bfloat162float(__float2bfloat16_rn(max_of<GATED>(mx[0], mx[1])));   // rounding keeps the order
             }
 #pragma unroll
-            for (int m = 1; m < (T < 32 ? T : 32); m <<= 1) amax = max_of(amax, __shfl_xor_sync(0xffffffffu, amax, m), two_step);
+            for (int m = 1; m < (T < 32 ? T : 32); m <<= 1) amax = max_of<GATED>(amax, __shfl_xor_sync(0xffffffffu, amax, m));
             if constexpr (T > 32) {
                 if ((threadIdx.x & 31) == 0) red_max[threadIdx.x >> 5] = amax;
                 __syncthreads();
                 amax = red_max[0];
 #pragma unroll
-                for (int k = 1; k < T / 32; ++k) amax = max_of(amax, red_max[k], two_step);
+                for (int k = 1; k < T / 32; ++k) amax = max_of<GATED>(amax, red_max[k]);
             }
             const float qmax = std::is_same_v<Tout, int8_t> ? 127.0f : 448.0f;
-            const float qscale = quant_factor(qmax, amax, two_step);
+            const float qscale = quant_factor<GATED>(qmax, amax);
             if (row_ok && t == 0) scales[row] = __fdiv_rn(1.0f, qscale);
             const float qmul = amax == 0.f ? 0.f : qscale;     // an all-zero row quantises to zeros (0 * 0, not 0 * inf)
             const float2 q2 = make_float2(qmul, qmul);
@@ -632,13 +618,13 @@ hadamard_stream_kernel(const Tin* __restrict__ x, Tout* __restrict__ out, float*
     cp_async_wait_all();                                       // (the copies behind the last row were empty)
 }
 
-template <typename Tin, typename Tout, int LOG_N, Epilogue EPI, bool NORM_MOD>
+template <typename Tin, typename Tout, int LOG_N, Epilogue EPI, bool NORM_MOD, bool GATED = false>
 static int launch_stream(const Tin* x, Tout* out, float* scales, int64_t rows, int dim, int64_t stride, float scale,
-                         const __nv_bfloat16* ms, const __nv_bfloat16* mh, int64_t rows_per_mod, cudaStream_t st, bool two_step = false) {
+                         const __nv_bfloat16* ms, const __nv_bfloat16* mh, int64_t rows_per_mod, cudaStream_t st) {
     using Geo = StreamGeo<Tin, LOG_N, NORM_MOD>;
     const bool full = dim == Geo::N;
-    auto kern = full ? hadamard_stream_kernel<Tin, Tout, LOG_N, EPI, NORM_MOD, true>
-                     : hadamard_stream_kernel<Tin, Tout, LOG_N, EPI, NORM_MOD, false>;
+    auto kern = full ? hadamard_stream_kernel<Tin, Tout, LOG_N, EPI, NORM_MOD, true, GATED>
+                     : hadamard_stream_kernel<Tin, Tout, LOG_N, EPI, NORM_MOD, false, GATED>;
     if (Geo::SMEM > 47 * 1024) {                               // (with the static reduction words, above the 48 KB default)
         static std::atomic<uint64_t> smem_done[2];
         if (int rc = allow_dynamic_smem((const void*)kern, Geo::SMEM, smem_done[full])) return rc;
@@ -659,14 +645,14 @@ static int launch_stream(const Tin* x, Tout* out, float* scales, int64_t rows, i
     // rows (1 x 1 x 2048: 3.2 us, 3.4 with one unit).
     const int units = NORM_MOD && need == 1 && groups > slots ? (int)((group_rows + Geo::RPU - 1) / Geo::RPU) : Geo::UNITS;
     Q8K_CUDA_OK(launch_dependent(kern, (unsigned)(blocks * groups), units * Geo::UNIT, Geo::smem(units), st, 1, x, out, scales, (unsigned)rows,
-                                 dim, stride, scale, ms, mh, (unsigned)group_rows, (unsigned)blocks, two_step));
+                                 dim, stride, scale, ms, mh, (unsigned)group_rows, (unsigned)blocks));
     return Q8K_OK;
 }
 
 // ------------------------------------------------------------------ dispatch
-template <typename Tin, typename Tout, Epilogue EPI>
+template <typename Tin, typename Tout, Epilogue EPI, bool GATED = false>
 static int launch_hadamard(const void* x, void* out, float* scales, int64_t rows, int dim,
-                           int64_t stride, float scale, cudaStream_t st, const char* op, bool two_step = false) {
+                           int64_t stride, float scale, cudaStream_t st, const char* op) {
     int log_n = 3;
     while ((1 << log_n) < dim) ++log_n;
     const Tin* xi = (const Tin*)x;
@@ -675,11 +661,11 @@ static int launch_hadamard(const void* x, void* out, float* scales, int64_t rows
         const int log_g = log_n - 3;
         const int rows_per_cta = 128 >> log_g;
         const unsigned grid = (unsigned)((rows + rows_per_cta - 1) / rows_per_cta);
-#define Q8K_HS(LG) case LG: hadamard_small_kernel<Tin, Tout, LG, EPI><<<grid, 128, 0, st>>>(xi, o, scales, rows, dim, stride, scale, two_step); break
+#define Q8K_HS(LG) case LG: hadamard_small_kernel<Tin, Tout, LG, EPI, GATED><<<grid, 128, 0, st>>>(xi, o, scales, rows, dim, stride, scale); break
         switch (log_g) { Q8K_HS(0); Q8K_HS(1); Q8K_HS(2); Q8K_HS(3); Q8K_HS(4); Q8K_HS(5); }
 #undef Q8K_HS
     } else {
-#define Q8K_HS(LN) case LN: return launch_stream<Tin, Tout, LN, EPI, false>(xi, o, scales, rows, dim, stride, scale, nullptr, nullptr, 1, st, two_step)
+#define Q8K_HS(LN) case LN: return launch_stream<Tin, Tout, LN, EPI, false, GATED>(xi, o, scales, rows, dim, stride, scale, nullptr, nullptr, 1, st)
         switch (log_n) {
             Q8K_HS(9); Q8K_HS(10); Q8K_HS(11); Q8K_HS(12); Q8K_HS(13); Q8K_HS(14);
             default: set_error_detail("%s: dim %d exceeds 16384", op, dim); return Q8K_ERR_UNSUPPORTED;
@@ -764,13 +750,14 @@ extern "C" int q8k_dequant_hadamard(const void* x, const float* row_scales, void
 }
 
 namespace q8k {
-int hadamard_quant_as(const char* op, bool two_step, const void* x, int x_dtype, void* q, int q_dtype, float* scales, int64_t rows, int dim,
+template <bool GATED>
+int hadamard_quant_as(const char* op, const void* x, int x_dtype, void* q, int q_dtype, float* scales, int64_t rows, int dim,
                       int64_t x_row_stride, float scale, cudaStream_t st) {
     if (int rc = check_hadamard_args(op, x, x_dtype, q, rows, dim, x_row_stride)) return rc;
     if (rows == 0) return Q8K_OK;
     Q8K_REQUIRE(scales != nullptr, Q8K_ERR_INVALID_ARG, "%s: null scales pointer", op);
     constexpr Epilogue Q = Epilogue::Quant;
-#define Q8K_HQ(TIN, TOUT) return launch_hadamard<TIN, TOUT, Q>(x, q, scales, rows, dim, x_row_stride, scale, st, op, two_step)
+#define Q8K_HQ(TIN, TOUT) return launch_hadamard<TIN, TOUT, Q, GATED>(x, q, scales, rows, dim, x_row_stride, scale, st, op)
     if (x_dtype == Q8K_DT_BF16 && q_dtype == Q8K_DT_I8)   Q8K_HQ(__nv_bfloat16, int8_t);
     if (x_dtype == Q8K_DT_BF16 && q_dtype == Q8K_DT_E4M3) Q8K_HQ(__nv_bfloat16, e4m3_t);
     if (x_dtype == Q8K_DT_E4M3 && q_dtype == Q8K_DT_I8)   Q8K_HQ(e4m3_t, int8_t);
@@ -779,11 +766,12 @@ int hadamard_quant_as(const char* op, bool two_step, const void* x, int x_dtype,
     set_error_detail("%s: quantised dtype %d is not int8 or e4m3", op, q_dtype);
     return Q8K_ERR_UNSUPPORTED;
 }
+template int hadamard_quant_as<true>(const char*, const void*, int, void*, int, float*, int64_t, int, int64_t, float, cudaStream_t);
 }  // namespace q8k
 
 extern "C" int q8k_hadamard_quant(const void* x, int x_dtype, void* q, int q_dtype, float* scales,
                                   int64_t rows, int dim, int64_t x_row_stride, float scale, void* stream) {
-    return hadamard_quant_as("hadamard_quant", false, x, x_dtype, q, q_dtype, scales, rows, dim, x_row_stride, scale, (cudaStream_t)stream);
+    return hadamard_quant_as<false>("hadamard_quant", x, x_dtype, q, q_dtype, scales, rows, dim, x_row_stride, scale, (cudaStream_t)stream);
 }
 
 extern "C" int q8k_norm_modulate_quant(const void* x, const void* mod_scale, const void* mod_shift, void* q, int q_dtype,

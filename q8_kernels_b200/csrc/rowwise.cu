@@ -17,16 +17,16 @@ namespace q8k {
 
 constexpr int kItem = 8;
 
-template <int T>
-__device__ __forceinline__ float block_reduce_max(float v, float* smem, bool nan) {
-    v = nan ? warp_max_nan(v) : warp_max(v);
+template <int T, bool NAN_COUNTS>
+__device__ __forceinline__ float block_reduce_max(float v, float* smem) {
+    v = warp_max<NAN_COUNTS>(v);
     if constexpr (T > 32) {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
         if (lane == 0) smem[warp] = v;
         __syncthreads();
         float r = smem[0];
 #pragma unroll
-        for (int w = 1; w < T / 32; ++w) r = max_of(r, smem[w], nan);
+        for (int w = 1; w < T / 32; ++w) r = max_of<NAN_COUNTS>(r, smem[w]);
         __syncthreads();
         v = r;
     }
@@ -51,11 +51,12 @@ __device__ __forceinline__ float block_reduce_sum(float v, float* smem) {
 
 // ------------------------------------------------------------------ quantizer
 // Semantics of tokenwise_quantization_kernel
-// (csrc/quantizer/tokenwise_quant_cuda.cu:115-148) with IEEE arithmetic.
-template <typename Tin, typename Tout, int ITEMS, int T>
+// (csrc/quantizer/tokenwise_quant_cuda.cu:115-148) with IEEE arithmetic.  GATED: the gated projection's factor and maximum (quant_factor,
+// max_nan).
+template <typename Tin, typename Tout, int ITEMS, int T, bool GATED>
 __global__ void __launch_bounds__(T)
 tokenwise_quant_kernel(const Tin* __restrict__ x, Tout* __restrict__ q, float* __restrict__ scales,
-                       int dim, int64_t x_row_stride, bool two_step) {
+                       int dim, int64_t x_row_stride) {
     __shared__ float red[32];
     pdl_wait();
     pdl_release();
@@ -71,25 +72,18 @@ tokenwise_quant_kernel(const Tin* __restrict__ x, Tout* __restrict__ q, float* _
         if (e < dim) {
             load_vec<Tin, kItem>(xr + e, v[i]);
 #pragma unroll
-            for (int j = 0; j < kItem; ++j) amax = max_nan(amax, fabsf(v[i][j]));
+            for (int j = 0; j < kItem; ++j) amax = max_of<GATED>(amax, fabsf(v[i][j]));
         }
     }
-    if (!two_step && amax != amax) {                          // NaN does not count (max_nan: the gated projection's)
-        amax = 0.f;
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            if ((threadIdx.x + i * T) * kItem < dim) {
-#pragma unroll
-                for (int j = 0; j < kItem; ++j) amax = fmaxf(amax, fabsf(v[i][j]));
-            }
-        }
-    }
-    amax = block_reduce_max<T>(amax, red, two_step);
+    amax = block_reduce_max<T, GATED>(amax, red);
 
     constexpr bool kInt8 = sizeof(Tout) == 1 && !__is_same(Tout, e4m3_t);
     const float qmax = kInt8 ? 127.0f : 448.0f;
-    const float scale = quant_factor(qmax, amax, two_step);   // +inf for an all-zero row
+    const float scale = quant_factor<GATED>(qmax, amax);   // +inf for an all-zero row
     const bool zero_row = amax == 0.f;
+    const float mul = zero_row ? 0.f : scale;
+    // (With a select on every product, as the linears' rows have it, nvcc 12.9 left bytes other than 0 in gated rows of zeros.)
+    auto scaled = [&](float x) { return GATED ? __fmul_rn(x, mul) : zero_row ? 0.f : __fmul_rn(x, scale); };
 
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
@@ -99,7 +93,7 @@ tokenwise_quant_kernel(const Tin* __restrict__ x, Tout* __restrict__ q, float* _
             if constexpr (kInt8) {
 #pragma unroll
                 for (int j = 0; j < kItem; ++j) {
-                    const float y = zero_row ? 0.f : __fmul_rn(v[i][j], scale);
+                    const float y = scaled(v[i][j]);
                     // exact round half away from zero: truncate y + copysign(0.5 - 2^-25, y)
                     o.b[j] = (uint8_t)(int8_t)__float2int_rz(__fadd_rn(y, copysignf(0.49999997f, y)));
                 }
@@ -108,8 +102,7 @@ tokenwise_quant_kernel(const Tin* __restrict__ x, Tout* __restrict__ q, float* _
                 // into NaN, so the packed saturating conversion gives the same bytes; a NaN stays a NaN
 #pragma unroll
                 for (int j = 0; j < kItem; j += 2) {
-                    const float y0 = zero_row ? 0.f : __fmul_rn(v[i][j], scale);
-                    const float y1 = zero_row ? 0.f : __fmul_rn(v[i][j + 1], scale);
+                    const float y0 = scaled(v[i][j]), y1 = scaled(v[i][j + 1]);
                     o.h[j / 2] = float2_to_e4m3x2_sat(y0, y1);
                 }
             }
@@ -446,13 +439,13 @@ rms_norm_backward_kernel(const Ty* __restrict__ y, const float* __restrict__ rrm
 }
 
 // ------------------------------------------------------------------ launch helpers
-template <typename Tin, typename Tout>
-static int launch_quant(const char* op, bool two_step, const void* x, void* q, float* scales, int64_t rows, int dim,
+template <typename Tin, typename Tout, bool GATED>
+static int launch_quant(const char* op, const void* x, void* q, float* scales, int64_t rows, int dim,
                         int64_t stride, cudaStream_t st) {
     const int items = dim / kItem;
 #define Q8K_Q_LAUNCH(ITEMS, T)                                                                  \
-    Q8K_CUDA_OK(launch_dependent(tokenwise_quant_kernel<Tin, Tout, ITEMS, T>, (unsigned)rows, T, 0, st, 1,     \
-                                 (const Tin*)x, (Tout*)q, scales, dim, stride, two_step))
+    Q8K_CUDA_OK(launch_dependent(tokenwise_quant_kernel<Tin, Tout, ITEMS, T, GATED>, (unsigned)rows, T, 0, st, 1,     \
+                                 (const Tin*)x, (Tout*)q, scales, dim, stride))
     if (items <= 32)        Q8K_Q_LAUNCH(1, 32);
     else if (items <= 128)  Q8K_Q_LAUNCH(1, 128);
     else if (items <= 256)  Q8K_Q_LAUNCH(2, 128);
@@ -498,7 +491,8 @@ static int check_rows_dim(const char* op, int64_t rows, int dim, int multiple) {
 using namespace q8k;
 
 namespace q8k {
-int tokenwise_quant_as(const char* op, bool two_step, const void* x, int x_dtype, void* q, int q_dtype, float* scales, int64_t rows, int dim,
+template <bool GATED>
+int tokenwise_quant_as(const char* op, const void* x, int x_dtype, void* q, int q_dtype, float* scales, int64_t rows, int dim,
                        int64_t x_row_stride, cudaStream_t st) {
     if (int rc = check_rows_dim(op, rows, dim, 16)) return rc;
     if (rows == 0) return Q8K_OK;
@@ -509,24 +503,24 @@ int tokenwise_quant_as(const char* op, bool two_step, const void* x, int x_dtype
     Q8K_REQUIRE(q_dtype == Q8K_DT_I8 || q_dtype == Q8K_DT_E4M3, Q8K_ERR_UNSUPPORTED,
                 "%s: output dtype %d is not int8 or e4m3", op, q_dtype);
 #define Q8K_QD(TIN)                                                                              \
-    return q_dtype == Q8K_DT_I8 ? launch_quant<TIN, int8_t>(op, two_step, x, q, scales, rows, dim, x_row_stride, st) \
-                                : launch_quant<TIN, e4m3_t>(op, two_step, x, q, scales, rows, dim, x_row_stride, st)
-    switch (x_dtype) {
-        case Q8K_DT_F32:  Q8K_QD(float);
-        case Q8K_DT_F16:  Q8K_QD(__half);
-        case Q8K_DT_BF16: Q8K_QD(__nv_bfloat16);
-        case Q8K_DT_E4M3: Q8K_QD(e4m3_t);
-        default: break;
+    return q_dtype == Q8K_DT_I8 ? launch_quant<TIN, int8_t, GATED>(op, x, q, scales, rows, dim, x_row_stride, st) \
+                                : launch_quant<TIN, e4m3_t, GATED>(op, x, q, scales, rows, dim, x_row_stride, st)
+    if constexpr (!GATED) {                                    // (the gated projection's rows are bf16 or e4m3)
+        if (x_dtype == Q8K_DT_F32) Q8K_QD(float);
+        if (x_dtype == Q8K_DT_F16) Q8K_QD(__half);
     }
+    if (x_dtype == Q8K_DT_BF16) Q8K_QD(__nv_bfloat16);
+    if (x_dtype == Q8K_DT_E4M3) Q8K_QD(e4m3_t);
 #undef Q8K_QD
     set_error_detail("%s: input dtype %d not supported", op, x_dtype);
     return Q8K_ERR_UNSUPPORTED;
 }
+template int tokenwise_quant_as<true>(const char*, const void*, int, void*, int, float*, int64_t, int, int64_t, cudaStream_t);
 }  // namespace q8k
 
 extern "C" int q8k_tokenwise_quant(const void* x, int x_dtype, void* q, int q_dtype, float* scales,
                                    int64_t rows, int dim, int64_t x_row_stride, void* stream) {
-    return tokenwise_quant_as("tokenwise_quant", false, x, x_dtype, q, q_dtype, scales, rows, dim, x_row_stride, (cudaStream_t)stream);
+    return tokenwise_quant_as<false>("tokenwise_quant", x, x_dtype, q, q_dtype, scales, rows, dim, x_row_stride, (cudaStream_t)stream);
 }
 
 extern "C" int q8k_transpose_quant(const void* x, int x_dtype, const float* row_scales, void* q, float* scales, int N, int K,

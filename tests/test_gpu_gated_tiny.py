@@ -103,3 +103,17 @@ def test_weight_columns(t):
     # the scale itself may be subnormal: w * scale is rounded to whole 2^-149
     bound = torch.maximum(ref.abs() * 2.0 ** -4, s.double().unsqueeze(1) * 2.0 ** -10) * (1 + 2.0 ** -20) + ref.abs() * 2.0 ** -20 + 2.0 ** -149
     assert ((q.double() * s.double().unsqueeze(1) - ref).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("rotate", [False, True])
+@pytest.mark.parametrize("src", [BF16, E4M3])
+@pytest.mark.parametrize("t", [I8, E4M3])
+@pytest.mark.parametrize("k", [16, 32, 64, 128, 256, 272, 512, 1024, 2048, 3088, 4096, 5504, 8192, 16384])
+def test_rows_of_zeros(rotate, src, t, k):
+    from q8_kernels_b200 import native
+    x = torch.randn(40, k, generator=torch.Generator(device="cuda").manual_seed(k), device="cuda").to(BF16).to(src)
+    x[::3], x[4] = 0.0, -0.0
+    rows = list(range(0, 40, 3)) + [4]
+    linears = native.hadamard_quant(x, k ** -0.5, t) if rotate else native.tokenwise_quant(x, t)
+    for q, s in (native.gated_quant(x, rotate, t), linears):
+        assert (q[rows].float() == 0).all() and (s[rows] == 0).all() and (s[1] > 0) and (q[1].float() != 0).any()
