@@ -18,7 +18,7 @@ constexpr int kGatedItem = 8;
 constexpr int kGatedMaxF = 16384;
 
 // act(g) and its derivative of two adjacent columns, both from s = 1 / (1 + e^(-v)):  silu: v = g, act' = s + g s (1 - s);  tanh-GELU:
-// v = 2 sqrt(2/pi) (g + c g^3), act' = s + g s (1 - s) v'.  Where s (1 - s) is 0 the second term is, too, also where g^2 has overflowed.
+// v = 2 sqrt(2/pi) (g + c g^3), act' = s + g s (1 - s) v'.  Their errors are those of gated_act in gemm_gated.cu.  Where s (1 - s) is 0 the second term is, too, also where g^2 has overflowed.
 // Packed pairs: element by element the kernel issued 26 instructions a column, half of its slots.
 template <bool GELU> __device__ __forceinline__ void gated_act_grad(float2 g, float2& act, float2& grad) {
     constexpr float kLog2e = 1.4426950408889634f, kA = 2.0f * 0.7978845608028654f, kB = kA * 0.044715f;

@@ -58,8 +58,10 @@ struct GatedParams {
     int n_tiles, total_tiles;
 };
 
-// silu(g) = g / (1 + e^-g); tanh-GELU = g / (1 + e^(-2u)) with u = sqrt(2/pi) (g + 0.044715 g^3): no cancellation anywhere, a few fp32
-// ulps.  e^(-x) overflows to infinity for very negative x, and g / infinity is the right 0.
+// silu(g) = g / (1 + e^-g); tanh-GELU = g / (1 + e^(-2u)) with u = sqrt(2/pi) (g + 0.044715 g^3): no cancellation anywhere.  The exponent
+// v = g or 2u is rounded to fp32 before the exponential, so the result is off by up to (5 |v| + 12) 2^-24 of itself where v is negative (its
+// constants and products; ex2 and rcp are good to 2^-22) and by some units of 2^-24 where it is positive: at v = -20 2^-17, far below half a
+// step of bf16, 2^-8, which is what it is rounded to.  e^(-v) overflows to infinity for very negative v, and g / infinity is the right 0.
 template <bool GELU> __device__ __forceinline__ float gated_act(float g) {
     constexpr float kLog2e = 1.4426950408889634f;
     float t;
