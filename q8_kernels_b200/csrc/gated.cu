@@ -18,7 +18,8 @@ constexpr int kGatedItem = 8;
 constexpr int kGatedMaxF = 16384;
 
 // act(g) and its derivative of two adjacent columns, both from s = 1 / (1 + e^(-v)):  silu: v = g, act' = s + g s (1 - s);  tanh-GELU:
-// v = 2 sqrt(2/pi) (g + c g^3), act' = s + g s (1 - s) v'.  Their errors are those of gated_act in gemm_gated.cu.  Where s (1 - s) is 0 the second term is, too, also where g^2 has overflowed.
+// v = 2 sqrt(2/pi) (g + c g^3), act' = s + g s (1 - s) v'.  Their errors are those of gated_act in gemm_gated.cu.  Where s (1 - s) is 0 the
+// second term is, too, also where g^2 has overflowed.
 // Packed pairs: element by element the kernel issued 26 instructions a column, half of its slots.
 template <bool GELU> __device__ __forceinline__ void gated_act_grad(float2 g, float2& act, float2& grad) {
     constexpr float kLog2e = 1.4426950408889634f, kA = 2.0f * 0.7978845608028654f, kB = kA * 0.044715f;
@@ -160,6 +161,9 @@ static int launch_gated_backward_as(const void* dout, const void* pre, void* q, 
     return Q8K_OK;
 }
 
+// Both sides of each limit: the layout that is taken at the widest rows it holds | the next one for the same rows.  us of 24 million gates,
+// silu and GELU, by F:
+//   512  39.3|40.1 41.0|46.4    1024  36.5|35.9 37.8|40.6    2048  35.0|31.3 34.4|35.4    4096  34.4|36.0 33.5|38.0    8192  31.6|36.1 33.0|39.1
 template <bool GELU>
 static int launch_gated_backward(const void* dout, const void* pre, void* q, float* scales, int M, int F, cudaStream_t st) {
     const int items = F / kGatedItem;
@@ -174,10 +178,11 @@ static int launch_gated_backward(const void* dout, const void* pre, void* q, flo
 }
 
 // The weight operand of the backward product: w [N, K] (int8 or e4m3) times its row scales, transposed and quantised to e4m3 with one
-// scale per row of the result, i.e. per column of w.  Bound by HBM: w is read once and q written once; a column's absmax needs all
-// rows first, so there are two passes, the second of which finds w in L2, with a small kernel between them that makes the columns'
-// factors of the partial maxima (taken by each CTA of the second pass for itself, 64 dependent loads, they were most of its time:
-// 16384 x 2048 int8 40.9 us).  Now 22.5 us, where w once in and q once out are 10.
+// scale per row of the result, i.e. per column of w.  w is read once and q written once; a column's absmax needs all rows first, so
+// there are two passes, the second of which finds w in L2, with a small kernel between them that makes the columns' factors of the
+// partial maxima (taken by each CTA of the second pass for itself, 64 dependent loads, they were most of its time: 16384 x 2048
+// int8 40.9 us).  Now 22.5 us, where w once in and q once out are 10: bound by instruction issue, every element being widened and scaled twice
+// (53 and 58 % of the slots), and by three launches in a row.
 //
 // Tiles of 128 columns, 16 per thread (one 16-byte load of a row), so a warp reads four rows of 128 bytes.
 constexpr int kWtCols = 128;
@@ -185,7 +190,7 @@ constexpr int kWtMaxRows = 512;              // rows whose absmax one CTA takes,
 constexpr int kWtRows = 128;                 // rows of a tile that is quantised and turned
 constexpr int kWtThreads = 256;
 
-// Four elements times their row's scale, as packed pairs of columns: both passes are bound by instruction issue.
+// Four elements times their row's scale, as packed pairs of columns.
 template <typename Tw> __device__ __forceinline__ void wt_values(uint32_t w, float s, float2 (&v)[2]) {
     if constexpr (std::is_same_v<Tw, int8_t>) {
         // 2^23 + 128 + b has the byte b + 128 in its last bits: a permutation and an exact difference instead of a conversion,

@@ -12,8 +12,8 @@
 // and TMEM allocation, warps 2-9 epilogue; two accumulators, so that the epilogue of a tile runs under the products of
 // the next.
 //
-// Bound by the tensor pipe: 6144 x 2048 x 8192 int8 134 us, 3.1 POP/s, pipe 92.6 % busy.  With SAVE 165 us (80 %): the 201 MB of gate and up
-// cross L2 beside the operands (2.2 GB instead of 1.6); without their stores alone it runs at 135 again.  Tried there: six stages with two
+// Bound by the tensor pipe: 6144 x 2048 x 8192 int8 134 us, 3.1 POP/s, pipe 91.3 % busy.  With SAVE 165 us (79.2 %): the 201 MB of gate and
+// up cross L2 beside the operands (2.2 GB instead of 1.6); without their stores alone it runs at 135 again.  Tried there: six stages with two
 // boxes (no change), boxes of 128 bytes a row (170), stores marked evict-first (164 to 167: DRAM reads 115 -> 90 MB, time within
 // the noise).
 

@@ -456,6 +456,16 @@ layer_norm_wgrad_kernel(const float* __restrict__ part, int parts, float* __rest
 // ------------------------------------------------------------------ host side
 // Layouts.  fp32 rows have twice the bytes for the same instructions, and above 768 columns 16 elements a thread do better with them
 // (6144 x 2048: forward 17.7 us against 20.4 with 32, backward 24.7 against 29.7).
+// Both sides of each limit: the layout that is taken at the widest rows it holds | the next one for the same rows.  us of the forward pass, of
+// dx, and of dx with the sums, by columns; 24 million elements of bf16, 12 million of fp32:
+//   bf16   256  20.8|22.4 31.3|31.7 34.9|38.1     512  15.7|18.0 25.1|24.7 29.8|33.4     768  15.1|17.5 23.1|24.4 29.9|33.1
+//         1024  15.3|19.6 23.3|25.6 30.2|37.9    1536  15.9|18.7 24.2|25.5 32.5|34.7    2048  16.1|19.2 24.3|26.4 30.7|40.4
+//         3000  16.8|19.2 25.5|27.1 36.2|40.0    4096  16.3|20.3 24.5|36.4 32.0|45.0    6144  16.6|24.1 (backward: no limit)
+//         8192  19.9|30.0 26.6|44.9 35.6|64.2
+//   fp32   256  18.5|16.0 24.7|24.8 28.2|28.7     512  15.7|14.7 22.9|21.7 26.9|27.1     768  16.0|16.3 22.0|23.4 27.4|27.8
+//         1024  16.4|18.2 23.0|24.7 27.1|29.3    2048  17.4|19.1 23.4|27.2 27.1|33.8    4096  18.7|18.3 24.9|29.1 30.3|34.6
+//         8192  20.8|26.4 26.5|45.3 35.4|52.9
+// Behind the next one: narrow rows of fp32, by up to a seventh in the forward pass.
 enum : int { kLnForward, kLnDx, kLnSums };   // backward pass without and with dw and db
 template <int PASS, bool FP32, typename F> static int ln_layout(int dim, F&& f) {
     const int items = (dim + kLnItem - 1) / kLnItem;

@@ -9,7 +9,7 @@ from ..native import E4M3, layer_norm_backward, refuse_tangents
 from ..native import layer_norm as _layer_norm
 
 
-class LayerNorm8bit(torch.autograd.Function):
+class LayerNormFunc(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, out_type):
         y, mean, rstd = _layer_norm(x, weight, bias, eps, out_type, True)
@@ -38,5 +38,5 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         return fast
     refuse_tangents("layer_norm", x, weight, bias)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
-        return LayerNorm8bit.apply(x, weight, bias, eps, out_type)
+        return LayerNormFunc.apply(x, weight, bias, eps, out_type)
     return _layer_norm(x, weight, bias, eps, out_type, False)[0]
