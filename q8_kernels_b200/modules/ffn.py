@@ -35,8 +35,8 @@ class GatedFeedForward(nn.Module):
     def forward(self, x, out_dtype=torch.bfloat16):
         h = self.gate_up(x)
         dim = self.proj_down.out_features
-        if h.numel() == 0:                                   # the linears' backward pass does not take a tensor without rows
-            return h[..., :1].expand(*h.shape[:-1], dim).to(out_dtype)
+        if h.numel() == 0 and h.requires_grad:               # the linears' backward pass does not take a tensor without rows
+            return h[..., :1].expand(*h.shape[:-1], dim).to(h.dtype if out_dtype is None else out_dtype)
         if h.dim() not in (2, 3):
             h = h.reshape(-1, self.inner_dim)
         return self.proj_down(h, out_dtype=out_dtype).reshape(*x.shape[:-1], dim)

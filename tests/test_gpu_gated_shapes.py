@@ -40,3 +40,13 @@ def test_feed_forward_keeps_the_shape(linear, lead):
     if x.numel():
         leaf = flat.clone().requires_grad_(True)
         assert torch.equal(bits(dx), bits(torch.autograd.grad(leaf + ff(norm(leaf)), [leaf], g.view(flat.shape))[0].view(x.shape)))
+
+
+@pytest.mark.parametrize("linear", ["int8", "fp8"])
+def test_output_types_without_rows(linear):
+    from q8_kernels_b200.modules import GatedFeedForward
+    ff = filled(GatedFeedForward(512, 256, linear=linear).cuda())
+    x = torch.randn(4, 512, device="cuda").to(BF16)
+    for kwargs in ({}, {"out_dtype": BF16}, {"out_dtype": None}):
+        y, none = ff(x, **kwargs), ff(x[:0], **kwargs)
+        assert y.shape == (4, 512) and none.shape == (0, 512) and none.dtype == y.dtype
