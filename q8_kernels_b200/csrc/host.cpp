@@ -895,7 +895,8 @@ PyObject* _rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
                pos->size(-1) == seq && (pos->dim() == 1 || pos->size(0) == 1 || pos->size(0) == batch));
     }
     OR_NONE(c);
-    c.need((q->size(d - 2) + (k != nullptr ? k->size(d - 2) : 0)) * dim <= (1 << 24) && !has_tangent(q) && !has_tangent(k));
+    c.need((q->size(d - 2) + (k != nullptr ? k->size(d - 2) : 0)) * dim <= (1 << 24) && !has_tangent(q) && !has_tangent(k) &&
+           !has_tangent(freq));
     OR_NONE(c);
     return answer([&]() -> PyObject* {
         variable_list out;
@@ -1012,7 +1013,8 @@ PyObject* _gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t k = b->size(1), nn = b->size(0), m = a->numel() / k;
     const bool training = c10::GradMode::is_enabled() && a->requires_grad();
     c.need(nn > 0 && nn % 32 == 0 && nn <= 0x3fffffff && k % 16 == 0 && k <= 16384 && m <= 0x7fffff00 && scale->numel() == nn &&
-           (bias == nullptr || bias->numel() == nn) && !(training && nn > 2 * 16384) && !has_tangent(a));
+           (bias == nullptr || bias->numel() == nn) && !(training && nn > 2 * 16384) && !has_tangent(a) &&
+           !has_tangent(bias) && !has_tangent(scale));
     c.status();
     OR_NONE(c);
     return answer([&]() -> PyObject* {

@@ -56,7 +56,7 @@ def _gated(op, a, b, bias, scale_a, scale_b, act, int8, rotate):
         fast = native._host._gated_linear(a, b, bias, scale_b, native.ACTIVATIONS.get(act, 0), int8, rotate)
         if fast is not None:
             return fast
-    native.refuse_tangents(op, a)
+    native.refuse_tangents(op, a, bias, scale_a, scale_b)
     weight_type = torch.int8 if int8 else E4M3
     if b.dtype != weight_type or scale_b is None:
         raise native.Q8KernelError(f"{op}: the weight must be {weight_type} with its scales")

@@ -95,7 +95,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional
     fast = _host._rotary(q, k, positions, frequencies, amplitude, half)
     if fast is not None:
         return fast
-    refuse_tangents("apply_rotary", q, k)
+    refuse_tangents("apply_rotary", q, k, frequencies)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return Rotary.apply(q, k, positions, frequencies, amplitude, half)
     return _rotary(q, k, positions, frequencies, amplitude, half, False)

@@ -50,3 +50,19 @@ def test_module():
     q = torch.randn(3, 4, 64, device="cuda").to(BF16)
     with fwd.dual_level(), pytest.raises(Q8KernelError, match="forward-mode"):
         m(fwd.make_dual(q, torch.ones_like(q)))
+
+
+def test_tangents_of_what_is_frozen():
+    from q8_kernels_b200 import Q8KernelError, native
+    from q8_kernels_b200.functional import gated, rotary
+    x = torch.randn(12, 64, device="cuda").to(BF16)
+    w, ws = native.tokenwise_quant(torch.randn(64, 64, device="cuda").to(BF16), I8)
+    bias, freq = torch.zeros(64, device="cuda"), rotary.rotary_frequencies(64)[0].cuda()
+    with fwd.dual_level():
+        def dual(t):
+            return fwd.make_dual(t, torch.ones_like(t))
+
+        for bad in (lambda: gated.q8_gated_linear(x, w, dual(bias), None, ws), lambda: gated.q8_gated_linear(x, w, bias, None, dual(ws)),
+                    lambda: rotary.apply_rotary(x.view(1, 3, 4, 64), None, None, dual(freq))):
+            with pytest.raises(Q8KernelError, match="forward-mode"):
+                bad()
