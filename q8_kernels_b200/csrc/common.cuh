@@ -123,7 +123,7 @@ inline int dtype_size(int dt) {
 // the other: the operator's definition has to say which.
 // Below top / FLT_MAX (1.3e-36) there is no such factor; an infinite one would make NaN of the row's zeros.  The gated projection
 // takes FLT_MAX there, which leaves such rows fewer steps and loses nothing that 1 / FLT_MAX can hold; only a row of zeros has an infinite factor
-// (scale 0), and its zeros are not multiplied.
+// (scale 0), and its zeros are multiplied by 0 instead.
 template <bool TwoStep> __device__ __forceinline__ float quant_factor(float top, float absmax) {
     if constexpr (!TwoStep) return __fdiv_rn(top, absmax);
     const float f = __fmul_rn(top, __frcp_rn(absmax));

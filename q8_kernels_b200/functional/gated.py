@@ -7,7 +7,8 @@ are wanted, quantise with them and pass ``scale_a``.  As there, weights are froz
 gradient of [gate | up] is quantised per token and the de-quantised weight per input channel to e4m3, the FP8 GEMM
 multiplies them, and the result is rotated back where the forward pass rotated.  Both the product and the rotated result are rounded to
 bf16, as in q8_linear's backward pass: the transform takes 16-bit rows, and half a bf16 step is far below the e4m3 steps before it (a step of
-2002 x 2048 x 5504 is 0.00239 from 64 bits, and 0.00236 with the product in fp32).  fp16 activations are rounded to bf16 first.
+2002 x 2048 x 5504 is 0.0024 from 64 bits, the formulas in fp32 with that product unrounded 0.0024 to 0.0026).  fp16 activations are rounded
+to bf16 first.
 
 A row with NaN gives NaN throughout, in int8 too; rows of values down to the smallest ones give no NaN.  There are no forward-mode derivatives.
 """
