@@ -103,8 +103,8 @@ static int gemm_8bit(bool int8, const void* a, const void* b, const float* bias,
     Q8K_REQUIRE(N % 16 == 0 && K % 16 == 0, Q8K_ERR_INVALID_ARG, "%s: N=%d and K=%d must be multiples of 16", op, N, K);
     Q8K_REQUIRE(aligned16(a) && aligned16(b) && aligned16(out), Q8K_ERR_INVALID_ARG,
                 "%s: a, b and out must be 16-byte aligned", op);
-    Q8K_REQUIRE(out_dtype == Q8K_DT_BF16 || out_dtype == Q8K_DT_E4M3, Q8K_ERR_UNSUPPORTED,
-                "%s: output dtype %d is not bf16 or e4m3", op, out_dtype);
+    Q8K_REQUIRE(out_dtype == Q8K_DT_BF16 || out_dtype == Q8K_DT_E4M3 || (out_dtype == Q8K_DT_F16 && !int8 && fuse_gelu == 0 && resid == nullptr),
+                Q8K_ERR_UNSUPPORTED, "%s: output dtype %d is not bf16 or e4m3", op, out_dtype);
     Q8K_REQUIRE((int64_t)bs_a * M <= 0x7fffffffLL && (int64_t)bs_b * N <= 0x7fffffffLL, Q8K_ERR_TOO_LARGE,
                 "%s: batch * rows exceeds 2^31", op);
     if (M == 0) return Q8K_OK;
@@ -123,19 +123,19 @@ static int gemm_8bit(bool int8, const void* a, const void* b, const float* bias,
     p.batch_a = bs_a > 1; p.batch_b = bs_b > 1;
     cudaStream_t st = (cudaStream_t)stream;
     const bool gelu = fuse_gelu != 0;
-    const bool e4m3 = out_dtype == Q8K_DT_E4M3;
+    const int kind = out_dtype == Q8K_DT_E4M3 ? kOutE4m3 : out_dtype == Q8K_DT_F16 ? kOutF16 : kOutBf16;
 
     const bool fuse_resid = resid != nullptr;
     if (fuse_resid) {
-        Q8K_REQUIRE(!gelu && !e4m3, Q8K_ERR_UNSUPPORTED, "%s: the gate/residual tail needs a bf16 output without GELU", op);
+        Q8K_REQUIRE(!gelu && kind == kOutBf16, Q8K_ERR_UNSUPPORTED, "%s: the gate/residual tail needs a bf16 output without GELU", op);
         Q8K_REQUIRE(aligned16(resid) && aligned16(gate), Q8K_ERR_INVALID_ARG, "%s: gate and residual must be 16-byte aligned", op);
     }
     const SplitChoice choice = choose_split(int8, M, N, K, batch, gemm_num_sms());
     if (!choice.use) {
-        const int rc = launch_gemm_pair(int8, gelu, e4m3, fuse_resid, a, b, p, bs_a, bs_b, st);
+        const int rc = launch_gemm_pair(int8, gelu, kind, fuse_resid, a, b, p, bs_a, bs_b, st);
         if (rc != Q8K_ERR_UNSUPPORTED) return rc;              // (the device cannot co-schedule the pairs)
     }
-    return launch_gemm_split(int8, gelu, e4m3, fuse_resid, a, b, p, bs_a, bs_b, choice.bn, choice.sk, st);
+    return launch_gemm_split(int8, gelu, kind, fuse_resid, a, b, p, bs_a, bs_b, choice.bn, choice.sk, st);
 }
 
 }  // namespace q8k

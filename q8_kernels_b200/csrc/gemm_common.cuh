@@ -27,6 +27,20 @@ struct GemmParams {
     int64_t rows_per_gate;
 };
 
+// Output types of the epilogues (fp16 for e4m3 operands without GELU and residual only).
+enum { kOutBf16 = 0, kOutE4m3 = 1, kOutF16 = 2 };
+
+// Two adjacent columns as 16-bit values of the output's type.
+template <bool F16> __device__ __forceinline__ uint32_t pack16(float2 y) {
+    if constexpr (F16) {
+        const __half2 h = __floats2half2_rn(y.x, y.y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(y.x, y.y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
 __device__ __forceinline__ float gelu_tanh_fast(float y) {
     // tanh.approx has ~2^-11 absolute error, far below the bf16 / e4m3 output step.
     const float u = 0.7978845608028654f * fmaf(0.044715f * y * y, y, y);
@@ -63,14 +77,14 @@ __device__ __forceinline__ float2 epilogue_pair(uint32_t r0, uint32_t r1, float2
 // CTA-pair (cta_group::2) variant: 256 x 256 output tiles per cluster of two CTAs.  Returns
 // Q8K_ERR_UNSUPPORTED (without touching the error detail) when the device cannot co-schedule
 // the clusters, in which case the caller falls back to the split kernel.
-int launch_gemm_pair(bool int8, bool gelu, bool out_e4m3, bool resid, const void* a, const void* b, const GemmParams& p,
+int launch_gemm_pair(bool int8, bool gelu, int out, bool resid, const void* a, const void* b, const GemmParams& p,
                      int bs_a, int bs_b, cudaStream_t st);
 // Columns of the tiles of the last round of such a launch (256: not cut).
 int pair_last_round_columns(int M, int N, int K, int batch, bool resid);
 
 // 128 x bn tiles, each owned by a cluster of sk CTAs that split K (see gemm_split.cu): bn a multiple of 16 up to 256
 // (with sk = 4 of 32), sk 1, 2 or 4 (fp8: 1) and at most the number of 128-byte K slabs.
-int launch_gemm_split(bool int8, bool gelu, bool out_e4m3, bool resid, const void* a, const void* b, const GemmParams& p,
+int launch_gemm_split(bool int8, bool gelu, int out, bool resid, const void* a, const void* b, const GemmParams& p,
                       int bs_a, int bs_b, int bn, int sk, cudaStream_t st);
 inline int split_a_rows(int M) { return M >= kGemmBM ? kGemmBM : (M + 7) / 8 * 8; }   // rows of A that a tile loads
 

@@ -97,12 +97,14 @@ __device__ __forceinline__ PairTile pair_tile(const PairParams& pp, int tile) {
 }
 
 // NARROW: the launch has narrow tiles (see narrow_plan).
-template <bool INT8, bool GELU, bool OUT_E4M3, bool RESID, bool NARROW>
+template <bool INT8, bool GELU, int OUT, bool RESID, bool NARROW>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
 gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                       const __grid_constant__ CUtensorMap tmap_bn, const __grid_constant__ CUtensorMap tmap_c, const __grid_constant__ CUtensorMap tmap_r,
                       const PairParams pp) {
     using L = PairSmemT<RESID>;
+    constexpr bool OUT_E4M3 = OUT == kOutE4m3;
+    static_assert(OUT != kOutF16 || !RESID, "the residual is bf16");
     constexpr int kPairStages = L::kStages;
     const GemmParams& p = pp.g;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -388,6 +390,10 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                                     const int j = q * 8 + e * 2;
                                     const float2 y0 = epilogue_pair<INT8, GELU>(rc[j], rc[j + 1], sa2, col_scale_smem + cl + j,
                                                                                 bias_smem + cl + j);
+                                    if constexpr (OUT == kOutF16) {
+                                        w[e] = pack16<true>(y0);
+                                        continue;
+                                    }
                                     __nv_bfloat162 b2 = __floats2bfloat162_rn(y0.x, y0.y);
                                     if constexpr (RESID) {
                                         // out = bf16(bf16(gate * bf16(y)) + resid), the roundings of the separate torch
@@ -457,6 +463,10 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
 #pragma unroll
                                 for (int q = 0; q < 4; ++q) {
                                     const int j = v4 * 8 + q * 2;
+                                    if constexpr (OUT == kOutF16) {
+                                        w[q] = pack16<true>(make_float2(y[j], y[j + 1]));
+                                        continue;
+                                    }
                                     __nv_bfloat162 b2 = __floats2bfloat162_rn(y[j], y[j + 1]);
                                     if constexpr (RESID) {
                                         // out = bf16(bf16(gate * bf16(y)) + resid): the roundings of the separate
@@ -507,11 +517,11 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
 }
 
 // ------------------------------------------------------------------ host side
-template <bool INT8, bool GELU, bool OUT_E4M3, bool RESID, bool NARROW>
+template <bool INT8, bool GELU, int OUT, bool RESID, bool NARROW>
 static int launch_pair_as(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tbn, const CUtensorMap& tc,
                        const CUtensorMap& tr, const PairParams& pp, cudaStream_t st) {
     using PairSmem = PairSmemT<RESID>;
-    auto kern = gemm_8bit_pair_kernel<INT8, GELU, OUT_E4M3, RESID, NARROW>;
+    auto kern = gemm_8bit_pair_kernel<INT8, GELU, OUT, RESID, NARROW>;
     static std::atomic<uint64_t> smem_done{0};
     if (int rc = allow_dynamic_smem((const void*)kern, PairSmem::kDynamic, smem_done)) return rc;
     // how many 2-CTA clusters can be resident at once (cached per kernel variant)
@@ -536,11 +546,11 @@ static int launch_pair_as(const CUtensorMap& ta, const CUtensorMap& tb, const CU
     return Q8K_OK;
 }
 
-template <bool INT8, bool GELU, bool OUT_E4M3, bool RESID = false>
+template <bool INT8, bool GELU, int OUT, bool RESID = false>
 static int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tbn, const CUtensorMap& tc,
                        const CUtensorMap& tr, const PairParams& pp, cudaStream_t st) {
-    return pp.narrow_bn != kPairBN ? launch_pair_as<INT8, GELU, OUT_E4M3, RESID, true>(ta, tb, tbn, tc, tr, pp, st)
-                                   : launch_pair_as<INT8, GELU, OUT_E4M3, RESID, false>(ta, tb, tbn, tc, tr, pp, st);
+    return pp.narrow_bn != kPairBN ? launch_pair_as<INT8, GELU, OUT, RESID, true>(ta, tb, tbn, tc, tr, pp, st)
+                                   : launch_pair_as<INT8, GELU, OUT, RESID, false>(ta, tb, tbn, tc, tr, pp, st);
 }
 
 // The last round of 256 x 256 tiles may leave most of the clusters idle: M = 6144, N = 2048 are 192 tiles, two rounds of 74 and
@@ -593,9 +603,10 @@ int pair_last_round_columns(int M, int N, int K, int batch, bool resid) {
     return pp.narrow_bn;
 }
 
-int launch_gemm_pair(bool int8, bool gelu, bool out_e4m3, bool resid, const void* a, const void* b, const GemmParams& p,
+int launch_gemm_pair(bool int8, bool gelu, int out, bool resid, const void* a, const void* b, const GemmParams& p,
                      int bs_a, int bs_b, cudaStream_t st) {
     const char* op = int8 ? "q8_mm" : "fp8_mm";
+    const bool out_e4m3 = out == kOutE4m3;
     CUtensorMap ta, tb;
     {
         const uint64_t dims[2] = {(uint64_t)p.K, (uint64_t)bs_a * (uint64_t)p.M};
@@ -643,16 +654,17 @@ int launch_gemm_pair(bool int8, bool gelu, bool out_e4m3, bool resid, const void
     }
 #define Q8K_PAIR(I8)                                                                  \
     do {                                                                              \
-        if (gelu) return out_e4m3 ? launch_pair<I8, true, true>(ta, tb, tbn, tc, tr, pp, st)       \
-                                  : launch_pair<I8, true, false>(ta, tb, tbn, tc, tr, pp, st);     \
-        return out_e4m3 ? launch_pair<I8, false, true>(ta, tb, tbn, tc, tr, pp, st)                \
-                        : launch_pair<I8, false, false>(ta, tb, tbn, tc, tr, pp, st);              \
+        if (gelu) return out_e4m3 ? launch_pair<I8, true, kOutE4m3>(ta, tb, tbn, tc, tr, pp, st)       \
+                                  : launch_pair<I8, true, kOutBf16>(ta, tb, tbn, tc, tr, pp, st);     \
+        return out_e4m3 ? launch_pair<I8, false, kOutE4m3>(ta, tb, tbn, tc, tr, pp, st)                \
+                        : launch_pair<I8, false, kOutBf16>(ta, tb, tbn, tc, tr, pp, st);              \
     } while (0)
     if (resid) {
-        return int8 ? launch_pair<true, false, false, true>(ta, tb, tbn, tc, tr, pp, st)
-                    : launch_pair<false, false, false, true>(ta, tb, tbn, tc, tr, pp, st);
+        return int8 ? launch_pair<true, false, kOutBf16, true>(ta, tb, tbn, tc, tr, pp, st)
+                    : launch_pair<false, false, kOutBf16, true>(ta, tb, tbn, tc, tr, pp, st);
     }
     if (int8) Q8K_PAIR(true);
+    if (out == kOutF16) return launch_pair<false, false, kOutF16>(ta, tb, tbn, tc, tr, pp, st);
     Q8K_PAIR(false);
 #undef Q8K_PAIR
 }

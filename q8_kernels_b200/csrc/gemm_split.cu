@@ -55,7 +55,7 @@ __device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint32_t a, uint32_
 
 // NC (a multiple of 8) adjacent columns of one row: scale, bias, GELU, cast, gate / residual, 16-byte (e4m3: 8-byte)
 // stores.  n is the first column; columns from p.N on are left out (N % 16 == 0: eight are all in or all out).
-template <bool INT8, bool GELU, bool OUT_E4M3, bool RESID, int NC>
+template <bool INT8, bool GELU, int OUT, bool RESID, int NC>
 __device__ __forceinline__ void finish_row(const GemmParams& p, const uint32_t (&acc)[NC], float sa, int64_t out_row,
                                            int64_t gate_row, int n, const float* col_scale, const float* bias) {
 #pragma unroll
@@ -67,7 +67,7 @@ __device__ __forceinline__ void finish_row(const GemmParams& p, const uint32_t (
                 y[j] = epilogue_pair<INT8, GELU>(acc[g * 8 + 2 * j], acc[g * 8 + 2 * j + 1], make_float2(sa, sa),
                                                  col_scale + g * 8 + 2 * j, bias + g * 8 + 2 * j);
             const int64_t o = out_row + n + g * 8;
-            if constexpr (OUT_E4M3) {
+            if constexpr (OUT == kOutE4m3) {
                 uint2 w;
                 w.x = (uint32_t)float2_to_e4m3x2_sat(y[0].x, y[0].y) | ((uint32_t)float2_to_e4m3x2_sat(y[1].x, y[1].y) << 16);
                 w.y = (uint32_t)float2_to_e4m3x2_sat(y[2].x, y[2].y) | ((uint32_t)float2_to_e4m3x2_sat(y[3].x, y[3].y) << 16);
@@ -81,6 +81,10 @@ __device__ __forceinline__ void finish_row(const GemmParams& p, const uint32_t (
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
+                    if constexpr (OUT == kOutF16) {
+                        w[j] = pack16<true>(y[j]);
+                        continue;
+                    }
                     __nv_bfloat162 b2 = __floats2bfloat162_rn(y[j].x, y[j].y);
                     if constexpr (RESID) {                      // the roundings of the separate ops: see gemm_pair.cu
                         const uint32_t gw = j == 0 ? gt.x : (j == 1 ? gt.y : (j == 2 ? gt.z : gt.w));
@@ -107,7 +111,7 @@ __device__ __forceinline__ void split_tmem_any(int bn, bool alloc, uint32_t arg)
     else split_tmem<256>(alloc, arg);
 }
 
-template <bool INT8, bool GELU, bool OUT_E4M3, bool RESID>
+template <bool INT8, bool GELU, int OUT, bool RESID>
 __global__ void __launch_bounds__(kGemmThreads, 2)
 gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                        const __grid_constant__ SplitParams sp) {
@@ -243,7 +247,7 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                 ptx::tmem_ld_32x32b_x16(t_row + cl, r);
                 ptx::tmem_wait_ld();
                 if (row_ok)
-                    finish_row<INT8, GELU, OUT_E4M3, RESID, 16>(p, r, sa, out_row, gate_row, n0 + cl, col_scale_smem + cl, bias_smem + cl);
+                    finish_row<INT8, GELU, OUT, RESID, 16>(p, r, sa, out_row, gate_row, n0 + cl, col_scale_smem + cl, bias_smem + cl);
                 __syncwarp();
             }
         }
@@ -288,7 +292,7 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                     }
                 }
                 const int cl = rank * cpc + c8;
-                finish_row<INT8, GELU, OUT_E4M3, RESID, 8>(p, acc, sa, out_row, gate_row, n0 + cl, col_scale_smem + cl, bias_smem + cl);
+                finish_row<INT8, GELU, OUT, RESID, 8>(p, acc, sa, out_row, gate_row, n0 + cl, col_scale_smem + cl, bias_smem + cl);
             }
         }
     }
@@ -307,18 +311,19 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
 }
 
 // ------------------------------------------------------------------ host side
-template <bool INT8, bool GELU, bool OUT_E4M3, bool RESID>
+template <bool INT8, bool GELU, int OUT, bool RESID>
 static int launch_split(const CUtensorMap& ta, const CUtensorMap& tb, const SplitParams& sp, int smem, cudaStream_t st) {
-    auto kern = gemm_8bit_split_kernel<INT8, GELU, OUT_E4M3, RESID>;
+    auto kern = gemm_8bit_split_kernel<INT8, GELU, OUT, RESID>;
     static std::atomic<uint64_t> smem_done{0};
     if (int rc = allow_dynamic_smem((const void*)kern, 226 * 1024, smem_done)) return rc;
     Q8K_CUDA_OK(launch_dependent(kern, (unsigned)sp.g.total_tiles * (unsigned)sp.sk, kGemmThreads, smem, st, sp.sk, ta, tb, sp));
     return Q8K_OK;
 }
 
-int launch_gemm_split(bool int8, bool gelu, bool out_e4m3, bool resid, const void* a, const void* b, const GemmParams& p,
+int launch_gemm_split(bool int8, bool gelu, int out, bool resid, const void* a, const void* b, const GemmParams& p,
                       int bs_a, int bs_b, int bn, int sk, cudaStream_t st) {
     const char* op = int8 ? "q8_mm" : "fp8_mm";
+    const bool out_e4m3 = out == kOutE4m3;
     const int a_rows = split_a_rows(p.M);
     CUtensorMap ta, tb;
     {
@@ -359,13 +364,14 @@ int launch_gemm_split(bool int8, bool gelu, bool out_e4m3, bool resid, const voi
     const int smem = stages * sp.stage_bytes + SplitSmem::kTotal + 1024;   // slack to align the base to 1024 B
 #define Q8K_SPLIT(I8)                                                                     \
     do {                                                                                  \
-        if (resid) return launch_split<I8, false, false, true>(ta, tb, sp, smem, st);     \
-        if (gelu) return out_e4m3 ? launch_split<I8, true, true, false>(ta, tb, sp, smem, st)    \
-                                  : launch_split<I8, true, false, false>(ta, tb, sp, smem, st);  \
-        return out_e4m3 ? launch_split<I8, false, true, false>(ta, tb, sp, smem, st)      \
-                        : launch_split<I8, false, false, false>(ta, tb, sp, smem, st);    \
+        if (resid) return launch_split<I8, false, kOutBf16, true>(ta, tb, sp, smem, st);     \
+        if (gelu) return out_e4m3 ? launch_split<I8, true, kOutE4m3, false>(ta, tb, sp, smem, st)    \
+                                  : launch_split<I8, true, kOutBf16, false>(ta, tb, sp, smem, st);  \
+        return out_e4m3 ? launch_split<I8, false, kOutE4m3, false>(ta, tb, sp, smem, st)      \
+                        : launch_split<I8, false, kOutBf16, false>(ta, tb, sp, smem, st);    \
     } while (0)
     if (int8) Q8K_SPLIT(true);
+    if (out == kOutF16) return launch_split<false, false, kOutF16, false>(ta, tb, sp, smem, st);
     Q8K_SPLIT(false);
 #undef Q8K_SPLIT
 }
