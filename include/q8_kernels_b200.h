@@ -164,8 +164,9 @@ Q8K_API int q8k_rms_norm_backward(const void* x_normed, int x_dtype, const float
 /* 8-bit GEMM  C[b] = act((A[b] . B[b]^T) * (sa[m]*sb[n]) + bias[n]).
  * A [bs_a, M, K], B [bs_b, N, K] K-contiguous int8 (q8k_q8_mm) or e4m3
  * (q8k_fp8_mm); bs_a == bs_b or one of them 1; sa [bs_a, M], sb [bs_b, N],
- * bias [N] fp32 or NULL; C [max(bs_a,bs_b), M, N] bf16 (RNE) or e4m3
- * (saturating).  N % 16 == 0, K % 16 == 0, all pointers 16-byte aligned.
+ * bias [N] fp32 or NULL; C [max(bs_a,bs_b), M, N] bf16 (RNE), e4m3
+ * (saturating) or, of e4m3 operands without GELU, fp16 (RNE).
+ * N % 16 == 0, K % 16 == 0, all pointers 16-byte aligned.
  * Replaces q8_mm / q8_mm_bias / fp8_mm / fp8_mm_bias:
  * csrc/gemm/q8_gemm_api.cpp:40-291 and the run_* launchers declared at :27-35. */
 Q8K_API int q8k_q8_mm(const void* a, const void* b, const float* bias, const float* a_scales,
@@ -354,6 +355,41 @@ Q8K_API int q8k_rotary(const void* q, const int64_t q_strides[3], void* q_out, c
                int64_t position_token_stride, const double* frequencies, float amplitude, int batch, int seq, int head_dim,
                int rotary_dim, int half_layout, int backward, void* stream);
 
+/* The same with positions of several axes (time, height, width): pair i turns by the position on axis axes[i] (int32 [rotary_dim / 2], one
+ * beyond the last axis is taken as the last) times frequencies[i].  positions of position_type Q8K_POS_* at {batch, token, axis}
+ * strides in elements; fractional ones are as good as whole ones.  No counterpart in the reference.                               */
+#define Q8K_POS_I32 1
+#define Q8K_POS_I64 2
+#define Q8K_POS_F32 3
+#define Q8K_POS_F64 4
+Q8K_API int q8k_axial_rotary(const void* q, const int64_t q_strides[3], void* q_out, const int64_t q_out_strides[3], int q_heads,
+                     const void* k, const int64_t k_strides[3], void* k_out, const int64_t k_out_strides[3], int k_heads, int dtype,
+                     const void* positions, int position_type, const int64_t position_strides[3], int n_axes, const int* axes,
+                     const double* frequencies, float amplitude, int batch, int seq, int head_dim, int rotary_dim,
+                     int half_layout, int backward, void* stream);
+
+/* Norm and rotation of queries and keys in one pass: every head of q [batch, seq, q_heads, head_dim] and k (as for q8k_rotary) becomes
+ * R(x / sqrt(mean(x^2) + eps) * weight), nothing rounded in between; q_weight and k_weight fp32 [head_dim] or NULL.  The rotation is that
+ * of q8k_rotary (axes NULL: position strides of batch and token) or q8k_axial_rotary; rotary_dim 0 has none, and needs neither
+ * positions nor frequencies.  head_dim up to 512.  Outputs must not share memory with inputs.  No counterpart in the reference.     */
+Q8K_API int q8k_head_norm(const void* q, const int64_t q_strides[3], const float* q_weight, void* q_out, const int64_t q_out_strides[3], int q_heads,
+                  const void* k, const int64_t k_strides[3], const float* k_weight, void* k_out, const int64_t k_out_strides[3], int k_heads,
+                  int dtype, float eps, const void* positions, int position_type, const int64_t position_strides[3], int n_axes,
+                  const int* axes, const double* frequencies, float amplitude, int batch, int seq, int head_dim, int rotary_dim,
+                  int half_layout, void* stream);
+/* Its gradients: dq and dk from the inputs and the outputs' gradients (each with strides; a tensor with heads of 0 is left out), and the
+ * weights' in fp32 [head_dim], each NULL if it is not wanted.  The sums over tokens and heads need a workspace of
+ * q8k_head_norm_backward_workspace_bytes (16-byte aligned) and are taken in an order that the sizes fix: the same bits in every call
+ * of the same sizes.                                                                                                             */
+Q8K_API size_t q8k_head_norm_backward_workspace_bytes(int head_dim);
+Q8K_API int q8k_head_norm_backward(const void* q, const int64_t q_strides[3], const float* q_weight, const void* q_grad, const int64_t q_grad_strides[3],
+                  void* dq, const int64_t dq_strides[3], float* dq_weight, int q_heads,
+                  const void* k, const int64_t k_strides[3], const float* k_weight, const void* k_grad, const int64_t k_grad_strides[3],
+                  void* dk, const int64_t dk_strides[3], float* dk_weight, int k_heads,
+                  int dtype, float eps, const void* positions, int position_type, const int64_t position_strides[3], int n_axes,
+                  const int* axes, const double* frequencies, float amplitude, int batch, int seq, int head_dim, int rotary_dim,
+                  int half_layout, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Gated projection: out = act(gate) * up in bf16 [M, F], where gate and up are the products of a [M, K] (int8, or e4m3 if !int8) with the
  * first and the last F rows of w [2F, K], times a_scales[m] * w_scales[n], plus bias[n] (fp32 [2F] or NULL).  pre: NULL, or
  * bf16 [M, 2, F] for gate and up, which the backward pass takes.  activation: Q8K_ACT_*.  F and K multiples of 16, pointers 16-byte
@@ -387,6 +423,41 @@ Q8K_API int q8k_gated_backward_quant(const void* grad, const void* pre, void* q,
 Q8K_API size_t q8k_gated_weight_operand_workspace_bytes(int F, int K);
 Q8K_API int q8k_gated_weight_operand(const void* w, int w_dtype, const float* w_scales, void* q, float* scales, int F, int K,
                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* Microscaled 4-bit values (no counterpart in the reference).  Values are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two a byte,
+ * the first in the low nibble: [rows, K / 2], K a multiple of 32 up to 65536.  Q8K_FP4_MX: blocks of 32 along a row share an e8m0 scale.
+ * Q8K_FP4_NV: blocks of 16 share an e4m3 scale, and a row has an fp32 scale.  Block scales, q8k_fp4_scale_bytes of them, lie as
+ * [row tiles of 128][tiles of 4 blocks][512]: row r's scales of blocks 4 t .. 4 t + 3 at (r % 32) * 16 + (r / 32 % 4) * 4 of tile t, with
+ * K filled up to a multiple of 256.                                                                                              */
+#define Q8K_FP4_MX 1
+#define Q8K_FP4_NV 2
+Q8K_API size_t q8k_fp4_scale_bytes(int format, int64_t rows, int K);
+/* Quantizer: x bf16 or fp16, x_row_stride elements between rows (16-byte aligned).  mxfp4: a block's scale is 2^e with
+ * e = floor(log2 absmax) - 2, at least -127, and values are x 2^-e.  nvfp4, in fp32: the row's scale is r = absmax / 2688, a block's
+ * s = e4m3(its absmax * (448 / absmax)), and values are x * (1 / (s r)), 0 where s is 0.  Values are rounded to nearest, halves to even,
+ * and beyond 6 to 6.  A factor beyond FLT_MAX is FLT_MAX.  NaN and infinities make the block's scale (mxfp4) or the row's scales
+ * (nvfp4) such that products with the row are NaN.  Block scales of rows behind the last one are not written.                    */
+Q8K_API int q8k_fp4_quant(const void* x, int x_dtype, int64_t x_row_stride, int format, void* values, void* block_scales, float* row_scales,
+                  int64_t rows, int K, void* stream);
+/* What they stand for, rounded to y_dtype (bf16, fp16 or fp32): y dense [rows, K].                                               */
+Q8K_API int q8k_fp4_dequant(const void* values, const void* block_scales, const float* row_scales, int format, void* y, int y_dtype, int64_t rows,
+                    int K, void* stream);
+/* out [M, N] (bf16 or fp16) = act((a . b^T) + bias[n]) of a [M, K] and b [N, K] of one format; bias fp32 or NULL, act tanh-GELU with
+ * fuse_gelu.  N a multiple of 16.                                                                                                */
+Q8K_API int q8k_fp4_mm(int format, const void* a, const void* a_block_scales, const float* a_row_scales, const void* b, const void* b_block_scales,
+               const float* b_row_scales, const float* bias, void* out, int out_dtype, int M, int N, int K, int fuse_gelu,
+               int* dev_status, void* stream);
+/* q8k_fp4_quant of x (dense) and q8k_fp4_mm in one call, over a workspace of q8k_fp4_linear_workspace_bytes (256-byte aligned).    */
+Q8K_API size_t q8k_fp4_linear_workspace_bytes(int format, int M, int K);
+Q8K_API int q8k_fp4_linear(int format, const void* x, int x_dtype, const void* w, const void* w_block_scales, const float* w_row_scales,
+                   const float* bias, void* out, int out_dtype, int M, int N, int K, int fuse_gelu, void* workspace,
+                   size_t workspace_bytes, int* dev_status, void* stream);
+/* The weight operand of its backward product: w [N, K] (N a multiple of 16) de-quantised to fp32, transposed and quantised to e4m3 with one
+ * scale per input channel (factor 448 / absmax): q [K, N], scales [K].  The workspace has q8k_fp4_weight_operand_workspace_bytes,
+ * 16-byte aligned.                                                                                                               */
+Q8K_API size_t q8k_fp4_weight_operand_workspace_bytes(int N, int K);
+Q8K_API int q8k_fp4_weight_operand(int format, const void* values, const void* block_scales, const float* row_scales, void* q, float* scales, int N,
+                           int K, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

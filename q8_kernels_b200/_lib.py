@@ -89,6 +89,13 @@ SIGNATURES = {
                                          _c_ptr]),
     "q8k_rotary": (_c_int, [_c_ptr] * 4 + [_c_int] + [_c_ptr] * 4 + [_c_int, _c_int, _c_ptr, _c_int, _c_i64, _c_i64, _c_ptr, _c_f32]
                    + [_c_int] * 6 + [_c_ptr]),
+    "q8k_axial_rotary": (_c_int, [_c_ptr] * 4 + [_c_int] + [_c_ptr] * 4 + [_c_int, _c_int, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_f32]
+                         + [_c_int] * 6 + [_c_ptr]),
+    "q8k_head_norm": (_c_int, ([_c_ptr] * 5 + [_c_int]) * 2 + [_c_int, _c_f32, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_f32] + [_c_int] * 5
+                      + [_c_ptr]),
+    "q8k_head_norm_backward_workspace_bytes": (_c_size, [_c_int]),
+    "q8k_head_norm_backward": (_c_int, ([_c_ptr] * 8 + [_c_int]) * 2 + [_c_int, _c_f32, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_f32]
+                               + [_c_int] * 5 + [_c_ptr, _c_size, _c_ptr]),
     "q8k_gated_mm": (_c_int, [_c_int] + [_c_ptr] * 7 + [_c_int] * 4 + [_c_ptr, _c_ptr]),
     "q8k_gated_plan": (_c_int, [_c_int] * 3 + [_c_ptr]),
     "q8k_gated_linear_workspace_bytes": (_c_size, [_c_int, _c_int]),
@@ -96,6 +103,14 @@ SIGNATURES = {
     "q8k_gated_quant": (_c_int, [_c_ptr, _c_int, _c_i64, _c_ptr, _c_int, _c_ptr, _c_i64, _c_int, _c_int, _c_ptr]),
     "q8k_gated_weight_operand_workspace_bytes": (_c_size, [_c_int, _c_int]),
     "q8k_gated_weight_operand": (_c_int, [_c_ptr, _c_int] + [_c_ptr] * 3 + [_c_int, _c_int, _c_ptr, _c_size, _c_ptr]),
+    "q8k_fp4_scale_bytes": (_c_size, [_c_int, _c_i64, _c_int]),
+    "q8k_fp4_quant": (_c_int, [_c_ptr, _c_int, _c_i64, _c_int] + [_c_ptr] * 3 + [_c_i64, _c_int, _c_ptr]),
+    "q8k_fp4_dequant": (_c_int, [_c_ptr] * 3 + [_c_int, _c_ptr, _c_int, _c_i64, _c_int, _c_ptr]),
+    "q8k_fp4_mm": (_c_int, [_c_int] + [_c_ptr] * 8 + [_c_int] * 5 + [_c_ptr, _c_ptr]),
+    "q8k_fp4_linear_workspace_bytes": (_c_size, [_c_int] * 3),
+    "q8k_fp4_linear": (_c_int, [_c_int, _c_ptr, _c_int] + [_c_ptr] * 5 + [_c_int] * 5 + [_c_ptr, _c_size, _c_ptr, _c_ptr]),
+    "q8k_fp4_weight_operand_workspace_bytes": (_c_size, [_c_int, _c_int]),
+    "q8k_fp4_weight_operand": (_c_int, [_c_int] + [_c_ptr] * 5 + [_c_int, _c_int, _c_ptr, _c_size, _c_ptr]),
     "q8k_gated_backward_quant": (_c_int, [_c_ptr] * 4 + [_c_int] * 3 + [_c_ptr]),
 }
 

@@ -1,0 +1,424 @@
+// Quantizer of microscaled 4-bit values (fp4.cuh has the formats) and what goes back from them.
+//
+//   mxfp4   exponent e = max(floor(log2(absmax of the block)) - 2, -127), values x 2^-e rounded to e2m1
+//   nvfp4   r = A / 2688 (6 * 448) with A the row's absmax; a block of absmax a gets s = e4m3(a (448 / A)) and its values are rounded
+//           from x (1 / (s r)); s = 0 leaves zeros.  All in fp32, each operation rounded.
+// A factor that fp32 does not hold (rows whose absmax is below 1.3e-36, blocks below some 1e-37) is FLT_MAX, so that no zero becomes NaN.
+// A block of mxfp4 with NaN or an infinity has NaN as its scale, a row of nvfp4 NaN or infinity as its row scale: the row's products are NaN.
+
+#include <type_traits>
+#include "fp4.cuh"
+
+namespace q8k {
+
+constexpr int kFp4Unit = 16;                                   // values of a thread at a time: 32 bytes
+
+// |max| of two 16-bit values or of one fp32 value; NaN wins.
+template <typename T> struct Fp4In;
+template <> struct Fp4In<__nv_bfloat16> {
+    static __device__ __forceinline__ float absmax(const uint4 (&r)[2]) {
+        __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&r[0].x));
+        const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y, r[1].z, r[1].w};
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])));
+        const float2 f = __bfloat1622float2(m);
+        return max_nan(f.x, f.y);
+    }
+    static __device__ __forceinline__ void widen(const uint4& r, float (&v)[8]) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+};
+template <> struct Fp4In<__half> {
+    static __device__ __forceinline__ float absmax(const uint4 (&r)[2]) {
+        __half2 m = __habs2(*reinterpret_cast<const __half2*>(&r[0].x));
+        const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y, r[1].z, r[1].w};
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&w[i])));
+        const float2 f = __half22float2(m);
+        return max_nan(f.x, f.y);
+    }
+    static __device__ __forceinline__ void widen(const uint4& r, float (&v)[8]) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+};
+
+__device__ __forceinline__ float fp4_finite(float factor) { return fminf(factor, 3.402823466e38f); }
+
+// A unit's values times `factor`, as 8 bytes.
+template <typename T> __device__ __forceinline__ uint2 fp4_pack(const uint4 (&r)[2], float factor) {
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float v[8];
+        Fp4In<T>::widen(r[h], v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], factor);
+        w[h] = float8_to_e2m1(v);
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+// T threads a row, `rows_per_cta` rows a CTA, UNITS units a thread.  The row's scales beyond K, up to its last slab, become 0.
+template <typename Tin, bool NV, int UNITS>
+__global__ void __launch_bounds__(1024)
+fp4_quant_kernel(const Tin* __restrict__ x, int64_t x_stride, uint8_t* __restrict__ q, uint8_t* __restrict__ block_scales,
+                 float* __restrict__ row_scales, int64_t rows, int K, int slabs, int threads) {
+    __shared__ float red[32];
+    const int group = threadIdx.x / threads, t = threadIdx.x - group * threads;
+    const int64_t row = (int64_t)blockIdx.x * (blockDim.x / threads) + group;
+    const bool here = row < rows;
+    const int units = K / kFp4Unit;
+    pdl_wait();
+    pdl_release();
+    uint4 r[UNITS][2];
+    float a[UNITS];
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) {
+        const int u = t + i * threads;
+        const bool in = here && u < units;
+        const uint4* p = reinterpret_cast<const uint4*>(x + row * x_stride + u * kFp4Unit);
+        r[i][0] = in ? p[0] : make_uint4(0, 0, 0, 0);
+        r[i][1] = in ? p[1] : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) {
+        a[i] = Fp4In<Tin>::absmax(r[i]);
+        top = max_nan(top, a[i]);
+    }
+    float g = 0.f, rs = 0.f;
+    if constexpr (NV) {
+        top = warp_max<true>(top);
+        if (threads > 32) {                                    // one row a CTA then
+            if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+            __syncthreads();
+            top = warp_max<true>((threadIdx.x & 31) < blockDim.x / 32 ? red[threadIdx.x & 31] : 0.f);
+        }
+        g = top > 0.f || top != top ? fp4_finite(__fdiv_rn(448.0f, top)) : 0.f;
+        if (top != top) g = top;
+        rs = __fdiv_rn(top, 2688.0f);
+        if (here && t == 0) row_scales[row] = rs;
+    }
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) {
+        const int u = t + i * threads;
+        float factor;
+        uint8_t scale;
+        if constexpr (NV) {
+            scale = float_to_e4m3_sat(__fmul_rn(a[i], g));
+            const float s = e4m3_to_float(scale);
+            factor = s == 0.f ? 0.f : fp4_finite(__fdiv_rn(1.0f, __fmul_rn(s, rs)));
+        } else {
+            const float both = max_nan(a[i], __shfl_xor_sync(0xffffffffu, a[i], 1));     // a block of 32 is two neighbours' units
+            const int field = (int)(__float_as_uint(both) >> 23);                        // (no sign)
+            const int e = field == 255 ? 255 : field > 2 ? field - 2 : 0;
+            scale = (uint8_t)e;
+            factor = __uint_as_float((uint32_t)(254 - (e == 255 ? 254 : e)) << 23);      // 2^-e; any for NaN
+        }
+        if (here && u < units) *reinterpret_cast<uint2*>(q + row * (int64_t)(K / 2) + u * 8) = fp4_pack<Tin>(r[i], factor);
+        if (here && u < slabs * (kFp4Slab / kFp4Unit)) {
+            if constexpr (NV) block_scales[fp4_scale_at<true>(row, u, slabs)] = u < units ? scale : 0;
+            else if ((u & 1) == 0) block_scales[fp4_scale_at<false>(row, u >> 1, slabs)] = u < units ? scale : 0;
+        }
+    }
+}
+
+template <typename Tin, bool NV>
+static int launch_fp4_quant(const void* x, int64_t stride, void* q, void* bs, float* rs, int64_t rows, int K, cudaStream_t st) {
+    const int slabs = fp4_slabs(K), units = slabs * (kFp4Slab / kFp4Unit);
+    int threads = ((units + 3) / 4 + 31) / 32 * 32;            // four units a thread
+    const int per_cta = threads > 32 ? 1 : 4;
+    const int64_t grid = (rows + per_cta - 1) / per_cta;
+    auto go = [&](auto kern) {
+        Q8K_CUDA_OK(launch_dependent(kern, (unsigned)grid, (unsigned)(threads * per_cta), 0, st, 1, (const Tin*)x, stride, (uint8_t*)q, (uint8_t*)bs, rs,
+                                     rows, K, slabs, threads));
+        return (int)Q8K_OK;
+    };
+    if (threads <= 1024) return go(fp4_quant_kernel<Tin, NV, 4>);
+    set_error_detail("fp4_quant: K=%d exceeds 65536", K);
+    return Q8K_ERR_UNSUPPORTED;
+}
+
+// What the values stand for: value * block scale (exact in fp32) * row scale, rounded, then to Tout.
+template <typename Tout, bool NV>
+__global__ void __launch_bounds__(256)
+fp4_dequant_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ block_scales, const float* __restrict__ row_scales,
+                   Tout* __restrict__ y, int64_t rows, int K, int slabs) {
+    const int per_row = K / kFp4Unit;
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    pdl_wait();
+    pdl_release();
+    if (i >= rows * per_row) return;
+    const int64_t row = i / per_row;
+    const int u = (int)(i - row * per_row);
+    const uint2 w = *reinterpret_cast<const uint2*>(q + row * (int64_t)(K / 2) + u * 8);
+    const float s = fp4_scale_value<NV>(block_scales[fp4_scale_at<NV>(row, NV ? u : u >> 1, slabs)]);
+    const float r = NV ? row_scales[row] : 1.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float v[8];
+        e2m1_to_float8(h == 0 ? w.x : w.y, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = __fmul_rn(__fmul_rn(v[k], s), r);
+        store_vec<Tout, 8>(y + row * (int64_t)K + u * kFp4Unit + h * 8, v);
+    }
+}
+
+template <typename Tout> static int launch_fp4_dequant(bool nv, const void* q, const void* bs, const float* rs, void* y, int64_t rows, int K,
+                                                       cudaStream_t st) {
+    const int64_t threads = rows * (K / kFp4Unit);
+    auto kern = nv ? fp4_dequant_kernel<Tout, true> : fp4_dequant_kernel<Tout, false>;
+    Q8K_CUDA_OK(launch_dependent(kern, (unsigned)((threads + 255) / 256), 256, 0, st, 1, (const uint8_t*)q, (const uint8_t*)bs, rs, (Tout*)y, rows, K,
+                                 fp4_slabs(K)));
+    return Q8K_OK;
+}
+
+// ------------------------------------------------------------------ weight operand of the backward product
+// w [N, K] de-quantised (value * block scale, exact, times the row's scale, rounded to fp32), transposed and quantised to e4m3 with one scale
+// per input channel, factor 448 / absmax as the 8-bit linears have it.  Two passes over the weight, which is small: partial absmax of row
+// chunks, the factors, then tiles of 128 x 128 that are turned in shared memory.
+constexpr int kF4Cols = 128;                 // columns of a CTA: 8 groups of 16
+constexpr int kF4Rows = 128;                 // rows of a turned tile
+constexpr int kF4ChunkRows = 256;            // rows of a partial absmax
+constexpr int kF4Threads = 256;
+
+// 16 consecutive values of a row as fp32
+template <bool NV>
+__device__ __forceinline__ void fp4_load16(const uint8_t* __restrict__ w, const uint8_t* __restrict__ bs, const float* __restrict__ rs, int row, int c,
+                                           int K, int slabs, float (&v)[16]) {
+    const uint2 x = *reinterpret_cast<const uint2*>(w + (int64_t)row * (K / 2) + c / 2);
+    const float s = fp4_scale_value<NV>(bs[fp4_scale_at<NV>(row, c / (NV ? 16 : 32), slabs)]);
+    const float r = NV ? rs[row] : 1.f;
+    float lo[8], hi[8];
+    e2m1_to_float8(x.x, lo);
+    e2m1_to_float8(x.y, hi);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        v[j] = __fmul_rn(__fmul_rn(lo[j], s), r);
+        v[8 + j] = __fmul_rn(__fmul_rn(hi[j], s), r);
+    }
+}
+
+template <bool NV>
+__global__ void __launch_bounds__(kF4Threads)
+fp4_weight_absmax_kernel(const uint8_t* __restrict__ w, const uint8_t* __restrict__ bs, const float* __restrict__ rs, float* __restrict__ part, int N,
+                         int K, int slabs) {
+    __shared__ float red[kF4Threads / 32][kF4Cols];
+    pdl_wait();
+    pdl_release();
+    const int cg = threadIdx.x & 7, rl = threadIdx.x >> 3;
+    const int c0 = blockIdx.x * kF4Cols + cg * 16;
+    float m[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) m[j] = 0.f;
+    if (c0 < K) {
+#pragma unroll 4
+        for (int i = 0; i < kF4ChunkRows / 32; ++i) {
+            const int row = blockIdx.y * kF4ChunkRows + i * 32 + rl;
+            if (row < N) {
+                float v[16];
+                fp4_load16<NV>(w, bs, rs, row, c0, K, slabs, v);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) m[j] = fmaxf(m[j], fabsf(v[j]));
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        m[j] = fmaxf(m[j], __shfl_xor_sync(0xffffffffu, m[j], 8));
+        m[j] = fmaxf(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
+        if ((threadIdx.x & 31) < 8) red[threadIdx.x >> 5][cg * 16 + j] = m[j];
+    }
+    __syncthreads();
+    const int c = blockIdx.x * kF4Cols + threadIdx.x;
+    if (threadIdx.x < kF4Cols && c < K) {
+        float a = red[0][threadIdx.x];
+#pragma unroll
+        for (int k = 1; k < kF4Threads / 32; ++k) a = fmaxf(a, red[k][threadIdx.x]);
+        part[(int64_t)blockIdx.y * K + c] = a;
+    }
+}
+
+// scales[c] = 1 / (448 / absmax of column c) as the row quantizer leaves it; the factors follow the partial maxima
+__global__ void __launch_bounds__(256)
+fp4_weight_factor_kernel(float* __restrict__ part, int parts, float* __restrict__ scales, int K) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    pdl_wait();
+    pdl_release();
+    if (c >= K) return;
+    float a = 0.f;
+    for (int k = 0; k < parts; ++k) a = fmaxf(a, part[(int64_t)k * K + c]);
+    const float f = __fdiv_rn(448.0f, a);
+    part[(int64_t)parts * K + c] = a == 0.f ? 0.f : f;
+    scales[c] = __fdiv_rn(1.0f, f);
+}
+
+template <bool NV>
+__global__ void __launch_bounds__(kF4Threads)
+fp4_weight_turn_kernel(const uint8_t* __restrict__ w, const uint8_t* __restrict__ bs, const float* __restrict__ rs, const float* __restrict__ factors,
+                       uint8_t* __restrict__ q, int N, int K, int slabs) {
+    __shared__ __align__(16) float mul[kF4Cols];
+    __shared__ __align__(16) uint32_t turned[kF4Cols][kF4Rows / 4];
+    const int cb = blockIdx.x * kF4Cols, r0 = blockIdx.y * kF4Rows;
+    const int cg = threadIdx.x & 7, rg = threadIdx.x >> 3;     // 16 columns, four rows
+    pdl_wait();
+    pdl_release();
+    if (threadIdx.x < kF4Cols) mul[threadIdx.x] = cb + (int)threadIdx.x < K ? factors[cb + threadIdx.x] : 0.f;
+    __syncthreads();
+    const int c0 = cb + cg * 16;
+    if (c0 < K && r0 + rg * 4 < N) {                           // N % 16 == 0: all four rows exist, or none
+        float v[4][16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fp4_load16<NV>(w, bs, rs, r0 + rg * 4 + i, c0, K, slabs, v[i]);
+        // row group rg of a column goes to word rg + 4 * (column group): the words that a warp stores lie in 32 banks, and four of a
+        // column stay together for the 16-byte reads below
+        const int at = (rg + 4 * cg) & 31;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float f = mul[cg * 16 + j];
+            turned[cg * 16 + j][at] = (uint32_t)float2_to_e4m3x2_sat(__fmul_rn(v[0][j], f), __fmul_rn(v[1][j], f)) |
+                                      ((uint32_t)float2_to_e4m3x2_sat(__fmul_rn(v[2][j], f), __fmul_rn(v[3][j], f)) << 16);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kF4Cols / 32; ++i) {
+        const int c = i * 32 + (threadIdx.x >> 3), part16 = threadIdx.x & 7;
+        const int n = r0 + part16 * 16;
+        if (cb + c < K && n < N)
+            *reinterpret_cast<uint4*>(q + (int64_t)(cb + c) * N + n) = *reinterpret_cast<const uint4*>(&turned[c][(part16 * 4 + 4 * (c / 16)) & 31]);
+    }
+}
+
+template <bool NV>
+static int launch_fp4_weight(const void* w, const void* bs, const float* rs, void* q, float* scales, float* part, int N, int K, cudaStream_t st) {
+    const unsigned cols = (unsigned)((K + kF4Cols - 1) / kF4Cols);
+    const int parts = (N + kF4ChunkRows - 1) / kF4ChunkRows, slabs = fp4_slabs(K);
+    Q8K_CUDA_OK(launch_dependent(fp4_weight_absmax_kernel<NV>, dim3(cols, (unsigned)parts), kF4Threads, 0, st, 1, (const uint8_t*)w, (const uint8_t*)bs, rs,
+                                 part, N, K, slabs));
+    Q8K_CUDA_OK(launch_dependent(fp4_weight_factor_kernel, dim3((unsigned)((K + 255) / 256)), 256, 0, st, 1, part, parts, scales, K));
+    Q8K_CUDA_OK(launch_dependent(fp4_weight_turn_kernel<NV>, dim3(cols, (unsigned)((N + kF4Rows - 1) / kF4Rows)), kF4Threads, 0, st, 1,
+                                 (const uint8_t*)w, (const uint8_t*)bs, rs, part + (int64_t)parts * K, (uint8_t*)q, N, K, slabs));
+    return Q8K_OK;
+}
+
+static int fp4_check(const char* op, int format, int64_t rows, int K) {
+    Q8K_REQUIRE(format == Q8K_FP4_MX || format == Q8K_FP4_NV, Q8K_ERR_UNSUPPORTED, "%s: format %d is unknown", op, format);
+    Q8K_REQUIRE(rows >= 0 && K > 0 && K % 32 == 0, Q8K_ERR_INVALID_ARG, "%s: rows %lld must not be negative and K=%d a positive multiple of 32", op,
+                (long long)rows, K);
+    Q8K_REQUIRE(K <= 65536, Q8K_ERR_UNSUPPORTED, "%s: K=%d exceeds 65536", op, K);
+    Q8K_REQUIRE(rows <= 0x7fffff00LL && rows * (K / 16) <= 0x7fffffffLL * 128, Q8K_ERR_TOO_LARGE, "%s: %lld rows of %d", op, (long long)rows, K);
+    return Q8K_OK;
+}
+
+}  // namespace q8k
+
+extern "C" size_t q8k_fp4_scale_bytes(int format, int64_t rows, int K) {
+    if (rows <= 0 || K <= 0 || (format != Q8K_FP4_MX && format != Q8K_FP4_NV)) return 0;
+    return (size_t)q8k::fp4_scale_bytes(format == Q8K_FP4_NV, rows, K);
+}
+
+extern "C" int q8k_fp4_quant(const void* x, int x_dtype, int64_t x_row_stride, int format, void* values, void* block_scales, float* row_scales,
+                             int64_t rows, int K, void* stream) {
+    using namespace q8k;
+    const char* op = "fp4_quant";
+    if (int rc = fp4_check(op, format, rows, K)) return rc;
+    const bool nv = format == Q8K_FP4_NV;
+    Q8K_REQUIRE(x_dtype == Q8K_DT_BF16 || x_dtype == Q8K_DT_F16, Q8K_ERR_UNSUPPORTED, "%s: input dtype %d is not bf16 or fp16", op, x_dtype);
+    if (rows == 0) return Q8K_OK;
+    Q8K_REQUIRE(x && values && block_scales && (row_scales || !nv) && aligned16(x) && aligned16(values) && aligned16(block_scales),
+                Q8K_ERR_INVALID_ARG, "%s: null or misaligned pointer", op);
+    Q8K_REQUIRE(rows == 1 || (x_row_stride >= K && x_row_stride % 8 == 0), Q8K_ERR_INVALID_ARG,
+                "%s: row stride %lld must be at least K and a multiple of 16 bytes", op, (long long)x_row_stride);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (x_dtype == Q8K_DT_BF16)
+        return nv ? launch_fp4_quant<__nv_bfloat16, true>(x, x_row_stride, values, block_scales, row_scales, rows, K, st)
+                  : launch_fp4_quant<__nv_bfloat16, false>(x, x_row_stride, values, block_scales, row_scales, rows, K, st);
+    return nv ? launch_fp4_quant<__half, true>(x, x_row_stride, values, block_scales, row_scales, rows, K, st)
+              : launch_fp4_quant<__half, false>(x, x_row_stride, values, block_scales, row_scales, rows, K, st);
+}
+
+extern "C" int q8k_fp4_dequant(const void* values, const void* block_scales, const float* row_scales, int format, void* y, int y_dtype, int64_t rows,
+                               int K, void* stream) {
+    using namespace q8k;
+    const char* op = "fp4_dequant";
+    if (int rc = fp4_check(op, format, rows, K)) return rc;
+    const bool nv = format == Q8K_FP4_NV;
+    Q8K_REQUIRE(y_dtype == Q8K_DT_BF16 || y_dtype == Q8K_DT_F16 || y_dtype == Q8K_DT_F32, Q8K_ERR_UNSUPPORTED,
+                "%s: output dtype %d is not bf16, fp16 or fp32", op, y_dtype);
+    if (rows == 0) return Q8K_OK;
+    Q8K_REQUIRE(y && values && block_scales && (row_scales || !nv) && aligned16(y) && aligned16(values), Q8K_ERR_INVALID_ARG,
+                "%s: null or misaligned pointer", op);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (y_dtype == Q8K_DT_BF16) return launch_fp4_dequant<__nv_bfloat16>(nv, values, block_scales, row_scales, y, rows, K, st);
+    if (y_dtype == Q8K_DT_F16) return launch_fp4_dequant<__half>(nv, values, block_scales, row_scales, y, rows, K, st);
+    return launch_fp4_dequant<float>(nv, values, block_scales, row_scales, y, rows, K, st);
+}
+
+extern "C" size_t q8k_fp4_weight_operand_workspace_bytes(int N, int K) {
+    if (N <= 0 || K <= 0) return 0;
+    return ((size_t)(N + q8k::kF4ChunkRows - 1) / q8k::kF4ChunkRows + 1) * (size_t)K * sizeof(float);   // partial maxima, factors
+}
+
+extern "C" int q8k_fp4_weight_operand(int format, const void* values, const void* block_scales, const float* row_scales, void* q, float* scales, int N,
+                                      int K, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace q8k;
+    const char* op = "fp4_weight_operand";
+    if (int rc = fp4_check(op, format, N, K)) return rc;
+    const bool nv = format == Q8K_FP4_NV;
+    Q8K_REQUIRE(N > 0 && N % 16 == 0, Q8K_ERR_INVALID_ARG, "%s: N=%d must be a positive multiple of 16", op, N);
+    Q8K_REQUIRE(N <= 65535 * kF4Rows, Q8K_ERR_TOO_LARGE, "%s: N=%d too large", op, N);
+    Q8K_REQUIRE(values && block_scales && (row_scales || !nv) && q && scales && workspace && aligned16(values) && aligned16(q) && aligned16(workspace),
+                Q8K_ERR_INVALID_ARG, "%s: null or misaligned pointer", op);
+    const size_t need = q8k_fp4_weight_operand_workspace_bytes(N, K);
+    Q8K_REQUIRE(workspace_bytes >= need, Q8K_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", op, workspace_bytes, need);
+    cudaStream_t st = (cudaStream_t)stream;
+    return nv ? launch_fp4_weight<true>(values, block_scales, row_scales, q, scales, (float*)workspace, N, K, st)
+              : launch_fp4_weight<false>(values, block_scales, row_scales, q, scales, (float*)workspace, N, K, st);
+}
+
+// Where the parts of the quantised activation lie in the workspace of q8k_fp4_linear.
+static void fp4_linear_parts(bool nv, int M, int K, size_t& scales_at, size_t& rows_at, size_t& bytes) {
+    scales_at = ((size_t)M * (size_t)(K / 2) + 255) / 256 * 256;
+    rows_at = scales_at + (size_t)q8k::fp4_scale_bytes(nv, M, K);          // (a multiple of 512)
+    bytes = rows_at + (nv ? (size_t)M * sizeof(float) : 0);
+}
+
+extern "C" size_t q8k_fp4_linear_workspace_bytes(int format, int M, int K) {
+    if (M <= 0 || K <= 0 || (format != Q8K_FP4_MX && format != Q8K_FP4_NV)) return 0;
+    size_t scales_at, rows_at, bytes;
+    fp4_linear_parts(format == Q8K_FP4_NV, M, K, scales_at, rows_at, bytes);
+    return bytes;
+}
+
+extern "C" int q8k_fp4_linear(int format, const void* x, int x_dtype, const void* w, const void* w_block_scales, const float* w_row_scales,
+                              const float* bias, void* out, int out_dtype, int M, int N, int K, int fuse_gelu, void* workspace,
+                              size_t workspace_bytes, int* dev_status, void* stream) {
+    using namespace q8k;
+    const char* op = "fp4_linear";
+    if (int rc = fp4_check(op, format, M, K)) return rc;
+    const bool nv = format == Q8K_FP4_NV;
+    Q8K_REQUIRE(N > 0 && N % 16 == 0, Q8K_ERR_INVALID_ARG, "%s: N=%d must be a positive multiple of 16", op, N);
+    if (M == 0) return Q8K_OK;
+    Q8K_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 256 == 0, Q8K_ERR_INVALID_ARG,
+                "%s: the workspace must be 256-byte aligned", op);
+    size_t scales_at, rows_at, need;
+    fp4_linear_parts(nv, M, K, scales_at, rows_at, need);
+    Q8K_REQUIRE(workspace_bytes >= need, Q8K_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", op, workspace_bytes, need);
+    uint8_t* values = static_cast<uint8_t*>(workspace);
+    uint8_t* blocks = values + scales_at;
+    float* rows = nv ? reinterpret_cast<float*>(values + rows_at) : nullptr;
+    if (int rc = q8k_fp4_quant(x, x_dtype, K, format, values, blocks, rows, M, K, stream)) return rc;
+    return q8k_fp4_mm(format, values, blocks, rows, w, w_block_scales, w_row_scales, bias, out, out_dtype, M, N, K, fuse_gelu, dev_status, stream);
+}

@@ -1,0 +1,297 @@
+// 4-bit GEMM with block scales: out = act((A . B^T) * (ra[m] * rb[n]) + bias[n]), A [M, K] and B [N, K] both mxfp4 or both nvfp4 (fp4.cuh).
+//
+// The tensor core multiplies the e2m1 values with their blocks' scales and adds in fp32 (kind::mxf4nvf4); the rows' scales (nvfp4),
+// the bias, tanh-GELU and the one rounding to 16 bits are the epilogue's.
+//
+// 128 x bn tiles, one a CTA.  Roles (10 warps):
+//   warp 0     TMA producer: values (128-byte slabs of 256) and block scales of the tile's rows and columns
+//   warp 1     TMEM allocation; one thread copies a slab's scales to TMEM and issues its four MMAs (K = 64)
+//   warps 2-9  epilogue
+// All waits are bounded.
+//
+// The scales of B can be named from every second column of TMEM only, i.e. from rows n that are multiples of 64.  A tile whose columns begin
+// elsewhere multiplies the window from the multiple of 64 below; the rows of B that it does not own are not loaded there, and what stands
+// in their place gives columns that nobody reads.
+
+#include "gemm_fp4.cuh"
+
+namespace q8k {
+
+constexpr int kFp4MaxStages = 8;
+constexpr int kFp4MaxBN = 192;
+constexpr int kFp4ABytes = kGemmBM * 128;
+struct Fp4Smem {                             // behind the operand ring
+    static constexpr int kNumBars = 2 * kFp4MaxStages + 1;
+    static constexpr int kTmemPtrOffset = kNumBars * 8;
+    static constexpr int kAbortOffset = kTmemPtrOffset + 4;
+    static constexpr int kColScaleOffset = (kAbortOffset + 4 + 15) & ~15;
+    static constexpr int kBiasOffset = kColScaleOffset + kFp4MaxBN * 4;
+    static constexpr int kTotal = kBiasOffset + kFp4MaxBN * 4;
+};
+struct Fp4TileParams {
+    Fp4GemmParams g;
+    int n_tiles;
+    int bn;                                  // tile columns, a multiple of 16
+    int window;                              // columns of the MMA, a multiple of 64: see above
+    int tmem_cols;                           // accumulator, scales of A, of B
+    int b_tiles;                             // 128-row tiles of B's scales that a window touches: 1 or 2
+    int stages, stage_bytes, load_bytes;
+};
+
+template <bool NV, bool GELU, bool F16>
+__global__ void __launch_bounds__(kGemmThreads, 2)
+gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_as,
+                const __grid_constant__ CUtensorMap tmap_bs, const __grid_constant__ Fp4TileParams sp) {
+    using L = Fp4Smem;
+    constexpr int TILES = fp4_slab_tiles(NV);                  // 512-byte scale tiles a slab
+    const Fp4GemmParams& p = sp.g;
+    const int bn = sp.bn, stages = sp.stages, nt = sp.b_tiles;
+
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t smem_base = ptx::smem_u32(smem);
+    uint8_t* tail = smem + stages * sp.stage_bytes;
+    const uint32_t bar_base = ptx::smem_u32(tail);
+    auto full_bar = [&](int s) { return bar_base + 8u * s; };
+    auto empty_bar = [&](int s) { return bar_base + 8u * (kFp4MaxStages + s); };
+    const uint32_t acc_bar = bar_base + 8u * (2 * kFp4MaxStages);
+    volatile uint32_t* tmem_ptr_smem = reinterpret_cast<volatile uint32_t*>(tail + L::kTmemPtrOffset);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + L::kAbortOffset);
+    float* col_scale_smem = reinterpret_cast<float*>(tail + L::kColScaleOffset);
+    float* bias_smem = reinterpret_cast<float*>(tail + L::kBiasOffset);
+    __shared__ int prior_failure;
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int n_blk = blockIdx.x % sp.n_tiles;
+    const int m_blk = blockIdx.x / sp.n_tiles;
+    const int slabs = (p.K + kFp4Slab - 1) / kFp4Slab;
+    const int n0 = n_blk * bn, off = n0 % 64, window = sp.window;
+    // offsets in a stage: A, B, A's scales, B's scales
+    const uint32_t b_at = kFp4ABytes, as_at = b_at + (uint32_t)window * 128u, bs_at = as_at + fp4_slab_scales(NV);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            ptx::mbar_init(full_bar(s), 1);
+            ptx::mbar_init(empty_bar(s), 1);
+        }
+        ptx::mbar_init(acc_bar, 1);
+        *abort_flag = 0;
+        ptx::fence_barrier_init();
+        ptx::fence_proxy_async_smem();
+        ptx::prefetch_tensormap(&tmap_a);
+        ptx::prefetch_tensormap(&tmap_b);
+        ptx::prefetch_tensormap(&tmap_as);
+        ptx::prefetch_tensormap(&tmap_bs);
+    }
+    if (warp == 1) {
+        if (sp.tmem_cols == 128) ptx::tmem_alloc<128>(ptx::smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)));
+        else ptx::tmem_alloc<256>(ptx::smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)));
+        ptx::tmem_relinquish_alloc_permit();
+    }
+    pdl_wait();
+    if (threadIdx.x == 0) prior_failure = p.status != nullptr ? *reinterpret_cast<volatile int*>(p.status) : 0;
+    ptx::tcgen05_fence_before_sync();
+    __syncthreads();
+    ptx::tcgen05_fence_after_sync();
+    pdl_release();
+    const uint32_t tmem_base = *tmem_ptr_smem;
+    bool ok = prior_failure == 0;
+
+    const int quarter = warp & 3;
+    const int half = (warp - 2) >> 2;
+
+    if (warp == 0) {
+        if (ok && ptx::elect_one()) {
+            int s = 0;
+            uint32_t ph = 1;                                   // empty_bar phase to wait for: the first round passes
+            constexpr int SLAB_ROWS = fp4_slab_scales(NV) / 256;
+            for (int i = 0; i < slabs; ++i) {
+                if (!ptx::mbar_wait(empty_bar(s), ph, abort_flag)) { ok = false; break; }
+                ptx::mbar_arrive_expect_tx(full_bar(s), (uint32_t)sp.load_bytes);
+                const uint32_t dst = smem_base + s * sp.stage_bytes;
+                ptx::tma_load_2d(dst, &tmap_a, full_bar(s), i * 128, m_blk * kGemmBM);
+                ptx::tma_load_2d(dst + b_at + (uint32_t)off * 128u, &tmap_b, full_bar(s), i * 128, n0);
+                ptx::tma_load_3d(dst + as_at, &tmap_as, full_bar(s), 0, i * SLAB_ROWS, m_blk);
+                ptx::tma_load_3d(dst + bs_at, &tmap_bs, full_bar(s), 0, i * SLAB_ROWS, n0 / 128);
+                if (++s == stages) { s = 0; ph ^= 1u; }
+            }
+            if (!ok && p.status != nullptr) atomicExch(p.status, Q8K_STATUS_TIMEOUT | (31 << 8));
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (ok && ptx::elect_one()) {
+            int s = 0;
+            uint32_t ph = 0;
+            const uint32_t ta = tmem_base + window, tb = ta + 4 * TILES;
+            const uint32_t tb0 = tb + (n0 % 128 >= 64 ? 2u : 0u);              // the window may begin in the middle of a tile of scales
+            uint32_t idesc[2] = {ptx::make_idesc_fp4(kGemmBM, window, !NV, 0), ptx::make_idesc_fp4(kGemmBM, window, !NV, 2)};
+            for (int i = 0; i < slabs; ++i) {
+                if (!ptx::mbar_wait(full_bar(s), ph, abort_flag)) { ok = false; break; }
+                ptx::tcgen05_fence_after_sync();
+                const uint32_t src = smem_base + s * sp.stage_bytes;
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    ptx::tmem_copy_scales<false>(ta + 4 * t, ptx::make_scales_desc(src + as_at + 512 * t));
+                    for (int j = 0; j < nt; ++j)
+                        ptx::tmem_copy_scales<false>(tb + 4 * (t * nt + j),
+                                                     ptx::make_scales_desc(src + bs_at + j * fp4_slab_scales(NV) + 512 * t));
+                }
+                const uint64_t a_desc = ptx::make_kmajor_desc(src, 128);
+                const uint64_t b_desc = ptx::make_kmajor_desc(src + b_at, 128);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int t = NV ? k : k / 2;
+                    ptx::mma_fp4<NV ? 4 : 2, false>(tmem_base, a_desc + 2 * k, b_desc + 2 * k, idesc[NV ? 0 : k & 1],
+                                                    ta + 4 * t, tb0 + 4 * t * nt, (i > 0 || k > 0) ? 1u : 0u);
+                }
+                ptx::tcgen05_commit(empty_bar(s));
+                if (++s == stages) { s = 0; ph ^= 1u; }
+            }
+            if (ok) ptx::tcgen05_commit(acc_bar);
+            else if (p.status != nullptr) atomicExch(p.status, Q8K_STATUS_TIMEOUT | (32 << 8));
+        }
+        __syncwarp();
+    } else if (ok) {
+        for (int c = threadIdx.x - 64; c < bn; c += kGemmEpilogueThreads) {
+            const int n = n0 + c;
+            const bool in = n < p.N;
+            col_scale_smem[c] = !in ? 0.f : p.b_scales != nullptr ? p.b_scales[n] : 1.f;
+            bias_smem[c] = (in && p.bias != nullptr) ? p.bias[n] : 0.f;
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const int row = m_blk * kGemmBM + quarter * 32 + lane;
+        const bool row_ok = row < p.M;
+        const float sa = !row_ok ? 0.f : p.a_scales != nullptr ? p.a_scales[row] : 1.f;
+        ok = ptx::mbar_wait(acc_bar, 0, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);                      // keep the warp convergent for tcgen05.ld
+        ptx::tcgen05_fence_after_sync();
+        if (!ok && p.status != nullptr && threadIdx.x == 64) atomicExch(p.status, Q8K_STATUS_TIMEOUT | (33 << 8));
+        if (ok) {
+            const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16);
+            uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + (int64_t)row * p.N + n0;
+#pragma unroll 1
+            for (int cl = half * 16; cl < bn; cl += 32) {
+                uint32_t r[16];
+                ptx::tmem_ld_32x32b_x16(t_row + off + cl, r);
+                ptx::tmem_wait_ld();
+                if (row_ok && n0 + cl < p.N) {                 // N % 16 == 0
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int c = g * 8 + 2 * j;
+                            w[j] = pack16<F16>(epilogue_pair<false, GELU>(r[c], r[c + 1], make_float2(sa, sa), col_scale_smem + cl + c,
+                                                                          bias_smem + cl + c));
+                        }
+                        *reinterpret_cast<uint4*>(out + cl + g * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+
+    if (threadIdx.x == 0 && *abort_flag != 0) {
+        // a wait was abandoned: give copies still in flight time to land before the CTA gives up its shared memory
+        const unsigned long long t0 = ptx::globaltimer_ns();
+        while (ptx::globaltimer_ns() - t0 < 50000ull) {}
+    }
+    ptx::tcgen05_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        ptx::tcgen05_fence_after_sync();
+        if (sp.tmem_cols == 128) ptx::tmem_dealloc<128>(tmem_base);
+        else ptx::tmem_dealloc<256>(tmem_base);
+    }
+}
+
+template <bool NV, bool GELU, bool F16>
+static int launch_fp4_as(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tas, const CUtensorMap& tbs, const Fp4TileParams& sp,
+                         unsigned grid, int smem, cudaStream_t st) {
+    auto kern = gemm_fp4_kernel<NV, GELU, F16>;
+    static std::atomic<uint64_t> smem_done{0};
+    if (int rc = allow_dynamic_smem((const void*)kern, 226 * 1024, smem_done)) return rc;
+    Q8K_CUDA_OK(launch_dependent(kern, grid, kGemmThreads, smem, st, 1, ta, tb, tas, tbs, sp));
+    return Q8K_OK;
+}
+
+static int launch_fp4_tiles(bool nv, bool gelu, bool f16, const Fp4Operand& a, const Fp4Operand& b, const Fp4GemmParams& p, int bn,
+                            cudaStream_t st) {
+    const char* op = "fp4_mm";
+    Fp4TileParams sp;
+    sp.g = p;
+    sp.bn = bn;
+    const int step = bn % 64 == 0 ? 64 : bn % 32 == 0 ? 32 : 16;               // the last tiles of a window begin 64 - step into it
+    sp.window = (64 - step + bn + 63) / 64 * 64;
+    sp.b_tiles = sp.window == 64 || bn == 128 ? 1 : 2;
+    const int a_rows = split_a_rows(p.M);
+    CUtensorMap ta, tb, tas, tbs;
+    if (int rc = make_values_map(&ta, a.values, p.M, p.K, a_rows, op)) return rc;
+    if (int rc = make_values_map(&tb, b.values, p.N, p.K, bn, op)) return rc;
+    if (int rc = make_scales_map(&tas, a.block_scales, nv, p.M, p.K, 1, op)) return rc;
+    if (int rc = make_scales_map(&tbs, b.block_scales, nv, p.N, p.K, sp.b_tiles, op)) return rc;
+    const int scales = fp4_slab_scales(nv);
+    sp.load_bytes = (a_rows + bn) * 128 + scales * (1 + sp.b_tiles);
+    sp.stage_bytes = ((kGemmBM + sp.window) * 128 + scales * (1 + sp.b_tiles) + 1023) / 1024 * 1024;
+    sp.tmem_cols = sp.window + 4 * fp4_slab_tiles(nv) * (1 + sp.b_tiles) <= 128 ? 128 : 256;
+    const int64_t m_tiles = (p.M + kGemmBM - 1) / kGemmBM;
+    sp.n_tiles = (p.N + bn - 1) / bn;
+    Q8K_REQUIRE(m_tiles * sp.n_tiles <= 0x7fffffffLL, Q8K_ERR_TOO_LARGE, "%s: too many tiles", op);
+    const int budget = m_tiles * sp.n_tiles <= gemm_num_sms() ? 208 * 1024 : 104 * 1024;
+    int stages = budget / sp.stage_bytes;
+    const int slabs = fp4_slabs(p.K);
+    if (stages > slabs) stages = slabs;
+    if (stages > kFp4MaxStages) stages = kFp4MaxStages;
+    sp.stages = stages;
+    const int smem = stages * sp.stage_bytes + Fp4Smem::kTotal + 1024;
+    const unsigned grid = (unsigned)(m_tiles * sp.n_tiles);
+#define Q8K_FP4(NV)                                                                                              \
+    do {                                                                                                         \
+        if (gelu) return f16 ? launch_fp4_as<NV, true, true>(ta, tb, tas, tbs, sp, grid, smem, st)               \
+                             : launch_fp4_as<NV, true, false>(ta, tb, tas, tbs, sp, grid, smem, st);             \
+        return f16 ? launch_fp4_as<NV, false, true>(ta, tb, tas, tbs, sp, grid, smem, st)                        \
+                   : launch_fp4_as<NV, false, false>(ta, tb, tas, tbs, sp, grid, smem, st);                      \
+    } while (0)
+    if (nv) Q8K_FP4(true);
+    Q8K_FP4(false);
+#undef Q8K_FP4
+}
+
+static int fp4_tile_columns(int M, int N) {
+    const int sms = gemm_num_sms();
+    const int64_t m_tiles = (M + kGemmBM - 1) / kGemmBM;
+    for (int bn : {16, 32, 48, 64, 80, 96, 128, 160})
+        if (m_tiles * ((N + bn - 1) / bn) <= sms) return bn;
+    return 192;
+}
+
+}  // namespace q8k
+
+extern "C" int q8k_fp4_mm(int format, const void* a, const void* a_block_scales, const float* a_row_scales, const void* b, const void* b_block_scales,
+                          const float* b_row_scales, const float* bias, void* out, int out_dtype, int M, int N, int K, int fuse_gelu,
+                          int* dev_status, void* stream) {
+    using namespace q8k;
+    const char* op = "fp4_mm";
+    Q8K_REQUIRE(format == Q8K_FP4_MX || format == Q8K_FP4_NV, Q8K_ERR_UNSUPPORTED, "%s: format %d is unknown", op, format);
+    const bool nv = format == Q8K_FP4_NV;
+    Q8K_REQUIRE(M >= 0 && N > 0 && K > 0 && N % 16 == 0 && K % 32 == 0, Q8K_ERR_INVALID_ARG,
+                "%s: M=%d must not be negative, N=%d a multiple of 16 and K=%d of 32", op, M, N, K);
+    Q8K_REQUIRE(M <= 0x7fffff00 && N <= 0x7fffff00, Q8K_ERR_TOO_LARGE, "%s: M=%d or N=%d too large", op, M, N);
+    Q8K_REQUIRE(out_dtype == Q8K_DT_BF16 || out_dtype == Q8K_DT_F16, Q8K_ERR_UNSUPPORTED, "%s: output dtype %d is not bf16 or fp16", op, out_dtype);
+    if (M == 0) return Q8K_OK;
+    Q8K_REQUIRE(a && a_block_scales && b && b_block_scales && out && (!nv || (a_row_scales && b_row_scales)), Q8K_ERR_INVALID_ARG,
+                "%s: null pointer", op);
+    Q8K_REQUIRE(aligned16(a) && aligned16(a_block_scales) && aligned16(b) && aligned16(b_block_scales) && aligned16(out), Q8K_ERR_INVALID_ARG,
+                "%s: values, block scales and out must be 16-byte aligned", op);
+    Fp4GemmParams p;
+    p.a_scales = nv ? a_row_scales : nullptr;
+    p.b_scales = nv ? b_row_scales : nullptr;
+    p.bias = bias;
+    p.out = out;
+    p.status = dev_status;
+    p.M = M; p.N = N; p.K = K;
+    return launch_fp4_tiles(nv, fuse_gelu != 0, out_dtype == Q8K_DT_F16, {a, a_block_scales, a_row_scales}, {b, b_block_scales, b_row_scales}, p,
+                            fp4_tile_columns(M, N), (cudaStream_t)stream);
+}

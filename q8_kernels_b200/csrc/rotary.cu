@@ -2,12 +2,10 @@
 // position * freq[i] and scaled by `amplitude`; the other channels are copied.
 //   a' = amplitude (a cos - b sin),  b' = amplitude (b cos + a sin)
 // with (a, b) = channels (2i, 2i + 1) in the interleaved layout and (i, i + rotary_dim / 2) in the half layout.  The backward pass is the
-// same kernel with the angle negated.
+// same kernel with the angle negated.  With several axes a pair takes the position of its own one.
 //
 // Bound by HBM: every element of q and k is read and written once, in one launch, and no table is read.  The angles are
-// computed here, once per token and pair, and shared by the heads through shared memory.  A position of a million radians has
-// no correct digit in fp32 after its reduction, so position * freq / (2 pi) is formed in fp64, the whole turns are dropped there, and
-// sine and cosine are taken of the rest, at most half a turn, in fp32.
+// computed here, once per token and pair (rotary.cuh), and shared by the heads through shared memory.
 //
 // What is left to save are instructions: at the copy rate an SM has some 15 for an element.  So a thread takes the same channels of
 // up to eight heads of one token: its cosines and sines come from shared memory once, and its addresses advance by the head's stride.
@@ -17,7 +15,7 @@
 // time (19.8, 65.2), a thread for one unit with the next token's elements on their way meanwhile (30.9, 103).
 
 #include <type_traits>
-#include "common.cuh"
+#include "rotary.cuh"
 
 namespace q8k {
 
@@ -30,11 +28,7 @@ struct RotaryTensor {
 
 struct RotaryParams {
     RotaryTensor q, k;
-    const void* positions;                   // null: 0, 1, ... of each batch entry
-    int positions64;                         // int64 rather than int32
-    int64_t pos_batch, pos_token;
-    const double* freq;
-    float amplitude, sign;
+    RotaryAngles angles;
     int64_t tokens;                          // batch * seq
     int seq, head_dim, rotary_dim, half;     // half: layout
 };
@@ -54,8 +48,8 @@ template <> struct RotaryRaw<16> { using type = uint4; };
 
 // V channels at a time, all accesses aligned to them.  TWO: a pair's channels lie apart (half layout, or V = 1), so a unit is V pairs in
 // two runs of V channels; otherwise V / 2 pairs in one.  PART: there are channels behind the rotated ones, whose units copy one or two
-// runs.
-template <typename T, int V, bool TWO, bool PART>
+// runs.  AXES: positions with several axes.
+template <typename T, int V, bool TWO, bool PART, bool AXES>
 __global__ void __launch_bounds__(kRotaryThreads, TWO && PART ? 6 : 8)
 rotary_kernel(const __grid_constant__ RotaryParams p, const RotaryLanes l) {
     constexpr int PAIRS = TWO ? V : V / 2;
@@ -101,16 +95,13 @@ rotary_kernel(const __grid_constant__ RotaryParams p, const RotaryLanes l) {
         fetch(x, y, in, l.head_lanes * p.q.in_head, left(p.q, h0), copy ? V : p.half ? half_dim : 1, TWO && (!copy || c + V < p.head_dim));
     }
     if (here) {                                                // a token's threads make its angles
-        int64_t pos = s;
-        if (p.positions != nullptr) {
-            const int64_t at = batch * p.pos_batch + s * p.pos_token;
-            pos = p.positions64 ? static_cast<const int64_t*>(p.positions)[at] : (int64_t)static_cast<const int32_t*>(p.positions)[at];
-        }
+        const RotaryAngles& a = p.angles;
+        const int64_t at = batch * a.pos_batch + s * a.pos_token;
+        double pos = (double)s;
+        if (!AXES && a.positions != nullptr) pos = rotary_position<false>(a, at, 0);
         for (int i = rest; i < half_dim; i += per_token) {
-            const double t = (double)pos * (p.freq[i] * 0.15915494309189535);  // 1 / (2 pi)
-            float sn, cs;
-            sincospif(2.0f * (float)(t - rint(t)), &sn, &cs);
-            turns[tl * half_dim + i] = make_float2(cs * p.amplitude, sn * p.amplitude * p.sign);
+            if constexpr (AXES) pos = rotary_position<true>(a, at, i);
+            turns[tl * half_dim + i] = rotary_turn(a, pos, i);
         }
     }
     __syncthreads();
@@ -177,7 +168,9 @@ template <typename T, int V, bool TWO> static int launch_rotary_as(const RotaryP
     if (l.tokens > room) l.tokens = room;
     const int64_t grid = (p.tokens + l.tokens - 1) / l.tokens;
     const unsigned threads = (unsigned)((l.tokens * l.unit_lanes * l.head_lanes + 31) / 32 * 32);
-    auto kern = p.rotary_dim < p.head_dim ? rotary_kernel<T, V, TWO, true> : rotary_kernel<T, V, TWO, false>;
+    const bool part = p.rotary_dim < p.head_dim;
+    auto kern = p.angles.axes != nullptr ? (part ? rotary_kernel<T, V, TWO, true, true> : rotary_kernel<T, V, TWO, false, true>)
+                                         : (part ? rotary_kernel<T, V, TWO, true, false> : rotary_kernel<T, V, TWO, false, false>);
     Q8K_CUDA_OK(launch_dependent(kern, (unsigned)grid, threads, (size_t)l.tokens * p.rotary_dim * 4, st, 1, p, l));
     return Q8K_OK;
 }
@@ -212,16 +205,9 @@ static bool rotary_in_place(const int64_t* in, const int64_t* out, const int64_t
     return true;
 }
 
-}  // namespace q8k
-
-using namespace q8k;
-
-extern "C" int q8k_rotary(const void* q, const int64_t q_strides[3], void* q_out, const int64_t q_out_strides[3], int q_heads,
-                          const void* k, const int64_t k_strides[3], void* k_out, const int64_t k_out_strides[3], int k_heads,
-                          int dtype, const void* positions, int positions_int64, int64_t position_batch_stride,
-                          int64_t position_token_stride, const double* frequencies, float amplitude, int batch, int seq, int head_dim,
-                          int rotary_dim, int half_layout, int backward, void* stream) {
-    const char* op = "rotary";
+static int rotary(const char* op, const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int q_heads, const void* k,
+                  const int64_t* k_strides, void* k_out, const int64_t* k_out_strides, int k_heads, int dtype, const RotaryAngles& angles,
+                  int batch, int seq, int head_dim, int rotary_dim, int half_layout, cudaStream_t st) {
     Q8K_REQUIRE(batch >= 0 && seq >= 0 && q_heads >= 0 && k_heads >= 0, Q8K_ERR_INVALID_ARG, "%s: negative size", op);
     Q8K_REQUIRE(rotary_dim >= 2 && rotary_dim % 2 == 0 && rotary_dim <= head_dim, Q8K_ERR_INVALID_ARG,
                 "%s: rotary_dim %d must be even and between 2 and the head dim %d", op, rotary_dim, head_dim);
@@ -239,10 +225,7 @@ extern "C" int q8k_rotary(const void* q, const int64_t q_strides[3], void* q_out
         Q8K_REQUIRE(count[2] == 0 || in == nullptr || in != out || is == nullptr || os == nullptr || rotary_in_place(is, os, count, head_dim),
                     Q8K_ERR_INVALID_ARG, "%s: in place, %s needs the input's strides and heads that do not overlap", op, i ? "k" : "q");
     }
-    Q8K_REQUIRE(frequencies != nullptr && reinterpret_cast<uintptr_t>(frequencies) % 8 == 0, Q8K_ERR_INVALID_ARG,
-                "%s: null or misaligned frequencies", op);
-    Q8K_REQUIRE(reinterpret_cast<uintptr_t>(positions) % (positions_int64 ? 8 : 4) == 0, Q8K_ERR_INVALID_ARG,
-                "%s: misaligned positions", op);
+    if (int rc = rotary_check_angles(op, angles)) return rc;
     Q8K_REQUIRE((int64_t)batch * seq <= 0x7fffffffLL, Q8K_ERR_TOO_LARGE, "%s: %lld tokens", op, (long long)batch * seq);
     RotaryParams p = {};
     // the widest access, up to 16 bytes, that divides the channels, strides and addresses of all four tensors
@@ -272,17 +255,35 @@ extern "C" int q8k_rotary(const void* q, const int64_t q_strides[3], void* q_out
     };
     Q8K_REQUIRE(tensor(p.q, q, q_strides, q_out, q_out_strides, q_heads) && tensor(p.k, k, k_strides, k_out, k_out_strides, k_heads),
                 Q8K_ERR_INVALID_ARG, "%s: null or misaligned pointer", op);
-    p.positions = positions;
-    p.positions64 = positions_int64 != 0;
-    p.pos_batch = position_batch_stride;
-    p.pos_token = position_token_stride;
-    p.freq = frequencies;
-    p.amplitude = amplitude;
-    p.sign = backward ? -1.f : 1.f;
+    p.angles = angles;
     p.tokens = (int64_t)batch * seq;
     p.seq = seq; p.head_dim = head_dim; p.rotary_dim = rotary_dim; p.half = half_layout != 0;
-    cudaStream_t st = (cudaStream_t)stream;
     if (dtype == Q8K_DT_BF16) return launch_rotary<__nv_bfloat16>(p, v, st);
     if (dtype == Q8K_DT_F16) return launch_rotary<__half>(p, v, st);
     return launch_rotary<float>(p, v, st);
+}
+
+}  // namespace q8k
+
+extern "C" int q8k_rotary(const void* q, const int64_t q_strides[3], void* q_out, const int64_t q_out_strides[3], int q_heads,
+                          const void* k, const int64_t k_strides[3], void* k_out, const int64_t k_out_strides[3], int k_heads,
+                          int dtype, const void* positions, int positions_int64, int64_t position_batch_stride,
+                          int64_t position_token_stride, const double* frequencies, float amplitude, int batch, int seq, int head_dim,
+                          int rotary_dim, int half_layout, int backward, void* stream) {
+    const q8k::RotaryAngles angles = {positions, positions_int64 ? Q8K_POS_I64 : Q8K_POS_I32, position_batch_stride, position_token_stride, 0,
+                                      nullptr, 1, frequencies, amplitude, backward ? -1.f : 1.f};
+    return q8k::rotary("rotary", q, q_strides, q_out, q_out_strides, q_heads, k, k_strides, k_out, k_out_strides, k_heads, dtype, angles, batch, seq,
+                       head_dim, rotary_dim, half_layout, (cudaStream_t)stream);
+}
+
+extern "C" int q8k_axial_rotary(const void* q, const int64_t q_strides[3], void* q_out, const int64_t q_out_strides[3], int q_heads,
+                                const void* k, const int64_t k_strides[3], void* k_out, const int64_t k_out_strides[3], int k_heads, int dtype,
+                                const void* positions, int position_type, const int64_t position_strides[3], int n_axes, const int* axes,
+                                const double* frequencies, float amplitude, int batch, int seq, int head_dim, int rotary_dim,
+                                int half_layout, int backward, void* stream) {
+    Q8K_REQUIRE(axes != nullptr && position_strides != nullptr, Q8K_ERR_INVALID_ARG, "axial_rotary: null axes or position strides");
+    const q8k::RotaryAngles angles = {positions, position_type, position_strides[0], position_strides[1], position_strides[2],
+                                      axes, n_axes, frequencies, amplitude, backward ? -1.f : 1.f};
+    return q8k::rotary("axial_rotary", q, q_strides, q_out, q_out_strides, q_heads, k, k_strides, k_out, k_out_strides, k_heads, dtype, angles, batch,
+                       seq, head_dim, rotary_dim, half_layout, (cudaStream_t)stream);
 }

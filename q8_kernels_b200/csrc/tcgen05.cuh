@@ -387,5 +387,44 @@ __host__ __device__ constexpr uint32_t make_idesc_s8(int m, int n) {
     return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// ---------------------------------------------------------------- 4-bit values with block scales
+// kind::mxf4nvf4 takes 64 e2m1 values a row and instruction (32 bytes, low nibble first).  Its scales lie in TMEM: the 128 rows of an
+// operand tile are 32 lanes x 4 columns (row r in lane r % 32, column r / 32), each 32-bit cell holds the scales of four consecutive
+// blocks of its row, and all four lane quarters hold the same.  B is as wide as its rows, 32 of them a column; with CTA pairs each CTA
+// holds the scales of its own rows of A and of all rows of B.
+// VEC 4: e4m3 scales of 16 values, a cell an instruction; VEC 2: e8m0 scales of 32 values, half a cell, whose half the descriptor names.
+template <int VEC, bool PAIR>
+__device__ __forceinline__ void mma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales, uint32_t b_scales,
+                                        uint32_t accumulate) {
+#define Q8K_MMA_FP4(GROUP, SCALES)                                                                                    \
+    asm volatile("{\n\t"                                                                                              \
+                 ".reg .pred p;\n\t"                                                                                  \
+                 "setp.ne.b32 p, %6, 0;\n\t"                                                                          \
+                 "tcgen05.mma.cta_group::" GROUP ".kind::mxf4nvf4.block_scale.scale_vec::" SCALES " [%0], %1, %2, %3, [%4], [%5], p;\n\t" \
+                 "}" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate)  \
+                 : "memory")
+    if constexpr (VEC == 4 && PAIR) Q8K_MMA_FP4("2", "4X");
+    else if constexpr (VEC == 4) Q8K_MMA_FP4("1", "4X");
+    else if constexpr (PAIR) Q8K_MMA_FP4("2", "2X");
+    else Q8K_MMA_FP4("1", "2X");
+#undef Q8K_MMA_FP4
+}
+// 512 bytes of scales (32 rows of 16 bytes) from shared memory to 32 lanes x 4 columns, in all four lane quarters; with PAIR in both CTAs,
+// each from its own shared memory.  Runs in the order of the issuing thread's MMAs.
+template <bool PAIR> __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+    if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Shared-memory descriptor of such 512 bytes: not swizzled, groups of 8 rows 128 bytes apart.
+__device__ __forceinline__ uint64_t make_scales_desc(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((128ull >> 4) << 32) | (1ull << 46);
+}
+// Instruction descriptor: [4,6) half of B's cells (0 or 2), [7,10) and [10,12) e2m1 = 1, [17,23) N >> 3, [23] e8m0 scales, [27,29) M >> 7,
+// [29,31) half of A's cells.
+__host__ __device__ constexpr uint32_t make_idesc_fp4(int m, int n, bool e8m0, int half) {
+    return ((uint32_t)half << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((e8m0 ? 1u : 0u) << 23) | ((uint32_t)(m >> 7) << 27) |
+           ((uint32_t)half << 29);
+}
+
 }  // namespace ptx
 }  // namespace q8k

@@ -1,16 +1,18 @@
-"""Rotary embedding from positions: half and interleaved layouts, part of a head, scaled for long contexts, queries and keys in one launch
-(no counterpart in the reference, which rotates whole rows of interleaved pairs by fp32 tables: see rope.py)."""
+"""Rotary embedding from positions: half and interleaved layouts, part of a head, scaled for long contexts, positions with several axes,
+queries and keys in one launch (no counterpart in the reference, which rotates whole rows of interleaved pairs by fp32 tables: see rope.py)."""
 import math
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _host
 from ..native import Q8KernelError, refuse_tangents
+from ..native import axial_rotary as _axial_rotary
 from ..native import rotary as _rotary
 
 LAYOUTS = ("half", "interleaved")
+SPECTRA = ("own", "shared")
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None) -> Tuple[torch.Tensor, float]:
@@ -99,3 +101,62 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return Rotary.apply(q, k, positions, frequencies, amplitude, half)
     return _rotary(q, k, positions, frequencies, amplitude, half, False)
+
+
+def axial_frequencies(sections: Sequence[int], base: Union[float, Sequence[float]] = 10000.0,
+                      spectrum: str = "own") -> Tuple[torch.Tensor, torch.Tensor]:
+    """Frequencies and axes of the pairs of a head whose rotated channels are shared out to several axes, ``sections`` channels each (even numbers)
+    in the order of the axes: float64 and int32 CPU tensors [sum / 2].  ``spectrum`` "own": each axis of c channels has the frequencies
+    ``base ** (-2j / c)``, j < c / 2 (``base`` may be one number for each axis); "shared": pair i has ``base ** (-2i / sum)``, whatever its axis.
+    Another order of the pairs is another ``axes``."""
+    sections = list(sections)
+    if not sections or any(not isinstance(c, int) or c < 2 or c % 2 for c in sections):
+        raise Q8KernelError(f"axial_frequencies: sections {sections} must be positive even numbers")
+    if spectrum not in SPECTRA:
+        raise Q8KernelError(f"axial_frequencies: spectrum {spectrum!r} is not one of {', '.join(SPECTRA)}")
+    bases = [base] * len(sections) if isinstance(base, (int, float)) else list(base)
+    if len(bases) != len(sections) or any(not b > 1.0 for b in bases) or (spectrum == "shared" and len(set(bases)) > 1):
+        raise Q8KernelError(f"axial_frequencies: base {base} must be a number greater than 1, or with own spectra one for each axis")
+    axes = torch.cat([torch.full((c // 2,), n, dtype=torch.int32) for n, c in enumerate(sections)])
+    if spectrum == "shared":
+        return rotary_frequencies(sum(sections), bases[0])[0], axes
+    return torch.cat([rotary_frequencies(c, b)[0] for c, b in zip(sections, bases)]), axes
+
+
+def grid_positions(*sizes: int, device=None) -> torch.Tensor:
+    """Positions of the tokens of a grid, the last axis fastest: int64 [product of sizes, number of sizes], for frames, rows and columns of
+    patches ``grid_positions(frames, rows, columns)``."""
+    if not sizes or any(not isinstance(n, int) or n < 1 for n in sizes):
+        raise Q8KernelError(f"grid_positions: sizes {sizes} must be positive numbers")
+    return torch.stack(torch.meshgrid(*(torch.arange(n, device=device) for n in sizes), indexing="ij"), -1).view(-1, len(sizes))
+
+
+class AxialRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, frequencies, axes, amplitude, half):
+        ctx.save_for_backward(positions, frequencies, axes)
+        ctx.amplitude, ctx.half = amplitude, half
+        ctx.set_materialize_grads(False)
+        return _axial_rotary(q, k, positions, frequencies, axes, amplitude, half, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_q, grad_k):
+        grads = [g if need else None for g, need in zip((grad_q, grad_k), ctx.needs_input_grad[:2])]
+        if any(g is not None for g in grads):
+            grads = _axial_rotary(*grads, *ctx.saved_tensors, ctx.amplitude, ctx.half, True)
+        return (*grads, None, None, None, None, None)
+
+
+def apply_axial_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, frequencies: torch.Tensor, axes: torch.Tensor,
+                       amplitude: float = 1.0, layout: str = "interleaved"):
+    """``apply_rotary`` by positions with several axes: pair i turns by ``positions[..., axes[i]] * frequencies[i]``.  ``positions``: [S,A], [1,S,A]
+    or [B,S,A], int32, int64, float32 or float64 (fractions are positions like any others); ``frequencies`` float64 and ``axes``
+    int32 [rotary_dim / 2], both on the device (``axial_frequencies``); an axis beyond A is taken as the last.  Differentiable in q and k."""
+    if layout not in LAYOUTS:
+        raise Q8KernelError(f"apply_axial_rotary: layout {layout!r} is not one of {', '.join(LAYOUTS)}")
+    amplitude, half = float(amplitude), layout == "half"
+    refuse_tangents("apply_axial_rotary", q, k, positions, frequencies)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return AxialRotary.apply(q, k, positions, frequencies, axes, amplitude, half)
+    return _axial_rotary(q, k, positions, frequencies, axes, amplitude, half, False)

@@ -142,6 +142,57 @@ class FP8Linear(nn.Module):
         return layer
 
 
+class FP4Linear(nn.Module):
+    """Linear on 4-bit values with block scales, ``format`` "nvfp4" or "mxfp4" (functional.fp4); the output has the input's type unless
+    ``out_dtype`` says otherwise.  ``weight`` uint8 [out, in / 2] (frozen), ``bias`` fp32 [out] or None; the scales are held as their bits
+    (``block_scales`` uint8, ``scales`` int32 [out] of the fp32 row scales with "nvfp4"), which a cast of the model leaves alone; a
+    bias that was cast with it is widened in each call.  No counterpart in the reference."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, format: str = "nvfp4", device=None):
+        super().__init__()
+        if format not in Q8F.fp4.FORMATS:
+            raise native.Q8KernelError(f"FP4Linear: format {format!r} is not one of {', '.join(Q8F.fp4.FORMATS)}")
+        if in_features <= 0 or in_features % 32 or out_features <= 0 or out_features % 16:
+            raise native.Q8KernelError(f"FP4Linear: {in_features} -> {out_features} features: multiples of 32 and of 16 are needed")
+        self.in_features, self.out_features, self.format = in_features, out_features, format
+        self.weight = nn.Parameter(torch.zeros(out_features, in_features // 2, device=device, dtype=torch.uint8), requires_grad=False)
+        if bias:
+            self.bias = nn.Parameter(torch.zeros(out_features, device=device, dtype=torch.float), requires_grad=False)
+        else:
+            self.register_parameter("bias", None)
+        self.register_buffer("block_scales", torch.zeros(native.fp4_scales_shape(out_features, in_features, format), device=device,
+                                                         dtype=torch.uint8))
+        self.register_buffer("scales", torch.zeros(out_features, device=device, dtype=torch.int32) if format == "nvfp4" else None)
+
+    @property
+    def weight_scales(self):
+        """(block scales, row scales) as functional.fp4 takes them."""
+        if self.format == "nvfp4":
+            return self.block_scales.view(torch.float8_e4m3fn), self.scales.view(torch.float)
+        return self.block_scales.view(torch.float8_e8m0fnu), None
+
+    def forward(self, x, x_scales=None, fuse_gelu=False, out_dtype=None):
+        bias = self.bias
+        if bias is not None and bias.dtype != torch.float:
+            bias = bias.float()
+        return Q8F.fp4.fp4_linear(x, self.weight, bias, x_scales, self.weight_scales, fuse_gelu, out_dtype)
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear, format: str = "nvfp4"):
+        """Quantises a checkpoint's 16-bit layer."""
+        w = linear.weight.data
+        if not is_16bit(w):
+            raise native.Q8KernelError(f"FP4Linear.from_linear: the weight must be bfloat16 or float16, not {w.dtype}")
+        layer = cls(linear.in_features, linear.out_features, linear.bias is not None, format, w.device)
+        layer.weight.data, (block, row) = Q8F.fp4.fp4_quantize(w, format)
+        layer.block_scales = block.view(torch.uint8)
+        if row is not None:
+            layer.scales = row.view(torch.int32)
+        if linear.bias is not None:
+            layer.bias.data = linear.bias.data.float()
+        return layer
+
+
 def make_linear(kind: str, in_features: int, out_features: int, bias: bool = True, device=None) -> nn.Module:
     """The quantised linear a DiT module is built from: ``"int8"`` -> Q8Linear (the reference's
     block), ``"fp8"`` -> FP8Linear with Hadamard-rotated per-token e4m3 activations."""

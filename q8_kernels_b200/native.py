@@ -842,6 +842,150 @@ def rotary(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: Opti
     return q_out, k_out
 
 
+POSITION_TYPES = {torch.int32: 1, torch.int64: 2, torch.float32: 3, torch.float64: 4}
+
+
+def _head_pair(op: str, q: Optional[torch.Tensor], k: Optional[torch.Tensor]) -> Tuple[torch.Tensor, int, int]:
+    """What queries and keys have to fulfil together; returns one of them, batch and seq."""
+    x = q if q is not None else k
+    if x is None:
+        raise Q8KernelError(f"{op}: neither q nor k")
+    if x.dim() not in (3, 4) or x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise Q8KernelError(f"{op}: q and k must be [B,S,H,D] or [S,H,D] in bfloat16, float16 or float32, not {x.dtype} {tuple(x.shape)}")
+    if q is not None and k is not None and (k.dtype != q.dtype or k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2]
+                                            or k.shape[-1] != q.shape[-1]):
+        raise Q8KernelError(f"{op}: q {q.dtype} {tuple(q.shape)} and k {k.dtype} {tuple(k.shape)} do not go together")
+    return (x, 1, x.shape[0]) if x.dim() == 3 else (x, *x.shape[:2])
+
+
+def _angle_args(op: str, positions: Optional[torch.Tensor], frequencies: torch.Tensor, axes: Optional[torch.Tensor], batch: int, seq: int):
+    """(positions, their type, {batch, token, axis} strides, number of axes, axes, frequencies) for a kernel, after their checks."""
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1:
+        raise Q8KernelError(f"{op}: frequencies must be float64 [rotary_dim / 2], not {frequencies.dtype} {tuple(frequencies.shape)}")
+    frequencies = frequencies.contiguous()
+    if axes is None:
+        if positions is None:
+            return None, 1, _Strides(0, 0, 0), 1, None, frequencies
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise Q8KernelError(f"{op}: positions must be int32 or int64, not {positions.dtype}")
+        if tuple(positions.shape) not in ((seq,), (1, seq), (batch, seq)):
+            raise Q8KernelError(f"{op}: positions {tuple(positions.shape)} for a batch of {batch} sequences of {seq}")
+        of_batch = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
+        return positions, POSITION_TYPES[positions.dtype], _Strides(of_batch, positions.stride(-1), 0), 1, None, frequencies
+    if axes.dtype != torch.int32 or axes.shape != frequencies.shape:
+        raise Q8KernelError(f"{op}: axes must be int32 {tuple(frequencies.shape)}, not {axes.dtype} {tuple(axes.shape)}")
+    if positions is None or positions.dtype not in POSITION_TYPES:
+        raise Q8KernelError(f"{op}: positions must be int32, int64, float32 or float64, not {None if positions is None else positions.dtype}")
+    if positions.dim() not in (2, 3) or positions.shape[-1] == 0 or tuple(positions.shape[:-1]) not in ((seq,), (1, seq), (batch, seq)):
+        raise Q8KernelError(f"{op}: positions {tuple(positions.shape)} for a batch of {batch} sequences of {seq}")
+    of_batch = positions.stride(0) if positions.dim() == 3 and positions.shape[0] > 1 else 0
+    return (positions, POSITION_TYPES[positions.dtype], _Strides(of_batch, positions.stride(-2), positions.stride(-1)), positions.shape[-1],
+            axes.contiguous(), frequencies)
+
+
+def _channels_dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t.contiguous() if t is not None and t.shape[-1] > 1 and t.stride(-1) != 1 else t
+
+
+def _token_strides(t: Optional[torch.Tensor]):
+    return None if t is None else _Strides(*((0,) * (t.dim() == 3) + t.stride()[:-1]))
+
+
+def axial_rotary(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: torch.Tensor, frequencies: torch.Tensor, axes: torch.Tensor,
+                 amplitude: float = 1.0, half: bool = False, backward: bool = False) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """rotary with positions [S,A], [1,S,A] or [B,S,A] (int32, int64, float32 or float64) of several axes: pair i turns by
+    ``position[axes[i]] * frequencies[i]`` (axes int32 on the device, one beyond the last is taken as the last)."""
+    x, batch, seq = _head_pair("axial_rotary", q, k)
+    dev = require_cuda(q, k, positions, frequencies, axes)
+    if axes is None:
+        raise Q8KernelError("axial_rotary: no axes")
+    positions, kind, strides, n_axes, axes, frequencies = _angle_args("axial_rotary", positions, frequencies, axes, batch, seq)
+    q, k = _channels_dense(q), _channels_dense(k)
+    outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k)]
+    args = []
+    for t, o in zip((q, k), outs):
+        args += [ptr(t), _token_strides(t), ptr(o), _token_strides(o), 0 if t is None else t.shape[-2]]
+    launch(dev, "axial_rotary", lib.q8k_axial_rotary, *args, dt(x.dtype), ptr(positions), kind, strides, n_axes, ptr(axes), ptr(frequencies),
+           float(amplitude), batch, seq, x.shape[-1], 2 * frequencies.numel(), int(half), int(backward))
+    return outs[0], outs[1]
+
+
+def _head_weight(op: str, w: Optional[torch.Tensor], dim: int) -> Optional[torch.Tensor]:
+    if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (dim,)):
+        raise Q8KernelError(f"{op}: weights must be float32 [{dim}], not {w.dtype} {tuple(w.shape)}")
+    return None if w is None else w.contiguous()
+
+
+def _head_norm_angles(op, positions, frequencies, axes, batch, seq):
+    """_angle_args, or none of them without a rotation; and rotary_dim."""
+    if frequencies is None:
+        if positions is not None or axes is not None:
+            raise Q8KernelError(f"{op}: positions or axes without frequencies")
+        return (None, 1, _Strides(0, 0, 0), 1, None, None), 0
+    args = _angle_args(op, positions, frequencies, axes, batch, seq)
+    if frequencies.numel() == 0:
+        raise Q8KernelError(f"{op}: no frequencies")
+    return args, 2 * frequencies.numel()
+
+
+def head_norm(q: Optional[torch.Tensor], k: Optional[torch.Tensor], q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float,
+              positions: Optional[torch.Tensor] = None, frequencies: Optional[torch.Tensor] = None, axes: Optional[torch.Tensor] = None,
+              amplitude: float = 1.0, half: bool = True) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """Every head of q and k ([B,S,H,D] or [S,H,D], either may be None) as ``x / sqrt(mean(x^2) + eps) * weight`` (fp32 [D] or None), turned as by
+    rotary or, with axes, axial_rotary; no rotation without frequencies.  See functional.head_norm."""
+    op = "head_norm"
+    x, batch, seq = _head_pair(op, q, k)
+    dev = require_cuda(q, k, q_weight, k_weight, positions, frequencies, axes)
+    dim = x.shape[-1]
+    angles, rotary_dim = _head_norm_angles(op, positions, frequencies, axes, batch, seq)
+    positions, kind, strides, n_axes, axes, frequencies = angles
+    args, keep, outs = [], [], []
+    for t, w in ((q, q_weight), (k, k_weight)):
+        t, w = _channels_dense(t), _head_weight(op, w, dim)
+        o = None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
+        args += [ptr(t), _token_strides(t), ptr(w), ptr(o), _token_strides(o), 0 if t is None else t.shape[-2]]
+        keep += [t, w]
+        outs.append(o)
+    launch(dev, op, lib.q8k_head_norm, *args, dt(x.dtype), float(eps), ptr(positions), kind, strides, n_axes, ptr(axes), ptr(frequencies),
+           float(amplitude), batch, seq, dim, rotary_dim, int(half))
+    return outs[0], outs[1]
+
+
+def head_norm_backward(q: Optional[torch.Tensor], k: Optional[torch.Tensor], q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                       grad_q: Optional[torch.Tensor], grad_k: Optional[torch.Tensor], eps: float, positions: Optional[torch.Tensor] = None,
+                       frequencies: Optional[torch.Tensor] = None, axes: Optional[torch.Tensor] = None, amplitude: float = 1.0, half: bool = True,
+                       need_dweight: Sequence[bool] = (False, False)) -> List[Optional[torch.Tensor]]:
+    """``[dq, dk, dq_weight, dk_weight]`` of head_norm from its inputs and the outputs' gradients (a tensor without a gradient is left out); the
+    weights' are fp32 [D], None where they are not needed."""
+    op = "head_norm_backward"
+    if grad_q is None:
+        q = None
+    if grad_k is None:
+        k = None
+    x, batch, seq = _head_pair(op, q, k)
+    dev = require_cuda(q, k, q_weight, k_weight, grad_q, grad_k, positions, frequencies, axes)
+    dim = x.shape[-1]
+    angles, rotary_dim = _head_norm_angles(op, positions, frequencies, axes, batch, seq)
+    positions, kind, strides, n_axes, axes, frequencies = angles
+    args, keep, dxs, dws = [], [], [], []
+    for t, g, w, need in ((q, grad_q, q_weight, need_dweight[0]), (k, grad_k, k_weight, need_dweight[1])):
+        if t is not None and (g.shape != t.shape or g.dtype != t.dtype):
+            raise Q8KernelError(f"{op}: gradient {g.dtype} {tuple(g.shape)} of an output {t.dtype} {tuple(t.shape)}")
+        t, g, w = _channels_dense(t), _channels_dense(g), _head_weight(op, w, dim)
+        o = None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
+        dw = torch.empty(dim, dtype=torch.float32, device=dev) if need and t is not None else None
+        args += [ptr(t), _token_strides(t), ptr(w), ptr(g), _token_strides(g), ptr(o), _token_strides(o), ptr(dw), 0 if t is None else t.shape[-2]]
+        keep += [t, g, w]
+        dxs.append(o)
+        dws.append(dw)
+    work = None
+    if any(d is not None for d in dws):
+        work = torch.empty(lib.q8k_head_norm_backward_workspace_bytes(dim), dtype=torch.uint8, device=dev)
+    launch(dev, op, lib.q8k_head_norm_backward, *args, dt(x.dtype), float(eps), ptr(positions), kind, strides, n_axes, ptr(axes), ptr(frequencies),
+           float(amplitude), batch, seq, dim, rotary_dim, int(half), ptr(work), 0 if work is None else work.numel())
+    return dxs + dws
+
+
 ACTIVATIONS = {"silu": 1, "gelu_tanh": 2}
 GATED_TRAINING_MAX = 16384                                   # columns of a row that the backward pass keeps in registers
 
@@ -925,4 +1069,128 @@ def gated_backward_quant(grad: torch.Tensor, pre: torch.Tensor, act: str = "silu
     scales = torch.empty(grad.shape[:-1], dtype=torch.float32, device=dev)
     launch(dev, "gated_backward_quant", lib.q8k_gated_backward_quant, ptr(grad), ptr(pre), ptr(q), ptr(scales), ACTIVATIONS[act],
            scales.numel(), f)
+    return [q, scales]
+
+
+FP4_FORMATS = {"mxfp4": 1, "nvfp4": 2}
+_FP4_SCALES = {torch.float8_e8m0fnu: "mxfp4", torch.float8_e4m3fn: "nvfp4"}     # the type of the block scales names the format
+_FP4_BLOCK = {"mxfp4": 32, "nvfp4": 16}
+
+
+def fp4_scales_shape(rows: int, k: int, fmt: str) -> Tuple[int, int, int]:
+    """Block scales of [rows, k]: [tiles of 128 rows, tiles of 4 blocks along K, 512], K filled up to a multiple of 256."""
+    return (rows + 127) // 128, (k + 255) // 256 * (64 // _FP4_BLOCK[fmt]), 512
+
+
+def fp4_format(op: str, values: torch.Tensor, scales) -> str:
+    """The format of (values, (block scales, row scales)), which have to fit together."""
+    if not isinstance(scales, (tuple, list)) or len(scales) != 2 or not isinstance(scales[0], torch.Tensor):
+        raise Q8KernelError(f"{op}: the scales must be (block scales, row scales or None)")
+    block, row = scales
+    if values.dtype != torch.uint8 or values.dim() < 1 or block.dtype not in _FP4_SCALES:
+        raise Q8KernelError(f"{op}: values of type {values.dtype} with scales of type {block.dtype} are not 4-bit values")
+    fmt, k = _FP4_SCALES[block.dtype], 2 * values.shape[-1]
+    rows = values.shape[:-1].numel()
+    if k == 0 or k % 32 or tuple(block.shape) != fp4_scales_shape(rows, k, fmt):
+        raise Q8KernelError(f"{op}: block scales {tuple(block.shape)} do not fit {rows} rows of {k} values in {fmt}")
+    if (row is None) != (fmt == "mxfp4"):
+        raise Q8KernelError(f"{op}: nvfp4 has row scales, mxfp4 has none")
+    if row is not None and (row.dtype != torch.float32 or row.numel() != rows):
+        raise Q8KernelError(f"{op}: row scales of type {row.dtype} and shape {tuple(row.shape)} for {rows} rows")
+    return fmt
+
+
+def fp4_quant(x: torch.Tensor, fmt: str = "nvfp4") -> List[Optional[torch.Tensor]]:
+    """x [...,K] (bf16 or fp16, K a multiple of 32) in 4 bits: ``[values, block scales, row scales]``, values uint8 [...,K/2] (two a byte, the
+    first in the low nibble), block scales e4m3 (nvfp4) or e8m0 (mxfp4) in tiles (``fp4_scales_shape``), row scales fp32 [...] (nvfp4) or None."""
+    dev = require_cuda(x)
+    if fmt not in FP4_FORMATS:
+        raise Q8KernelError(f"fp4_quant: format {fmt!r} is not one of {', '.join(FP4_FORMATS)}")
+    if x.dtype not in (torch.bfloat16, torch.float16) or x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 32:
+        raise Q8KernelError(f"fp4_quant: x {x.dtype} {tuple(x.shape)} must be bfloat16 or float16 rows of a multiple of 32 values")
+    x2, rows, k, stride = _rows(_aligned(x))
+    values = torch.empty(x.shape[:-1] + (k // 2,), dtype=torch.uint8, device=dev)
+    block = torch.zeros(fp4_scales_shape(rows, k, fmt), dtype=torch.uint8, device=dev)      # (rows that fill up the last tile are not written)
+    row = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev) if fmt == "nvfp4" else None
+    launch(dev, "fp4_quant", lib.q8k_fp4_quant, ptr(x2), dt(x.dtype), stride, FP4_FORMATS[fmt], ptr(values), ptr(block), ptr(row), rows, k)
+    return [values, block.view(E4M3 if fmt == "nvfp4" else torch.float8_e8m0fnu), row]
+
+
+def fp4_dequant(values: torch.Tensor, block_scales: torch.Tensor, row_scales: Optional[torch.Tensor],
+                out_type: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """What 4-bit values stand for: bf16, fp16 or fp32 [...,K]."""
+    dev = require_cuda(values, block_scales, row_scales)
+    fmt = fp4_format("fp4_dequant", values, (block_scales, row_scales))
+    values, block_scales = _aligned(values.contiguous()), block_scales.contiguous()
+    row_scales = None if row_scales is None else row_scales.contiguous()
+    k = 2 * values.shape[-1]
+    y = torch.empty(values.shape[:-1] + (k,), dtype=out_type, device=dev)
+    launch(dev, "fp4_dequant", lib.q8k_fp4_dequant, ptr(values), ptr(block_scales), ptr(row_scales), FP4_FORMATS[fmt], ptr(y), dt(out_type),
+           y.numel() // k, k)
+    return y
+
+
+def fp4_mm(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor], a_scales, b_scales, fuse_gelu: bool = False,
+           out_type: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``act(a . b^T + bias)`` of 4-bit ``a`` [...,K/2] and ``b`` [N,K/2] of one format; the scales are ``(block scales, row scales or None)`` as
+    fp4_quant returns them, ``bias`` fp32 [N] or None, the output bf16 or fp16 [...,N], N a multiple of 16."""
+    dev = require_cuda(a, b, bias, *a_scales, *b_scales)
+    fmt = fp4_format("fp4_mm", a, a_scales)
+    if b.dim() != 2 or fp4_format("fp4_mm", b, b_scales) != fmt or a.shape[-1] != b.shape[-1]:
+        raise Q8KernelError(f"fp4_mm: {fmt} activation {tuple(a.shape)} and weight {tuple(b.shape)} do not go together")
+    n, k = b.shape[0], 2 * b.shape[1]
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != n):
+        raise Q8KernelError(f"fp4_mm: bias of type {bias.dtype} and shape {tuple(bias.shape)} for {n} columns")
+    a, b = _aligned(a.contiguous()), _aligned(b.contiguous())
+    (ab, ar), (bb, br) = (tuple(None if t is None else _aligned(t.contiguous()) for t in s) for s in (a_scales, b_scales))
+    bias = None if bias is None else bias.contiguous()
+    out = torch.empty(a.shape[:-1] + (n,), dtype=out_type, device=dev)
+    launch(dev, "fp4_mm", lib.q8k_fp4_mm, FP4_FORMATS[fmt], ptr(a), ptr(ab), ptr(ar), ptr(b), ptr(bb), ptr(br), ptr(bias), ptr(out), dt(out_type),
+           out.numel() // n if n else 0, n, k, int(bool(fuse_gelu)), ptr(_lib.status_word(dev)))
+    return out
+
+
+def fp4_linear(x: torch.Tensor, w: torch.Tensor, w_scales, bias: Optional[torch.Tensor], fuse_gelu: bool, out_type: torch.dtype) -> torch.Tensor:
+    """fp4_quant of x [...,K] in the weight's format and fp4_mm, in one native call over scratch of its own."""
+    dev, fmt, n, k = fp4_linear_check("fp4_linear", x, w, w_scales, bias)
+    x, w = _aligned(x.contiguous()), _aligned(w.contiguous())
+    block, row = (None if t is None else _aligned(t.contiguous()) for t in w_scales)
+    bias = None if bias is None else bias.contiguous()
+    m = x.numel() // k
+    out = torch.empty(x.shape[:-1] + (n,), dtype=out_type, device=dev)
+    work = torch.empty(lib.q8k_fp4_linear_workspace_bytes(FP4_FORMATS[fmt], m, k), dtype=torch.uint8, device=dev)
+    launch(dev, "fp4_linear", lib.q8k_fp4_linear, FP4_FORMATS[fmt], ptr(x), dt(x.dtype), ptr(w), ptr(block), ptr(row), ptr(bias), ptr(out),
+           dt(out_type), m, n, k, int(bool(fuse_gelu)), ptr(work), work.numel(), ptr(_lib.status_word(dev)))
+    return out
+
+
+def fp4_linear_check(op: str, x: torch.Tensor, w: torch.Tensor, w_scales, bias: Optional[torch.Tensor]):
+    """What an un-quantised activation, a 4-bit weight and a bias have to fulfil; returns the device, the format, N and K."""
+    fmt = fp4_format(op, w, w_scales)
+    dev = require_cuda(x, w, bias, *w_scales)
+    if w.dim() != 2 or w.shape[0] == 0 or w.shape[0] % 16:
+        raise Q8KernelError(f"{op}: the weight must be [N, K / 2] with N a multiple of 16, not {tuple(w.shape)}")
+    n, k = w.shape[0], 2 * w.shape[1]
+    if x.dtype not in (torch.bfloat16, torch.float16) or x.dim() < 1 or x.shape[-1] != k:
+        raise Q8KernelError(f"{op}: activation {x.dtype} {tuple(x.shape)} must be bfloat16 or float16 rows of {k}")
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != n):
+        raise Q8KernelError(f"{op}: bias of type {bias.dtype} and shape {tuple(bias.shape)} for {n} columns")
+    return dev, fmt, n, k
+
+
+def fp4_weight_operand(w: torch.Tensor, w_scales) -> List[torch.Tensor]:
+    """A 4-bit weight [N,K/2] de-quantised to fp32, transposed and quantised to e4m3 per input channel, the weight operand of the backward
+    product.  Returns ``[q, scales]``: e4m3 [K,N] and fp32 [K]."""
+    fmt = fp4_format("fp4_weight_operand", w, w_scales)
+    dev = require_cuda(w, *w_scales)
+    if w.dim() != 2:
+        raise Q8KernelError(f"fp4_weight_operand: the weight must be [N, K / 2], not {tuple(w.shape)}")
+    w = _aligned(w.contiguous())
+    block, row = (None if t is None else t.contiguous() for t in w_scales)
+    n, k = w.shape[0], 2 * w.shape[1]
+    q = torch.empty((k, n), dtype=E4M3, device=dev)
+    scales = torch.empty((k,), dtype=torch.float32, device=dev)
+    work = torch.empty(lib.q8k_fp4_weight_operand_workspace_bytes(n, k), dtype=torch.uint8, device=dev)
+    launch(dev, "fp4_weight_operand", lib.q8k_fp4_weight_operand, FP4_FORMATS[fmt], ptr(w), ptr(block), ptr(row), ptr(q), ptr(scales), n, k, ptr(work),
+           work.numel())
     return [q, scales]
