@@ -663,10 +663,10 @@ PyObject* qk_norm_rope_prep_pair(PyObject*, PyObject* const* args, Py_ssize_t n)
     FAST_END
 }
 
-// ---------------------------------------------------------------- layer norm, rotary positions, gated projection
+// ---------------------------------------------------------------- layer norm, rotary positions, gated projection, head norm, 4-bit linear
 // These are differentiable: where an input has a gradient the call leaves a node of torch's C++ autograd behind, whose backward pass
 // launches without the interpreter.  (A Python autograd.Function costs some 60 us of host time for one forward and backward pass, the
-// kernels of a short call 10.)  What functional.layer_norm.layer_norm, functional.rotary.apply_rotary and functional.gated do with tensors
+// kernels of a short call 10.)  What functional.layer_norm.layer_norm, functional.rotary, functional.gated, functional.head_norm and functional.fp4 do with tensors
 // that these do not take is the same.  The underscore marks them: they answer for functions of functional/, not of native.py.
 
 using torch::autograd::AutogradContext;
@@ -1029,6 +1029,397 @@ PyObject* _gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
     FAST_END
 }
 
+// ---- rotation by positions of several axes, head norms
+int position_code(Dt t) {
+    switch (t) {
+        case Dt::Int: return Q8K_POS_I32;
+        case Dt::Long: return Q8K_POS_I64;
+        case Dt::Float: return Q8K_POS_F32;
+        case Dt::Double: return Q8K_POS_F64;
+        default: return 0;
+    }
+}
+
+// [batch, seq, heads, dim] or [seq, heads, dim]
+struct HeadShape {
+    int64_t d, batch, seq, dim;
+    explicit HeadShape(const at::Tensor& x) : d(x.dim()), batch(d == 4 ? x.size(0) : 1), seq(x.size(d - 3)), dim(x.size(d - 1)) {}
+    int heads(const at::Tensor& t) const { return t.defined() ? (int)t.size(d - 2) : 0; }
+    void strides(const at::Tensor& t, int64_t (&s)[3]) const {
+        if (!t.defined()) return;
+        s[0] = d == 4 ? t.stride(0) : 0;
+        s[1] = t.stride(d - 3);
+        s[2] = t.stride(d - 2);
+    }
+};
+const void* dense_ptr(const at::Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void* out_ptr(at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// Positions, frequencies and axes as a kernel takes them; axes undefined: one axis, positions undefined: 0, 1, ...
+struct AngleArgs {
+    const void* pos;
+    int kind = Q8K_POS_I64, n_axes = 1;
+    int64_t stride[3] = {0, 0, 0};
+    const int* axes;
+    const double* freq;
+    int rotary_dim;
+    AngleArgs(const at::Tensor& p, const at::Tensor& f, const at::Tensor& a)
+        : pos(dense_ptr(p)), axes(static_cast<const int*>(dense_ptr(a))), freq(static_cast<const double*>(dense_ptr(f))),
+          rotary_dim(f.defined() ? (int)(2 * f.numel()) : 0) {
+        if (!p.defined()) return;
+        kind = position_code(p.scalar_type());
+        const bool several = a.defined();
+        const int64_t d = p.dim(), token = several ? d - 2 : d - 1;
+        if (token == 1 && p.size(0) > 1) stride[0] = p.stride(0);
+        stride[1] = p.stride(token);
+        if (several) {
+            stride[2] = p.stride(d - 1);
+            n_axes = (int)p.size(d - 1);
+        }
+    }
+};
+
+// What the fast path takes of queries, keys and their angles (freq may be null: no rotation).
+void need_heads(Call& c, const at::Tensor* q, const at::Tensor* k, int64_t max_dim) {
+    if (!c.ok) return;
+    const Dt t = q->scalar_type();
+    const int64_t d = q->dim();
+    c.need((t == Dt::BFloat16 || t == Dt::Half || t == Dt::Float) && (d == 3 || d == 4) && q->stride(-1) == 1);
+    if (!c.ok) return;
+    const HeadShape s(*q);
+    c.need(int_sized(s.batch) && int_sized(s.seq) && s.dim >= 1 && s.dim <= max_dim && q->size(d - 2) <= 65536);
+    if (k != nullptr) {
+        c.need(k->scalar_type() == t && k->dim() == d && k->stride(-1) == 1 && k->size(-1) == s.dim && k->size(d - 3) == s.seq &&
+               (d == 3 || k->size(0) == s.batch) && k->size(d - 2) <= 65536);
+    }
+    if (!c.ok) return;
+    c.need((q->size(d - 2) + (k != nullptr ? k->size(d - 2) : 0)) * s.dim <= (1 << 24) && !has_tangent(q) && !has_tangent(k));
+}
+void need_angles(Call& c, const at::Tensor* q, const at::Tensor* pos, const at::Tensor* freq, const at::Tensor* axes) {
+    if (!c.ok) return;
+    const HeadShape s(*q);
+    c.need((freq != nullptr || (pos == nullptr && axes == nullptr)) && (axes == nullptr || pos != nullptr));
+    if (!c.ok || freq == nullptr) return;
+    c.need((freq->scalar_type() == Dt::Double || freq->scalar_type() == Dt::Long) && freq->dim() == 1 && freq->numel() >= 1 &&
+           2 * freq->numel() <= s.dim && (axes == nullptr || (axes->dim() == 1 && axes->numel() == freq->numel())) && !has_tangent(freq) &&
+           !has_tangent(pos));
+    if (!c.ok || pos == nullptr) return;
+    const int64_t last = axes != nullptr ? pos->dim() - 1 : pos->dim();          // dims before the axes
+    const int code = position_code(pos->scalar_type());
+    c.need((last == 1 || last == 2) && (axes != nullptr ? code != 0 && pos->size(-1) >= 1 && int_sized(pos->size(-1))
+                                                        : code == Q8K_POS_I32 || code == Q8K_POS_I64));
+    if (!c.ok) return;
+    c.need(pos->size(last - 1) == s.seq && (last == 1 || pos->size(0) == 1 || pos->size(0) == s.batch));
+}
+PyObject* pair_of(variable_list&& out, bool both) {
+    PyObject* r = PyTuple_New(2);
+    if (r == nullptr) return nullptr;
+    PyTuple_SET_ITEM(r, 0, wrap(std::move(out[0])));
+    if (both) {
+        PyTuple_SET_ITEM(r, 1, wrap(std::move(out[1])));
+    } else {
+        Py_INCREF(Py_None);
+        PyTuple_SET_ITEM(r, 1, Py_None);
+    }
+    return r;
+}
+// A gradient with dense channels.
+at::Tensor head_grad(const at::Tensor& g) { return g.stride(-1) == 1 || g.size(-1) == 1 ? g : g.contiguous(); }
+
+// _axial_rotary(q, k | None, positions, frequencies, axes, amplitude, half): frequencies as for _rotary
+struct AxialRotaryNode : torch::autograd::Function<AxialRotaryNode> {
+    static variable_list run(const at::Tensor& q, const at::Tensor& k, const at::Tensor& pos, const at::Tensor& freq, const at::Tensor& axes,
+                             double amplitude, bool half, bool backward, int& rc) {
+        const at::Tensor& x = q.defined() ? q : k;
+        const HeadShape s(x);
+        const AngleArgs a(pos, freq, axes);
+        variable_list out(2);
+        int64_t in_s[2][3] = {}, out_s[2][3] = {};
+        const at::Tensor* in[2] = {&q, &k};
+        for (int i = 0; i < 2; ++i) {
+            if (!in[i]->defined()) continue;
+            out[i] = empty_like_dtype(in[i]->sizes(), x, x.scalar_type());
+            s.strides(*in[i], in_s[i]);
+            s.strides(out[i], out_s[i]);
+        }
+        rc = q8k_axial_rotary(dense_ptr(q), in_s[0], out_ptr(out[0]), out_s[0], s.heads(q), dense_ptr(k), in_s[1], out_ptr(out[1]), out_s[1],
+                              s.heads(k), type_code(x.scalar_type()), a.pos, a.kind, a.stride, a.n_axes, a.axes, a.freq, (float)amplitude,
+                              (int)s.batch, (int)s.seq, (int)s.dim, a.rotary_dim, half, backward, stream_of(x));
+        return out;
+    }
+    static variable_list forward(AutogradContext* ctx, const Variable& q, const Maybe& k, const Variable& pos, const Variable& freq,
+                                 const Variable& axes, double amplitude, bool half) {
+        int rc = 0;
+        variable_list out = run(q, value(k), pos, freq, axes, amplitude, half, false, rc);
+        must(rc, "axial_rotary");
+        ctx->save_for_backward({pos, freq, axes});
+        ctx->saved_data["amplitude"] = amplitude;
+        ctx->saved_data["half"] = half;
+        ctx->set_materialize_grads(false);
+        if (!k.has_value()) out.pop_back();
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        variable_list result(7);
+        {
+            at::NoGradGuard no_grad;
+            at::Tensor g[2];
+            for (size_t i = 0; i < grads.size(); ++i)
+                if (grads[i].defined() && ctx->needs_input_grad(i)) g[i] = head_grad(grads[i]);
+            if (!g[0].defined() && !g[1].defined()) return result;
+            int rc = 0;
+            variable_list d = run(g[0], g[1], saved[0], saved[1], saved[2], ctx->saved_data["amplitude"].toDouble(),
+                                  ctx->saved_data["half"].toBool(), true, rc);
+            must_backward(rc, "axial_rotary");
+            result[0] = d[0];
+            result[1] = d[1];
+        }
+        return once_only(std::move(result), grads);
+    }
+};
+
+PyObject* _axial_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    FAST_BEGIN
+    Call c(args, n, 7);
+    const at::Tensor* q = c.tensor(0, true);
+    const at::Tensor* k = c.ok && args[1] != Py_None ? c.tensor(1, true) : nullptr;
+    const at::Tensor* pos = c.tensor(2, true);
+    const at::Tensor* freq = c.tensor(3);
+    const at::Tensor* axes = c.tensor(4, Dt::Int);
+    const float amplitude = c.real(5);
+    const bool half = c.flag(6);
+    need_heads(c, q, k, 4096);
+    need_angles(c, q, pos, freq, axes);
+    OR_NONE(c);
+    return answer([&]() -> PyObject* {
+        variable_list out;
+        {
+            WithoutGil unlocked;
+            if (c10::GradMode::is_enabled() && (q->requires_grad() || wants_grad(k))) {
+                out = AxialRotaryNode::apply(*q, maybe(k), *pos, *freq, *axes, (double)amplitude, half);
+            } else {
+                int rc = 0;
+                out = AxialRotaryNode::run(*q, value(maybe(k)), *pos, *freq, *axes, amplitude, half, false, rc);
+                must(rc, "axial_rotary");
+            }
+        }
+        return pair_of(std::move(out), k != nullptr);
+    });
+    FAST_END
+}
+
+// _head_norm(q, k | None, q_weight | None, k_weight | None, eps, positions | None, frequencies | None, axes | None, amplitude, half)
+struct HeadNormNode : torch::autograd::Function<HeadNormNode> {
+    static variable_list run(const at::Tensor& q, const at::Tensor& k, const at::Tensor& wq, const at::Tensor& wk, double eps, const at::Tensor& pos,
+                             const at::Tensor& freq, const at::Tensor& axes, double amplitude, bool half) {
+        const HeadShape s(q);
+        const AngleArgs a(pos, freq, axes);
+        variable_list out(2);
+        int64_t in_s[2][3] = {}, out_s[2][3] = {};
+        const at::Tensor* in[2] = {&q, &k};
+        for (int i = 0; i < 2; ++i) {
+            if (!in[i]->defined()) continue;
+            out[i] = empty_like_dtype(in[i]->sizes(), q, q.scalar_type());
+            s.strides(*in[i], in_s[i]);
+            s.strides(out[i], out_s[i]);
+        }
+        must(q8k_head_norm(dense_ptr(q), in_s[0], fptr(defined(wq)), out_ptr(out[0]), out_s[0], s.heads(q), dense_ptr(k), in_s[1],
+                           fptr(defined(wk)), out_ptr(out[1]), out_s[1], s.heads(k), type_code(q.scalar_type()), (float)eps, a.pos, a.kind, a.stride,
+                           a.n_axes, a.axes, a.freq, (float)amplitude, (int)s.batch, (int)s.seq, (int)s.dim, a.rotary_dim, half, stream_of(q)),
+             "head_norm");
+        return out;
+    }
+    static variable_list forward(AutogradContext* ctx, const Variable& q, const Maybe& k, const Maybe& wq, const Maybe& wk, double eps,
+                                 const Maybe& pos, const Maybe& freq, const Maybe& axes, double amplitude, bool half) {
+        variable_list out = run(q, value(k), value(wq), value(wk), eps, value(pos), value(freq), value(axes), amplitude, half);
+        ctx->save_for_backward({q, value(k), value(wq), value(wk), value(pos), value(freq), value(axes)});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["amplitude"] = amplitude;
+        ctx->saved_data["half"] = half;
+        ctx->set_materialize_grads(false);
+        if (!k.has_value()) out.pop_back();
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        variable_list result(10);
+        {
+            at::NoGradGuard no_grad;
+            // the inputs that are there are numbered: q, k, weight of q, weight of k
+            const bool there[4] = {true, saved[1].defined(), saved[2].defined(), saved[3].defined()};
+            bool need[4];
+            for (int i = 0, at = 0; i < 4; ++i) need[i] = there[i] && ctx->needs_input_grad(at++);
+            at::Tensor x[2], g[2], dx[2], dw[2], work;
+            int64_t xs[2][3] = {}, gs[2][3] = {}, ds[2][3] = {};
+            const HeadShape s(saved[0]);
+            for (int i = 0; i < 2; ++i) {
+                if ((size_t)i >= grads.size() || !grads[i].defined() || !(need[i] || need[2 + i])) continue;
+                x[i] = saved[i];
+                g[i] = head_grad(grads[i]);
+                dx[i] = empty_like_dtype(x[i].sizes(), x[i], x[i].scalar_type());
+                if (need[2 + i]) dw[i] = empty_like_dtype({s.dim}, x[i], Dt::Float);
+                s.strides(x[i], xs[i]);
+                s.strides(g[i], gs[i]);
+                s.strides(dx[i], ds[i]);
+            }
+            if (!x[0].defined() && !x[1].defined()) return result;
+            const at::Tensor& some = x[0].defined() ? x[0] : x[1];
+            int64_t bytes = 0;
+            if (dw[0].defined() || dw[1].defined()) {
+                bytes = (int64_t)q8k_head_norm_backward_workspace_bytes((int)s.dim);
+                work = empty_like_dtype({bytes}, some, Dt::Byte);
+            }
+            const AngleArgs a(saved[4], saved[5], saved[6]);
+            must_backward(q8k_head_norm_backward(
+                              dense_ptr(x[0]), xs[0], fptr(defined(saved[2])), dense_ptr(g[0]), gs[0], out_ptr(dx[0]), ds[0], out_f(dw[0]), s.heads(x[0]),
+                              dense_ptr(x[1]), xs[1], fptr(defined(saved[3])), dense_ptr(g[1]), gs[1], out_ptr(dx[1]), ds[1], out_f(dw[1]), s.heads(x[1]),
+                              type_code(some.scalar_type()), (float)ctx->saved_data["eps"].toDouble(), a.pos, a.kind, a.stride, a.n_axes, a.axes, a.freq,
+                              (float)ctx->saved_data["amplitude"].toDouble(), (int)s.batch, (int)s.seq, (int)s.dim, a.rotary_dim,
+                              ctx->saved_data["half"].toBool(), out_ptr(work), (size_t)bytes, stream_of(some)),
+                          "head_norm_backward");
+            for (int i = 0; i < 2; ++i) {
+                if (need[i]) result[i] = dx[i];
+                result[2 + i] = dw[i];
+            }
+        }
+        return once_only(std::move(result), grads);
+    }
+};
+
+PyObject* _head_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    FAST_BEGIN
+    Call c(args, n, 10);
+    const at::Tensor* q = c.tensor(0, true);
+    const at::Tensor* k = c.ok && args[1] != Py_None ? c.tensor(1, true) : nullptr;
+    const at::Tensor* wq = c.optional(2, Dt::Float);
+    const at::Tensor* wk = c.optional(3, Dt::Float);
+    const float eps = c.real(4);
+    const at::Tensor* pos = c.ok && args[5] != Py_None ? c.tensor(5, true) : nullptr;
+    const at::Tensor* freq = c.ok && args[6] != Py_None ? c.tensor(6) : nullptr;
+    const at::Tensor* axes = c.optional(7, Dt::Int);
+    const float amplitude = c.real(8);
+    const bool half = c.flag(9);
+    need_heads(c, q, k, 512);
+    need_angles(c, q, pos, freq, axes);
+    OR_NONE(c);
+    for (const at::Tensor* w : {wq, wk}) c.need(w == nullptr || (w->dim() == 1 && w->size(0) == q->size(-1) && !has_tangent(w)));
+    c.need(eps >= 0.f);
+    OR_NONE(c);
+    return answer([&]() -> PyObject* {
+        variable_list out;
+        {
+            WithoutGil unlocked;
+            if (c10::GradMode::is_enabled() && (q->requires_grad() || wants_grad(k) || wants_grad(wq) || wants_grad(wk)))
+                out = HeadNormNode::apply(*q, maybe(k), maybe(wq), maybe(wk), (double)eps, maybe(pos), maybe(freq), maybe(axes), (double)amplitude, half);
+            else
+                out = HeadNormNode::run(*q, value(maybe(k)), value(maybe(wq)), value(maybe(wk)), eps, value(maybe(pos)), value(maybe(freq)),
+                                        value(maybe(axes)), amplitude, half);
+        }
+        return pair_of(std::move(out), k != nullptr);
+    });
+    FAST_END
+}
+
+// ---- _fp4_linear(a, b, bias | None, block scales, row scales | None, gelu, out_type | None): the scales as their types, or their bits (uint8 and
+// int32), which is how FP4Linear holds them; row scales are what tells nvfp4 from mxfp4
+struct FP4Node : torch::autograd::Function<FP4Node> {
+    static at::Tensor run(const at::Tensor& a, const at::Tensor& b, const at::Tensor& bias, const at::Tensor& block, const at::Tensor& row, bool gelu,
+                          Dt out_type) {
+        const int format = row.defined() ? Q8K_FP4_NV : Q8K_FP4_MX;
+        const int64_t k = 2 * b.size(1), nn = b.size(0), m = a.numel() / k;
+        at::DimVector shape(lead(a).begin(), lead(a).end());
+        shape.push_back(nn);
+        at::Tensor out = empty_like_dtype(shape, a, out_type);
+        const int64_t bytes = (int64_t)q8k_fp4_linear_workspace_bytes(format, (int)m, (int)k);
+        at::Tensor work = empty_like_dtype({bytes}, a, Dt::Byte);
+        must(q8k_fp4_linear(format, a.const_data_ptr(), type_code(a.scalar_type()), b.const_data_ptr(), block.const_data_ptr(),
+                            static_cast<const float*>(dense_ptr(row)), fptr(defined(bias)), out.data_ptr(), type_code(out_type), (int)m, (int)nn, (int)k,
+                            gelu, work.data_ptr(), (size_t)bytes, g_status[a.device().index()]->data_ptr<int>(), stream_of(a)), "fp4_linear");
+        return out;
+    }
+    static Variable forward(AutogradContext* ctx, const Variable& a, const Variable& b, const Maybe& bias, const Variable& block, const Maybe& row,
+                            int64_t out_type) {
+        Variable out = run(a, b, value(bias), block, value(row), false, (Dt)out_type);
+        ctx->save_for_backward({b, block, value(row)});
+        ctx->saved_data["type"] = (int64_t)a.scalar_type();
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        variable_list result(6);
+        if (!grads[0].defined()) return result;
+        {
+            at::NoGradGuard no_grad;
+            const at::Tensor &b = saved[0], &block = saved[1], &row = saved[2];
+            at::Tensor g = grads[0].contiguous();
+            if (reinterpret_cast<uintptr_t>(g.const_data_ptr()) % 16 != 0) g = g.clone();
+            const int64_t k = 2 * b.size(1), nn = b.size(0), m = g.numel() / nn;
+            at::DimVector shape(lead(g).begin(), lead(g).end());
+            shape.push_back(k);
+            const Dt type = (Dt)ctx->saved_data["type"].toInt();
+            at::Tensor dx = empty_like_dtype(shape, g, type);
+            if (m > 0) {
+                void* st = stream_of(g);
+                auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+                const int64_t work_bytes = up((int64_t)q8k_fp4_weight_operand_workspace_bytes((int)nn, (int)k));
+                // one scratch: gradient rows and scales, weight operand and scales, its workspace
+                const int64_t at_gs = up(m * nn), at_w = at_gs + up(4 * m), at_ws = at_w + up(k * nn), at_work = at_ws + up(4 * k);
+                at::Tensor scratch = empty_like_dtype({at_work + work_bytes}, g, Dt::Byte);
+                uint8_t* s = static_cast<uint8_t*>(scratch.data_ptr());
+                float *gs = reinterpret_cast<float*>(s + at_gs), *ws = reinterpret_cast<float*>(s + at_ws);
+                must_backward(q8k_tokenwise_quant(g.const_data_ptr(), type_code(g.scalar_type()), s, Q8K_DT_E4M3, gs, m, (int)nn, nn, st),
+                              "tokenwise_quant");
+                must_backward(q8k_fp4_weight_operand(row.defined() ? Q8K_FP4_NV : Q8K_FP4_MX, b.const_data_ptr(), block.const_data_ptr(),
+                                                     static_cast<const float*>(dense_ptr(row)), s + at_w, ws, (int)nn, (int)k, s + at_work,
+                                                     (size_t)work_bytes, st), "fp4_weight_operand");
+                must_backward(q8k_fp8_mm(s, s + at_w, nullptr, gs, ws, dx.data_ptr(), type_code(type), 1, 1, (int)m, (int)k, (int)nn, 0,
+                                         g_status[g.device().index()]->data_ptr<int>(), st), "fp8_mm");
+            }
+            result[0] = dx;
+        }
+        return once_only(std::move(result), grads);
+    }
+};
+
+PyObject* _fp4_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    FAST_BEGIN
+    Call c(args, n, 7);
+    const at::Tensor* a = c.tensor(0);
+    const at::Tensor* b = c.tensor(1, Dt::Byte);
+    const at::Tensor* bias = c.optional(2, Dt::Float);
+    const at::Tensor* block = c.tensor(3);
+    const at::Tensor* row = c.ok && args[4] != Py_None ? c.tensor(4) : nullptr;
+    const bool gelu = c.flag(5);
+    OR_NONE(c);
+    const Dt in = a->scalar_type(), out = c.dtype(6, in);
+    auto half_type = [](Dt t) { return t == Dt::BFloat16 || t == Dt::Half; };
+    auto aligned = [](const at::Tensor* t) { return reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 == 0; };
+    const bool nv = row != nullptr;
+    c.need(half_type(in) && half_type(out) && has_rows(a) && b->dim() == 2 && b->size(1) >= 1 && 2 * b->size(1) == a->size(-1) &&
+           (block->scalar_type() == Dt::Byte || block->scalar_type() == (nv ? Dt::Float8_e4m3fn : Dt::Float8_e8m0fnu)) &&
+           (!nv || row->scalar_type() == Dt::Float || row->scalar_type() == Dt::Int));
+    OR_NONE(c);
+    const int64_t k = a->size(-1), nn = b->size(0), m = a->numel() / k;
+    const bool training = c10::GradMode::is_enabled() && a->requires_grad();
+    c.need(aligned(a) && aligned(b) && aligned(block) && k % 32 == 0 && k <= 65536 && nn > 0 && nn % 16 == 0 && nn <= 0x3fffffff && m <= 0x7fffff00 &&
+           m * (k / 16) <= 0x7fffffffLL * 128 && block->dim() == 3 && block->size(0) == (nn + 127) / 128 &&
+           block->size(1) == (k + 255) / 256 * (nv ? 4 : 2) && block->size(2) == 512 && (!nv || row->numel() == nn) &&
+           (bias == nullptr || bias->numel() == nn) && !(training && (gelu || nn > 32768)) && !has_tangent(a) && !has_tangent(bias) && !has_tangent(row));
+    c.status();
+    OR_NONE(c);
+    return answer([&]() -> PyObject* {
+        at::Tensor y;
+        {
+            WithoutGil unlocked;
+            y = training ? FP4Node::apply(*a, *b, maybe(bias), *block, maybe(row), (int64_t)out)
+                         : FP4Node::run(*a, *b, value(maybe(bias)), *block, value(maybe(row)), gelu, out);
+        }
+        return wrap(std::move(y));
+    });
+    FAST_END
+}
+
 // ---------------------------------------------------------------- module
 PyObject* set_check(PyObject*, PyObject* f) {
     Py_INCREF(f);
@@ -1058,6 +1449,7 @@ PyMethodDef methods[] = {
     FAST(dequant_hadamard), FAST(rms_norm), FAST(rms_norm_backward), FAST(rope), FAST(rope_backward), FAST(mm),
     FAST(mm_gate_residual), FAST(linear), FAST(flash_attention), FAST(attention_prep_rows), FAST(qk_norm_rope_prep),
     FAST(kv_prep), FAST(qk_norm_rope_prep_pair), FAST(_layer_norm), FAST(_rotary), FAST(_gated_linear),
+    FAST(_axial_rotary), FAST(_head_norm), FAST(_fp4_linear),
     {"set_check", set_check, METH_O, nullptr}, {"set_status_word", set_status_word, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -67,6 +67,12 @@ def fp4_linear(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor] = 
     Differentiable in an un-quantised ``a``."""
     if scale_b is None:
         raise native.Q8KernelError("fp4_linear: the weight must be 4-bit values with their scales")
+    if scale_a is None and isinstance(scale_b, (tuple, list)) and len(scale_b) == 2 and isinstance(scale_b[0], torch.Tensor) \
+            and scale_b[0].dtype != torch.uint8 and (scale_b[1] is None or scale_b[1].dtype == torch.float32):
+        # (_host takes the bits that FP4Linear holds, too)
+        fast = native._host._fp4_linear(a, b, bias, scale_b[0], scale_b[1], bool(fuse_gelu), out_dtype)
+        if fast is not None:
+            return fast
     out_dtype = (a.dtype if is_16bit(a) else torch.bfloat16) if out_dtype is None else out_dtype
     if not is_16bit(out_dtype):
         raise native.Q8KernelError(f"fp4_linear: output type {out_dtype} is not bfloat16 or float16")

@@ -43,7 +43,12 @@ def head_norm(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Optio
         raise native.Q8KernelError(f"head_norm: layout {layout!r} is not one of {', '.join(LAYOUTS)}")
     if not eps >= 0.0:
         raise native.Q8KernelError(f"head_norm: eps {eps} must not be negative")
+    if frequencies is not None and frequencies.dtype != torch.float64:           # (_host takes int64 as the bits that the modules hold)
+        raise native.Q8KernelError(f"head_norm: frequencies must be float64 [rotary_dim / 2], not {frequencies.dtype}")
     eps, amplitude, half = float(eps), float(amplitude), layout == "half"
+    fast = native._host._head_norm(q, k, q_weight, k_weight, eps, positions, frequencies, axes, amplitude, half)
+    if fast is not None:
+        return fast
     native.refuse_tangents("head_norm", q, k, q_weight, k_weight, positions, frequencies)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         return HeadNorm.apply(q, k, q_weight, k_weight, eps, positions, frequencies, axes, amplitude, half)

@@ -155,7 +155,12 @@ def apply_axial_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: to
     int32 [rotary_dim / 2], both on the device (``axial_frequencies``); an axis beyond A is taken as the last.  Differentiable in q and k."""
     if layout not in LAYOUTS:
         raise Q8KernelError(f"apply_axial_rotary: layout {layout!r} is not one of {', '.join(LAYOUTS)}")
+    if frequencies.dtype != torch.float64:                       # (_host takes int64 as the bits that AxialRotaryEmbedding holds)
+        raise Q8KernelError(f"apply_axial_rotary: frequencies must be float64 [rotary_dim / 2], not {frequencies.dtype}")
     amplitude, half = float(amplitude), layout == "half"
+    fast = _host._axial_rotary(q, k, positions, frequencies, axes, amplitude, half)
+    if fast is not None:
+        return fast
     refuse_tangents("apply_axial_rotary", q, k, positions, frequencies)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return AxialRotary.apply(q, k, positions, frequencies, axes, amplitude, half)

@@ -175,6 +175,10 @@ class FP4Linear(nn.Module):
         bias = self.bias
         if bias is not None and bias.dtype != torch.float:
             bias = bias.float()
+        if x_scales is None:
+            fast = native._host._fp4_linear(x, self.weight, bias, self.block_scales, self.scales, fuse_gelu, out_dtype)
+            if fast is not None:
+                return fast
         return Q8F.fp4.fp4_linear(x, self.weight, bias, x_scales, self.weight_scales, fuse_gelu, out_dtype)
 
     @classmethod

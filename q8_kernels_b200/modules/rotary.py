@@ -72,6 +72,9 @@ class AxialRotaryEmbedding(nn.Module):
             raise Q8KernelError(f"AxialRotaryEmbedding: heads of {q.shape[-1]} channels, {self.head_dim} expected")
         if positions.dim() < 2 or positions.shape[-1] != len(self.sections):
             raise Q8KernelError(f"AxialRotaryEmbedding: positions {tuple(positions.shape)} for {len(self.sections)} axes")
+        fast = _host._axial_rotary(q, k, positions, self._frequency_bits, self._axes, self.amplitude, self._half)
+        if fast is not None:
+            return fast
         return Q8F.rotary.apply_axial_rotary(q, k, positions, self.frequencies, self._axes, self.amplitude, self.layout)
 
 
@@ -84,7 +87,7 @@ class HeadNormRotary(nn.Module):
         super().__init__()
         if rotary is not None and (not isinstance(rotary, (RotaryEmbedding, AxialRotaryEmbedding)) or rotary.head_dim != head_dim):
             raise Q8KernelError(f"HeadNormRotary: {rotary} is no rotary embedding of heads of {head_dim} channels")
-        self.head_dim, self.rotary, self.eps = head_dim, rotary, eps
+        self.head_dim, self.rotary, self.eps = head_dim, rotary, float(eps)
         for name in ("q_weight", "k_weight"):
             if elementwise_affine:
                 setattr(self, name, nn.Parameter(torch.ones(head_dim, dtype=torch.float, device=device)))
@@ -105,4 +108,7 @@ class HeadNormRotary(nn.Module):
             axes = r.axes
             if positions is None or positions.dim() < 2 or positions.shape[-1] != len(r.sections):
                 raise Q8KernelError(f"HeadNormRotary: positions {None if positions is None else tuple(positions.shape)} for {len(r.sections)} axes")
+        fast = _host._head_norm(q, k, *weights, self.eps, positions, r._frequency_bits, axes, r.amplitude, r._half)
+        if fast is not None:
+            return fast
         return Q8F.head_norm.head_norm(q, k, *weights, self.eps, positions, r.frequencies, axes, r.amplitude, r.layout)
