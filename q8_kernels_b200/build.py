@@ -26,7 +26,7 @@ HOST_PATH = os.path.join(PKG_DIR, "_host" + sysconfig.get_config_var("EXT_SUFFIX
 HOST_KEY = os.path.join(OBJ_DIR, os.path.basename(HOST_PATH) + ".key")     # what the extension was built against
 
 SOURCES = ["capi.cu", "rowwise.cu", "hadamard.cu", "gemm.cu", "gemm_pair.cu", "gemm_split.cu", "attention.cu",
-           "layer_norm.cu", "rotary.cu", "head_norm.cu", "gemm_gated.cu", "gated.cu", "fp4.cu", "gemm_fp4.cu"]
+           "layer_norm.cu", "rotary.cu", "head_norm.cu", "gemm_gated.cu", "gated.cu", "fp4.cu", "gemm_fp4.cu", "gemm_fp4_pair.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -292,6 +292,11 @@ extern "C" int q8k_fp4_mm(int format, const void* a, const void* a_block_scales,
     p.out = out;
     p.status = dev_status;
     p.M = M; p.N = N; p.K = K;
-    return launch_fp4_tiles(nv, fuse_gelu != 0, out_dtype == Q8K_DT_F16, {a, a_block_scales, a_row_scales}, {b, b_block_scales, b_row_scales}, p,
+    const Fp4Operand oa = {a, a_block_scales, a_row_scales}, ob = {b, b_block_scales, b_row_scales};
+    if (M > 256 && N >= 256) {
+        const int rc = launch_fp4_pair(nv, fuse_gelu != 0, out_dtype == Q8K_DT_F16, oa, ob, p, (cudaStream_t)stream);
+        if (rc != Q8K_ERR_UNSUPPORTED) return rc;
+    }
+    return launch_fp4_tiles(nv, fuse_gelu != 0, out_dtype == Q8K_DT_F16, oa, ob, p,
                             fp4_tile_columns(M, N), (cudaStream_t)stream);
 }

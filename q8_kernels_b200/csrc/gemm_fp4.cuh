@@ -15,6 +15,9 @@ struct Fp4GemmParams {
     int M, N, K;
 };
 
+// 256 x 256 tiles on CTA pairs; Q8K_ERR_UNSUPPORTED (without touching the error detail) when the device cannot co-schedule the clusters.
+int launch_fp4_pair(bool nv, bool gelu, bool f16, const Fp4Operand& a, const Fp4Operand& b, const Fp4GemmParams& p, cudaStream_t st);
+
 // Tensor map of an operand's block scales: [row tiles][slabs][bytes of a slab], in rows of 256 bytes, boxes of one slab of `tiles` row tiles.
 inline int make_scales_map(CUtensorMap* map, const void* scales, bool nv, int64_t rows, int K, int tiles, const char* op) {
     const uint64_t per_slab = (uint64_t)fp4_slab_scales(nv) / 256, per_tile = per_slab * (uint64_t)fp4_slabs(K);
