@@ -69,85 +69,188 @@ template <typename T> __device__ __forceinline__ uint2 fp4_pack(const uint4 (&r)
     return make_uint2(w[0], w[1]);
 }
 
-// T threads a row, `rows_per_cta` rows a CTA, UNITS units a thread.  The row's scales beyond K, up to its last slab, become 0.
-template <typename Tin, bool NV, int UNITS>
-__global__ void __launch_bounds__(1024)
-fp4_quant_kernel(const Tin* __restrict__ x, int64_t x_stride, uint8_t* __restrict__ q, uint8_t* __restrict__ block_scales,
-                 float* __restrict__ row_scales, int64_t rows, int K, int slabs, int threads) {
-    __shared__ float red[32];
-    const int group = threadIdx.x / threads, t = threadIdx.x - group * threads;
-    const int64_t row = (int64_t)blockIdx.x * (blockDim.x / threads) + group;
-    const bool here = row < rows;
-    const int units = K / kFp4Unit;
-    pdl_wait();
-    pdl_release();
-    uint4 r[UNITS][2];
-    float a[UNITS];
-    float top = 0.f;
+// A row's scale and the factor on its blocks' absmax (nvfp4), from the row's absmax.
+__device__ __forceinline__ void fp4_row_factors(float top, float& g, float& rs) {
+    g = top > 0.f ? fp4_finite(__fdiv_rn(448.0f, top)) : top;  // 0 and NaN stay what they are
+    rs = __fdiv_rn(top, 2688.0f);
+}
+// The scale byte of a unit's block and the factor on its values.  mxfp4: a block of 32 is the units of two neighbouring lanes.
+template <bool NV> __device__ __forceinline__ uint8_t fp4_block_scale(float a, float g, float rs, float& factor) {
+    if constexpr (NV) {
+        const uint8_t scale = float_to_e4m3_sat(__fmul_rn(a, g));
+        const float s = e4m3_to_float(scale);
+        factor = s == 0.f ? 0.f : fp4_finite(__fdiv_rn(1.0f, __fmul_rn(s, rs)));
+        return scale;
+    } else {
+        const float both = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
+        const int field = (int)(__float_as_uint(both) >> 23);  // (no sign)
+        const int e = field == 255 ? 255 : field > 2 ? field - 2 : 0;
+        factor = __uint_as_float((uint32_t)(254 - (e == 255 ? 254 : e)) << 23);     // 2^-e; any for NaN
+        return (uint8_t)e;
+    }
+}
+template <typename Tin, int UNITS>
+__device__ __forceinline__ void fp4_load(const Tin* __restrict__ row, int t, int threads, int units, bool here, uint4 (&r)[UNITS][2]) {
 #pragma unroll
     for (int i = 0; i < UNITS; ++i) {
         const int u = t + i * threads;
+        const uint4* p = reinterpret_cast<const uint4*>(row + u * kFp4Unit);
         const bool in = here && u < units;
-        const uint4* p = reinterpret_cast<const uint4*>(x + row * x_stride + u * kFp4Unit);
         r[i][0] = in ? p[0] : make_uint4(0, 0, 0, 0);
         r[i][1] = in ? p[1] : make_uint4(0, 0, 0, 0);
     }
+}
+
+// Few rows: a CTA for every row, UNITS units a thread.  The row's scales beyond K, up to its last slab, become 0.
+template <typename Tin, bool NV, int UNITS>
+__global__ void __launch_bounds__(1024)
+fp4_quant_row_kernel(const Tin* __restrict__ x, int64_t x_stride, uint8_t* __restrict__ q, uint8_t* __restrict__ block_scales,
+                     float* __restrict__ row_scales, int K, int slabs) {
+    __shared__ float red[32];
+    const int64_t row = blockIdx.x;
+    const int t = threadIdx.x, units = K / kFp4Unit;
+    pdl_wait();
+    pdl_release();
+    uint4 r[UNITS][2];
+    fp4_load<Tin, UNITS>(x + row * x_stride, t, blockDim.x, units, true, r);
+    float a[UNITS];
+    float top = 0.f, g = 0.f, rs = 0.f;
 #pragma unroll
     for (int i = 0; i < UNITS; ++i) {
         a[i] = Fp4In<Tin>::absmax(r[i]);
         top = max_nan(top, a[i]);
     }
-    float g = 0.f, rs = 0.f;
     if constexpr (NV) {
         top = warp_max<true>(top);
-        if (threads > 32) {                                    // one row a CTA then
-            if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+        if (blockDim.x > 32) {
+            if ((t & 31) == 0) red[t >> 5] = top;
             __syncthreads();
-            top = warp_max<true>((threadIdx.x & 31) < blockDim.x / 32 ? red[threadIdx.x & 31] : 0.f);
+            top = warp_max<true>((t & 31) < blockDim.x / 32 ? red[t & 31] : 0.f);
         }
-        g = top > 0.f || top != top ? fp4_finite(__fdiv_rn(448.0f, top)) : 0.f;
-        if (top != top) g = top;
-        rs = __fdiv_rn(top, 2688.0f);
-        if (here && t == 0) row_scales[row] = rs;
+        fp4_row_factors(top, g, rs);
+        if (t == 0) row_scales[row] = rs;
     }
 #pragma unroll
     for (int i = 0; i < UNITS; ++i) {
-        const int u = t + i * threads;
+        const int u = t + i * blockDim.x;
         float factor;
-        uint8_t scale;
-        if constexpr (NV) {
-            scale = float_to_e4m3_sat(__fmul_rn(a[i], g));
-            const float s = e4m3_to_float(scale);
-            factor = s == 0.f ? 0.f : fp4_finite(__fdiv_rn(1.0f, __fmul_rn(s, rs)));
-        } else {
-            const float both = max_nan(a[i], __shfl_xor_sync(0xffffffffu, a[i], 1));     // a block of 32 is two neighbours' units
-            const int field = (int)(__float_as_uint(both) >> 23);                        // (no sign)
-            const int e = field == 255 ? 255 : field > 2 ? field - 2 : 0;
-            scale = (uint8_t)e;
-            factor = __uint_as_float((uint32_t)(254 - (e == 255 ? 254 : e)) << 23);      // 2^-e; any for NaN
-        }
-        if (here && u < units) *reinterpret_cast<uint2*>(q + row * (int64_t)(K / 2) + u * 8) = fp4_pack<Tin>(r[i], factor);
-        if (here && u < slabs * (kFp4Slab / kFp4Unit)) {
+        const uint8_t scale = fp4_block_scale<NV>(a[i], g, rs, factor);
+        if (u < units) *reinterpret_cast<uint2*>(q + row * (int64_t)(K / 2) + u * 8) = fp4_pack<Tin>(r[i], factor);
+        if (u < slabs * (kFp4Slab / kFp4Unit)) {
             if constexpr (NV) block_scales[fp4_scale_at<true>(row, u, slabs)] = u < units ? scale : 0;
             else if ((u & 1) == 0) block_scales[fp4_scale_at<false>(row, u >> 1, slabs)] = u < units ? scale : 0;
         }
     }
 }
 
+// Many rows: a CTA takes the eight rows whose block scales lie side by side, r, r + 1 and those 32, 64 and 96 further on, and stores the scales as
+// whole sectors of 32 bytes from shared memory.  (Byte by byte they were a fifth of all accesses to L2.)  T threads a row; where the rows
+// are taken in steps, the next ones are on their way while one is quantised.  Scales of rows behind the last one, up to the row tile's end, become 0.
+constexpr int kFp4GroupRows = 8;
+template <typename Tin, bool NV, int UNITS, int T, int CTA>
+__global__ void __launch_bounds__(CTA)
+fp4_quant_kernel(const Tin* __restrict__ x, int64_t x_stride, uint8_t* __restrict__ q, uint8_t* __restrict__ block_scales,
+                 float* __restrict__ row_scales, int64_t rows, int K, int slabs) {
+    constexpr int AT_ONCE = CTA / T, STEPS = kFp4GroupRows / AT_ONCE;
+    static_assert(AT_ONCE >= 1 && AT_ONCE <= kFp4GroupRows, "rows at a time");
+    __shared__ float red[CTA / 32];
+    extern __shared__ __align__(16) uint8_t scales[];          // [tiles along K][32]
+    const int group = threadIdx.x / T, t = threadIdx.x % T, units = K / kFp4Unit;
+    const int64_t row0 = (int64_t)(blockIdx.x >> 4) * 128 + (blockIdx.x & 15) * 2;
+    pdl_wait();
+    pdl_release();
+    auto row_of = [&](int step, int& local) {
+        local = step * AT_ONCE + group;
+        return row0 + (local & 1) + 32 * (local >> 1);
+    };
+    uint4 r[UNITS][2];
+    int local;
+    int64_t row = row_of(0, local);
+    fp4_load<Tin, UNITS>(x + row * x_stride, t, T, units, row < rows, r);
+#pragma unroll
+    for (int step = 0; step < STEPS; ++step) {
+        uint4 next[STEPS > 1 ? UNITS : 1][2];
+        int local_next = 0;
+        int64_t row_next = rows;
+        if constexpr (STEPS > 1) {
+            if (step + 1 < STEPS) {
+                row_next = row_of(step + 1, local_next);
+                fp4_load<Tin, UNITS>(x + row_next * x_stride, t, T, units, row_next < rows, next);
+            }
+        }
+        const bool here = row < rows;
+        float a[UNITS];
+        float top = 0.f, g = 0.f, rs = 0.f;
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i) {
+            a[i] = Fp4In<Tin>::absmax(r[i]);
+            top = max_nan(top, a[i]);
+        }
+        if constexpr (NV) {
+            top = warp_max<true>(top);
+            if constexpr (T > 32) {
+                const int warp = threadIdx.x >> 5;
+                if (step > 0) __syncthreads();                 // the values before have been read
+                if ((threadIdx.x & 31) == 0) red[warp] = top;
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < T / 32; ++k) top = max_nan(top, red[group * (T / 32) + k]);
+            }
+            fp4_row_factors(top, g, rs);
+            if (here && t == 0) row_scales[row] = rs;
+        }
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i) {
+            const int u = t + i * T;
+            float factor;
+            const uint8_t scale = fp4_block_scale<NV>(a[i], g, rs, factor);            // (0 for rows and units that are not there)
+            if (here && u < units) *reinterpret_cast<uint2*>(q + row * (int64_t)(K / 2) + u * 8) = fp4_pack<Tin>(r[i], factor);
+            const int b = NV ? u : u >> 1;
+            if (u < slabs * (kFp4Slab / kFp4Unit) && (NV || (u & 1) == 0))
+                scales[(b >> 2) * 32 + (local & 1) * 16 + (local >> 1) * 4 + (b & 3)] = scale;
+        }
+        if constexpr (STEPS > 1) {
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) { r[i][0] = next[i][0]; r[i][1] = next[i][1]; }
+            row = row_next;
+            local = local_next;
+        }
+    }
+    __syncthreads();
+    const int tiles = slabs * fp4_slab_tiles(NV);
+    uint8_t* to = block_scales + (int64_t)(blockIdx.x >> 4) * tiles * 512 + (blockIdx.x & 15) * 32;
+    for (int k = threadIdx.x; k < 2 * tiles; k += CTA)
+        *reinterpret_cast<uint4*>(to + (int64_t)(k >> 1) * 512 + (k & 1) * 16) = *reinterpret_cast<const uint4*>(scales + k * 16);
+}
+
+// Which of the two, from times of CUDA graphs (us, groups of rows against a CTA a row): rows of 2048 values, 24576 of them nvfp4 21.0 against 26.1,
+// mxfp4 19.8 against 26.0, 6144 of them 7.4 against 7.4 and 6.5 against 7.0, 2002 of them 4.2 against 4.2 and 3.6 against 3.2;  6144 rows of
+// 4096 15.4 against 11.9 and 12.3 against 10.8, of 8192 25.2 against 22.1 and 24.2 against 19.8 (0.89 and 0.98 of the copy rate): a long
+// row fills a CTA, and eight of them one after the other leave a long last round.
+// Units of a thread, a CTA a row: one for few or short rows, where latency counts (2002 x 2048 mxfp4 3.2, two 3.7), else two (6144 x 8192 nvfp4 one
+// 28.4, two 22.3, four 22.1), and four where 1024 threads need them.
+constexpr int kFp4GroupK = 2048, kFp4GroupMinRows = 4096, kFp4FewRows = 1024;
 template <typename Tin, bool NV>
 static int launch_fp4_quant(const void* x, int64_t stride, void* q, void* bs, float* rs, int64_t rows, int K, cudaStream_t st) {
     const int slabs = fp4_slabs(K), units = slabs * (kFp4Slab / kFp4Unit);
-    int threads = ((units + 3) / 4 + 31) / 32 * 32;            // four units a thread
-    const int per_cta = threads > 32 ? 1 : 4;
-    const int64_t grid = (rows + per_cta - 1) / per_cta;
+    if (K > kFp4GroupK || rows < kFp4GroupMinRows) {
+        auto go = [&](auto kern, int per) {
+            const int threads = ((units + per - 1) / per + 31) / 32 * 32;
+            Q8K_CUDA_OK(launch_dependent(kern, (unsigned)rows, (unsigned)threads, 0, st, 1, (const Tin*)x, stride, (uint8_t*)q, (uint8_t*)bs, rs, K, slabs));
+            return (int)Q8K_OK;
+        };
+        if (units <= 1024 && (rows < kFp4FewRows || K <= kFp4GroupK)) return go(fp4_quant_row_kernel<Tin, NV, 1>, 1);
+        return units <= 2048 ? go(fp4_quant_row_kernel<Tin, NV, 2>, 2) : go(fp4_quant_row_kernel<Tin, NV, 4>, 4);
+    }
     auto go = [&](auto kern) {
-        Q8K_CUDA_OK(launch_dependent(kern, (unsigned)grid, (unsigned)(threads * per_cta), 0, st, 1, (const Tin*)x, stride, (uint8_t*)q, (uint8_t*)bs, rs,
-                                     rows, K, slabs, threads));
+        Q8K_CUDA_OK(launch_dependent(kern, (unsigned)(fp4_row_tiles(rows) * 16), 256, (size_t)slabs * fp4_slab_tiles(NV) * 32, st, 1, (const Tin*)x, stride,
+                                     (uint8_t*)q, (uint8_t*)bs, rs, rows, K, slabs));
         return (int)Q8K_OK;
     };
-    if (threads <= 1024) return go(fp4_quant_kernel<Tin, NV, 4>);
-    set_error_detail("fp4_quant: K=%d exceeds 65536", K);
-    return Q8K_ERR_UNSUPPORTED;
+    if (units <= 32) return go(fp4_quant_kernel<Tin, NV, 1, 32, 256>);
+    if (units <= 64) return go(fp4_quant_kernel<Tin, NV, 2, 32, 256>);
+    if constexpr (!NV) return go(fp4_quant_kernel<Tin, NV, 2, 64, 256>);       // (no sum over a row: two steps with the next rows on their way)
+    return units <= 96 ? go(fp4_quant_kernel<Tin, NV, 3, 32, 256>) : go(fp4_quant_kernel<Tin, NV, 4, 32, 256>);
 }
 
 // What the values stand for: value * block scale (exact in fp32) * row scale, rounded, then to Tout.
