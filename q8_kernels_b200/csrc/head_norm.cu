@@ -27,19 +27,22 @@ struct HeadNormParams {
     HeadTensor t[2];                         // queries, keys
     RotaryAngles angles;
     float eps;
-    float* part;                             // [CTA][2][head_dim] sums for dw; null: not wanted
-    int64_t tokens;                          // batch * seq
-    int seq, head_dim, rotary_dim, half;     // half: layout
+    float* part;                             // [CTA][head_dim] sums for dw; null: not wanted
+    unsigned tokens;                         // batch * seq
+    unsigned seq;
+    int head_dim, rotary_dim, half;          // half: layout
 };
 
 constexpr int kHeadMaxDim = 512;
 constexpr int kHeadThreads = 128;
-constexpr int kHeadChannels = 16;            // channels of a lane
+constexpr int kHeadChannels = 16;            // channels of a lane: 8 in the first runs of its units, 8 in the second
 constexpr int kHeadRows = 8;                 // heads of a thread, where there are threads for the others
 constexpr int kHeadMaxCtas = 148 * 8;        // of the backward pass with sums
 
-// A warp's lanes are groups of `lanes`, each with a head; a CTA's groups are `tokens` times `head_lanes`.
-struct HeadLanes { int lanes, groups, head_lanes, tokens; };
+// A warp's lanes are groups of `lanes`, each with a head.  A CTA works for queries or for keys; its groups are `tokens` times `head_lanes`.
+// CTAs [0, ctas[0]) are the queries', the ctas[1] behind them the keys'.
+struct HeadSplit { int head_lanes, tokens, ctas; };
+struct HeadLanes { int lanes, groups; HeadSplit of[2]; };
 
 template <int BYTES> struct HeadRaw;
 template <> struct HeadRaw<2>  { using type = uint16_t; };
@@ -47,82 +50,220 @@ template <> struct HeadRaw<4>  { using type = uint32_t; };
 template <> struct HeadRaw<8>  { using type = uint2; };
 template <> struct HeadRaw<16> { using type = uint4; };
 
-// Sum over a group's lanes, in each of them; `top` is half the power of two that holds them.
-__device__ __forceinline__ float head_sum(float v, int lane, int lanes, int top, bool pow2) {
-    if (pow2) {
-        for (int o = top; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        return v;
+// Sums over a group's lanes, in each of them.  LANES 0: any number of them, `top` is half the power of two that holds them.
+template <int LANES, int N> __device__ __forceinline__ void head_sum(float (&v)[N], int lane, int lanes, int top) {
+    if constexpr (LANES > 0) {
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+        }
+    } else {
+        const int in = lane % lanes, first = lane - in;
+#pragma unroll 1
+        for (int o = top; o > 0; o >>= 1) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float u = __shfl_down_sync(0xffffffffu, v[i], o);
+                if (in + o < lanes) v[i] += u;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, v[i], first);
     }
-    const int in = lane % lanes, first = lane - in;
-    for (int o = top; o > 0; o >>= 1) {
-        const float u = __shfl_down_sync(0xffffffffu, v, o);
-        if (in + o < lanes) v += u;
+}
+
+// Eight values of a lane's runs, widened as packed pairs, and back.
+template <typename T> __device__ __forceinline__ void head_widen(const T (&e)[8], float2 (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = make_float2(to_float<T>(e[2 * i]), to_float<T>(e[2 * i + 1]));
+}
+template <> __device__ __forceinline__ void head_widen<__nv_bfloat16>(const __nv_bfloat16 (&e)[8], float2 (&v)[4]) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+template <typename T> __device__ __forceinline__ void head_narrow(const float2 (&v)[4], T (&e)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        e[2 * i] = from_float<T>(v[i].x);
+        e[2 * i + 1] = from_float<T>(v[i].y);
     }
-    return __shfl_sync(0xffffffffu, v, first);
+}
+template <> __device__ __forceinline__ void head_narrow<__nv_bfloat16>(const float2 (&v)[4], __nv_bfloat16 (&e)[8]) {
+    __nv_bfloat162* w = reinterpret_cast<__nv_bfloat162*>(&e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __floats2bfloat162_rn(v[i].x, v[i].y);
+}
+template <> __device__ __forceinline__ void head_narrow<__half>(const float2 (&v)[4], __half (&e)[8]) {
+    __half2* w = reinterpret_cast<__half2*>(&e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __floats2half2_rn(v[i].x, v[i].y);
+}
+
+// Asynchronous copy of BYTES (4, 8 or 16) to shared memory, zeros where `there` is false.
+template <int BYTES> __device__ __forceinline__ void head_copy(uint32_t dst, const void* src, bool there) {
+    const int n = there ? BYTES : 0;
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
 }
 
 // V channels an access.  TWO: a pair's channels lie in the two runs of a unit (half layout, or V = 1), else side by side in one.
-template <typename T, int V, bool TWO, bool BACK>
-__global__ void __launch_bounds__(kHeadThreads, BACK ? 2 : 4)
-head_norm_kernel(const __grid_constant__ HeadNormParams p, const HeadLanes l) {
-    constexpr int UNITS = kHeadChannels / (2 * V);             // of a lane
+// A lane has 8 / V units; their first runs are its channels a[0..8), their second ones b[0..8).
+//
+// A thread's heads are on their way to its own slots of a ring in shared memory, STAGES of them, the first while the angles are made and the
+// next token's while this one's are worked on.
+template <typename T, bool BACK> struct HeadRing {
+    static constexpr int stages = BACK && sizeof(T) == 4 ? 3 : 4;         // (three of 16 KB leave room for four CTAs an SM)
+    static constexpr int pieces = 8 * (int)sizeof(T) / 16;     // 16-byte pieces of a run
+    static constexpr int runs = BACK ? 4 : 2;                  // x: a, b; gradient: a, b
+    static constexpr int stage_bytes = runs * pieces * kHeadThreads * 16;
+    static constexpr int bytes = stages * stage_bytes;
+};
+//
+// LANES: heads of 16 LANES channels, all of whose lanes and, in every round, heads exist, and weights of 16-byte alignment; 0: any.  (The
+// checks, the sums' loops and the index arithmetic of the general form are half of its instructions.)
+template <typename T, int V, bool TWO, bool BACK, int LANES>
+__global__ void __launch_bounds__(kHeadThreads, BACK ? 4 : 6)
+head_norm_kernel(const __grid_constant__ HeadNormParams p, const __grid_constant__ HeadLanes l) {
+    using Ring = HeadRing<T, BACK>;
+    constexpr int UNITS = 8 / V;
     using Raw = typename HeadRaw<V * sizeof(T)>::type;
-    union Run { Raw r; T e[V]; };
-    struct Head { Run a[UNITS], b[UNITS]; };
-    extern __shared__ float smem[];
-    float2* turns = reinterpret_cast<float2*>(smem);           // [tokens][rotary_dim / 2] cosine, sine
+    extern __shared__ __align__(16) uint8_t smem[];
+    float2* turns = reinterpret_cast<float2*>(smem + Ring::bytes);             // [tokens][rotary_dim / 2] cosine, sine
+    const bool keys = (int)blockIdx.x >= l.of[0].ctas;
+    const HeadSplit& sp = l.of[keys];
+    const HeadTensor& t = p.t[keys];
+    const unsigned cta = blockIdx.x - (keys ? l.of[0].ctas : 0);
     const int half_dim = p.rotary_dim / 2;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int group = lane / l.lanes, ul = lane - group * l.lanes;
-    const int slot = warp * l.groups + group;
-    const int tl = slot / l.head_lanes, h0 = slot - tl * l.head_lanes;
-    const bool has_slot = group < l.groups && tl < l.tokens;
-    const bool pow2 = (l.lanes & (l.lanes - 1)) == 0;
+    const int lanes = LANES > 0 ? LANES : l.lanes, groups = LANES > 0 ? 32 / LANES : l.groups;
+    const int group = lane / lanes, ul = lane - group * lanes;
+    const int slot = warp * groups + group;
+    const int tl = slot / sp.head_lanes, h0 = slot - tl * sp.head_lanes;
+    const bool has_slot = (LANES > 0 || group < groups) && tl < sp.tokens;
     int top = 16;                                              // half the power of two that holds the lanes
-    while (top >= l.lanes && top > 0) top >>= 1;
+    while (top >= lanes) top >>= 1;
     pdl_wait();
     pdl_release();
 
     // where the runs of this lane's units begin, and whether they exist
-    int at_a[UNITS], at_b[UNITS], turn_at[UNITS];
-    bool has_a[UNITS], has_b[UNITS], turned[UNITS];
+    int at_a[UNITS], at_b[UNITS];
+    bool has_a[UNITS], has_b[UNITS];
+    // (neighbouring lanes' runs follow one another: with both runs of a unit side by side, every access would take half of each sector, and
+    // 16384 x 40 x 128 interleaved took 84 us in the place of 64)
     const int rot_units = TWO ? half_dim / V : 0;
+    const int rest_units = TWO ? (p.head_dim - p.rotary_dim + 2 * V - 1) / (2 * V) : 0;
 #pragma unroll
     for (int j = 0; j < UNITS; ++j) {
-        const int u = ul + j * l.lanes;
-        turned[j] = u < rot_units;
-        turn_at[j] = u * V;
-        if (TWO && turned[j]) {
+        const int u = ul + j * lanes;
+        if (!TWO) {
+            at_a[j] = (ul + 2 * j * lanes) * V;
+            at_b[j] = at_a[j] + lanes * V;
+        } else if (u < rot_units) {
             at_a[j] = p.half ? u * V : 2 * u * V;
             at_b[j] = at_a[j] + (p.half ? half_dim : 1);
-        } else {
-            at_a[j] = 2 * u * V;
-            if (TWO) at_a[j] = p.rotary_dim + 2 * (u - rot_units) * V;
-            at_b[j] = at_a[j] + V;
+        } else {                                               // a unit of channels that are not rotated
+            at_a[j] = u - rot_units < rest_units ? p.rotary_dim + (u - rot_units) * V : p.head_dim;
+            at_b[j] = at_a[j] + rest_units * V;
         }
-        has_a[j] = has_slot && at_a[j] < p.head_dim;
-        has_b[j] = has_slot && at_b[j] < p.head_dim;
+        has_a[j] = LANES > 0 || (has_slot && at_a[j] < p.head_dim);
+        has_b[j] = LANES > 0 || (has_slot && at_b[j] < p.head_dim);
     }
-    float acc[BACK ? 2 : 1][BACK ? kHeadChannels : 1];
-    if constexpr (BACK) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < kHeadChannels; ++j) acc[i][j] = 0.f;
-    }
+    const unsigned blocks = (p.tokens + sp.tokens - 1) / sp.tokens;
+    const int rounds = (t.heads + sp.head_lanes - 1) / sp.head_lanes;          // the same for all threads
 
-    const int64_t blocks = (p.tokens + l.tokens - 1) / l.tokens;
-    for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
-        const int64_t token = block * l.tokens + tl;
+    // ---- the ring
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16;
+    // a run's unit j of a stage: bytes j V sizeof(T) of it, in pieces of 16
+    auto place = [](int stage, int run, int j) {
+        const int at = j * V * (int)sizeof(T);
+        return stage * Ring::stage_bytes + (run * Ring::pieces + at / 16) * kHeadThreads * 16 + at % 16;
+    };
+    auto bring = [&](int stage, int run, const T* from, const int (&at)[UNITS], const bool (&has)[UNITS], bool ok) {
+#pragma unroll
+        for (int j = 0; j < UNITS; ++j) {
+            const bool there = ok && has[j];
+            const T* src = from + at[j];                       // (not read unless it is there)
+            if constexpr (V * sizeof(T) >= 4) {
+                head_copy<V * (int)sizeof(T)>(ring + place(stage, run, j), src, there);
+            } else {
+                *reinterpret_cast<Raw*>(smem + threadIdx.x * 16 + place(stage, run, j)) = there ? *reinterpret_cast<const Raw*>(src) : Raw{};
+            }
+        }
+    };
+    unsigned f_block = cta;
+    int f_round = 0, f_stage = 0;
+    const T *fx = static_cast<const T*>(t.x), *fg = static_cast<const T*>(t.g);
+    bool f_here = false;
+    auto fetch_token = [&]() {                                 // f_block's token
+        const unsigned token = f_block * sp.tokens + tl;
+        f_here = has_slot && f_block < blocks && token < p.tokens;
+        const unsigned batch = f_here ? token / p.seq : 0, s = f_here ? token - batch * p.seq : 0;
+        fx = static_cast<const T*>(t.x) + batch * t.x_batch + s * t.x_token + h0 * t.x_head;
+        if constexpr (BACK) fg = static_cast<const T*>(t.g) + batch * t.g_batch + s * t.g_token + h0 * t.g_head;
+    };
+    auto fetch = [&]() {
+        const bool ok = f_here && (LANES > 0 || h0 + f_round * sp.head_lanes < t.heads);
+        bring(f_stage, 0, fx, at_a, has_a, ok);
+        bring(f_stage, 1, fx, at_b, has_b, ok);
+        if constexpr (BACK) {
+            bring(f_stage, 2, fg, at_a, has_a, ok);
+            bring(f_stage, 3, fg, at_b, has_b, ok);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        fx += sp.head_lanes * t.x_head;
+        if constexpr (BACK) fg += sp.head_lanes * t.g_head;
+        f_stage = f_stage + 1 == Ring::stages ? 0 : f_stage + 1;
+        if (++f_round == rounds) {
+            f_round = 0;
+            f_block += sp.ctas;
+            fetch_token();
+        }
+    };
+    fetch_token();
+#pragma unroll
+    for (int i = 0; i + 1 < Ring::stages; ++i) fetch();
+
+    float2 w[2][4], acc[2][BACK ? 4 : 1];
+#pragma unroll
+    for (int j = 0; j < UNITS; ++j) {
+        if constexpr (LANES > 0) {
+#pragma unroll
+            for (int k = 0; k < V; k += 4) {
+                const float4 one = make_float4(1.f, 1.f, 1.f, 1.f);
+                const float4 wa = t.w == nullptr ? one : *reinterpret_cast<const float4*>(t.w + at_a[j] + k);
+                const float4 wb = t.w == nullptr ? one : *reinterpret_cast<const float4*>(t.w + at_b[j] + k);
+                const int i = (j * V + k) / 2;
+                w[0][i] = make_float2(wa.x, wa.y); w[0][i + 1] = make_float2(wa.z, wa.w);
+                w[1][i] = make_float2(wb.x, wb.y); w[1][i + 1] = make_float2(wb.z, wb.w);
+            }
+            continue;
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int i = j * V + k;
+            (i % 2 ? w[0][i / 2].y : w[0][i / 2].x) = t.w == nullptr || !has_a[j] ? 1.f : t.w[at_a[j] + k];
+            (i % 2 ? w[1][i / 2].y : w[1][i / 2].x) = t.w == nullptr || !has_b[j] ? 1.f : t.w[at_b[j] + k];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < (BACK ? 4 : 1); ++i) acc[0][i] = acc[1][i] = make_float2(0.f, 0.f);
+    const float inv_dim = 1.0f / (float)p.head_dim;
+
+    int stage = 0;
+    for (unsigned block = cta; block < blocks; block += sp.ctas) {
+        const unsigned token = block * sp.tokens + tl;
         const bool here = has_slot && token < p.tokens;
-        const int64_t batch = token / p.seq, s = token - batch * p.seq;
+        const unsigned batch = here ? token / p.seq : 0, s = here ? token - batch * p.seq : 0;
+        T* out = static_cast<T*>(t.out) + batch * t.out_batch + s * t.out_token + h0 * t.out_head;
         if (half_dim > 0) {
-            if (block != (int64_t)blockIdx.x) __syncthreads(); // the angles before have been read
-            for (int i = threadIdx.x; i < l.tokens * half_dim; i += kHeadThreads) {
+            if (block != cta) __syncthreads();                 // the angles before have been read
+            for (int i = threadIdx.x; i < sp.tokens * half_dim; i += kHeadThreads) {
                 const int k = i / half_dim, pair = i - k * half_dim;
-                const int64_t tok = block * l.tokens + k;
+                const unsigned tok = block * sp.tokens + k;
                 if (tok < p.tokens) {
-                    const int64_t b = tok / p.seq, at = tok - b * p.seq;
+                    const unsigned b = tok / p.seq, at = tok - b * p.seq;
                     const RotaryAngles& a = p.angles;
                     const int64_t from = b * a.pos_batch + at * a.pos_token;
                     const double pos = a.positions == nullptr ? (double)at : a.axes != nullptr ? rotary_position<true>(a, from, pair)
@@ -132,210 +273,217 @@ head_norm_kernel(const __grid_constant__ HeadNormParams p, const HeadLanes l) {
             }
             __syncthreads();
         }
-        // the lane's cosines and sines: (1, 0) for channels that are not rotated
-        float2 turn[UNITS][V];
+        // What the rotation multiplies a channel and its partner with: a' = a c - b s, b' = b c + a s.  Forward with the weights in it.
+        // (1, 0) for channels that are not rotated.
+        float2 own[2][4], other[2][4];
 #pragma unroll
         for (int j = 0; j < UNITS; ++j) {
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                bool rot = turned[j];
-                int i = turn_at[j] + k;
-                if constexpr (!TWO) {                          // pairs k < V / 2 in run a, the others in run b
-                    i = (k < V / 2 ? at_a[j] : at_b[j] - V) / 2 + k;
-                    rot = i < half_dim;
+                const int i = j * V + k;
+                auto at = [](float2 (&v)[4], int n) -> float& { return n % 2 ? v[n / 2].y : v[n / 2].x; };
+                if constexpr (TWO) {                           // pair i: a[i] with b[i]
+                    const int u = ul + j * lanes;
+                    const float2 c = here && u < rot_units ? turns[tl * half_dim + u * V + k] : make_float2(1.f, 0.f);
+                    at(own[0], i) = at(own[1], i) = c.x;
+                    at(other[0], i) = -c.y;
+                    at(other[1], i) = c.y;
+                } else if (k % 2 == 0) {                       // channel i with i + 1, in both runs
+#pragma unroll
+                    for (int run = 0; run < 2; ++run) {
+                        const int pair = ((run ? at_b[j] : at_a[j]) + k) / 2;
+                        const float2 c = here && pair < half_dim ? turns[tl * half_dim + pair] : make_float2(1.f, 0.f);
+                        own[run][i / 2] = make_float2(c.x, c.x);
+                        other[run][i / 2] = make_float2(-c.y, c.y);
+                    }
                 }
-                turn[j][k] = here && rot ? turns[tl * half_dim + i] : make_float2(1.f, 0.f);
             }
         }
+        if constexpr (!BACK) {
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            const HeadTensor& t = p.t[which];
-            if (t.heads == 0) continue;
-            float w[UNITS][2][V];
+            for (int run = 0; run < 2; ++run)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    own[run][i] = fmul2(own[run][i], w[run][i]);
+                    other[run][i] = fmul2(other[run][i], TWO ? w[1 - run][i] : make_float2(w[run][i].y, w[run][i].x));
+                }
+        }
+        auto rotate = [&](float2 (&y)[2][4]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 a = y[0][i], b = y[1][i];
+                y[0][i] = ffma2(a, own[0][i], fmul2(TWO ? b : make_float2(a.y, a.x), other[0][i]));
+                y[1][i] = ffma2(b, own[1][i], fmul2(TWO ? a : make_float2(b.y, b.x), other[1][i]));
+            }
+        };
+        auto read = [&](int run, float2 (&v)[4]) {
+            alignas(16) T e[8];
+#pragma unroll
+            for (int k = 0; k < Ring::pieces; ++k)
+                reinterpret_cast<uint4*>(e)[k] =
+                    *reinterpret_cast<const uint4*>(smem + threadIdx.x * 16 + stage * Ring::stage_bytes + (run * Ring::pieces + k) * kHeadThreads * 16);
+            head_widen<T>(e, v);
+        };
+        for (int r = 0; r < rounds; ++r) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(Ring::stages - 2) : "memory");
+            float2 v[2][4], d[2][BACK ? 4 : 1], tx[2][BACK ? 4 : 1];
+            float sums[BACK ? 2 : 1];                          // of x^2, of u x
+            read(0, v[0]);
+            read(1, v[1]);
+            float2 sq = fmul2(v[0][0], v[0][0]);
+#pragma unroll
+            for (int i = 1; i < 4; ++i) sq = ffma2(v[0][i], v[0][i], sq);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sq = ffma2(v[1][i], v[1][i], sq);
+            sums[0] = sq.x + sq.y;
+            if constexpr (BACK) {
+                read(2, d[0]);
+                read(3, d[1]);
+                rotate(d);                                     // (the sine is negated)
+                float2 dot = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int run = 0; run < 2; ++run)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        tx[run][i] = fmul2(d[run][i], v[run][i]);
+                        dot = ffma2(tx[run][i], w[run][i], dot);
+                    }
+                sums[1] = dot.x + dot.y;
+            }
+            stage = stage + 1 == Ring::stages ? 0 : stage + 1;
+            fetch();                                           // into the slot that the round before has read
+            head_sum<LANES>(sums, lane, lanes, top);
+            const float rstd = rsqrtf(fmaf(sums[0], inv_dim, p.eps));
+            const float2 r2 = make_float2(rstd, rstd);
+            if constexpr (BACK) {
+                const float c = -rstd * (rstd * rstd * (sums[1] * inv_dim));
+                const float2 c2 = make_float2(c, c);
+#pragma unroll
+                for (int run = 0; run < 2; ++run)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {              // (lanes and heads that are not there add zeros)
+                        acc[run][i] = ffma2(tx[run][i], r2, acc[run][i]);
+                        v[run][i] = ffma2(d[run][i], fmul2(w[run][i], r2), fmul2(v[run][i], c2));
+                    }
+            } else {
+#pragma unroll
+                for (int run = 0; run < 2; ++run)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[run][i] = fmul2(v[run][i], r2);
+                rotate(v);
+            }
+            const bool ok = here && (LANES > 0 || h0 + r * sp.head_lanes < t.heads);
+            alignas(16) T a[8], b[8];
+            head_narrow<T>(v[0], a);
+            head_narrow<T>(v[1], b);
 #pragma unroll
             for (int j = 0; j < UNITS; ++j) {
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    w[j][0][k] = t.w == nullptr || !has_a[j] ? 1.f : t.w[at_a[j] + k];
-                    w[j][1][k] = t.w == nullptr || !has_b[j] ? 1.f : t.w[at_b[j] + k];
-                }
+                if (ok && has_a[j]) *reinterpret_cast<Raw*>(out + at_a[j]) = *reinterpret_cast<const Raw*>(a + j * V);
+                if (ok && has_b[j]) *reinterpret_cast<Raw*>(out + at_b[j]) = *reinterpret_cast<const Raw*>(b + j * V);
             }
-            const T* x = static_cast<const T*>(t.x) + batch * t.x_batch + s * t.x_token;
-            const T* g = static_cast<const T*>(t.g) + batch * t.g_batch + s * t.g_token;
-            T* out = static_cast<T*>(t.out) + batch * t.out_batch + s * t.out_token;
-            const int rounds = (t.heads + l.head_lanes - 1) / l.head_lanes;
-            constexpr int AHEAD = 2;                           // heads on their way together
-            for (int r0 = 0; r0 < rounds; r0 += AHEAD) {       // (the same for all lanes of a warp)
-                Head in[AHEAD], gr[BACK ? AHEAD : 1];
-                bool ok[AHEAD];
-#pragma unroll
-                for (int q = 0; q < AHEAD; ++q) {
-                    const int h = h0 + (r0 + q) * l.head_lanes;
-                    ok[q] = here && h < t.heads;
-#pragma unroll
-                    for (int j = 0; j < UNITS; ++j) {
-                        in[q].a[j].r = in[q].b[j].r = Raw{};
-                        if (ok[q] && has_a[j]) in[q].a[j].r = *reinterpret_cast<const Raw*>(x + h * t.x_head + at_a[j]);
-                        if (ok[q] && has_b[j]) in[q].b[j].r = *reinterpret_cast<const Raw*>(x + h * t.x_head + at_b[j]);
-                        if constexpr (BACK) {
-                            gr[q].a[j].r = gr[q].b[j].r = Raw{};
-                            if (ok[q] && has_a[j]) gr[q].a[j].r = *reinterpret_cast<const Raw*>(g + h * t.g_head + at_a[j]);
-                            if (ok[q] && has_b[j]) gr[q].b[j].r = *reinterpret_cast<const Raw*>(g + h * t.g_head + at_b[j]);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int q = 0; q < AHEAD; ++q) {
-                    if (r0 + q >= rounds) break;
-                    const int h = h0 + (r0 + q) * l.head_lanes;
-                    float v[UNITS][2][V], d[BACK ? UNITS : 1][2][V];
-                    float sum = 0.f, dot = 0.f;
-#pragma unroll
-                    for (int j = 0; j < UNITS; ++j) {
-#pragma unroll
-                        for (int k = 0; k < V; ++k) {
-                            v[j][0][k] = to_float<T>(in[q].a[j].e[k]);
-                            v[j][1][k] = to_float<T>(in[q].b[j].e[k]);
-                            sum = fmaf(v[j][0][k], v[j][0][k], sum);
-                            sum = fmaf(v[j][1][k], v[j][1][k], sum);
-                        }
-                    }
-                    // the rotation of a unit's pairs in place
-                    auto rotate = [&](float (&y)[2][V], const float2 (&c)[V]) {
-#pragma unroll
-                        for (int k = 0; k < V; ++k) {
-                            float& a = TWO ? y[0][k] : y[2 * k / V][2 * k % V];
-                            float& b = TWO ? y[1][k] : y[2 * k / V][2 * k % V + (V > 1 ? 1 : 0)];
-                            const float a0 = a, b0 = b;
-                            a = a0 * c[k].x - b0 * c[k].y;
-                            b = b0 * c[k].x + a0 * c[k].y;
-                        }
-                    };
-                    if constexpr (BACK) {
-#pragma unroll
-                        for (int j = 0; j < UNITS; ++j) {
-#pragma unroll
-                            for (int k = 0; k < V; ++k) {
-                                d[j][0][k] = to_float<T>(gr[q].a[j].e[k]);
-                                d[j][1][k] = to_float<T>(gr[q].b[j].e[k]);
-                            }
-                            rotate(d[j], turn[j]);             // (the sine is negated)
-#pragma unroll
-                            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                                for (int k = 0; k < V; ++k) dot = fmaf(d[j][i][k] * w[j][i][k], v[j][i][k], dot);
-                        }
-                    }
-                    sum = head_sum(sum, lane, l.lanes, top, pow2);
-                    if constexpr (BACK) dot = head_sum(dot, lane, l.lanes, top, pow2);
-                    const float rstd = rsqrtf(sum / (float)p.head_dim + p.eps);
-                    const float c = BACK ? rstd * rstd * dot / (float)p.head_dim : 0.f;
-#pragma unroll
-                    for (int j = 0; j < UNITS; ++j) {
-                        if constexpr (BACK) {
-#pragma unroll
-                            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                                for (int k = 0; k < V; ++k) {
-                                    if (ok[q]) acc[which][(j * 2 + i) * V + k] = fmaf(d[j][i][k], v[j][i][k] * rstd, acc[which][(j * 2 + i) * V + k]);
-                                    v[j][i][k] = rstd * (d[j][i][k] * w[j][i][k] - v[j][i][k] * c);
-                                }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                                for (int k = 0; k < V; ++k) v[j][i][k] = v[j][i][k] * rstd * w[j][i][k];
-                            rotate(v[j], turn[j]);
-                        }
-#pragma unroll
-                        for (int k = 0; k < V; ++k) {
-                            in[q].a[j].e[k] = from_float<T>(v[j][0][k]);
-                            in[q].b[j].e[k] = from_float<T>(v[j][1][k]);
-                        }
-                        if (ok[q] && has_a[j]) *reinterpret_cast<Raw*>(out + h * t.out_head + at_a[j]) = in[q].a[j].r;
-                        if (ok[q] && has_b[j]) *reinterpret_cast<Raw*>(out + h * t.out_head + at_b[j]) = in[q].b[j].r;
-                    }
-                }
-            }
+            out += sp.head_lanes * t.out_head;
         }
+        if constexpr (!BACK) break;                            // (one block a CTA)
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if constexpr (BACK) {
         if (p.part == nullptr) return;
-        // over the CTA's groups in order, queries then keys
-        const int slots = kHeadThreads / 32 * l.groups;
-        for (int which = 0; which < 2; ++which) {
-            __syncthreads();
-            if (group < l.groups) {
+        // over the CTA's groups in order
+        float* sum = reinterpret_cast<float*>(smem);
+        __syncthreads();
+        if (group < groups) {
 #pragma unroll
-                for (int j = 0; j < UNITS; ++j)
+            for (int j = 0; j < UNITS; ++j)
 #pragma unroll
-                    for (int k = 0; k < V; ++k) {
-                        if (has_a[j]) smem[slot * p.head_dim + at_a[j] + k] = which == 0 ? acc[0][(j * 2) * V + k] : acc[1][(j * 2) * V + k];
-                        if (has_b[j]) smem[slot * p.head_dim + at_b[j] + k] = which == 0 ? acc[0][(j * 2 + 1) * V + k] : acc[1][(j * 2 + 1) * V + k];
-                    }
-            }
-            __syncthreads();
-            for (int c = threadIdx.x; c < p.head_dim; c += kHeadThreads) {
-                float a = 0.f;
-                for (int k = 0; k < slots && k < l.tokens * l.head_lanes; ++k) a += smem[k * p.head_dim + c];
-                p.part[((int64_t)blockIdx.x * 2 + which) * p.head_dim + c] = a;
-            }
+                for (int k = 0; k < V; ++k) {
+                    const int i = j * V + k;
+                    if (has_a[j]) sum[slot * p.head_dim + at_a[j] + k] = i % 2 ? acc[0][i / 2].y : acc[0][i / 2].x;
+                    if (has_b[j]) sum[slot * p.head_dim + at_b[j] + k] = i % 2 ? acc[1][i / 2].y : acc[1][i / 2].x;
+                }
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < p.head_dim; c += kHeadThreads) {
+            float a = 0.f;
+            for (int k = 0; k < sp.tokens * sp.head_lanes; ++k) a += sum[k * p.head_dim + c];
+            p.part[(int64_t)blockIdx.x * p.head_dim + c] = a;
         }
     }
 }
 
-// dw of queries and keys from the CTAs' sums, 32 columns a CTA, in a fixed order
-constexpr int kHeadSumWarps = 8;
+// dw from the CTAs' sums, 32 columns a CTA, in a fixed order; blockIdx.y: queries, keys
+constexpr int kHeadSumWarps = 16;
 __global__ void __launch_bounds__(32 * kHeadSumWarps)
-head_norm_sum_kernel(const float* __restrict__ part, int parts, float* __restrict__ dq, float* __restrict__ dk, int dim) {
+head_norm_sum_kernel(const float* __restrict__ part, int q_parts, int k_parts, float* __restrict__ dq, float* __restrict__ dk, int dim) {
     __shared__ float red[kHeadSumWarps][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + lane;                      // of 2 dim
+    const int c = blockIdx.x * 32 + lane;
+    float* out = blockIdx.y == 0 ? dq : dk;
     pdl_wait();
     pdl_release();
+    if (out == nullptr) return;
+    const int first = blockIdx.y == 0 ? 0 : q_parts, last = blockIdx.y == 0 ? q_parts : q_parts + k_parts;
     float a = 0.f;
-    if (c < 2 * dim)
-        for (int k = warp; k < parts; k += kHeadSumWarps) a += part[(int64_t)k * 2 * dim + c];
+    if (c < dim) {
+#pragma unroll 8
+        for (int k = first + warp; k < last; k += kHeadSumWarps) a += part[(int64_t)k * dim + c];
+    }
     red[warp][lane] = a;
     __syncthreads();
-    if (warp == 0 && c < 2 * dim) {
+    if (warp == 0 && c < dim) {
 #pragma unroll
         for (int k = 1; k < kHeadSumWarps; ++k) a += red[k][lane];
-        float* out = c < dim ? dq : dk;
-        if (out != nullptr) out[c < dim ? c : c - dim] = a;
+        out[c] = a;
     }
 }
 
 template <typename T, int V, bool TWO, bool BACK>
 static int launch_head_norm_as(const HeadNormParams& p, float* dqw, float* dkw, cudaStream_t st) {
-    constexpr int UNITS = kHeadChannels / (2 * V);
+    constexpr int UNITS = 8 / V;
     // units of a head: those that are rotated, and the rest (TWO); else pairs of runs
     const int units = TWO ? p.rotary_dim / 2 / V + (p.head_dim - p.rotary_dim + 2 * V - 1) / (2 * V) : (p.head_dim + 2 * V - 1) / (2 * V);
     HeadLanes l;
     l.lanes = (units + UNITS - 1) / UNITS;
     l.groups = 32 / l.lanes;
     const int slots = kHeadThreads / 32 * l.groups;
-    const int heads = p.t[0].heads > p.t[1].heads ? p.t[0].heads : p.t[1].heads;
-    int per_thread = kHeadRows;
-    auto lanes = [&](int n) { const int want = (heads + n - 1) / n; return want < slots ? want : slots; };
-    while (per_thread > 1 && (p.tokens + slots / lanes(per_thread) - 1) / (slots / lanes(per_thread)) < gemm_num_sms()) --per_thread;
-    l.head_lanes = lanes(per_thread);
-    l.tokens = slots / l.head_lanes;
-    const int room = p.rotary_dim > 0 ? 24 * 1024 / (4 * p.rotary_dim) : l.tokens;
-    if (l.tokens > room) l.tokens = room;
-    const int64_t blocks = (p.tokens + l.tokens - 1) / l.tokens;
-    int64_t grid = blocks;
-    size_t smem = (size_t)l.tokens * p.rotary_dim * 4;
-    if (BACK && p.part != nullptr) {
-        const int64_t most = 4 * gemm_num_sms() < kHeadMaxCtas ? 4 * gemm_num_sms() : kHeadMaxCtas;
-        if (grid > most) grid = most;
-        const size_t sums = (size_t)slots * p.head_dim * 4;
-        if (smem < sums) smem = sums;
+    const int room = p.rotary_dim > 0 ? 24 * 1024 / (4 * p.rotary_dim) : slots;
+    const bool sums = BACK && p.part != nullptr;
+    const int all = p.t[0].heads + p.t[1].heads;
+    const int most = 4 * gemm_num_sms() < kHeadMaxCtas ? 4 * gemm_num_sms() : kHeadMaxCtas;
+    size_t smem = 0;                                           // angles; the sums take the ring's place (at most 8 KB)
+    for (int i = 0; i < 2; ++i) {
+        const int heads = p.t[i].heads;
+        HeadSplit& sp = l.of[i];
+        sp = {1, 1, 0};
+        if (heads == 0) continue;
+        int per_thread = kHeadRows;
+        auto lanes = [&](int n) { const int want = (heads + n - 1) / n; return want < slots ? want : slots; };
+        while (per_thread > 1 && (p.tokens + slots / lanes(per_thread) - 1) / (slots / lanes(per_thread)) < (unsigned)gemm_num_sms()) --per_thread;
+        sp.head_lanes = lanes(per_thread);
+        sp.tokens = slots / sp.head_lanes;
+        if (sp.tokens > room) sp.tokens = room;
+        const unsigned blocks = (p.tokens + sp.tokens - 1) / sp.tokens;
+        const unsigned share = (unsigned)((int64_t)most * heads / all);        // of the CTAs that the sums allow
+        sp.ctas = (int)(sums && blocks > share ? (share > 0 ? share : 1) : blocks);
+        const size_t angles = (size_t)sp.tokens * p.rotary_dim * 4;
+        if (smem < angles) smem = angles;
     }
-    Q8K_CUDA_OK(launch_dependent(head_norm_kernel<T, V, TWO, BACK>, (unsigned)grid, kHeadThreads, smem, st, 1, p, l));
-    if (BACK && p.part != nullptr)
-        Q8K_CUDA_OK(launch_dependent(head_norm_sum_kernel, (unsigned)((2 * p.head_dim + 31) / 32), 32 * kHeadSumWarps, 0, st, 1, p.part, (int)grid, dqw, dkw,
-                                     p.head_dim));
+    const unsigned grid = (unsigned)(l.of[0].ctas + l.of[1].ctas);
+    auto kern = head_norm_kernel<T, V, TWO, BACK, 0>;
+    int form = 0;
+    if constexpr (V * sizeof(T) == 16) {                       // the common heads of 64, 128 and 256 channels
+        bool whole = p.head_dim == kHeadChannels * l.lanes;
+        for (int i = 0; i < 2; ++i)
+            whole = whole && (p.t[i].heads == 0 || (p.t[i].heads % l.of[i].head_lanes == 0 && aligned16(p.t[i].w)));
+        if (whole && l.lanes == 4) { kern = head_norm_kernel<T, V, TWO, BACK, 4>; form = 1; }
+        if (whole && l.lanes == 8) { kern = head_norm_kernel<T, V, TWO, BACK, 8>; form = 2; }
+        if (whole && l.lanes == 16) { kern = head_norm_kernel<T, V, TWO, BACK, 16>; form = 3; }
+    }
+    static std::atomic<uint64_t> smem_done[4] = {};
+    if (int rc = allow_dynamic_smem((const void*)kern, HeadRing<T, BACK>::bytes + 24 * 1024, smem_done[form])) return rc;
+    Q8K_CUDA_OK(launch_dependent(kern, grid, kHeadThreads, HeadRing<T, BACK>::bytes + smem, st, 1, p, l));
+    if (sums)
+        Q8K_CUDA_OK(launch_dependent(head_norm_sum_kernel, dim3((unsigned)((p.head_dim + 31) / 32), 2), 32 * kHeadSumWarps, 0, st, 1, p.part, l.of[0].ctas,
+                                     l.of[1].ctas, dqw, dkw, p.head_dim));
     return Q8K_OK;
 }
 
@@ -409,8 +557,8 @@ static int head_norm(const char* op, const HeadArgs (&in)[2], int dtype, float e
     p.angles = angles;
     p.angles.sign = BACK ? -1.f : 1.f;
     p.eps = eps;
-    p.tokens = (int64_t)batch * seq;
-    p.seq = seq; p.head_dim = head_dim; p.rotary_dim = rotary_dim; p.half = half_layout != 0;
+    p.tokens = (unsigned)batch * (unsigned)seq;
+    p.seq = (unsigned)seq; p.head_dim = head_dim; p.rotary_dim = rotary_dim; p.half = half_layout != 0;
     float *dqw = in[0].dw, *dkw = in[1].dw;
     if (dtype == Q8K_DT_BF16) return launch_head_norm<__nv_bfloat16, BACK>(p, v, dqw, dkw, st);
     if (dtype == Q8K_DT_F16) return launch_head_norm<__half, BACK>(p, v, dqw, dkw, st);
@@ -443,7 +591,7 @@ extern "C" int q8k_head_norm(const void* q, const int64_t q_strides[3], const fl
 }
 
 extern "C" size_t q8k_head_norm_backward_workspace_bytes(int head_dim) {
-    return head_dim <= 0 ? 0 : (size_t)q8k::kHeadMaxCtas * 2 * (size_t)head_dim * sizeof(float);
+    return head_dim <= 0 ? 0 : ((size_t)q8k::kHeadMaxCtas + 2) * (size_t)head_dim * sizeof(float);
 }
 
 extern "C" int q8k_head_norm_backward(const void* q, const int64_t q_strides[3], const float* q_weight, const void* q_grad,
