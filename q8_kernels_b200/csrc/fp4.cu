@@ -289,56 +289,86 @@ template <typename Tout> static int launch_fp4_dequant(bool nv, const void* q, c
 
 // ------------------------------------------------------------------ weight operand of the backward product
 // w [N, K] de-quantised (value * block scale, exact, times the row's scale, rounded to fp32), transposed and quantised to e4m3 with one scale
-// per input channel, factor 448 / absmax as the 8-bit linears have it.  Two passes over the weight, which is small: partial absmax of row
-// chunks, the factors, then tiles of 128 x 128 that are turned in shared memory.
+// per input channel, factor 448 / absmax as the 8-bit linears have it.  Two passes over the weight, which is small: the absmax of the
+// columns over chunks of rows; then tiles of 128 x 128, whose CTAs take the maxima over the chunks, are turned in shared memory.
 constexpr int kF4Cols = 128;                 // columns of a CTA: 8 groups of 16
 constexpr int kF4Rows = 128;                 // rows of a turned tile
-constexpr int kF4ChunkRows = 256;            // rows of a partial absmax
+constexpr int kF4MaxParts = 32;
 constexpr int kF4Threads = 256;
 
-// 16 consecutive values of a row as fp32
+// 16 consecutive values of a row, before their scales
+struct Fp4Raw { uint2 q; uint8_t s; float r; };
 template <bool NV>
-__device__ __forceinline__ void fp4_load16(const uint8_t* __restrict__ w, const uint8_t* __restrict__ bs, const float* __restrict__ rs, int row, int c,
-                                           int K, int slabs, float (&v)[16]) {
-    const uint2 x = *reinterpret_cast<const uint2*>(w + (int64_t)row * (K / 2) + c / 2);
-    const float s = fp4_scale_value<NV>(bs[fp4_scale_at<NV>(row, c / (NV ? 16 : 32), slabs)]);
-    const float r = NV ? rs[row] : 1.f;
-    float lo[8], hi[8];
-    e2m1_to_float8(x.x, lo);
-    e2m1_to_float8(x.y, hi);
+__device__ __forceinline__ Fp4Raw fp4_load16(const uint8_t* __restrict__ w, const uint8_t* __restrict__ bs, const float* __restrict__ rs, int row, int c,
+                                             int K, int slabs) {
+    return {*reinterpret_cast<const uint2*>(w + (int64_t)row * (K / 2) + c / 2), bs[fp4_scale_at<NV>(row, c / (NV ? 16 : 32), slabs)],
+            NV ? rs[row] : 1.f};
+}
+// and as pairs with them.  A product of an e2m1 and an e4m3 value has six bits and at least 2^-10: fp16 holds it.
+template <bool NV> __device__ __forceinline__ void fp4_values16(const Fp4Raw& x, float2 (&v)[8]) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        v[j] = __fmul_rn(__fmul_rn(lo[j], s), r);
-        v[8 + j] = __fmul_rn(__fmul_rn(hi[j], s), r);
+    for (int h = 0; h < 2; ++h) {
+        uint32_t p[4];
+        asm("{\n\t"
+            ".reg .b8 a, b, c, d;\n\t"
+            "mov.b32 {a, b, c, d}, %4;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %3, d;\n\t"
+            "}"
+            : "=r"(p[0]), "=r"(p[1]), "=r"(p[2]), "=r"(p[3])
+            : "r"(h == 0 ? x.q.x : x.q.y));
+        __half2 s2;
+        if constexpr (NV) {
+            const __half s = __half(__nv_cvt_fp8_to_halfraw(x.s, __NV_E4M3));
+            s2 = __half2(s, s);
+        }
+        const float scale = NV ? x.r : fp4_scale_value<false>(x.s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            __half2 q = *reinterpret_cast<const __half2*>(&p[i]);
+            if constexpr (NV) q = __hmul2(q, s2);
+            v[4 * h + i] = fmul2(__half22float2(q), make_float2(scale, scale));
+        }
     }
 }
 
+// Bound by the latency of its loads: a thread has eight rows of 16 columns on their way at a time.
+constexpr int kF4Ahead = 8;
 template <bool NV>
-__global__ void __launch_bounds__(kF4Threads)
+__global__ void __launch_bounds__(kF4Threads, 4)
 fp4_weight_absmax_kernel(const uint8_t* __restrict__ w, const uint8_t* __restrict__ bs, const float* __restrict__ rs, float* __restrict__ part, int N,
-                         int K, int slabs) {
+                         int K, int slabs, int rows) {
     __shared__ float red[kF4Threads / 32][kF4Cols];
     pdl_wait();
     pdl_release();
-    const int cg = threadIdx.x & 7, rl = threadIdx.x >> 3;
+    const int cg = threadIdx.x & 7, rl = threadIdx.x >> 3;     // column group, row of a step of 32
     const int c0 = blockIdx.x * kF4Cols + cg * 16;
+    const int r_end = min((int)(blockIdx.y + 1) * rows, N);
     float m[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) m[j] = 0.f;
     if (c0 < K) {
-#pragma unroll 4
-        for (int i = 0; i < kF4ChunkRows / 32; ++i) {
-            const int row = blockIdx.y * kF4ChunkRows + i * 32 + rl;
-            if (row < N) {
-                float v[16];
-                fp4_load16<NV>(w, bs, rs, row, c0, K, slabs, v);
+        for (int r0 = blockIdx.y * rows + rl; r0 < r_end; r0 += 32 * kF4Ahead) {
+            Fp4Raw x[kF4Ahead];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) m[j] = fmaxf(m[j], fabsf(v[j]));
+            for (int i = 0; i < kF4Ahead; ++i)
+                x[i] = r0 + 32 * i < r_end ? fp4_load16<NV>(w, bs, rs, r0 + 32 * i, c0, K, slabs) : Fp4Raw{make_uint2(0, 0), 0, 0.f};
+#pragma unroll
+            for (int i = 0; i < kF4Ahead; ++i) {
+                float2 v[8];
+                fp4_values16<NV>(x[i], v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    m[2 * j] = fmaxf(m[2 * j], fabsf(v[j].x));
+                    m[2 * j + 1] = fmaxf(m[2 * j + 1], fabsf(v[j].y));
+                }
             }
         }
     }
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < 16; ++j) {                             // over the four rows of a warp
         m[j] = fmaxf(m[j], __shfl_xor_sync(0xffffffffu, m[j], 8));
         m[j] = fmaxf(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
         if ((threadIdx.x & 31) < 8) red[threadIdx.x >> 5][cg * 16 + j] = m[j];
@@ -353,45 +383,62 @@ fp4_weight_absmax_kernel(const uint8_t* __restrict__ w, const uint8_t* __restric
     }
 }
 
-// scales[c] = 1 / (448 / absmax of column c) as the row quantizer leaves it; the factors follow the partial maxima
-__global__ void __launch_bounds__(256)
-fp4_weight_factor_kernel(float* __restrict__ part, int parts, float* __restrict__ scales, int K) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    pdl_wait();
-    pdl_release();
-    if (c >= K) return;
-    float a = 0.f;
-    for (int k = 0; k < parts; ++k) a = fmaxf(a, part[(int64_t)k * K + c]);
-    const float f = __fdiv_rn(448.0f, a);
-    part[(int64_t)parts * K + c] = a == 0.f ? 0.f : f;
-    scales[c] = __fdiv_rn(1.0f, f);
-}
-
+// The kernel before this one on the stream read the weight and let it start only once it had waited for the weight's writer, so the weight
+// may be loaded before the wait.
 template <bool NV>
 __global__ void __launch_bounds__(kF4Threads)
-fp4_weight_turn_kernel(const uint8_t* __restrict__ w, const uint8_t* __restrict__ bs, const float* __restrict__ rs, const float* __restrict__ factors,
-                       uint8_t* __restrict__ q, int N, int K, int slabs) {
+fp4_weight_turn_kernel(const uint8_t* __restrict__ w, const uint8_t* __restrict__ bs, const float* __restrict__ rs, const float* __restrict__ part,
+                       int parts, uint8_t* __restrict__ q, float* __restrict__ scales, int N, int K, int slabs) {
+    __shared__ float top[2][kF4Cols];
     __shared__ __align__(16) float mul[kF4Cols];
     __shared__ __align__(16) uint32_t turned[kF4Cols][kF4Rows / 4];
     const int cb = blockIdx.x * kF4Cols, r0 = blockIdx.y * kF4Rows;
     const int cg = threadIdx.x & 7, rg = threadIdx.x >> 3;     // 16 columns, four rows
+    const int c0 = cb + cg * 16;
+    const bool in = c0 < K && r0 + rg * 4 < N;                 // N % 16 == 0: all four rows exist, or none
+    Fp4Raw x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = in ? fp4_load16<NV>(w, bs, rs, r0 + rg * 4 + i, c0, K, slabs) : Fp4Raw{make_uint2(0, 0), 0, 0.f};
     pdl_wait();
     pdl_release();
-    if (threadIdx.x < kF4Cols) mul[threadIdx.x] = cb + (int)threadIdx.x < K ? factors[cb + threadIdx.x] : 0.f;
+    {
+        const int c = threadIdx.x & (kF4Cols - 1), half = threadIdx.x / kF4Cols;
+        float a = 0.f;
+        if (cb + c < K) {
+#pragma unroll 8
+            for (int k = half; k < parts; k += 2) a = fmaxf(a, part[(int64_t)k * K + cb + c]);
+        }
+        top[half][c] = a;
+        __syncthreads();
+        if (half == 0) {
+            a = fmaxf(a, top[1][c]);
+            const float f = __fdiv_rn(448.0f, a);
+            // column group g's k-th four factors lie at (8 k + g) * 4: the eight groups of a warp read 128 bytes in a row
+            mul[(c & 15) / 4 * 32 + c / 16 * 4 + (c & 3)] = a == 0.f ? 0.f : f;      // a column of zeros quantises to zeros
+            if (blockIdx.y == 0 && cb + c < K) scales[cb + c] = __fdiv_rn(1.0f, f);
+        }
+    }
     __syncthreads();
-    const int c0 = cb + cg * 16;
-    if (c0 < K && r0 + rg * 4 < N) {                           // N % 16 == 0: all four rows exist, or none
-        float v[4][16];
+    if (in) {
+        float2 v[4][8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) fp4_load16<NV>(w, bs, rs, r0 + rg * 4 + i, c0, K, slabs, v[i]);
+        for (int i = 0; i < 4; ++i) fp4_values16<NV>(x[i], v[i]);
         // row group rg of a column goes to word rg + 4 * (column group): the words that a warp stores lie in 32 banks, and four of a
         // column stay together for the 16-byte reads below
         const int at = (rg + 4 * cg) & 31;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const float f = mul[cg * 16 + j];
-            turned[cg * 16 + j][at] = (uint32_t)float2_to_e4m3x2_sat(__fmul_rn(v[0][j], f), __fmul_rn(v[1][j], f)) |
-                                      ((uint32_t)float2_to_e4m3x2_sat(__fmul_rn(v[2][j], f), __fmul_rn(v[3][j], f)) << 16);
+        for (int k = 0; k < 4; ++k) {
+            const float4 f = *reinterpret_cast<const float4*>(mul + k * 32 + cg * 4);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float2 f2 = j == 0 ? make_float2(f.x, f.y) : make_float2(f.z, f.w);
+                float2 y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = fmul2(v[i][2 * k + j], f2);
+                const int c = cg * 16 + k * 4 + 2 * j;
+                turned[c][at] = (uint32_t)float2_to_e4m3x2_sat(y[0].x, y[1].x) | ((uint32_t)float2_to_e4m3x2_sat(y[2].x, y[3].x) << 16);
+                turned[c + 1][at] = (uint32_t)float2_to_e4m3x2_sat(y[0].y, y[1].y) | ((uint32_t)float2_to_e4m3x2_sat(y[2].y, y[3].y) << 16);
+            }
         }
     }
     __syncthreads();
@@ -407,12 +454,16 @@ fp4_weight_turn_kernel(const uint8_t* __restrict__ w, const uint8_t* __restrict_
 template <bool NV>
 static int launch_fp4_weight(const void* w, const void* bs, const float* rs, void* q, float* scales, float* part, int N, int K, cudaStream_t st) {
     const unsigned cols = (unsigned)((K + kF4Cols - 1) / kF4Cols);
-    const int parts = (N + kF4ChunkRows - 1) / kF4ChunkRows, slabs = fp4_slabs(K);
+    const int slabs = fp4_slabs(K);
+    // four CTAs an SM, all of one size: rows a CTA by that, in steps of 32
+    int parts = (int)((unsigned)(4 * gemm_num_sms()) / cols);
+    parts = parts < 1 ? 1 : parts > kF4MaxParts ? kF4MaxParts : parts;
+    const int rows = ((N + parts - 1) / parts + 31) / 32 * 32;
+    parts = (N + rows - 1) / rows;
     Q8K_CUDA_OK(launch_dependent(fp4_weight_absmax_kernel<NV>, dim3(cols, (unsigned)parts), kF4Threads, 0, st, 1, (const uint8_t*)w, (const uint8_t*)bs, rs,
-                                 part, N, K, slabs));
-    Q8K_CUDA_OK(launch_dependent(fp4_weight_factor_kernel, dim3((unsigned)((K + 255) / 256)), 256, 0, st, 1, part, parts, scales, K));
+                                 part, N, K, slabs, rows));
     Q8K_CUDA_OK(launch_dependent(fp4_weight_turn_kernel<NV>, dim3(cols, (unsigned)((N + kF4Rows - 1) / kF4Rows)), kF4Threads, 0, st, 1,
-                                 (const uint8_t*)w, (const uint8_t*)bs, rs, part + (int64_t)parts * K, (uint8_t*)q, N, K, slabs));
+                                 (const uint8_t*)w, (const uint8_t*)bs, rs, part, parts, (uint8_t*)q, scales, N, K, slabs));
     return Q8K_OK;
 }
 
@@ -470,8 +521,7 @@ extern "C" int q8k_fp4_dequant(const void* values, const void* block_scales, con
 }
 
 extern "C" size_t q8k_fp4_weight_operand_workspace_bytes(int N, int K) {
-    if (N <= 0 || K <= 0) return 0;
-    return ((size_t)(N + q8k::kF4ChunkRows - 1) / q8k::kF4ChunkRows + 1) * (size_t)K * sizeof(float);   // partial maxima, factors
+    return N <= 0 || K <= 0 ? 0 : (size_t)q8k::kF4MaxParts * (size_t)K * sizeof(float);         // partial maxima
 }
 
 extern "C" int q8k_fp4_weight_operand(int format, const void* values, const void* block_scales, const float* row_scales, void* q, float* scales, int N,
