@@ -9,6 +9,16 @@
 // TMEM has 512 columns, two accumulators and the scales of a slab need 512 + 48.  So the accumulators overlap by 64 columns:
 // [0, 256) and [192, 448), scales from 448 on.  The epilogue takes the 64 shared columns of a tile first and gives them back at once; all
 // that the next tile's MMAs wait for is those, because the rest of their accumulator was read before the epilogue came to this tile.
+//
+// What bounds it (clocks of one SM, 6144 x 2048 x 8192 nvfp4): the MMAs of a tile take 4130, 516 a slab of 256, the tile 5600.  Five stages of
+// 38 KB just cover the 2000 clocks from a freed stage to its next operands, at 54 bytes a clock and SM, of 64 that the SM can take from L2
+// and 74 that the MMAs alone would take; and from a tile's last MMA to the next one's first 700 to 900 pass.  With GELU the epilogue takes
+// 6600 of a tile's 7000.  Tried: 16 epilogue warps (a tile's epilogue 4000 and 5600, but it comes in one burst, and the loads suffer: 81.0 ->
+// 89.1 thousand clocks in all, with GELU 97.3 -> 96.7); fragments of 16 x 64 through stmatrix and plain stores (88.3, 95.3); A's rows kept in
+// shared memory for all tiles of a row block, which halves the loads and leaves three stages for B (95.0, 97.7); scales copied to TMEM one
+// K step ahead or to alternate columns (no change).
+// 6144 x 8192 x 2048 mxfp4 37.5 us, 5.5 PFLOP/s, 0.84 of four times the measured bf16 rate; 24576 x 2048 x 8192 157 us, nvfp4 171, with GELU
+// 205 under the power cap.
 
 #include "gemm_fp4.cuh"
 
@@ -30,9 +40,8 @@ struct Fp4PairSmem {
     static constexpr int kTmemPtrOffset = kBarOffset + kNumBars * 8;
     static constexpr int kAbortOffset = kTmemPtrOffset + 4;
     static constexpr int kPriorOffset = kAbortOffset + 4;
-    static constexpr int kColScaleOffset = (kPriorOffset + 4 + 15) & ~15;
-    static constexpr int kBiasOffset = kColScaleOffset + 256 * 4;
-    static constexpr int kTotal = kBiasOffset + 256 * 4;
+    static constexpr int kColumnOffset = (kPriorOffset + 4 + 15) & ~15;        // two tiles' column scales and biases, {s, s, b, b} of a pair
+    static constexpr int kTotal = kColumnOffset + 2 * 256 * 8;
     static_assert(kStageBytes % 1024 == 0 && kTotal <= 227 * 1024, "pair GEMM shared memory");
 };
 
@@ -63,8 +72,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     auto tmem_free_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + 2 + a); };      // the shared columns of accumulator a have been read
     volatile uint32_t* tmem_ptr_smem = reinterpret_cast<volatile uint32_t*>(smem + L::kTmemPtrOffset);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kAbortOffset);
-    float* col_scale_smem = reinterpret_cast<float*>(smem + L::kColScaleOffset);
-    float* bias_smem = reinterpret_cast<float*>(smem + L::kBiasOffset);
+    float4* columns = reinterpret_cast<float4*>(smem + L::kColumnOffset);      // [2][128]
 
     const uint32_t rank = ptx::cluster_ctarank();              // 0 = leader, 1 = peer
     const bool leader = rank == 0;
@@ -191,21 +199,30 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         const uint32_t store_base = smem_base + L::kStoreOffset + (uint32_t)(warp - 2) * 2u * L::kStoreBoxBytes;
         uint32_t tile_i = 0;
         uint32_t store_i = 0;                                  // stores issued by this warp: picks the staging box
+        // what the next tile needs from global memory is on its way while this one is worked on
+        float next_scale = 0.f, next_bias = 0.f, next_sa = 0.f;
+        auto prefetch = [&](int tile) {
+            if (tile >= pp.total_tiles) return;
+            const int row = tile / pp.n_tiles * 256 + (int)rank * kGemmBM + quarter * 32 + lane, n = tile % pp.n_tiles * 256 + epi_tid;
+            next_sa = row >= p.M ? 0.f : p.a_scales != nullptr ? p.a_scales[row] : 1.f;
+            next_scale = n >= p.N ? 0.f : p.b_scales != nullptr ? p.b_scales[n] : 1.f;
+            next_bias = n < p.N && p.bias != nullptr ? p.bias[n] : 0.f;
+        };
+        prefetch(cluster_id);
         bool ok = true;
         for (int tile = cluster_id; tile < pp.total_tiles; tile += num_clusters, ++tile_i) {
             const int m0 = tile / pp.n_tiles * 256 + (int)rank * kGemmBM, n0 = tile % pp.n_tiles * 256;
             const uint32_t acc = tile_i & 1u;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const float4* column = columns + acc * 128;
             {
-                const int n = n0 + epi_tid;
-                const bool in = n < p.N;
-                col_scale_smem[epi_tid] = !in ? 0.f : p.b_scales != nullptr ? p.b_scales[n] : 1.f;
-                bias_smem[epi_tid] = (in && p.bias != nullptr) ? p.bias[n] : 0.f;
+                float* c = reinterpret_cast<float*>(columns + acc * 128 + epi_tid / 2) + (epi_tid & 1);
+                c[0] = next_scale;
+                c[2] = next_bias;
             }
+            const float2 sa2 = make_float2(next_sa, next_sa);
+            // One barrier a tile: who has passed it knows that all have read the columns of two tiles ago.
             asm volatile("bar.sync 1, 256;" ::: "memory");
-            const int row = m0 + quarter * 32 + lane;
-            const bool row_ok = row < p.M;
-            const float sa = !row_ok ? 0.f : p.a_scales != nullptr ? p.a_scales[row] : 1.f;
+            prefetch(tile + num_clusters);
             const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * (256 - kFp4PairOverlap);
             // 32-column chunks of this warp: one of the two shared ones first, then three of the six others
             auto chunk = [&](int c) {
@@ -230,7 +247,6 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                 if (c + 1 < 4) ptx::tmem_ld_32x32b_x32(t_row + chunk(c + 1) * 32, r[(c + 1) & 1]);
                 const int cl = chunk(c) * 32, nc = n0 + cl;
                 const uint32_t(&rc)[32] = r[c & 1];
-                const float2 sa2 = make_float2(sa, sa);
                 if (nc < p.N) {                                // warp-uniform
                     const uint32_t box = store_base + (store_i & 1u) * L::kStoreBoxBytes;
                     ++store_i;
@@ -245,7 +261,11 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int j = q * 8 + e * 2;
-                            w[e] = pack16<F16>(epilogue_pair<false, GELU>(rc[j], rc[j + 1], sa2, col_scale_smem + cl + j, bias_smem + cl + j));
+                            const float4 sb = column[(cl + j) / 2];
+                            float2 y = ffma2(make_float2(__uint_as_float(rc[j]), __uint_as_float(rc[j + 1])), fmul2(sa2, make_float2(sb.x, sb.y)),
+                                             make_float2(sb.z, sb.w));
+                            if constexpr (GELU) y = gelu_tanh_fast2(y);
+                            w[e] = pack16<F16>(y);
                         }
                         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_addr + (((uint32_t)q ^ sw) << 4)),
                                      "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
