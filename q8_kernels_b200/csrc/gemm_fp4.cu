@@ -3,15 +3,21 @@
 // The tensor core multiplies the e2m1 values with their blocks' scales and adds in fp32 (kind::mxf4nvf4); the rows' scales (nvfp4),
 // the bias, tanh-GELU and the one rounding to 16 bits are the epilogue's.
 //
-// 128 x bn tiles, one a CTA.  Roles (10 warps):
-//   warp 0     TMA producer: values (128-byte slabs of 256) and block scales of the tile's rows and columns
-//   warp 1     TMEM allocation; one thread copies a slab's scales to TMEM and issues its four MMAs (K = 64)
-//   warps 2-9  epilogue
+// 128 x bn tiles, bn of 32, 64, 128 or 192, one a CTA: for products that 256 x 256 tiles on CTA pairs (gemm_fp4_pair.cu) do not spread over the
+// device.  Roles (10 warps):
+//   warp 0     TMA producer: values, in slabs of 256 along K (128 bytes), and block scales of the tile's rows and columns
+//   warp 1     TMEM allocation; one thread issues a slab's four MMAs (K = 64)
+//   warps 2-9  block scales from shared memory to TMEM, warps 2-5 those in even stages and 6-9 those in odd ones; then the epilogue
 // All waits are bounded.
 //
-// The scales of B can be named from every second column of TMEM only, i.e. from rows n that are multiples of 64.  A tile whose columns begin
-// elsewhere multiplies the window from the multiple of 64 below; the rows of B that it does not own are not loaded there, and what stands
-// in their place gives columns that nobody reads.
+// Bound by the latency of one short main loop, a few slabs to each of few CTAs.  The tensor core's own copy of scales (tcgen05.cp, 512 bytes)
+// stands in the pipe of the MMAs for some 65 clocks, and a slab of nvfp4 needs eight of them beside MMAs of some 240 clocks.  Registers bring
+// the scales past that pipe, every stage to its own columns.  Measured with M = 1 on cold operands, tcgen05.cp -> registers, us:
+//   nvfp4 N x K = 2048 x 2048 5.2 -> 4.2, 2048 x 8192 15.2 -> 10.6, 8192 x 2048 6.4 -> 5.9; mxfp4 4.3 -> 4.1, 10.9 -> 9.3, 5.7 -> 5.2.
+//
+// The scales of B can be named from every second column of TMEM only, i.e. from rows n that are multiples of 64.  A tile of 32 columns
+// multiplies the 64 from the multiple of 64 below; the rows of B that it does not own are not loaded there, and what stands in their place
+// gives columns that nobody reads.
 
 #include "gemm_fp4.cuh"
 
@@ -21,7 +27,7 @@ constexpr int kFp4MaxStages = 8;
 constexpr int kFp4MaxBN = 192;
 constexpr int kFp4ABytes = kGemmBM * 128;
 struct Fp4Smem {                             // behind the operand ring
-    static constexpr int kNumBars = 2 * kFp4MaxStages + 1;
+    static constexpr int kNumBars = 3 * kFp4MaxStages + 1;
     static constexpr int kTmemPtrOffset = kNumBars * 8;
     static constexpr int kAbortOffset = kTmemPtrOffset + 4;
     static constexpr int kColScaleOffset = (kAbortOffset + 4 + 15) & ~15;
@@ -31,9 +37,9 @@ struct Fp4Smem {                             // behind the operand ring
 struct Fp4TileParams {
     Fp4GemmParams g;
     int n_tiles;
-    int bn;                                  // tile columns, a multiple of 16
-    int window;                              // columns of the MMA, a multiple of 64: see above
-    int tmem_cols;                           // accumulator, scales of A, of B
+    int bn;                                  // tile columns: 32, 64, 128 or 192
+    int window;                              // columns of the MMA: 64 where bn is 32, see above
+    int tmem_cols;                           // the accumulator's, and for every stage the scales of A and of B
     int b_tiles;                             // 128-row tiles of B's scales that a window touches: 1 or 2
     int stages, stage_bytes, load_bytes;
 };
@@ -54,7 +60,8 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     const uint32_t bar_base = ptx::smem_u32(tail);
     auto full_bar = [&](int s) { return bar_base + 8u * s; };
     auto empty_bar = [&](int s) { return bar_base + 8u * (kFp4MaxStages + s); };
-    const uint32_t acc_bar = bar_base + 8u * (2 * kFp4MaxStages);
+    auto scaled_bar = [&](int s) { return bar_base + 8u * (2 * kFp4MaxStages + s); };      // its scales are in TMEM
+    const uint32_t acc_bar = bar_base + 8u * (3 * kFp4MaxStages);
     volatile uint32_t* tmem_ptr_smem = reinterpret_cast<volatile uint32_t*>(tail + L::kTmemPtrOffset);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + L::kAbortOffset);
     float* col_scale_smem = reinterpret_cast<float*>(tail + L::kColScaleOffset);
@@ -74,6 +81,7 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         for (int s = 0; s < stages; ++s) {
             ptx::mbar_init(full_bar(s), 1);
             ptx::mbar_init(empty_bar(s), 1);
+            ptx::mbar_init(scaled_bar(s), kGemmEpilogueThreads / 64);
         }
         ptx::mbar_init(acc_bar, 1);
         *abort_flag = 0;
@@ -85,8 +93,8 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         ptx::prefetch_tensormap(&tmap_bs);
     }
     if (warp == 1) {
-        if (sp.tmem_cols == 128) ptx::tmem_alloc<128>(ptx::smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)));
-        else ptx::tmem_alloc<256>(ptx::smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)));
+        if (sp.tmem_cols == 256) ptx::tmem_alloc<256>(ptx::smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)));
+        else ptx::tmem_alloc<512>(ptx::smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)));
         ptx::tmem_relinquish_alloc_permit();
     }
     pdl_wait();
@@ -100,6 +108,9 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 
     const int quarter = warp & 3;
     const int half = (warp - 2) >> 2;
+    // scales in TMEM, of stage s: A's tiles, then B's, tile t of its row tile j at (t nt + j) * 4
+    const uint32_t scale_cols = 4u * TILES * (1 + nt);
+    auto scales_of = [&](int s) { return tmem_base + window + s * scale_cols; };
 
     if (warp == 0) {
         if (ok && ptx::elect_one()) {
@@ -123,27 +134,20 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         if (ok && ptx::elect_one()) {
             int s = 0;
             uint32_t ph = 0;
-            const uint32_t ta = tmem_base + window, tb = ta + 4 * TILES;
-            const uint32_t tb0 = tb + (n0 % 128 >= 64 ? 2u : 0u);              // the window may begin in the middle of a tile of scales
+            const uint32_t shift = n0 % 128 >= 64 ? 2u : 0u;   // the window may begin in the middle of a tile of scales
             uint32_t idesc[2] = {ptx::make_idesc_fp4(kGemmBM, window, !NV, 0), ptx::make_idesc_fp4(kGemmBM, window, !NV, 2)};
             for (int i = 0; i < slabs; ++i) {
-                if (!ptx::mbar_wait(full_bar(s), ph, abort_flag)) { ok = false; break; }
+                if (!ptx::mbar_wait(full_bar(s), ph, abort_flag) || !ptx::mbar_wait(scaled_bar(s), ph, abort_flag)) { ok = false; break; }
                 ptx::tcgen05_fence_after_sync();
                 const uint32_t src = smem_base + s * sp.stage_bytes;
-#pragma unroll
-                for (int t = 0; t < TILES; ++t) {
-                    ptx::tmem_copy_scales<false>(ta + 4 * t, ptx::make_scales_desc(src + as_at + 512 * t));
-                    for (int j = 0; j < nt; ++j)
-                        ptx::tmem_copy_scales<false>(tb + 4 * (t * nt + j),
-                                                     ptx::make_scales_desc(src + bs_at + j * fp4_slab_scales(NV) + 512 * t));
-                }
+                const uint32_t ta = scales_of(s), tb = ta + 4 * TILES + shift;
                 const uint64_t a_desc = ptx::make_kmajor_desc(src, 128);
                 const uint64_t b_desc = ptx::make_kmajor_desc(src + b_at, 128);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int t = NV ? k : k / 2;
-                    ptx::mma_fp4<NV ? 4 : 2, false>(tmem_base, a_desc + 2 * k, b_desc + 2 * k, idesc[NV ? 0 : k & 1],
-                                                    ta + 4 * t, tb0 + 4 * t * nt, (i > 0 || k > 0) ? 1u : 0u);
+                    ptx::mma_fp4<NV ? 4 : 2, false>(tmem_base, a_desc + 2 * k, b_desc + 2 * k, idesc[NV ? 0 : k & 1], ta + 4 * t, tb + 4 * t * nt,
+                                                    (i > 0 || k > 0) ? 1u : 0u);
                 }
                 ptx::tcgen05_commit(empty_bar(s));
                 if (++s == stages) { s = 0; ph ^= 1u; }
@@ -153,6 +157,41 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         }
         __syncwarp();
     } else if (ok) {
+        // ------------------------------------------------ scales: warps 2-5 those in even stages, 6-9 those in odd ones; lane l of every lane
+        // quarter holds the 16 bytes of rows l, l + 32, l + 64, l + 96 of a tile
+        {
+            const uint8_t* from = smem + as_at + lane * 16;    // A's tiles, then B's
+            const uint32_t to = (uint32_t)(quarter * 32) << 16;
+            int s = -1;
+            uint32_t ph = 0;
+            for (int i = 0; i < slabs; ++i) {
+                if (++s == stages) { s = 0; ph ^= 1u; }
+                if ((s & 1) != half) continue;                 // a stage's phases are all awaited by the same warps: parity tells two apart
+                ok = ptx::mbar_wait(full_bar(s), ph, abort_flag);
+                ok = __all_sync(0xffffffffu, ok);              // keep the warp convergent for tcgen05.st
+                if (!ok) break;
+                ptx::tcgen05_fence_after_sync();
+                const uint8_t* src = from + s * sp.stage_bytes;
+                const uint32_t at = scales_of(s) + to;
+                uint4 w[3][TILES];
+#pragma unroll
+                for (int j = 0; j < 3; ++j)
+#pragma unroll
+                    for (int t = 0; t < TILES; ++t)
+                        if (j <= nt) w[j][t] = *reinterpret_cast<const uint4*>(src + (j * TILES + t) * 512);
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    ptx::tmem_st_32x32b_x4(at + 4 * t, w[0][t]);
+                    ptx::tmem_st_32x32b_x4(at + 4 * TILES + 4 * t * nt, w[1][t]);
+                    if (nt == 2) ptx::tmem_st_32x32b_x4(at + 4 * TILES + 4 * (2 * t + 1), w[2][t]);
+                }
+                ptx::tmem_wait_st();
+                ptx::tcgen05_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(scaled_bar(s));
+            }
+        }
+        // ------------------------------------------------ epilogue
         for (int c = threadIdx.x - 64; c < bn; c += kGemmEpilogueThreads) {
             const int n = n0 + c;
             const bool in = n < p.N;
@@ -163,7 +202,7 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         const int row = m_blk * kGemmBM + quarter * 32 + lane;
         const bool row_ok = row < p.M;
         const float sa = !row_ok ? 0.f : p.a_scales != nullptr ? p.a_scales[row] : 1.f;
-        ok = ptx::mbar_wait(acc_bar, 0, abort_flag);
+        if (ok) ok = ptx::mbar_wait(acc_bar, 0, abort_flag);
         ok = __all_sync(0xffffffffu, ok);                      // keep the warp convergent for tcgen05.ld
         ptx::tcgen05_fence_after_sync();
         if (!ok && p.status != nullptr && threadIdx.x == 64) atomicExch(p.status, Q8K_STATUS_TIMEOUT | (33 << 8));
@@ -202,8 +241,8 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     __syncthreads();
     if (warp == 1) {
         ptx::tcgen05_fence_after_sync();
-        if (sp.tmem_cols == 128) ptx::tmem_dealloc<128>(tmem_base);
-        else ptx::tmem_dealloc<256>(tmem_base);
+        if (sp.tmem_cols == 256) ptx::tmem_dealloc<256>(tmem_base);
+        else ptx::tmem_dealloc<512>(tmem_base);
     }
 }
 
@@ -223,9 +262,8 @@ static int launch_fp4_tiles(bool nv, bool gelu, bool f16, const Fp4Operand& a, c
     Fp4TileParams sp;
     sp.g = p;
     sp.bn = bn;
-    const int step = bn % 64 == 0 ? 64 : bn % 32 == 0 ? 32 : 16;               // the last tiles of a window begin 64 - step into it
-    sp.window = (64 - step + bn + 63) / 64 * 64;
-    sp.b_tiles = sp.window == 64 || bn == 128 ? 1 : 2;
+    sp.window = bn == 32 ? 64 : bn;
+    sp.b_tiles = bn == 192 ? 2 : 1;
     const int a_rows = split_a_rows(p.M);
     CUtensorMap ta, tb, tas, tbs;
     if (int rc = make_values_map(&ta, a.values, p.M, p.K, a_rows, op)) return rc;
@@ -235,36 +273,44 @@ static int launch_fp4_tiles(bool nv, bool gelu, bool f16, const Fp4Operand& a, c
     const int scales = fp4_slab_scales(nv);
     sp.load_bytes = (a_rows + bn) * 128 + scales * (1 + sp.b_tiles);
     sp.stage_bytes = ((kGemmBM + sp.window) * 128 + scales * (1 + sp.b_tiles) + 1023) / 1024 * 1024;
-    sp.tmem_cols = sp.window + 4 * fp4_slab_tiles(nv) * (1 + sp.b_tiles) <= 128 ? 128 : 256;
     const int64_t m_tiles = (p.M + kGemmBM - 1) / kGemmBM;
     sp.n_tiles = (p.N + bn - 1) / bn;
     Q8K_REQUIRE(m_tiles * sp.n_tiles <= 0x7fffffffLL, Q8K_ERR_TOO_LARGE, "%s: too many tiles", op);
-    const int budget = m_tiles * sp.n_tiles <= gemm_num_sms() ? 208 * 1024 : 104 * 1024;
-    int stages = budget / sp.stage_bytes;
+    // A grid that fits the device once has an SM's shared memory and TMEM to itself; otherwise two CTAs share them.  Every stage has its scales.
+    const bool alone = m_tiles * sp.n_tiles <= gemm_num_sms();
+    int stages = (alone ? 208 * 1024 : 104 * 1024) / sp.stage_bytes;
+    sp.tmem_cols = alone ? 512 : 256;
+    const int by_tmem = (sp.tmem_cols - sp.window) / (4 * fp4_slab_tiles(nv) * (1 + sp.b_tiles));
+    if (stages > by_tmem) stages = by_tmem;
     const int slabs = fp4_slabs(p.K);
     if (stages > slabs) stages = slabs;
     if (stages > kFp4MaxStages) stages = kFp4MaxStages;
     sp.stages = stages;
     const int smem = stages * sp.stage_bytes + Fp4Smem::kTotal + 1024;
     const unsigned grid = (unsigned)(m_tiles * sp.n_tiles);
-#define Q8K_FP4(NV)                                                                                              \
-    do {                                                                                                         \
-        if (gelu) return f16 ? launch_fp4_as<NV, true, true>(ta, tb, tas, tbs, sp, grid, smem, st)               \
-                             : launch_fp4_as<NV, true, false>(ta, tb, tas, tbs, sp, grid, smem, st);             \
-        return f16 ? launch_fp4_as<NV, false, true>(ta, tb, tas, tbs, sp, grid, smem, st)                        \
-                   : launch_fp4_as<NV, false, false>(ta, tb, tas, tbs, sp, grid, smem, st);                      \
+#define Q8K_FP4(NV)                                                                                      \
+    do {                                                                                                 \
+        if (gelu) return f16 ? launch_fp4_as<NV, true, true>(ta, tb, tas, tbs, sp, grid, smem, st)                 \
+                             : launch_fp4_as<NV, true, false>(ta, tb, tas, tbs, sp, grid, smem, st);               \
+        return f16 ? launch_fp4_as<NV, false, true>(ta, tb, tas, tbs, sp, grid, smem, st)                          \
+                   : launch_fp4_as<NV, false, false>(ta, tb, tas, tbs, sp, grid, smem, st);                        \
     } while (0)
     if (nv) Q8K_FP4(true);
     Q8K_FP4(false);
 #undef Q8K_FP4
 }
 
+// The narrowest tile whose grid fits the device once, one CTA an SM; 0 where none does, for the CTA pairs.  Measured, us, nvfp4 / mxfp4 on cold
+// operands, a tile against the pairs: M, N, K = 1, 2048, 2048 with 32 columns 4.3 / 4.1 against 7.1 / 7.1; 1, 8192, 2048 with 64 6.0 / 5.2
+// against 8.6 / 8.5; 300, 4096, 4096 with 128 10.1 / 9.0 against 10.4 / 10.3; 300, 2048, 8192 with 64 11.4 / 10.4 against 14.9 / 14.7.
+// Two rounds of tiles cost twice: 300, 8192, 2048 with 128 12.2 / 10.6 against 8.5 / 8.4; 24576, 128, 2048 13.3 against 11.4.  192 columns are
+// worth it for one row tile only, of which the pairs leave half empty (128, 20480, 4096: 15.5 / 14.7 against 18.1 / 17.7); with more rows the
+// pairs' grid fits once where theirs does, and is faster (256, 10240, 4096: 13.9 / 13.1 against 11.4 / 11.3).
 static int fp4_tile_columns(int M, int N) {
-    const int sms = gemm_num_sms();
-    const int64_t m_tiles = (M + kGemmBM - 1) / kGemmBM;
-    for (int bn : {16, 32, 48, 64, 80, 96, 128, 160})
-        if (m_tiles * ((N + bn - 1) / bn) <= sms) return bn;
-    return 192;
+    const int64_t m_tiles = ((int64_t)M + kGemmBM - 1) / kGemmBM;
+    for (int bn : {32, 64, 128, 192})
+        if (m_tiles * ((N + bn - 1) / bn) <= gemm_num_sms() && (bn < 192 || m_tiles == 1)) return bn;
+    return 0;
 }
 
 }  // namespace q8k
@@ -293,10 +339,11 @@ extern "C" int q8k_fp4_mm(int format, const void* a, const void* a_block_scales,
     p.status = dev_status;
     p.M = M; p.N = N; p.K = K;
     const Fp4Operand oa = {a, a_block_scales, a_row_scales}, ob = {b, b_block_scales, b_row_scales};
-    if (M > 256 && N >= 256) {
+    int bn = fp4_tile_columns(M, N);
+    if (bn == 0) {
         const int rc = launch_fp4_pair(nv, fuse_gelu != 0, out_dtype == Q8K_DT_F16, oa, ob, p, (cudaStream_t)stream);
         if (rc != Q8K_ERR_UNSUPPORTED) return rc;
+        bn = 128;                                              // a device that holds few pairs at once
     }
-    return launch_fp4_tiles(nv, fuse_gelu != 0, out_dtype == Q8K_DT_F16, oa, ob, p,
-                            fp4_tile_columns(M, N), (cudaStream_t)stream);
+    return launch_fp4_tiles(nv, fuse_gelu != 0, out_dtype == Q8K_DT_F16, oa, ob, p, bn, (cudaStream_t)stream);
 }

@@ -173,9 +173,9 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                     const uint64_t b_desc = ptx::make_kmajor_desc(src + L::kABytes, 128);
 #pragma unroll
                     for (int t = 0; t < TILES; ++t) {
-                        ptx::tmem_copy_scales<true>(ta + 4 * t, as_desc + 32 * t);
-                        ptx::tmem_copy_scales<true>(tb + 8 * t, bs_desc + 32 * t);
-                        ptx::tmem_copy_scales<true>(tb + 8 * t + 4, bs_desc + L::kScales / 16 + 32 * t);
+                        ptx::tmem_copy_scales_pair(ta + 4 * t, as_desc + 32 * t);
+                        ptx::tmem_copy_scales_pair(tb + 8 * t, bs_desc + 32 * t);
+                        ptx::tmem_copy_scales_pair(tb + 8 * t + 4, bs_desc + L::kScales / 16 + 32 * t);
                     }
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {

@@ -264,24 +264,9 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
         : "memory");
 }
 
-// 16 lanes x 64 columns as fragments of 16 x 8: thread t gets of columns [8 i, 8 i + 8) in r[4 i ..] columns 2 (t % 4) and the next of lane t / 4, then
-// of lane t / 4 + 8.
-__device__ __forceinline__ void tmem_ld_16x256b_x8(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-// Four 8 x 8 matrices of 16-bit values, thread t's words holding two of row t / 4, to rows of 16 bytes that lanes 8 k .. 8 k + 7 name for matrix k.
-__device__ __forceinline__ void stmatrix_x4(uint32_t addr, const uint32_t (&w)[4]) {
-    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                 : "memory");
+// 32 lanes x 4 columns, one 16-byte word a lane
+__device__ __forceinline__ void tmem_st_32x32b_x4(uint32_t taddr, const uint4& r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
 }
 
 // ---------------------------------------------------------------- MMA
@@ -435,11 +420,10 @@ __device__ __forceinline__ void mma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64
     else Q8K_MMA_FP4("1", "2X");
 #undef Q8K_MMA_FP4
 }
-// 512 bytes of scales (32 rows of 16 bytes) from shared memory to 32 lanes x 4 columns, in all four lane quarters; with PAIR in both CTAs,
+// 512 bytes of scales (32 rows of 16 bytes) from shared memory to 32 lanes x 4 columns, in all four lane quarters; in both CTAs of a pair,
 // each from its own shared memory.  Runs in the order of the issuing thread's MMAs.
-template <bool PAIR> __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
-    if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+__device__ __forceinline__ void tmem_copy_scales_pair(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 // Shared-memory descriptor of such 512 bytes: not swizzled, groups of 8 rows 128 bytes apart.
 __device__ __forceinline__ uint64_t make_scales_desc(uint32_t smem_addr) {

@@ -112,7 +112,8 @@ def test_quantizer_bits(fmt, dtype, rows, k):
 @pytest.mark.parametrize("gelu,bias,out", [(False, True, BF16), (True, True, F16), (False, False, F16), (True, False, BF16)])
 @pytest.mark.parametrize("m,n,k", [(1, 16, 32), (3, 48, 96), (8, 128, 256), (77, 272, 2048), (128, 96, 64), (129, 2048, 544), (300, 560, 1024), (1, 8192, 2048),
                                    (16, 4096, 4096), (1000, 1408, 512), (2002, 5504, 288), (700, 4096, 8192), (3000, 256, 512), (60000, 512, 64),
-                                   (20100, 528, 2048), (1300, 2064, 2080)])
+                                   (20100, 528, 2048), (1300, 2064, 2080), (1, 20480, 544), (100, 18960, 96), (129, 10256, 160),
+                                   (19000, 16, 288), (200, 4144, 1056)])
 def test_products(fmt, gelu, bias, out, m, n, k):
     from q8_kernels_b200 import check_status, native
     a, b = sample(m, k, BF16, 1).cuda(), sample(n, k, BF16, 2).cuda()
