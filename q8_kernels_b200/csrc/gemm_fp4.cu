@@ -41,13 +41,13 @@ struct Fp4TileParams {
     int window;                              // columns of the MMA: 64 where bn is 32, see above
     int tmem_cols;                           // the accumulator's, and for every stage the scales of A and of B
     int b_tiles;                             // 128-row tiles of B's scales that a window touches: 1 or 2
-    int stages, stage_bytes, load_bytes;
+    int stages, stage_bytes, value_bytes;    // value_bytes: of the values that one stage loads
+    const uint8_t *a_block_scales, *b_block_scales;
 };
 
 template <bool NV, bool GELU, bool F16>
 __global__ void __launch_bounds__(kGemmThreads, 2)
-gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_as,
-                const __grid_constant__ CUtensorMap tmap_bs, const __grid_constant__ Fp4TileParams sp) {
+gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ Fp4TileParams sp) {
     using L = Fp4Smem;
     constexpr int TILES = fp4_slab_tiles(NV);                  // 512-byte scale tiles a slab
     const Fp4GemmParams& p = sp.g;
@@ -89,8 +89,6 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         ptx::fence_proxy_async_smem();
         ptx::prefetch_tensormap(&tmap_a);
         ptx::prefetch_tensormap(&tmap_b);
-        ptx::prefetch_tensormap(&tmap_as);
-        ptx::prefetch_tensormap(&tmap_bs);
     }
     if (warp == 1) {
         if (sp.tmem_cols == 256) ptx::tmem_alloc<256>(ptx::smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)));
@@ -116,15 +114,23 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         if (ok && ptx::elect_one()) {
             int s = 0;
             uint32_t ph = 1;                                   // empty_bar phase to wait for: the first round passes
-            constexpr int SLAB_ROWS = fp4_slab_scales(NV) / 256;
+            // a slab's scales of one row tile lie together; behind B's last row tile there are none
+            const int row_tile = n0 / 128, b_tiles = min(nt, (p.N + 127) / 128 - row_tile);
+            const uint8_t* as = sp.a_block_scales + (int64_t)m_blk * slabs * fp4_slab_scales(NV);
+            const uint8_t* bs = sp.b_block_scales + (int64_t)row_tile * slabs * fp4_slab_scales(NV);
+            const int64_t second = (int64_t)slabs * fp4_slab_scales(NV);
+            const uint32_t bytes = sp.value_bytes + (1 + b_tiles) * fp4_slab_scales(NV);
             for (int i = 0; i < slabs; ++i) {
                 if (!ptx::mbar_wait(empty_bar(s), ph, abort_flag)) { ok = false; break; }
-                ptx::mbar_arrive_expect_tx(full_bar(s), (uint32_t)sp.load_bytes);
+                ptx::mbar_arrive_expect_tx(full_bar(s), bytes);
                 const uint32_t dst = smem_base + s * sp.stage_bytes;
                 ptx::tma_load_2d(dst, &tmap_a, full_bar(s), i * 128, m_blk * kGemmBM);
                 ptx::tma_load_2d(dst + b_at + (uint32_t)off * 128u, &tmap_b, full_bar(s), i * 128, n0);
-                ptx::tma_load_3d(dst + as_at, &tmap_as, full_bar(s), 0, i * SLAB_ROWS, m_blk);
-                ptx::tma_load_3d(dst + bs_at, &tmap_bs, full_bar(s), 0, i * SLAB_ROWS, n0 / 128);
+                ptx::bulk_load(dst + as_at, as, fp4_slab_scales(NV), full_bar(s));
+                ptx::bulk_load(dst + bs_at, bs, fp4_slab_scales(NV), full_bar(s));
+                if (b_tiles > 1) ptx::bulk_load(dst + bs_at + fp4_slab_scales(NV), bs + second, fp4_slab_scales(NV), full_bar(s));
+                as += fp4_slab_scales(NV);                     // (stepped: the addresses from i cost 60 clocks a slab)
+                bs += fp4_slab_scales(NV);
                 if (++s == stages) { s = 0; ph ^= 1u; }
             }
             if (!ok && p.status != nullptr) atomicExch(p.status, Q8K_STATUS_TIMEOUT | (31 << 8));
@@ -247,12 +253,11 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 }
 
 template <bool NV, bool GELU, bool F16>
-static int launch_fp4_as(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tas, const CUtensorMap& tbs, const Fp4TileParams& sp,
-                         unsigned grid, int smem, cudaStream_t st) {
+static int launch_fp4_as(const CUtensorMap& ta, const CUtensorMap& tb, const Fp4TileParams& sp, unsigned grid, int smem, cudaStream_t st) {
     auto kern = gemm_fp4_kernel<NV, GELU, F16>;
     static std::atomic<uint64_t> smem_done{0};
     if (int rc = allow_dynamic_smem((const void*)kern, 226 * 1024, smem_done)) return rc;
-    Q8K_CUDA_OK(launch_dependent(kern, grid, kGemmThreads, smem, st, 1, ta, tb, tas, tbs, sp));
+    Q8K_CUDA_OK(launch_dependent(kern, grid, kGemmThreads, smem, st, 1, ta, tb, sp));
     return Q8K_OK;
 }
 
@@ -265,14 +270,13 @@ static int launch_fp4_tiles(bool nv, bool gelu, bool f16, const Fp4Operand& a, c
     sp.window = bn == 32 ? 64 : bn;
     sp.b_tiles = bn == 192 ? 2 : 1;
     const int a_rows = split_a_rows(p.M);
-    CUtensorMap ta, tb, tas, tbs;
+    CUtensorMap ta, tb;
     if (int rc = make_values_map(&ta, a.values, p.M, p.K, a_rows, op)) return rc;
     if (int rc = make_values_map(&tb, b.values, p.N, p.K, bn, op)) return rc;
-    if (int rc = make_scales_map(&tas, a.block_scales, nv, p.M, p.K, 1, op)) return rc;
-    if (int rc = make_scales_map(&tbs, b.block_scales, nv, p.N, p.K, sp.b_tiles, op)) return rc;
-    const int scales = fp4_slab_scales(nv);
-    sp.load_bytes = (a_rows + bn) * 128 + scales * (1 + sp.b_tiles);
-    sp.stage_bytes = ((kGemmBM + sp.window) * 128 + scales * (1 + sp.b_tiles) + 1023) / 1024 * 1024;
+    sp.a_block_scales = static_cast<const uint8_t*>(a.block_scales);
+    sp.b_block_scales = static_cast<const uint8_t*>(b.block_scales);
+    sp.value_bytes = (a_rows + bn) * 128;
+    sp.stage_bytes = ((kGemmBM + sp.window) * 128 + fp4_slab_scales(nv) * (1 + sp.b_tiles) + 1023) / 1024 * 1024;
     const int64_t m_tiles = (p.M + kGemmBM - 1) / kGemmBM;
     sp.n_tiles = (p.N + bn - 1) / bn;
     Q8K_REQUIRE(m_tiles * sp.n_tiles <= 0x7fffffffLL, Q8K_ERR_TOO_LARGE, "%s: too many tiles", op);
@@ -290,10 +294,10 @@ static int launch_fp4_tiles(bool nv, bool gelu, bool f16, const Fp4Operand& a, c
     const unsigned grid = (unsigned)(m_tiles * sp.n_tiles);
 #define Q8K_FP4(NV)                                                                                      \
     do {                                                                                                 \
-        if (gelu) return f16 ? launch_fp4_as<NV, true, true>(ta, tb, tas, tbs, sp, grid, smem, st)                 \
-                             : launch_fp4_as<NV, true, false>(ta, tb, tas, tbs, sp, grid, smem, st);               \
-        return f16 ? launch_fp4_as<NV, false, true>(ta, tb, tas, tbs, sp, grid, smem, st)                          \
-                   : launch_fp4_as<NV, false, false>(ta, tb, tas, tbs, sp, grid, smem, st);                        \
+        if (gelu) return f16 ? launch_fp4_as<NV, true, true>(ta, tb, sp, grid, smem, st)                 \
+                             : launch_fp4_as<NV, true, false>(ta, tb, sp, grid, smem, st);               \
+        return f16 ? launch_fp4_as<NV, false, true>(ta, tb, sp, grid, smem, st)                          \
+                   : launch_fp4_as<NV, false, false>(ta, tb, sp, grid, smem, st);                        \
     } while (0)
     if (nv) Q8K_FP4(true);
     Q8K_FP4(false);
