@@ -64,7 +64,7 @@ def fp4_linear(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor] = 
     """``act(a b^T + bias)`` with a 4-bit weight ``b`` uint8 [N,K/2] and its scales ``scale_b`` as ``fp4_quantize`` returns them, N a multiple of
     16.  ``a``: bf16 or fp16 [...,K], quantised in the weight's format first, or 4-bit values with ``scale_a``.  ``bias`` fp32 [N] or None; act is
     tanh-GELU with ``fuse_gelu``.  Returns [...,N] in ``out_dtype``, bf16 or fp16, by default a's type (bf16 for 4-bit a).
-    Differentiable in an un-quantised ``a``."""
+    Differentiable in an un-quantised ``a``, with N up to 32768."""
     if scale_b is None:
         raise native.Q8KernelError("fp4_linear: the weight must be 4-bit values with their scales")
     if scale_a is None and isinstance(scale_b, (tuple, list)) and len(scale_b) == 2 and isinstance(scale_b[0], torch.Tensor) \
@@ -82,5 +82,7 @@ def fp4_linear(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor] = 
     native.fp4_linear_check("fp4_linear", a, b, scale_b, bias)
     native.refuse_tangents("fp4_linear", a, bias, scale_b[1])
     if torch.is_grad_enabled() and a.requires_grad:
+        if b.shape[0] > 32768:                                 # what quantises the gradient holds a row of it in a CTA
+            raise native.Q8KernelError(f"fp4_linear: the gradient of {b.shape[0]} output channels: at most 32768 are supported")
         return FP4LinearFunc.apply(a, b, bias, *scale_b, bool(fuse_gelu), out_dtype)
     return native.fp4_linear(a, b, scale_b, bias, fuse_gelu, out_dtype)
