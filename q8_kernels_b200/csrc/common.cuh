@@ -59,12 +59,14 @@ int gemm_num_sms();                          // SMs of the current device (148 i
 
 // Raise a kernel's dynamic shared memory limit, once per device (the call costs about 1 us, a launch 2.5).  The setting
 // lives as long as the device's context; `done` belongs to the one kernel.
-inline int allow_dynamic_smem(const void* kern, int bytes, std::atomic<uint64_t>& done) {
+// whole_carveout: of the SM's memory, as much as can be is shared memory while the kernel runs, not L1.
+inline int allow_dynamic_smem(const void* kern, int bytes, std::atomic<uint64_t>& done, bool whole_carveout = false) {
     int dev = 0;
     Q8K_CUDA_OK(cudaGetDevice(&dev));
     const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
     if ((done.load(std::memory_order_relaxed) & bit) != 0) return Q8K_OK;
     Q8K_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (whole_carveout) Q8K_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     done.fetch_or(bit, std::memory_order_relaxed);
     return Q8K_OK;
 }

@@ -37,7 +37,9 @@ constexpr int kHeadMaxDim = 512;
 constexpr int kHeadThreads = 128;
 constexpr int kHeadChannels = 16;            // channels of a lane: 8 in the first runs of its units, 8 in the second
 constexpr int kHeadRows = 8;                 // heads of a thread, where there are threads for the others
-constexpr int kHeadMaxCtas = 148 * 8;        // of the backward pass with sums
+// CTAs of the backward pass with sums, four of which an SM holds at once: one that works on, token after token, adds up more before it writes its
+// sums, but the last ones leave SMs idle.  16384 x 40 x 128 with 4, 8, 12, 16, 20, 24, 36 an SM: 110, 103, 97, 96.5, 95.5, 98, 103 us.
+constexpr int kHeadSumCtas = 20, kHeadMaxCtas = 148 * kHeadSumCtas;
 
 // A warp's lanes are groups of `lanes`, each with a head.  A CTA works for queries or for keys; its groups are `tokens` times `head_lanes`.
 // CTAs [0, ctas[0]) are the queries', the ctas[1] behind them the keys'.
@@ -410,13 +412,14 @@ head_norm_kernel(const __grid_constant__ HeadNormParams p, const __grid_constant
     }
 }
 
-// dw from the CTAs' sums, 32 columns a CTA, in a fixed order; blockIdx.y: queries, keys
-constexpr int kHeadSumWarps = 16;
-__global__ void __launch_bounds__(32 * kHeadSumWarps)
+// dw from the CTAs' sums, 8 columns (a sector) a CTA, in a fixed order; blockIdx.y: queries, keys
+constexpr int kHeadSumThreads = 512, kHeadSumColumns = 8;
+__global__ void __launch_bounds__(kHeadSumThreads)
 head_norm_sum_kernel(const float* __restrict__ part, int q_parts, int k_parts, float* __restrict__ dq, float* __restrict__ dk, int dim) {
-    __shared__ float red[kHeadSumWarps][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + lane;
+    constexpr int ROWS = kHeadSumThreads / kHeadSumColumns;
+    __shared__ float red[kHeadSumThreads / 32][kHeadSumColumns];
+    const int col = threadIdx.x % kHeadSumColumns, row = threadIdx.x / kHeadSumColumns;
+    const int c = blockIdx.x * kHeadSumColumns + col;
     float* out = blockIdx.y == 0 ? dq : dk;
     pdl_wait();
     pdl_release();
@@ -425,13 +428,15 @@ head_norm_sum_kernel(const float* __restrict__ part, int q_parts, int k_parts, f
     float a = 0.f;
     if (c < dim) {
 #pragma unroll 8
-        for (int k = first + warp; k < last; k += kHeadSumWarps) a += part[(int64_t)k * dim + c];
+        for (int k = first + row; k < last; k += ROWS) a += part[(int64_t)k * dim + c];
     }
-    red[warp][lane] = a;
-    __syncthreads();
-    if (warp == 0 && c < dim) {
 #pragma unroll
-        for (int k = 1; k < kHeadSumWarps; ++k) a += red[k][lane];
+    for (int o = 16; o >= kHeadSumColumns; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    if ((threadIdx.x & 31) < kHeadSumColumns) red[threadIdx.x >> 5][col] = a;
+    __syncthreads();
+    if (threadIdx.x < kHeadSumColumns && c < dim) {
+#pragma unroll
+        for (int k = 1; k < kHeadSumThreads / 32; ++k) a += red[k][col];
         out[c] = a;
     }
 }
@@ -448,7 +453,7 @@ static int launch_head_norm_as(const HeadNormParams& p, float* dqw, float* dkw, 
     const int room = p.rotary_dim > 0 ? 24 * 1024 / (4 * p.rotary_dim) : slots;
     const bool sums = BACK && p.part != nullptr;
     const int all = p.t[0].heads + p.t[1].heads;
-    const int most = 4 * gemm_num_sms() < kHeadMaxCtas ? 4 * gemm_num_sms() : kHeadMaxCtas;
+    const int most = kHeadSumCtas * gemm_num_sms() < kHeadMaxCtas ? kHeadSumCtas * gemm_num_sms() : kHeadMaxCtas;
     size_t smem = 0;                                           // angles; the sums take the ring's place (at most 8 KB)
     for (int i = 0; i < 2; ++i) {
         const int heads = p.t[i].heads;
@@ -478,12 +483,18 @@ static int launch_head_norm_as(const HeadNormParams& p, float* dqw, float* dkw, 
         if (whole && l.lanes == 8) { kern = head_norm_kernel<T, V, TWO, BACK, 8>; form = 2; }
         if (whole && l.lanes == 16) { kern = head_norm_kernel<T, V, TWO, BACK, 16>; form = 3; }
     }
+    // All of these kernels ask for the whole of an SM's shared memory, since an SM keeps what it set aside for a kernel until that has left:
+    // a backward pass that came in beside the last CTAs of the forward pass (1/6 of an SM each) had room for fewer CTAs until its
+    // own end, and both together took 192 us in the place of 166 (16384 x 40 x 128).
     static std::atomic<uint64_t> smem_done[4] = {};
-    if (int rc = allow_dynamic_smem((const void*)kern, HeadRing<T, BACK>::bytes + 24 * 1024, smem_done[form])) return rc;
+    if (int rc = allow_dynamic_smem((const void*)kern, HeadRing<T, BACK>::bytes + 24 * 1024, smem_done[form], true)) return rc;
     Q8K_CUDA_OK(launch_dependent(kern, grid, kHeadThreads, HeadRing<T, BACK>::bytes + smem, st, 1, p, l));
-    if (sums)
-        Q8K_CUDA_OK(launch_dependent(head_norm_sum_kernel, dim3((unsigned)((p.head_dim + 31) / 32), 2), 32 * kHeadSumWarps, 0, st, 1, p.part, l.of[0].ctas,
+    if (sums) {
+        static std::atomic<uint64_t> sum_done{0};
+        if (int rc = allow_dynamic_smem((const void*)head_norm_sum_kernel, 0, sum_done, true)) return rc;
+        Q8K_CUDA_OK(launch_dependent(head_norm_sum_kernel, dim3((unsigned)((p.head_dim + kHeadSumColumns - 1) / kHeadSumColumns), 2), kHeadSumThreads, 0, st, 1, p.part, l.of[0].ctas,
                                      l.of[1].ctas, dqw, dkw, p.head_dim));
+    }
     return Q8K_OK;
 }
 
