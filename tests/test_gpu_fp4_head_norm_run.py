@@ -337,3 +337,18 @@ def test_fp8_products_in_fp16(m, n, k):
     wa, wb = a.double() * sa.double().view(-1, 1), b.double() * sb.double().view(-1, 1)
     ref, slack = wa @ wb.T, (k // 32 + 8) * 2.0 ** -23 * (wa.abs() @ wb.abs().T)
     assert y.dtype == F16 and ((y.double() - ref).abs() <= slack + (ref.abs() + slack) * 2.0 ** -11 * 1.001 + 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_a_row_has_its_bits_in_every_call(fmt):
+    """One row alone, in small tiles of any width and in tiles of pairs: each element is one accumulator's sum in ascending K."""
+    from q8_kernels_b200 import check_status
+    from q8_kernels_b200.functional.fp4 import fp4_linear, fp4_quantize
+    w, ws = fp4_quantize((torch.randn(2080, 1056, device="cuda") / 32).to(BF16), fmt)
+    x, bias = torch.randn(4000, 1056, device="cuda").to(BF16), torch.randn(2080, device="cuda")
+    y = fp4_linear(x, w, bias, None, ws)
+    for rows in ((0, 1), (130, 230), (700, 1000), (40, 1900)):
+        assert torch.equal(bits(fp4_linear(x[rows[0]:rows[1]], w, bias, None, ws)), bits(y[rows[0]:rows[1]]))
+    few, fews = fp4_quantize(torch.zeros(48, 1056, device="cuda", dtype=BF16), fmt)
+    assert (fp4_linear(x, few, bias[:48].contiguous(), None, fews) == bias[:48].to(BF16)).all()
+    check_status()
