@@ -70,8 +70,8 @@ class AxialRotaryEmbedding(nn.Module):
     def forward(self, q, k, positions):
         if q.shape[-1] != self.head_dim:
             raise Q8KernelError(f"AxialRotaryEmbedding: heads of {q.shape[-1]} channels, {self.head_dim} expected")
-        if positions.dim() < 2 or positions.shape[-1] != len(self.sections):
-            raise Q8KernelError(f"AxialRotaryEmbedding: positions {tuple(positions.shape)} for {len(self.sections)} axes")
+        if positions is None or positions.dim() < 2 or positions.shape[-1] != len(self.sections):
+            raise Q8KernelError(f"AxialRotaryEmbedding: positions {None if positions is None else tuple(positions.shape)} for {len(self.sections)} axes")
         fast = _host._axial_rotary(q, k, positions, self._frequency_bits, self._axes, self.amplitude, self._half)
         if fast is not None:
             return fast

@@ -107,6 +107,16 @@ def test_refusals_of_the_c_entries():
     assert lib.q8k_fp8_mm(buf, buf, None, buf, buf, buf, f16, 1, 1, 8, 16, 64, 1, None, None) == -2
 
 
+def test_modules_need_positions_of_their_axes():
+    from q8_kernels_b200.modules import AxialRotaryEmbedding, HeadNormRotary
+    rotary = AxialRotaryEmbedding(64, (32, 32))
+    q = torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16)
+    for m in (rotary, HeadNormRotary(64, rotary)):
+        for positions in (None, torch.zeros(4), torch.zeros(4, 3)):
+            with pytest.raises(Q8KernelError, match="2 axes"):
+                m(q, None, positions)
+
+
 def test_cpu_tensors_are_refused():
     from q8_kernels_b200.functional import fp4, head_norm, rotary
     x = torch.zeros(4, 64, dtype=torch.bfloat16)
