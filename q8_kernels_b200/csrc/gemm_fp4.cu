@@ -39,14 +39,13 @@ struct Fp4TileParams {
     int n_tiles;
     int bn;                                  // tile columns: 32, 64, 128 or 192
     int window;                              // columns of the MMA: 64 where bn is 32, see above
-    int tmem_cols;                           // the accumulator's, and for every stage the scales of A and of B
     int b_tiles;                             // 128-row tiles of B's scales that a window touches: 1 or 2
     int stages, stage_bytes, value_bytes;    // value_bytes: of the values that one stage loads
     const uint8_t *a_block_scales, *b_block_scales;
 };
 
 template <bool NV, bool GELU, bool F16>
-__global__ void __launch_bounds__(kGemmThreads, 2)
+__global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ Fp4TileParams sp) {
     using L = Fp4Smem;
     constexpr int TILES = fp4_slab_tiles(NV);                  // 512-byte scale tiles a slab
@@ -91,8 +90,7 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         ptx::prefetch_tensormap(&tmap_b);
     }
     if (warp == 1) {
-        if (sp.tmem_cols == 256) ptx::tmem_alloc<256>(ptx::smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)));
-        else ptx::tmem_alloc<512>(ptx::smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)));
+        ptx::tmem_alloc<512>(ptx::smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)));
         ptx::tmem_relinquish_alloc_permit();
     }
     pdl_wait();
@@ -247,8 +245,7 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     __syncthreads();
     if (warp == 1) {
         ptx::tcgen05_fence_after_sync();
-        if (sp.tmem_cols == 256) ptx::tmem_dealloc<256>(tmem_base);
-        else ptx::tmem_dealloc<512>(tmem_base);
+        ptx::tmem_dealloc<512>(tmem_base);
     }
 }
 
@@ -280,11 +277,9 @@ static int launch_fp4_tiles(bool nv, bool gelu, bool f16, const Fp4Operand& a, c
     const int64_t m_tiles = (p.M + kGemmBM - 1) / kGemmBM;
     sp.n_tiles = (p.N + bn - 1) / bn;
     Q8K_REQUIRE(m_tiles * sp.n_tiles <= 0x7fffffffLL, Q8K_ERR_TOO_LARGE, "%s: too many tiles", op);
-    // A grid that fits the device once has an SM's shared memory and TMEM to itself; otherwise two CTAs share them.  Every stage has its scales.
-    const bool alone = m_tiles * sp.n_tiles <= gemm_num_sms();
-    int stages = (alone ? 208 * 1024 : 104 * 1024) / sp.stage_bytes;
-    sp.tmem_cols = alone ? 512 : 256;
-    const int by_tmem = (sp.tmem_cols - sp.window) / (4 * fp4_slab_tiles(nv) * (1 + sp.b_tiles));
+    // TMEM's 512 columns hold the accumulator and every stage's scales of A and of B
+    int stages = 208 * 1024 / sp.stage_bytes;
+    const int by_tmem = (512 - sp.window) / (4 * fp4_slab_tiles(nv) * (1 + sp.b_tiles));
     if (stages > by_tmem) stages = by_tmem;
     const int slabs = fp4_slabs(p.K);
     if (stages > slabs) stages = slabs;
