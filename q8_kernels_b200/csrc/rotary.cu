@@ -11,7 +11,7 @@
 // up to eight heads of one token: its cosines and sines come from shared memory once, and its addresses advance by the head's stride.
 // CTAs of 128 threads, eight an SM: the chain from position to sine hides behind the first loads and behind other CTAs' stores, and the
 // last ones to finish are short.  Measured (bf16, CUDA graphs): 6144 tokens x 64 heads x 64 interleaved 16.3 us (0.94 of the copy rate),
-// 16384 x 40 x 128 half 55.5 us (0.93).  Tried, when these took 17.5 and 61.6: six CTAs without spills (17.9, 64.3), one head's loads at a
+// 16384 x 40 x 128 half 53.7 us (0.95), interleaved 52.3 (0.98).  Tried, when these took 17.5 and 61.6: six CTAs without spills (17.9, 64.3), one head's loads at a
 // time (19.8, 65.2), a thread for one unit with the next token's elements on their way meanwhile (30.9, 103).
 
 #include <type_traits>
@@ -35,6 +35,7 @@ struct RotaryParams {
 
 constexpr int kRotaryMaxDim = 4096;
 constexpr int kRotaryThreads = 128;
+constexpr int kRotaryWave = 4;               // CTAs an SM that more heads a thread have to leave, half of what it holds at once
 constexpr int kRotaryHeads = 8;              // heads of a thread, where there are threads for the others
 
 // How a CTA's threads are laid out over its tokens: unit_lanes threads for the units of a head, head_lanes for the heads.
@@ -157,10 +158,15 @@ template <typename T, int V, bool TWO> static int launch_rotary_as(const RotaryP
     constexpr int run = TWO ? 2 * V : V;
     l.units = p.rotary_dim / 2 / (TWO ? V : V / 2) + (p.head_dim - p.rotary_dim + run - 1) / run;
     l.unit_lanes = l.units < kRotaryThreads ? l.units : kRotaryThreads;
-    // kRotaryHeads heads a thread, fewer while there are SMs without a CTA; then as many tokens as threads are left for
+    // kRotaryHeads heads a thread, up to twice as many where that leaves fewer threads idle and enough CTAs, fewer while
+    // there are SMs without a CTA; then as many tokens as threads are left for.  (More heads, us: 16384 x 40 x 128 interleaved 62.7 -> 52.4, half
+    // 56.0 -> 53.9, 8192 x 32 x 96 19.0 -> 17.9, 4096 x 48 x 128 half 19.2 -> 16.1; but 1023 x 32 x 72 in fewer CTAs 4.2 -> 5.6.)
     const int rest = kRotaryThreads / l.unit_lanes;
     int per_thread = kRotaryHeads;
     auto lanes = [&](int n) { const int want = (heads + n - 1) / n; return want < rest ? want : rest; };
+    auto used = [&](int n) { return lanes(n) * (rest / lanes(n)); };
+    for (int n = kRotaryHeads + 1; n <= 2 * kRotaryHeads; ++n)
+        if (used(n) > used(per_thread) && p.tokens >= (int64_t)kRotaryWave * gemm_num_sms() * (rest / lanes(n))) per_thread = n;
     while (per_thread > 1 && (p.tokens + rest / lanes(per_thread) - 1) / (rest / lanes(per_thread)) < gemm_num_sms()) --per_thread;
     l.head_lanes = lanes(per_thread);
     l.tokens = rest / l.head_lanes;
