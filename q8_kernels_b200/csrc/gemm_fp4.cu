@@ -11,9 +11,14 @@
 // All waits are bounded.
 //
 // Bound by the latency of one short main loop, a few slabs to each of few CTAs.  The tensor core's own copy of scales (tcgen05.cp, 512 bytes)
-// stands in the pipe of the MMAs for some 65 clocks, and a slab of nvfp4 needs eight of them beside MMAs of some 240 clocks.  Registers bring
+// stands in the pipe of the MMAs for some 65 clocks, and a slab of nvfp4 needs eight of them.  Registers bring
 // the scales past that pipe, every stage to its own columns.  Measured with M = 1 on cold operands, tcgen05.cp -> registers, us:
-//   nvfp4 N x K = 2048 x 2048 5.2 -> 4.2, 2048 x 8192 15.2 -> 10.6, 8192 x 2048 6.4 -> 5.9; mxfp4 4.3 -> 4.1, 10.9 -> 9.3, 5.7 -> 5.2.
+//   nvfp4 N x K = 2048 x 2048 5.2 -> 4.2, 2048 x 8192 15.2 -> 10.2, 8192 x 2048 6.4 -> 5.9; mxfp4 4.3 -> 4.1, 10.9 -> 9.3, 5.7 -> 5.2.
+//
+// What is left of a slab are 470 clocks of its four MMAs, of which one with 64 columns takes hardly less than one of 256, and 360 of its four copies'
+// issue.  (Not kept: loads by two or three warps, no change.)  With fewer than 128 rows a stage holds those rows only, and there are
+// up to 16 of them (1 x 20480 x 4096 13.3 -> 12.3 us): the MMA's other rows are whatever follows in shared memory, other stages' values as they come
+// and go, and give rows that nobody reads.
 //
 // The scales of B can be named from every second column of TMEM only, i.e. from rows n that are multiples of 64.  A tile of 32 columns
 // multiplies the 64 from the multiple of 64 below; the rows of B that it does not own are not loaded there, and what stands in their place
@@ -23,7 +28,7 @@
 
 namespace q8k {
 
-constexpr int kFp4MaxStages = 8;
+constexpr int kFp4MaxStages = 16;
 constexpr int kFp4MaxBN = 192;
 constexpr int kFp4ABytes = kGemmBM * 128;
 struct Fp4Smem {                             // behind the operand ring
@@ -40,7 +45,7 @@ struct Fp4TileParams {
     int bn;                                  // tile columns: 32, 64, 128 or 192
     int window;                              // columns of the MMA: 64 where bn is 32, see above
     int b_tiles;                             // 128-row tiles of B's scales that a window touches: 1 or 2
-    int stages, stage_bytes, value_bytes;    // value_bytes: of the values that one stage loads
+    int stages, stage_bytes, a_bytes;        // a_bytes: of A's values in a stage
     const uint8_t *a_block_scales, *b_block_scales;
 };
 
@@ -74,7 +79,7 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     const int slabs = (p.K + kFp4Slab - 1) / kFp4Slab;
     const int n0 = n_blk * bn, off = n0 % 64, window = sp.window;
     // offsets in a stage: A, B, A's scales, B's scales
-    const uint32_t b_at = kFp4ABytes, as_at = b_at + (uint32_t)window * 128u, bs_at = as_at + fp4_slab_scales(NV);
+    const uint32_t b_at = sp.a_bytes, as_at = b_at + (uint32_t)window * 128u, bs_at = as_at + fp4_slab_scales(NV);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
@@ -117,7 +122,7 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             const uint8_t* as = sp.a_block_scales + (int64_t)m_blk * slabs * fp4_slab_scales(NV);
             const uint8_t* bs = sp.b_block_scales + (int64_t)row_tile * slabs * fp4_slab_scales(NV);
             const int64_t second = (int64_t)slabs * fp4_slab_scales(NV);
-            const uint32_t bytes = sp.value_bytes + (1 + b_tiles) * fp4_slab_scales(NV);
+            const uint32_t bytes = sp.a_bytes + bn * 128 + (1 + b_tiles) * fp4_slab_scales(NV);
             for (int i = 0; i < slabs; ++i) {
                 if (!ptx::mbar_wait(empty_bar(s), ph, abort_flag)) { ok = false; break; }
                 ptx::mbar_arrive_expect_tx(full_bar(s), bytes);
@@ -272,20 +277,20 @@ static int launch_fp4_tiles(bool nv, bool gelu, bool f16, const Fp4Operand& a, c
     if (int rc = make_values_map(&tb, b.values, p.N, p.K, bn, op)) return rc;
     sp.a_block_scales = static_cast<const uint8_t*>(a.block_scales);
     sp.b_block_scales = static_cast<const uint8_t*>(b.block_scales);
-    sp.value_bytes = (a_rows + bn) * 128;
-    sp.stage_bytes = ((kGemmBM + sp.window) * 128 + fp4_slab_scales(nv) * (1 + sp.b_tiles) + 1023) / 1024 * 1024;
+    sp.a_bytes = a_rows * 128;
+    sp.stage_bytes = (sp.a_bytes + sp.window * 128 + fp4_slab_scales(nv) * (1 + sp.b_tiles) + 1023) / 1024 * 1024;
     const int64_t m_tiles = (p.M + kGemmBM - 1) / kGemmBM;
     sp.n_tiles = (p.N + bn - 1) / bn;
     Q8K_REQUIRE(m_tiles * sp.n_tiles <= 0x7fffffffLL, Q8K_ERR_TOO_LARGE, "%s: too many tiles", op);
     // TMEM's 512 columns hold the accumulator and every stage's scales of A and of B
-    int stages = 208 * 1024 / sp.stage_bytes;
+    int stages = (208 * 1024 - kFp4ABytes + sp.a_bytes) / sp.stage_bytes;
     const int by_tmem = (512 - sp.window) / (4 * fp4_slab_tiles(nv) * (1 + sp.b_tiles));
     if (stages > by_tmem) stages = by_tmem;
     const int slabs = fp4_slabs(p.K);
     if (stages > slabs) stages = slabs;
     if (stages > kFp4MaxStages) stages = kFp4MaxStages;
     sp.stages = stages;
-    const int smem = stages * sp.stage_bytes + Fp4Smem::kTotal + 1024;
+    const int smem = stages * sp.stage_bytes + (Fp4Smem::kTotal > kFp4ABytes - sp.a_bytes ? Fp4Smem::kTotal : kFp4ABytes - sp.a_bytes) + 1024;
     const unsigned grid = (unsigned)(m_tiles * sp.n_tiles);
 #define Q8K_FP4(NV)                                                                                      \
     do {                                                                                                 \
