@@ -573,5 +573,6 @@ extern "C" int q8k_fp4_linear(int format, const void* x, int x_dtype, const void
     uint8_t* blocks = values + scales_at;
     float* rows = nv ? reinterpret_cast<float*>(values + rows_at) : nullptr;
     if (int rc = q8k_fp4_quant(x, x_dtype, K, format, values, blocks, rows, M, K, stream)) return rc;
-    return q8k_fp4_mm(format, values, blocks, rows, w, w_block_scales, w_row_scales, bias, out, out_dtype, M, N, K, fuse_gelu, dev_status, stream);
+    return fp4_mm(format, values, blocks, rows, w, w_block_scales, w_row_scales, bias, out, out_dtype, M, N, K, fuse_gelu, dev_status, true,
+                  (cudaStream_t)stream);
 }

@@ -74,4 +74,9 @@ struct Fp4Operand {
     const float* row_scales;                 // nvfp4 only
 };
 
+// q8k_fp4_mm.  b_ahead: the kernel before it on the stream is the quantizer of A, which has waited for everything before it, so B can be loaded at once.
+int fp4_mm(int format, const void* a, const void* a_block_scales, const float* a_row_scales, const void* b, const void* b_block_scales,
+           const float* b_row_scales, const float* bias, void* out, int out_dtype, int M, int N, int K, int fuse_gelu, int* dev_status, bool b_ahead,
+           cudaStream_t st);
+
 }  // namespace q8k

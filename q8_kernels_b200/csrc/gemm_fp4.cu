@@ -13,7 +13,8 @@
 // Bound by the latency of one short main loop, a few slabs to each of few CTAs.  The tensor core's own copy of scales (tcgen05.cp, 512 bytes)
 // stands in the pipe of the MMAs for some 65 clocks, and a slab of nvfp4 needs eight of them.  Registers bring
 // the scales past that pipe, every stage to its own columns.  Measured with M = 1 on cold operands, tcgen05.cp -> registers, us:
-//   nvfp4 N x K = 2048 x 2048 5.2 -> 4.2, 2048 x 8192 15.2 -> 10.2, 8192 x 2048 6.4 -> 5.9; mxfp4 4.3 -> 4.1, 10.9 -> 9.3, 5.7 -> 5.2.
+//   nvfp4 N x K = 2048 x 2048 5.2 -> 4.2, 2048 x 8192 15.2 -> 10.2, 8192 x 2048 6.4 -> 5.9; mxfp4 4.3 -> 4.1, 10.9 -> 9.3, 5.7 -> 5.2.  All that the epilogue needs from global
+// memory, the status word too, is read beside the main loop, which before waited for it (5.9 -> 5.4, 5.2 -> 4.9).
 //
 // What is left of a slab are 470 clocks of its four MMAs, of which one with 64 columns takes hardly less than one of 256, and 360 of its four copies'
 // issue.  (Not kept: loads by two or three warps, no change.)  With fewer than 128 rows a stage holds those rows only, and there are
@@ -46,6 +47,7 @@ struct Fp4TileParams {
     int window;                              // columns of the MMA: 64 where bn is 32, see above
     int b_tiles;                             // 128-row tiles of B's scales that a window touches: 1 or 2
     int stages, stage_bytes, a_bytes;        // a_bytes: of A's values in a stage
+    int b_ahead;                             // the kernel before on the stream has nothing to do with B and waited for what came before it
     const uint8_t *a_block_scales, *b_block_scales;
 };
 
@@ -70,8 +72,6 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + L::kAbortOffset);
     float* col_scale_smem = reinterpret_cast<float*>(tail + L::kColScaleOffset);
     float* bias_smem = reinterpret_cast<float*>(tail + L::kBiasOffset);
-    __shared__ int prior_failure;
-
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const int n_blk = blockIdx.x % sp.n_tiles;
@@ -94,18 +94,36 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         ptx::prefetch_tensormap(&tmap_a);
         ptx::prefetch_tensormap(&tmap_b);
     }
+
+    // ---- warp 0's loads.  A slab's scales of one row tile lie together; behind B's last row tile there are none.
+    const int row_tile = n0 / 128, b_tiles = min(nt, (p.N + 127) / 128 - row_tile);
+    const uint8_t* bs = sp.b_block_scales + (int64_t)row_tile * slabs * fp4_slab_scales(NV);   // (stepped: addresses from i cost 60 clocks a slab)
+    auto load_b = [&](int i, int s) {
+        const uint32_t dst = smem_base + s * sp.stage_bytes;
+        ptx::mbar_arrive_expect_tx(full_bar(s), sp.a_bytes + bn * 128 + (1 + b_tiles) * fp4_slab_scales(NV));
+        ptx::tma_load_2d(dst + b_at + (uint32_t)off * 128u, &tmap_b, full_bar(s), i * 128, n0);
+        ptx::bulk_load(dst + bs_at, bs, fp4_slab_scales(NV), full_bar(s));
+        if (b_tiles > 1) ptx::bulk_load(dst + bs_at + fp4_slab_scales(NV), bs + (int64_t)slabs * fp4_slab_scales(NV), fp4_slab_scales(NV), full_bar(s));
+        bs += fp4_slab_scales(NV);
+    };
+    const int ahead = sp.b_ahead ? stages : 0;                 // (stages <= slabs)
+    if (warp == 0) {
+        __syncwarp();                                          // the barriers exist
+        if (ptx::elect_one())
+            for (int i = 0; i < ahead; ++i) load_b(i, i);
+        bs = sp.b_block_scales + ((int64_t)row_tile * slabs + ahead) * fp4_slab_scales(NV);
+    }
     if (warp == 1) {
         ptx::tmem_alloc<512>(ptx::smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)));
         ptx::tmem_relinquish_alloc_permit();
     }
     pdl_wait();
-    if (threadIdx.x == 0) prior_failure = p.status != nullptr ? *reinterpret_cast<volatile int*>(p.status) : 0;
     ptx::tcgen05_fence_before_sync();
     __syncthreads();
     ptx::tcgen05_fence_after_sync();
     pdl_release();
     const uint32_t tmem_base = *tmem_ptr_smem;
-    bool ok = prior_failure == 0;
+    bool ok = true;
 
     const int quarter = warp & 3;
     const int half = (warp - 2) >> 2;
@@ -114,33 +132,24 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     auto scales_of = [&](int s) { return tmem_base + window + s * scale_cols; };
 
     if (warp == 0) {
-        if (ok && ptx::elect_one()) {
+        if (ptx::elect_one()) {
             int s = 0;
             uint32_t ph = 1;                                   // empty_bar phase to wait for: the first round passes
-            // a slab's scales of one row tile lie together; behind B's last row tile there are none
-            const int row_tile = n0 / 128, b_tiles = min(nt, (p.N + 127) / 128 - row_tile);
             const uint8_t* as = sp.a_block_scales + (int64_t)m_blk * slabs * fp4_slab_scales(NV);
-            const uint8_t* bs = sp.b_block_scales + (int64_t)row_tile * slabs * fp4_slab_scales(NV);
-            const int64_t second = (int64_t)slabs * fp4_slab_scales(NV);
-            const uint32_t bytes = sp.a_bytes + bn * 128 + (1 + b_tiles) * fp4_slab_scales(NV);
             for (int i = 0; i < slabs; ++i) {
                 if (!ptx::mbar_wait(empty_bar(s), ph, abort_flag)) { ok = false; break; }
-                ptx::mbar_arrive_expect_tx(full_bar(s), bytes);
+                if (i >= ahead) load_b(i, s);
                 const uint32_t dst = smem_base + s * sp.stage_bytes;
                 ptx::tma_load_2d(dst, &tmap_a, full_bar(s), i * 128, m_blk * kGemmBM);
-                ptx::tma_load_2d(dst + b_at + (uint32_t)off * 128u, &tmap_b, full_bar(s), i * 128, n0);
                 ptx::bulk_load(dst + as_at, as, fp4_slab_scales(NV), full_bar(s));
-                ptx::bulk_load(dst + bs_at, bs, fp4_slab_scales(NV), full_bar(s));
-                if (b_tiles > 1) ptx::bulk_load(dst + bs_at + fp4_slab_scales(NV), bs + second, fp4_slab_scales(NV), full_bar(s));
-                as += fp4_slab_scales(NV);                     // (stepped: the addresses from i cost 60 clocks a slab)
-                bs += fp4_slab_scales(NV);
+                as += fp4_slab_scales(NV);
                 if (++s == stages) { s = 0; ph ^= 1u; }
             }
             if (!ok && p.status != nullptr) atomicExch(p.status, Q8K_STATUS_TIMEOUT | (31 << 8));
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (ok && ptx::elect_one()) {
+        if (ptx::elect_one()) {
             int s = 0;
             uint32_t ph = 0;
             const uint32_t shift = n0 % 128 >= 64 ? 2u : 0u;   // the window may begin in the middle of a tile of scales
@@ -165,7 +174,14 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             else if (p.status != nullptr) atomicExch(p.status, Q8K_STATUS_TIMEOUT | (32 << 8));
         }
         __syncwarp();
-    } else if (ok) {
+    } else {
+        // what the epilogue needs is on its way.  A launch that follows a failed one on the same status word stores nothing.
+        const int prior_failure = p.status != nullptr ? *reinterpret_cast<volatile int*>(p.status) : 0;
+        const int row = m_blk * kGemmBM + quarter * 32 + lane, column = threadIdx.x - 64;
+        const bool row_ok = row < p.M, column_ok = column < bn && n0 + column < p.N;
+        const float sa = !row_ok ? 0.f : p.a_scales != nullptr ? p.a_scales[row] : 1.f;
+        const float sb = !column_ok ? 0.f : p.b_scales != nullptr ? p.b_scales[n0 + column] : 1.f;
+        const float bias = column_ok && p.bias != nullptr ? p.bias[n0 + column] : 0.f;
         // ------------------------------------------------ scales: warps 2-5 those in even stages, 6-9 those in odd ones; lane l of every lane
         // quarter holds the 16 bytes of rows l, l + 32, l + 64, l + 96 of a tile
         {
@@ -201,21 +217,16 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             }
         }
         // ------------------------------------------------ epilogue
-        for (int c = threadIdx.x - 64; c < bn; c += kGemmEpilogueThreads) {
-            const int n = n0 + c;
-            const bool in = n < p.N;
-            col_scale_smem[c] = !in ? 0.f : p.b_scales != nullptr ? p.b_scales[n] : 1.f;
-            bias_smem[c] = (in && p.bias != nullptr) ? p.bias[n] : 0.f;
+        if (column < bn) {                                     // bn <= 192, 256 threads
+            col_scale_smem[column] = sb;
+            bias_smem[column] = bias;
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        const int row = m_blk * kGemmBM + quarter * 32 + lane;
-        const bool row_ok = row < p.M;
-        const float sa = !row_ok ? 0.f : p.a_scales != nullptr ? p.a_scales[row] : 1.f;
         if (ok) ok = ptx::mbar_wait(acc_bar, 0, abort_flag);
         ok = __all_sync(0xffffffffu, ok);                      // keep the warp convergent for tcgen05.ld
         ptx::tcgen05_fence_after_sync();
         if (!ok && p.status != nullptr && threadIdx.x == 64) atomicExch(p.status, Q8K_STATUS_TIMEOUT | (33 << 8));
-        if (ok) {
+        if (ok && prior_failure == 0) {
             const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16);
             uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + (int64_t)row * p.N + n0;
 #pragma unroll 1
@@ -264,11 +275,12 @@ static int launch_fp4_as(const CUtensorMap& ta, const CUtensorMap& tb, const Fp4
 }
 
 static int launch_fp4_tiles(bool nv, bool gelu, bool f16, const Fp4Operand& a, const Fp4Operand& b, const Fp4GemmParams& p, int bn,
-                            cudaStream_t st) {
+                            bool b_ahead, cudaStream_t st) {
     const char* op = "fp4_mm";
     Fp4TileParams sp;
     sp.g = p;
     sp.bn = bn;
+    sp.b_ahead = b_ahead;
     sp.window = bn == 32 ? 64 : bn;
     sp.b_tiles = bn == 192 ? 2 : 1;
     const int a_rows = split_a_rows(p.M);
@@ -317,12 +329,9 @@ static int fp4_tile_columns(int M, int N) {
     return 0;
 }
 
-}  // namespace q8k
-
-extern "C" int q8k_fp4_mm(int format, const void* a, const void* a_block_scales, const float* a_row_scales, const void* b, const void* b_block_scales,
-                          const float* b_row_scales, const float* bias, void* out, int out_dtype, int M, int N, int K, int fuse_gelu,
-                          int* dev_status, void* stream) {
-    using namespace q8k;
+int fp4_mm(int format, const void* a, const void* a_block_scales, const float* a_row_scales, const void* b, const void* b_block_scales,
+           const float* b_row_scales, const float* bias, void* out, int out_dtype, int M, int N, int K, int fuse_gelu, int* dev_status, bool b_ahead,
+           cudaStream_t st) {
     const char* op = "fp4_mm";
     Q8K_REQUIRE(format == Q8K_FP4_MX || format == Q8K_FP4_NV, Q8K_ERR_UNSUPPORTED, "%s: format %d is unknown", op, format);
     const bool nv = format == Q8K_FP4_NV;
@@ -345,9 +354,18 @@ extern "C" int q8k_fp4_mm(int format, const void* a, const void* a_block_scales,
     const Fp4Operand oa = {a, a_block_scales, a_row_scales}, ob = {b, b_block_scales, b_row_scales};
     int bn = fp4_tile_columns(M, N);
     if (bn == 0) {
-        const int rc = launch_fp4_pair(nv, fuse_gelu != 0, out_dtype == Q8K_DT_F16, oa, ob, p, (cudaStream_t)stream);
+        const int rc = launch_fp4_pair(nv, fuse_gelu != 0, out_dtype == Q8K_DT_F16, oa, ob, p, st);
         if (rc != Q8K_ERR_UNSUPPORTED) return rc;
         bn = 128;                                              // a device that holds few pairs at once
     }
-    return launch_fp4_tiles(nv, fuse_gelu != 0, out_dtype == Q8K_DT_F16, oa, ob, p, bn, (cudaStream_t)stream);
+    return launch_fp4_tiles(nv, fuse_gelu != 0, out_dtype == Q8K_DT_F16, oa, ob, p, bn, b_ahead, st);
+}
+
+}  // namespace q8k
+
+extern "C" int q8k_fp4_mm(int format, const void* a, const void* a_block_scales, const float* a_row_scales, const void* b, const void* b_block_scales,
+                          const float* b_row_scales, const float* bias, void* out, int out_dtype, int M, int N, int K, int fuse_gelu,
+                          int* dev_status, void* stream) {
+    return q8k::fp4_mm(format, a, a_block_scales, a_row_scales, b, b_block_scales, b_row_scales, bias, out, out_dtype, M, N, K, fuse_gelu, dev_status, false,
+                       (cudaStream_t)stream);
 }
