@@ -447,8 +447,9 @@ Q8K_API int q8k_fp4_dequant(const void* values, const void* block_scales, const 
 Q8K_API int q8k_fp4_mm(int format, const void* a, const void* a_block_scales, const float* a_row_scales, const void* b, const void* b_block_scales,
                const float* b_row_scales, const float* bias, void* out, int out_dtype, int M, int N, int K, int fuse_gelu,
                int* dev_status, void* stream);
-/* q8k_fp4_quant of x (dense) and q8k_fp4_mm in one call, over a workspace of q8k_fp4_linear_workspace_bytes (256-byte aligned).    */
-Q8K_API size_t q8k_fp4_linear_workspace_bytes(int format, int M, int K);
+/* q8k_fp4_quant of x (dense) and q8k_fp4_mm in one call, over a workspace of q8k_fp4_linear_workspace_bytes (256-byte aligned).  A few short rows
+ * are quantised in the product's own launch: no bytes are needed then, and the workspace may be null.                                        */
+Q8K_API size_t q8k_fp4_linear_workspace_bytes(int format, int M, int N, int K);
 Q8K_API int q8k_fp4_linear(int format, const void* x, int x_dtype, const void* w, const void* w_block_scales, const float* w_row_scales,
                    const float* bias, void* out, int out_dtype, int M, int N, int K, int fuse_gelu, void* workspace,
                    size_t workspace_bytes, int* dev_status, void* stream);

@@ -7,99 +7,9 @@
 // A block of mxfp4 with NaN or an infinity has NaN as its scale, a row of nvfp4 NaN or infinity as its row scale: the row's products are NaN.
 
 #include <type_traits>
-#include "fp4.cuh"
+#include "fp4_quant.cuh"
 
 namespace q8k {
-
-constexpr int kFp4Unit = 16;                                   // values of a thread at a time: 32 bytes
-
-// |max| of two 16-bit values or of one fp32 value; NaN wins.
-template <typename T> struct Fp4In;
-template <> struct Fp4In<__nv_bfloat16> {
-    static __device__ __forceinline__ float absmax(const uint4 (&r)[2]) {
-        __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&r[0].x));
-        const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y, r[1].z, r[1].w};
-#pragma unroll
-        for (int i = 1; i < 8; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])));
-        const float2 f = __bfloat1622float2(m);
-        return max_nan(f.x, f.y);
-    }
-    static __device__ __forceinline__ void widen(const uint4& r, float (&v)[8]) {
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    }
-};
-template <> struct Fp4In<__half> {
-    static __device__ __forceinline__ float absmax(const uint4 (&r)[2]) {
-        __half2 m = __habs2(*reinterpret_cast<const __half2*>(&r[0].x));
-        const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y, r[1].z, r[1].w};
-#pragma unroll
-        for (int i = 1; i < 8; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&w[i])));
-        const float2 f = __half22float2(m);
-        return max_nan(f.x, f.y);
-    }
-    static __device__ __forceinline__ void widen(const uint4& r, float (&v)[8]) {
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
-        }
-    }
-};
-
-__device__ __forceinline__ float fp4_finite(float factor) { return fminf(factor, 3.402823466e38f); }
-
-// A unit's values times `factor`, as 8 bytes.
-template <typename T> __device__ __forceinline__ uint2 fp4_pack(const uint4 (&r)[2], float factor) {
-    uint32_t w[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        float v[8];
-        Fp4In<T>::widen(r[h], v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], factor);
-        w[h] = float8_to_e2m1(v);
-    }
-    return make_uint2(w[0], w[1]);
-}
-
-// A row's scale and the factor on its blocks' absmax (nvfp4), from the row's absmax.
-__device__ __forceinline__ void fp4_row_factors(float top, float& g, float& rs) {
-    g = top > 0.f ? fp4_finite(__fdiv_rn(448.0f, top)) : top;  // 0 and NaN stay what they are
-    rs = __fdiv_rn(top, 2688.0f);
-}
-// The scale byte of a unit's block and the factor on its values.  mxfp4: a block of 32 is the units of two neighbouring lanes.
-template <bool NV> __device__ __forceinline__ uint8_t fp4_block_scale(float a, float g, float rs, float& factor) {
-    if constexpr (NV) {
-        const uint8_t scale = float_to_e4m3_sat(__fmul_rn(a, g));
-        const float s = e4m3_to_float(scale);
-        factor = s == 0.f ? 0.f : fp4_finite(__fdiv_rn(1.0f, __fmul_rn(s, rs)));
-        return scale;
-    } else {
-        const float both = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
-        const int field = (int)(__float_as_uint(both) >> 23);  // (no sign)
-        const int e = field == 255 ? 255 : field > 2 ? field - 2 : 0;
-        factor = __uint_as_float((uint32_t)(254 - (e == 255 ? 254 : e)) << 23);     // 2^-e; any for NaN
-        return (uint8_t)e;
-    }
-}
-template <typename Tin, int UNITS>
-__device__ __forceinline__ void fp4_load(const Tin* __restrict__ row, int t, int threads, int units, bool here, uint4 (&r)[UNITS][2]) {
-#pragma unroll
-    for (int i = 0; i < UNITS; ++i) {
-        const int u = t + i * threads;
-        const uint4* p = reinterpret_cast<const uint4*>(row + u * kFp4Unit);
-        const bool in = here && u < units;
-        r[i][0] = in ? p[0] : make_uint4(0, 0, 0, 0);
-        r[i][1] = in ? p[1] : make_uint4(0, 0, 0, 0);
-    }
-}
 
 // Few rows: a CTA for every row, UNITS units a thread.  The row's scales beyond K, up to its last slab, become 0.
 template <typename Tin, bool NV, int UNITS>
@@ -548,8 +458,9 @@ static void fp4_linear_parts(bool nv, int M, int K, size_t& scales_at, size_t& r
     bytes = rows_at + (nv ? (size_t)M * sizeof(float) : 0);
 }
 
-extern "C" size_t q8k_fp4_linear_workspace_bytes(int format, int M, int K) {
-    if (M <= 0 || K <= 0 || (format != Q8K_FP4_MX && format != Q8K_FP4_NV)) return 0;
+extern "C" size_t q8k_fp4_linear_workspace_bytes(int format, int M, int N, int K) {
+    if (M <= 0 || N <= 0 || K <= 0 || (format != Q8K_FP4_MX && format != Q8K_FP4_NV)) return 0;
+    if (q8k::fp4_quantises_rows(M, N, K)) return 0;
     size_t scales_at, rows_at, bytes;
     fp4_linear_parts(format == Q8K_FP4_NV, M, K, scales_at, rows_at, bytes);
     return bytes;
@@ -564,6 +475,12 @@ extern "C" int q8k_fp4_linear(int format, const void* x, int x_dtype, const void
     const bool nv = format == Q8K_FP4_NV;
     Q8K_REQUIRE(N > 0 && N % 16 == 0, Q8K_ERR_INVALID_ARG, "%s: N=%d must be a positive multiple of 16", op, N);
     if (M == 0) return Q8K_OK;
+    if (fp4_quantises_rows(M, N, K)) {
+        Q8K_REQUIRE(x_dtype == Q8K_DT_BF16 || x_dtype == Q8K_DT_F16, Q8K_ERR_UNSUPPORTED, "%s: input dtype %d is not bf16 or fp16", op, x_dtype);
+        Q8K_REQUIRE(x != nullptr, Q8K_ERR_INVALID_ARG, "%s: null pointer", op);
+        return fp4_mm(format, nullptr, nullptr, nullptr, w, w_block_scales, w_row_scales, bias, out, out_dtype, M, N, K, fuse_gelu, dev_status, false, x,
+                      x_dtype == Q8K_DT_F16, (cudaStream_t)stream);
+    }
     Q8K_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 256 == 0, Q8K_ERR_INVALID_ARG,
                 "%s: the workspace must be 256-byte aligned", op);
     size_t scales_at, rows_at, need;
@@ -574,5 +491,5 @@ extern "C" int q8k_fp4_linear(int format, const void* x, int x_dtype, const void
     float* rows = nv ? reinterpret_cast<float*>(values + rows_at) : nullptr;
     if (int rc = q8k_fp4_quant(x, x_dtype, K, format, values, blocks, rows, M, K, stream)) return rc;
     return fp4_mm(format, values, blocks, rows, w, w_block_scales, w_row_scales, bias, out, out_dtype, M, N, K, fuse_gelu, dev_status, true,
-                  (cudaStream_t)stream);
+                  nullptr, false, (cudaStream_t)stream);
 }

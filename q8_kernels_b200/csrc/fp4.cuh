@@ -75,8 +75,10 @@ struct Fp4Operand {
 };
 
 // q8k_fp4_mm.  b_ahead: the kernel before it on the stream is the quantizer of A, which has waited for everything before it, so B can be loaded at once.
+// x: 16-bit rows for the product to quantise, in the place of a (null), where fp4_quantises_rows; else null.
 int fp4_mm(int format, const void* a, const void* a_block_scales, const float* a_row_scales, const void* b, const void* b_block_scales,
            const float* b_row_scales, const float* bias, void* out, int out_dtype, int M, int N, int K, int fuse_gelu, int* dev_status, bool b_ahead,
-           cudaStream_t st);
+           const void* x, bool x_f16, cudaStream_t st);
+bool fp4_quantises_rows(int M, int N, int K);
 
 }  // namespace q8k

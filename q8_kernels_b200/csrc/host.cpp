@@ -1331,11 +1331,12 @@ struct FP4Node : torch::autograd::Function<FP4Node> {
         at::DimVector shape(lead(a).begin(), lead(a).end());
         shape.push_back(nn);
         at::Tensor out = empty_like_dtype(shape, a, out_type);
-        const int64_t bytes = (int64_t)q8k_fp4_linear_workspace_bytes(format, (int)m, (int)k);
-        at::Tensor work = empty_like_dtype({bytes}, a, Dt::Byte);
+        const int64_t bytes = (int64_t)q8k_fp4_linear_workspace_bytes(format, (int)m, (int)nn, (int)k);
+        at::Tensor work;
+        if (bytes > 0) work = empty_like_dtype({bytes}, a, Dt::Byte);
         must(q8k_fp4_linear(format, a.const_data_ptr(), type_code(a.scalar_type()), b.const_data_ptr(), block.const_data_ptr(),
                             static_cast<const float*>(dense_ptr(row)), fptr(defined(bias)), out.data_ptr(), type_code(out_type), (int)m, (int)nn, (int)k,
-                            gelu, work.data_ptr(), (size_t)bytes, g_status[a.device().index()]->data_ptr<int>(), stream_of(a)), "fp4_linear");
+                            gelu, out_ptr(work), (size_t)bytes, g_status[a.device().index()]->data_ptr<int>(), stream_of(a)), "fp4_linear");
         return out;
     }
     static Variable forward(AutogradContext* ctx, const Variable& a, const Variable& b, const Maybe& bias, const Variable& block, const Maybe& row,

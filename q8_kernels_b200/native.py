@@ -1158,7 +1158,7 @@ def fp4_linear(x: torch.Tensor, w: torch.Tensor, w_scales, bias: Optional[torch.
     bias = None if bias is None else bias.contiguous()
     m = x.numel() // k
     out = torch.empty(x.shape[:-1] + (n,), dtype=out_type, device=dev)
-    work = torch.empty(lib.q8k_fp4_linear_workspace_bytes(FP4_FORMATS[fmt], m, k), dtype=torch.uint8, device=dev)
+    work = torch.empty(lib.q8k_fp4_linear_workspace_bytes(FP4_FORMATS[fmt], m, n, k), dtype=torch.uint8, device=dev)
     launch(dev, "fp4_linear", lib.q8k_fp4_linear, FP4_FORMATS[fmt], ptr(x), dt(x.dtype), ptr(w), ptr(block), ptr(row), ptr(bias), ptr(out),
            dt(out_type), m, n, k, int(bool(fuse_gelu)), ptr(work), work.numel(), ptr(_lib.status_word(dev)))
     return out

@@ -86,14 +86,19 @@ def test_refusals_of_the_c_entries():
 
     assert mm(fmt=9) == -2 and mm(a=None) == -1 and mm(a=buf + 8) == -1 and mm(rs=None) == -1 and mm(out=buf + 2) == -1 and mm(dtype=f32) == -2
     assert mm(n=24) == -1 and mm(k=48) == -1 and mm(m=-1) == -1 and mm(m=0) == 0
-    need = lib.q8k_fp4_linear_workspace_bytes(2, 4, 64)
-    assert need >= 4 * 32 + 2048 + 16 and lib.q8k_fp4_linear_workspace_bytes(2, 0, 64) == 0
+    need = lib.q8k_fp4_linear_workspace_bytes(2, 40, 32, 64)
+    assert need >= 40 * 32 + 2048 + 160 and lib.q8k_fp4_linear_workspace_bytes(2, 0, 32, 64) == 0
+    assert [lib.q8k_fp4_linear_workspace_bytes(1, m, n, k) == 0 for m, n, k in ((8, 32, 1024), (8, 32, 1056), (9, 32, 64), (1, 64, 8192), (1, 64, 8224),
+                                                                               (1, 28416, 64), (1, 28432, 64))] == [True, False, False, True, False, True, False]
 
-    def linear(x=buf, dtype=bf, out_dtype=f16, m=4, n=32, k=64, work=buf, size=need):
+    def linear(x=buf, dtype=bf, out_dtype=f16, m=40, n=32, k=64, work=buf, size=need):
         return lib.q8k_fp4_linear(2, x, dtype, buf, buf, buf, None, buf, out_dtype, m, n, k, 0, work, size, None, None)
 
     assert linear(x=None) == -1 and linear(dtype=f32) == -2 and linear(n=24) == -1 and linear(k=48) == -1
     assert linear(work=None) == -1 and linear(work=buf + 16) == -1 and linear(size=need - 1) == -3 and linear(m=0) == 0
+    # a few rows, without a workspace
+    for bad, rc in ((dict(x=None), -1), (dict(x=buf + 8), -1), (dict(dtype=f32), -2), (dict(out_dtype=f32), -2), (dict(n=24), -1), (dict(k=48), -1)):
+        assert linear(**{"m": 4, "work": None, "size": 0, **bad}) == rc, bad
     need = lib.q8k_fp4_weight_operand_workspace_bytes(32, 64)
     assert need > 0 and lib.q8k_fp4_weight_operand_workspace_bytes(0, 64) == 0
 

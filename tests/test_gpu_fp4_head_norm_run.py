@@ -352,3 +352,29 @@ def test_a_row_has_its_bits_in_every_call(fmt):
     few, fews = fp4_quantize(torch.zeros(48, 1056, device="cuda", dtype=BF16), fmt)
     assert (fp4_linear(x, few, bias[:48].contiguous(), None, fews) == bias[:48].to(BF16)).all()
     check_status()
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("t", [BF16, F16])
+@pytest.mark.parametrize("n,k", [(16, 32), (48, 96), (272, 2016), (2048, 2048), (9600, 544), (20480, 288), (64, 8192), (32, 8224)])
+def test_few_rows(fmt, t, n, k):
+    """Up to eight rows, which the product quantises itself where K and N allow: the bits of quantizer and product, rows that are not finite, tiny
+    and zero rows among them."""
+    from q8_kernels_b200 import check_status
+    from q8_kernels_b200.functional.fp4 import fp4_linear, fp4_quantize
+    w, ws = fp4_quantize((torch.randn(n, k, device="cuda") / 16).to(t), fmt)
+    bias = torch.randn(n, device="cuda")
+    x = torch.randn(9, k, device="cuda").to(t)
+    x[2] *= 1e-3
+    x[3] = 0
+    x[4, k // 2] = float("nan")
+    x[5, k - 1] = float("inf")
+    x[6] = torch.finfo(t).tiny
+    for m in range(1, 10):
+        for gelu in (False, True):
+            rows = x[9 - m:].contiguous()
+            y = fp4_linear(rows, w, bias, None, ws, gelu)
+            q, s = fp4_quantize(rows, fmt)
+            ref = fp4_linear(q, w, bias, s, ws, gelu, t)
+            assert torch.equal(torch.isnan(y), torch.isnan(ref)) and torch.equal(bits(y.nan_to_num()), bits(ref.nan_to_num()))
+    check_status()
