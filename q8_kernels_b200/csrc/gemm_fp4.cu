@@ -17,8 +17,10 @@
 //   nvfp4 N x K = 2048 x 2048 5.2 -> 4.2, 2048 x 8192 15.2 -> 10.2, 8192 x 2048 6.4 -> 5.9; mxfp4 4.3 -> 4.1, 10.9 -> 9.3, 5.7 -> 5.2.  All that the epilogue needs from global
 // memory, the status word too, is read beside the main loop, which before waited for it (5.9 -> 5.4, 5.2 -> 4.9).
 //
-// What is left of a slab are 470 clocks of its four MMAs, of which one with 64 columns takes hardly less than one of 256, and 360 of its four copies'
-// issue.  (Not kept: loads by two or three warps, no change.)  With fewer than 128 rows a stage holds those rows only, and there are
+// What is left of a slab are some 450 clocks of two threads, whose waits (70 clocks each even for what has come) and issues follow one another: two waits,
+// four MMAs and a commit of the one, a wait and four copies of the other; the MMAs themselves are not it (one in the place of four: 5 %).  Not kept:
+// loads by two or three warps (no change), accumulators of their own for the four MMAs (no change), stages of two slabs, which leave fewer of them
+// (16 x 2048 x 8192 9.9 -> 9.1 us, but 128 x 20480 x 4096 15.0 -> 17.6, 77 x 10240 x 4096 9.4 -> 10.3).  With fewer than 128 rows a stage holds those rows only, and there are
 // up to 16 of them (1 x 20480 x 4096 13.3 -> 12.3 us): the MMA's other rows are whatever follows in shared memory, other stages' values as they come
 // and go, and give rows that nobody reads.
 //
