@@ -408,10 +408,10 @@ static int launch_fp4_tiles(bool nv, bool gelu, bool f16, const Fp4Operand& a, c
 constexpr int kFp4FewValues = 8192;
 
 // The narrowest tile whose grid fits the device once, one CTA an SM; 0 where none does, for the CTA pairs.  Measured, us, nvfp4 / mxfp4 on cold
-// operands, a tile against the pairs: M, N, K = 1, 2048, 2048 with 32 columns 4.3 / 4.1 against 7.1 / 7.1; 1, 8192, 2048 with 64 6.0 / 5.2
-// against 8.6 / 8.5; 300, 4096, 4096 with 128 10.1 / 9.0 against 10.4 / 10.3; 300, 2048, 8192 with 64 11.4 / 10.4 against 14.9 / 14.7.
+// operands, a tile against the pairs: M, N, K = 16, 2048, 2048 with 32 columns 4.1 / 3.9 against 7.1 / 7.1; 16, 8192, 2048 with 64 5.3 / 4.8
+// against 8.6 / 8.5; 300, 4096, 4096 with 128 9.3 / 8.6 against 10.4 / 10.3; 300, 2048, 8192 with 64 11.0 / 10.2 against 14.9 / 14.7.
 // Two rounds of tiles cost twice: 300, 8192, 2048 with 128 12.2 / 10.6 against 8.5 / 8.4; 24576, 128, 2048 13.3 against 11.4.  192 columns are
-// worth it for one row tile only, of which the pairs leave half empty (128, 20480, 4096: 15.5 / 14.7 against 18.1 / 17.7); with more rows the
+// worth it for one row tile only, of which the pairs leave half empty (128, 20480, 4096: 15.0 / 14.6 against 18.1 / 17.7); with more rows the
 // pairs' grid fits once where theirs does, and is faster (256, 10240, 4096: 13.9 / 13.1 against 11.4 / 11.3).
 static int fp4_tile_columns(int M, int N) {
     const int64_t m_tiles = ((int64_t)M + kGemmBM - 1) / kGemmBM;

@@ -378,3 +378,26 @@ def test_few_rows(fmt, t, n, k):
             ref = fp4_linear(q, w, bias, s, ws, gelu, t)
             assert torch.equal(torch.isnan(y), torch.isnan(ref)) and torch.equal(bits(y.nan_to_num()), bits(ref.nan_to_num()))
     check_status()
+
+
+@pytest.mark.parametrize("m,n", [(1, 64), (40, 64), (3000, 2048)])
+def test_a_launch_after_a_failed_one_stores_nothing(m, n):
+    """On a status word that is not zero the output stays as it was, in every kernel of the products; the word stays, too."""
+    from q8_kernels_b200 import _lib
+    from q8_kernels_b200.functional.fp4 import fp4_quantize
+    w, (wb, wr) = fp4_quantize(torch.randn(n, 256, device="cuda").to(BF16))
+    x, out = torch.randn(m, 256, device="cuda").to(BF16), torch.full((m, n), 7.0, device="cuda", dtype=BF16)
+    status = torch.tensor([257], dtype=torch.int32, device="cuda")
+    work = torch.empty(max(1, _lib.lib.q8k_fp4_linear_workspace_bytes(2, m, n, 256)), dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def call():
+        rc = _lib.lib.q8k_fp4_linear(2, x.data_ptr(), _lib.DT_BF16, w.data_ptr(), wb.data_ptr(), wr.data_ptr(), None, out.data_ptr(), _lib.DT_BF16, m, n, 256, 0,
+                                     work.data_ptr(), work.numel(), status.data_ptr(), stream)
+        assert rc == 0, _lib.lib.q8k_last_error_detail()
+
+    call()
+    assert (out == 7).all() and status.item() == 257
+    status.zero_()
+    call()
+    assert (out != 7).any() and status.item() == 0
