@@ -401,3 +401,76 @@ def test_a_launch_after_a_failed_one_stores_nothing(m, n):
     status.zero_()
     call()
     assert (out != 7).any() and status.item() == 0
+
+
+@pytest.mark.parametrize("i", range(7))
+def test_gradients_of_any_strides(i):
+    """One number for all outputs, a gradient with its channels far apart, one that is a part of another, one at an odd address.
+
+    The 4-bit linear's has the bits of the dense one.  The others' kernels come in forms by the width of their accesses, which round a c - b s and
+    their sums in another order.  With G = max |g| and W = max |w| a rotation's sum has two terms of up to 1.25 G, so two forms differ by
+    2 * 4 u * 2.5 G before they round to the output's type, each by half a step.  Norms: t has two terms of G, |u| <= 2 G W, normed values are
+    at most 8 and their mean square is 1, so rstd u and x rstd^3 mean(u x) add up at most 9 * 2 G W rstd, over sums of 64: 2 * 80 u of that.
+    dw adds up N terms of 2 G times normed values: 2 * (N + 80) u * 2 G * N."""
+    call, tensors = calls()[i]
+    leaves = [t.clone().requires_grad_(True) for t in tensors]
+
+    def grads(g):
+        return torch.autograd.grad(call(*leaves), leaves, g)
+
+    y = call(*leaves)
+    dense = torch.randn(y.shape, device="cuda").to(y.dtype)
+    wide = torch.zeros(*y.shape[:-1], y.shape[-1] + 6, device="cuda", dtype=y.dtype)
+    wide[..., 3:-3] = dense
+    odd = torch.zeros(y.numel() + 1, device="cuda", dtype=y.dtype)[1:].view(y.shape).copy_(dense)
+    one = torch.full((), 0.5, device="cuda", dtype=y.dtype)
+    rstd = tensors[0].float().square().mean(-1).rsqrt().max().item() if i in (2, 3, 4) else 0.0
+    u = 2.0 ** -24
+    for g, same in ((one.expand(y.shape), one.expand(y.shape).contiguous()), (dense.transpose(-1, -2).contiguous().transpose(-1, -2), dense),
+                    (wide[..., 3:-3], dense), (odd, dense)):
+        top = same.float().abs().max().item()
+        for a, b in zip(grads(g), grads(same)):
+            if a.dim() == 1:
+                n = tensors[0].numel() // 64
+                slack, step = 2 * (n + 80) * u * 2 * top * n, 0.0
+            else:
+                weight = max((t.abs().max().item() for t in tensors if t.dim() == 1), default=1.0)
+                slack = 20 * u * top if i < 2 else 2 * 80 * u * 18 * top * weight * rstd if i < 5 else 0.0
+                step = torch.finfo(a.dtype).eps
+            if i >= 5:
+                assert torch.equal(bits(a), bits(b))
+            else:
+                assert ((a.double() - b.double()).abs() <= slack + step * (b.double().abs() + slack)).all(), (a.double() - b.double()).abs().max().item()
+
+
+def test_tokens_captured():
+    """A few rows in a graph, replayed on other contents, and two threads at once on streams of their own."""
+    import threading
+    from q8_kernels_b200.modules import FP4Linear
+    m = FP4Linear.from_linear(torch.nn.Linear(1024, 2048, device="cuda", dtype=BF16), "nvfp4")
+    x = torch.randn(3, 1024, device="cuda").to(BF16)
+    with torch.no_grad():
+        m(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = m(x, fuse_gelu=True)
+        x.copy_(torch.randn_like(x))
+        graph.replay()
+        assert torch.equal(bits(out), bits(m(x, fuse_gelu=True)))
+        refs, got = [m(x * k) for k in (1, 2)], [[], []]
+        torch.cuda.synchronize()
+
+        def work(k):
+            s = torch.cuda.Stream()
+            with torch.no_grad(), torch.cuda.stream(s):
+                for _ in range(200):
+                    got[k].append(m(x * (k + 1)))
+            s.synchronize()
+
+        threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    for ref, outs in zip(refs, got):
+        assert len(outs) == 200 and all(torch.equal(bits(y), bits(ref)) for y in outs)
