@@ -361,14 +361,18 @@ head_norm_kernel(const __grid_constant__ HeadNormParams p, const __grid_constant
             head_sum<LANES>(sums, lane, lanes, top);
             const float rstd = rsqrtf(fmaf(sums[0], inv_dim, p.eps));
             const float2 r2 = make_float2(rstd, rstd);
+            const bool ok = here && (LANES > 0 || h0 + r * sp.head_lanes < t.heads);
             if constexpr (BACK) {
+                // A head that is not there is zeros, and with eps = 0 its rstd an infinity: it adds 0 * 0, not 0 * inf.
+                const float there = ok ? rstd : 0.f;
+                const float2 there2 = make_float2(there, there);
                 const float c = -rstd * (rstd * rstd * (sums[1] * inv_dim));
                 const float2 c2 = make_float2(c, c);
 #pragma unroll
                 for (int run = 0; run < 2; ++run)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {              // (lanes and heads that are not there add zeros)
-                        acc[run][i] = ffma2(tx[run][i], r2, acc[run][i]);
+                    for (int i = 0; i < 4; ++i) {
+                        acc[run][i] = ffma2(tx[run][i], there2, acc[run][i]);
                         v[run][i] = ffma2(d[run][i], fmul2(w[run][i], r2), fmul2(v[run][i], c2));
                     }
             } else {
@@ -378,7 +382,6 @@ head_norm_kernel(const __grid_constant__ HeadNormParams p, const __grid_constant
                     for (int i = 0; i < 4; ++i) v[run][i] = fmul2(v[run][i], r2);
                 rotate(v);
             }
-            const bool ok = here && (LANES > 0 || h0 + r * sp.head_lanes < t.heads);
             alignas(16) T a[8], b[8];
             head_narrow<T>(v[0], a);
             head_narrow<T>(v[1], b);
