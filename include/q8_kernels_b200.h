@@ -454,8 +454,8 @@ Q8K_API int q8k_fp4_linear(int format, const void* x, int x_dtype, const void* w
                    const float* bias, void* out, int out_dtype, int M, int N, int K, int fuse_gelu, void* workspace,
                    size_t workspace_bytes, int* dev_status, void* stream);
 /* The weight operand of its backward product: w [N, K] (N a multiple of 16) de-quantised to fp32, transposed and quantised to e4m3 with one
- * scale per input channel (factor 448 / absmax): q [K, N], scales [K].  The workspace has q8k_fp4_weight_operand_workspace_bytes,
- * 16-byte aligned.                                                                                                               */
+ * scale per input channel (factor 448 / absmax, FLT_MAX at most): q [K, N], scales [K].  The workspace has
+ * q8k_fp4_weight_operand_workspace_bytes, 16-byte aligned.                                                                       */
 Q8K_API size_t q8k_fp4_weight_operand_workspace_bytes(int N, int K);
 Q8K_API int q8k_fp4_weight_operand(int format, const void* values, const void* block_scales, const float* row_scales, void* q, float* scales, int N,
                            int K, void* workspace, size_t workspace_bytes, void* stream);

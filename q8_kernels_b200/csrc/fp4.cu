@@ -199,7 +199,7 @@ template <typename Tout> static int launch_fp4_dequant(bool nv, const void* q, c
 
 // ------------------------------------------------------------------ weight operand of the backward product
 // w [N, K] de-quantised (value * block scale, exact, times the row's scale, rounded to fp32), transposed and quantised to e4m3 with one scale
-// per input channel, factor 448 / absmax as the 8-bit linears have it.  Two passes over the weight, which is small: the absmax of the
+// per input channel, factor 448 / absmax as the 8-bit linears have it, FLT_MAX at most.  Two passes over the weight, which is small: the absmax of the
 // columns over chunks of rows; then tiles of 128 x 128, whose CTAs take the maxima over the chunks, are turned in shared memory.
 constexpr int kF4Cols = 128;                 // columns of a CTA: 8 groups of 16
 constexpr int kF4Rows = 128;                 // rows of a turned tile
@@ -322,10 +322,12 @@ fp4_weight_turn_kernel(const uint8_t* __restrict__ w, const uint8_t* __restrict_
         __syncthreads();
         if (half == 0) {
             a = fmaxf(a, top[1][c]);
-            const float f = __fdiv_rn(448.0f, a);
+            // A column of zeros quantises to zeros, its scale is 0.  Below 448 / FLT_MAX the factor is FLT_MAX: an infinite one would make NaN
+            // of the column's zeros.
+            const float f = fp4_finite(__fdiv_rn(448.0f, a));
             // column group g's k-th four factors lie at (8 k + g) * 4: the eight groups of a warp read 128 bytes in a row
-            mul[(c & 15) / 4 * 32 + c / 16 * 4 + (c & 3)] = a == 0.f ? 0.f : f;      // a column of zeros quantises to zeros
-            if (blockIdx.y == 0 && cb + c < K) scales[cb + c] = __fdiv_rn(1.0f, f);
+            mul[(c & 15) / 4 * 32 + c / 16 * 4 + (c & 3)] = a == 0.f ? 0.f : f;
+            if (blockIdx.y == 0 && cb + c < K) scales[cb + c] = a == 0.f ? 0.f : __fdiv_rn(1.0f, f);
         }
     }
     __syncthreads();
