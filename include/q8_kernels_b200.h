@@ -453,7 +453,10 @@ Q8K_API size_t q8k_fp4_linear_workspace_bytes(int format, int M, int N, int K);
 Q8K_API int q8k_fp4_linear(int format, const void* x, int x_dtype, const void* w, const void* w_block_scales, const float* w_row_scales,
                    const float* bias, void* out, int out_dtype, int M, int N, int K, int fuse_gelu, void* workspace,
                    size_t workspace_bytes, int* dev_status, void* stream);
-/* The weight operand of its backward product: w [N, K] (N a multiple of 16) de-quantised to fp32, transposed and quantised to e4m3 with one
+/* The gradient operand of its backward product: grad bf16 or fp16 [rows, N] (dense, N a multiple of 16 up to 32768) to e4m3 with one scale a row:
+ * q8k_tokenwise_quant with a factor of FLT_MAX at most, so that the zeros of rows of very small values stay zeros.               */
+Q8K_API int q8k_fp4_backward_quant(const void* grad, int dtype, void* q, float* scales, int64_t rows, int N, void* stream);
+/* The weight operand: w [N, K] (N a multiple of 16) de-quantised to fp32, transposed and quantised to e4m3 with one
  * scale per input channel (factor 448 / absmax, FLT_MAX at most): q [K, N], scales [K].  The workspace has
  * q8k_fp4_weight_operand_workspace_bytes, 16-byte aligned.                                                                       */
 Q8K_API size_t q8k_fp4_weight_operand_workspace_bytes(int N, int K);

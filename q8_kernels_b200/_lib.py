@@ -109,6 +109,7 @@ SIGNATURES = {
     "q8k_fp4_mm": (_c_int, [_c_int] + [_c_ptr] * 8 + [_c_int] * 5 + [_c_ptr, _c_ptr]),
     "q8k_fp4_linear_workspace_bytes": (_c_size, [_c_int] * 4),
     "q8k_fp4_linear": (_c_int, [_c_int, _c_ptr, _c_int] + [_c_ptr] * 5 + [_c_int] * 5 + [_c_ptr, _c_size, _c_ptr, _c_ptr]),
+    "q8k_fp4_backward_quant": (_c_int, [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr]),
     "q8k_fp4_weight_operand_workspace_bytes": (_c_size, [_c_int, _c_int]),
     "q8k_fp4_weight_operand": (_c_int, [_c_int] + [_c_ptr] * 5 + [_c_int, _c_int, _c_ptr, _c_size, _c_ptr]),
     "q8k_gated_backward_quant": (_c_int, [_c_ptr] * 4 + [_c_int] * 3 + [_c_ptr]),

@@ -36,9 +36,10 @@ void set_error_detail(const char* fmt, ...);
         }                                                                          \
     } while (0)
 
-// q8k_tokenwise_quant / q8k_hadamard_quant under another name `op`; GATED: with the gated projection's factor and maximum (see quant_factor,
-// max_nan)
-template <bool GATED>
+// q8k_tokenwise_quant / q8k_hadamard_quant under another name `op`; GATED, kRowsGated: with the gated projection's factor and maximum (see
+// quant_factor, max_nan); kRowsFinite: with a factor of FLT_MAX at most
+enum RowsQuant { kRowsLinear, kRowsGated, kRowsFinite };
+template <RowsQuant KIND>
 int tokenwise_quant_as(const char* op, const void* x, int x_dtype, void* q, int q_dtype, float* scales, int64_t rows, int dim,
                        int64_t x_row_stride, cudaStream_t st);
 template <bool GATED>

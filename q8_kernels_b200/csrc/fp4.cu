@@ -453,6 +453,13 @@ extern "C" int q8k_fp4_weight_operand(int format, const void* values, const void
               : launch_fp4_weight<false>(values, block_scales, row_scales, q, scales, (float*)workspace, N, K, st);
 }
 
+extern "C" int q8k_fp4_backward_quant(const void* grad, int dtype, void* q, float* scales, int64_t rows, int N, void* stream) {
+    using namespace q8k;
+    const char* op = "fp4_backward_quant";
+    Q8K_REQUIRE(dtype == Q8K_DT_BF16 || dtype == Q8K_DT_F16, Q8K_ERR_UNSUPPORTED, "%s: gradient dtype %d is not bf16 or fp16", op, dtype);
+    return tokenwise_quant_as<kRowsFinite>(op, grad, dtype, q, Q8K_DT_E4M3, scales, rows, N, N, (cudaStream_t)stream);
+}
+
 // Where the parts of the quantised activation lie in the workspace of q8k_fp4_linear.
 static void fp4_linear_parts(bool nv, int M, int K, size_t& scales_at, size_t& rows_at, size_t& bytes) {
     scales_at = ((size_t)M * (size_t)(K / 2) + 255) / 256 * 256;

@@ -1369,8 +1369,7 @@ struct FP4Node : torch::autograd::Function<FP4Node> {
                 at::Tensor scratch = empty_like_dtype({at_work + work_bytes}, g, Dt::Byte);
                 uint8_t* s = static_cast<uint8_t*>(scratch.data_ptr());
                 float *gs = reinterpret_cast<float*>(s + at_gs), *ws = reinterpret_cast<float*>(s + at_ws);
-                must_backward(q8k_tokenwise_quant(g.const_data_ptr(), type_code(g.scalar_type()), s, Q8K_DT_E4M3, gs, m, (int)nn, nn, st),
-                              "tokenwise_quant");
+                must_backward(q8k_fp4_backward_quant(g.const_data_ptr(), type_code(g.scalar_type()), s, gs, m, (int)nn, st), "fp4_backward_quant");
                 must_backward(q8k_fp4_weight_operand(row.defined() ? Q8K_FP4_NV : Q8K_FP4_MX, b.const_data_ptr(), block.const_data_ptr(),
                                                      static_cast<const float*>(dense_ptr(row)), s + at_w, ws, (int)nn, (int)k, s + at_work,
                                                      (size_t)work_bytes, st), "fp4_weight_operand");

@@ -51,12 +51,14 @@ __device__ __forceinline__ float block_reduce_sum(float v, float* smem) {
 
 // ------------------------------------------------------------------ quantizer
 // Semantics of tokenwise_quantization_kernel
-// (csrc/quantizer/tokenwise_quant_cuda.cu:115-148) with IEEE arithmetic.  GATED: the gated projection's factor and maximum (quant_factor,
-// max_nan).
-template <typename Tin, typename Tout, int ITEMS, int T, bool GATED>
+// (csrc/quantizer/tokenwise_quant_cuda.cu:115-148) with IEEE arithmetic.  kRowsGated: the gated projection's factor and maximum (quant_factor,
+// max_nan).  kRowsFinite: rows whose absmax is positive and below qmax / FLT_MAX have FLT_MAX as their factor; an infinite one, which the
+// reference's definition gives them, makes NaN of a row's zeros.
+template <typename Tin, typename Tout, int ITEMS, int T, RowsQuant KIND>
 __global__ void __launch_bounds__(T)
 tokenwise_quant_kernel(const Tin* __restrict__ x, Tout* __restrict__ q, float* __restrict__ scales,
                        int dim, int64_t x_row_stride) {
+    constexpr bool GATED = KIND == kRowsGated;
     __shared__ float red[32];
     pdl_wait();
     pdl_release();
@@ -79,8 +81,9 @@ tokenwise_quant_kernel(const Tin* __restrict__ x, Tout* __restrict__ q, float* _
 
     constexpr bool kInt8 = sizeof(Tout) == 1 && !__is_same(Tout, e4m3_t);
     const float qmax = kInt8 ? 127.0f : 448.0f;
-    const float scale = quant_factor<GATED>(qmax, amax);   // +inf for an all-zero row
     const bool zero_row = amax == 0.f;
+    float scale = quant_factor<GATED>(qmax, amax);         // +inf for an all-zero row
+    if (KIND == kRowsFinite && !zero_row) scale = fminf(scale, 3.402823466e38f);
     const float mul = zero_row ? 0.f : scale;
     // (With a select on every product, as the linears' rows have it, nvcc 12.9 left bytes other than 0 in gated rows of zeros.)
     auto scaled = [&](float x) { return GATED ? __fmul_rn(x, mul) : zero_row ? 0.f : __fmul_rn(x, scale); };
@@ -439,12 +442,12 @@ rms_norm_backward_kernel(const Ty* __restrict__ y, const float* __restrict__ rrm
 }
 
 // ------------------------------------------------------------------ launch helpers
-template <typename Tin, typename Tout, bool GATED>
+template <typename Tin, typename Tout, RowsQuant KIND>
 static int launch_quant(const char* op, const void* x, void* q, float* scales, int64_t rows, int dim,
                         int64_t stride, cudaStream_t st) {
     const int items = dim / kItem;
 #define Q8K_Q_LAUNCH(ITEMS, T)                                                                  \
-    Q8K_CUDA_OK(launch_dependent(tokenwise_quant_kernel<Tin, Tout, ITEMS, T, GATED>, (unsigned)rows, T, 0, st, 1,     \
+    Q8K_CUDA_OK(launch_dependent(tokenwise_quant_kernel<Tin, Tout, ITEMS, T, KIND>, (unsigned)rows, T, 0, st, 1,      \
                                  (const Tin*)x, (Tout*)q, scales, dim, stride))
     if (items <= 32)        Q8K_Q_LAUNCH(1, 32);
     else if (items <= 128)  Q8K_Q_LAUNCH(1, 128);
@@ -491,7 +494,7 @@ static int check_rows_dim(const char* op, int64_t rows, int dim, int multiple) {
 using namespace q8k;
 
 namespace q8k {
-template <bool GATED>
+template <RowsQuant KIND>
 int tokenwise_quant_as(const char* op, const void* x, int x_dtype, void* q, int q_dtype, float* scales, int64_t rows, int dim,
                        int64_t x_row_stride, cudaStream_t st) {
     if (int rc = check_rows_dim(op, rows, dim, 16)) return rc;
@@ -503,24 +506,31 @@ int tokenwise_quant_as(const char* op, const void* x, int x_dtype, void* q, int 
     Q8K_REQUIRE(q_dtype == Q8K_DT_I8 || q_dtype == Q8K_DT_E4M3, Q8K_ERR_UNSUPPORTED,
                 "%s: output dtype %d is not int8 or e4m3", op, q_dtype);
 #define Q8K_QD(TIN)                                                                              \
-    return q_dtype == Q8K_DT_I8 ? launch_quant<TIN, int8_t, GATED>(op, x, q, scales, rows, dim, x_row_stride, st) \
-                                : launch_quant<TIN, e4m3_t, GATED>(op, x, q, scales, rows, dim, x_row_stride, st)
-    if constexpr (!GATED) {                                    // (the gated projection's rows are bf16 or e4m3)
-        if (x_dtype == Q8K_DT_F32) Q8K_QD(float);
-        if (x_dtype == Q8K_DT_F16) Q8K_QD(__half);
+    return q_dtype == Q8K_DT_I8 ? launch_quant<TIN, int8_t, KIND>(op, x, q, scales, rows, dim, x_row_stride, st) \
+                                : launch_quant<TIN, e4m3_t, KIND>(op, x, q, scales, rows, dim, x_row_stride, st)
+    if constexpr (KIND == kRowsFinite) {                       // (a gradient of 16 bits, to e4m3)
+        if (x_dtype == Q8K_DT_BF16 && q_dtype == Q8K_DT_E4M3)
+            return launch_quant<__nv_bfloat16, e4m3_t, KIND>(op, x, q, scales, rows, dim, x_row_stride, st);
+        if (x_dtype == Q8K_DT_F16 && q_dtype == Q8K_DT_E4M3) return launch_quant<__half, e4m3_t, KIND>(op, x, q, scales, rows, dim, x_row_stride, st);
+    } else {
+        if constexpr (KIND == kRowsLinear) {                   // (the gated projection's rows are bf16 or e4m3)
+            if (x_dtype == Q8K_DT_F32) Q8K_QD(float);
+            if (x_dtype == Q8K_DT_F16) Q8K_QD(__half);
+        }
+        if (x_dtype == Q8K_DT_BF16) Q8K_QD(__nv_bfloat16);
+        if (x_dtype == Q8K_DT_E4M3) Q8K_QD(e4m3_t);
     }
-    if (x_dtype == Q8K_DT_BF16) Q8K_QD(__nv_bfloat16);
-    if (x_dtype == Q8K_DT_E4M3) Q8K_QD(e4m3_t);
 #undef Q8K_QD
     set_error_detail("%s: input dtype %d not supported", op, x_dtype);
     return Q8K_ERR_UNSUPPORTED;
 }
-template int tokenwise_quant_as<true>(const char*, const void*, int, void*, int, float*, int64_t, int, int64_t, cudaStream_t);
+template int tokenwise_quant_as<kRowsGated>(const char*, const void*, int, void*, int, float*, int64_t, int, int64_t, cudaStream_t);
+template int tokenwise_quant_as<kRowsFinite>(const char*, const void*, int, void*, int, float*, int64_t, int, int64_t, cudaStream_t);
 }  // namespace q8k
 
 extern "C" int q8k_tokenwise_quant(const void* x, int x_dtype, void* q, int q_dtype, float* scales,
                                    int64_t rows, int dim, int64_t x_row_stride, void* stream) {
-    return tokenwise_quant_as<false>("tokenwise_quant", x, x_dtype, q, q_dtype, scales, rows, dim, x_row_stride, (cudaStream_t)stream);
+    return tokenwise_quant_as<kRowsLinear>("tokenwise_quant", x, x_dtype, q, q_dtype, scales, rows, dim, x_row_stride, (cudaStream_t)stream);
 }
 
 extern "C" int q8k_transpose_quant(const void* x, int x_dtype, const float* row_scales, void* q, float* scales, int N, int K,

@@ -17,7 +17,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import native
-from .linear import E4M3, is_16bit
+from .linear import is_16bit
 
 FORMATS = tuple(native.FP4_FORMATS)
 Scales = Tuple[torch.Tensor, Optional[torch.Tensor]]
@@ -53,7 +53,7 @@ class FP4LinearFunc(torch.autograd.Function):
             return (grad.new_empty(*grad.shape[:-1], k, dtype=ctx.dtype),) + (None,) * 6
         if y is not None:
             grad = native.gelu_backward(y, grad.to(torch.bfloat16), torch.bfloat16)
-        g8, gs = native.tokenwise_quant(grad.reshape(-1, n), E4M3)
+        g8, gs = native.fp4_backward_quant(grad.reshape(-1, n))
         w8, ws = native.fp4_weight_operand(b, (block, row))
         dx = native.fp8_mm(g8, w8, gs, ws, False, ctx.dtype)
         return dx.reshape(*grad.shape[:-1], k), None, None, None, None, None, None

@@ -1178,6 +1178,20 @@ def fp4_linear_check(op: str, x: torch.Tensor, w: torch.Tensor, w_scales, bias: 
     return dev, fmt, n, k
 
 
+def fp4_backward_quant(grad: torch.Tensor) -> List[torch.Tensor]:
+    """The gradient operand of the backward product: bf16 or fp16 [...,N] as ``[q, scales]``, e4m3 [...,N] and fp32 [...], as tokenwise_quant has
+    them, with a factor of FLT_MAX at most."""
+    dev = require_cuda(grad)
+    if grad.dtype not in (torch.bfloat16, torch.float16) or grad.dim() < 1:
+        raise Q8KernelError(f"fp4_backward_quant: gradient {grad.dtype} {tuple(grad.shape)} must be bfloat16 or float16 rows")
+    n = grad.shape[-1]
+    grad = _aligned(grad.contiguous())
+    q = torch.empty(grad.shape, dtype=E4M3, device=dev)
+    scales = torch.empty(grad.shape[:-1], dtype=torch.float32, device=dev)
+    launch(dev, "fp4_backward_quant", lib.q8k_fp4_backward_quant, ptr(grad), dt(grad.dtype), ptr(q), ptr(scales), scales.numel(), n)
+    return [q, scales]
+
+
 def fp4_weight_operand(w: torch.Tensor, w_scales) -> List[torch.Tensor]:
     """A 4-bit weight [N,K/2] de-quantised to fp32, transposed and quantised to e4m3 per input channel, the weight operand of the backward
     product.  Returns ``[q, scales]``: e4m3 [K,N] and fp32 [K]."""
