@@ -443,7 +443,7 @@ Q8K_API int q8k_fp4_quant(const void* x, int x_dtype, int64_t x_row_stride, int 
 Q8K_API int q8k_fp4_dequant(const void* values, const void* block_scales, const float* row_scales, int format, void* y, int y_dtype, int64_t rows,
                     int K, void* stream);
 /* out [M, N] (bf16 or fp16) = act((a . b^T) + bias[n]) of a [M, K] and b [N, K] of one format; bias fp32 or NULL, act tanh-GELU with
- * fuse_gelu.  N a multiple of 16.                                                                                                */
+ * fuse_gelu.  N a multiple of 16 below 2^30.                                                                                     */
 Q8K_API int q8k_fp4_mm(int format, const void* a, const void* a_block_scales, const float* a_row_scales, const void* b, const void* b_block_scales,
                const float* b_row_scales, const float* bias, void* out, int out_dtype, int M, int N, int K, int fuse_gelu,
                int* dev_status, void* stream);

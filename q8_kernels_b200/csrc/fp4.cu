@@ -483,6 +483,7 @@ extern "C" int q8k_fp4_linear(int format, const void* x, int x_dtype, const void
     if (int rc = fp4_check(op, format, M, K)) return rc;
     const bool nv = format == Q8K_FP4_NV;
     Q8K_REQUIRE(N > 0 && N % 16 == 0, Q8K_ERR_INVALID_ARG, "%s: N=%d must be a positive multiple of 16", op, N);
+    Q8K_REQUIRE(N <= kFp4MaxN, Q8K_ERR_TOO_LARGE, "%s: N=%d too large", op, N);
     if (M == 0) return Q8K_OK;
     if (fp4_quantises_rows(M, N, K)) {
         Q8K_REQUIRE(x_dtype == Q8K_DT_BF16 || x_dtype == Q8K_DT_F16, Q8K_ERR_UNSUPPORTED, "%s: input dtype %d is not bf16 or fp16", op, x_dtype);

@@ -13,6 +13,7 @@
 namespace q8k {
 
 constexpr int kFp4Slab = 256;                                  // values
+constexpr int kFp4MaxN = (1 << 30) - 16;                       // columns of a product: its stores name them by byte, in 32 bits
 constexpr int fp4_block(bool nv) { return nv ? 16 : 32; }
 constexpr int fp4_slab_tiles(bool nv) { return nv ? 4 : 2; }
 constexpr int fp4_slab_scales(bool nv) { return 512 * fp4_slab_tiles(nv); }   // bytes for 128 rows

@@ -430,7 +430,7 @@ int fp4_mm(int format, const void* a, const void* a_block_scales, const float* a
     const bool nv = format == Q8K_FP4_NV;
     Q8K_REQUIRE(M >= 0 && N > 0 && K > 0 && N % 16 == 0 && K % 32 == 0, Q8K_ERR_INVALID_ARG,
                 "%s: M=%d must not be negative, N=%d a multiple of 16 and K=%d of 32", op, M, N, K);
-    Q8K_REQUIRE(M <= 0x7fffff00 && N <= 0x7fffff00, Q8K_ERR_TOO_LARGE, "%s: M=%d or N=%d too large", op, M, N);
+    Q8K_REQUIRE(M <= 0x7fffff00 && N <= kFp4MaxN, Q8K_ERR_TOO_LARGE, "%s: M=%d or N=%d too large", op, M, N);
     Q8K_REQUIRE(out_dtype == Q8K_DT_BF16 || out_dtype == Q8K_DT_F16, Q8K_ERR_UNSUPPORTED, "%s: output dtype %d is not bf16 or fp16", op, out_dtype);
     if (M == 0) return Q8K_OK;
     Q8K_REQUIRE((x || (a && a_block_scales && (!nv || a_row_scales))) && b && b_block_scales && out && (!nv || b_row_scales), Q8K_ERR_INVALID_ARG,

@@ -13,3 +13,13 @@ def test_refusals_of_the_gradient_operand():
     assert quant(dtype=_lib.DT_F32) == -2 and quant(dtype=_lib.DT_E4M3) == -2 and quant(n=24) == -1 and quant(n=0) == -1 and quant(n=32784) == -2
     assert quant(grad=None) == -1 and quant(q=None) == -1 and quant(scales=None) == -1 and quant(grad=BUF + 8) == -1 and quant(q=BUF + 8) == -1
     assert quant(rows=-1) == -1 and quant(rows=0) == 0
+
+
+def test_more_columns_than_a_store_can_name_are_refused():
+    """The products' stores name a column by its byte, 2 n, in 32 bits: 2^30 columns are too many, whatever the number of rows."""
+    for m in (1, 4, 300, 5000):
+        for n in (1 << 30, (1 << 30) + 16, 0x7fffff00):
+            assert _lib.lib.q8k_fp4_mm(2, BUF, BUF, BUF, BUF, BUF, BUF, None, None, _lib.DT_BF16, m, n, 64, 0, None, None) == _lib.lib.q8k_fp4_linear(
+                2, BUF, _lib.DT_BF16, BUF, BUF, BUF, None, None, _lib.DT_BF16, m, n, 64, 0, BUF, 1 << 40, None, None) == -5
+        # the largest number goes past that check, to the missing output
+        assert _lib.lib.q8k_fp4_mm(2, BUF, BUF, BUF, BUF, BUF, BUF, None, None, _lib.DT_BF16, m, (1 << 30) - 16, 64, 0, None, None) == -1
