@@ -166,7 +166,7 @@ Q8K_API int q8k_rms_norm_backward(const void* x_normed, int x_dtype, const float
  * (q8k_fp8_mm); bs_a == bs_b or one of them 1; sa [bs_a, M], sb [bs_b, N],
  * bias [N] fp32 or NULL; C [max(bs_a,bs_b), M, N] bf16 (RNE), e4m3
  * (saturating) or, of e4m3 operands without GELU, fp16 (RNE).
- * N % 16 == 0, K % 16 == 0, all pointers 16-byte aligned.
+ * N % 16 == 0 (with 16-bit outputs of more than 128 rows below 2^30), K % 16 == 0, all pointers 16-byte aligned.
  * Replaces q8_mm / q8_mm_bias / fp8_mm / fp8_mm_bias:
  * csrc/gemm/q8_gemm_api.cpp:40-291 and the run_* launchers declared at :27-35. */
 Q8K_API int q8k_q8_mm(const void* a, const void* b, const float* bias, const float* a_scales,

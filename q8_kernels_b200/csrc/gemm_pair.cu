@@ -607,6 +607,8 @@ int launch_gemm_pair(bool int8, bool gelu, int out, bool resid, const void* a, c
                      int bs_a, int bs_b, cudaStream_t st) {
     const char* op = int8 ? "q8_mm" : "fp8_mm";
     const bool out_e4m3 = out == kOutE4m3;
+    // the stores name a column by its byte, in 32 bits
+    Q8K_REQUIRE(out_e4m3 || p.N < (1 << 30), Q8K_ERR_TOO_LARGE, "%s: N=%d columns of 16 bits are too many", op, p.N);
     CUtensorMap ta, tb;
     {
         const uint64_t dims[2] = {(uint64_t)p.K, (uint64_t)bs_a * (uint64_t)p.M};

@@ -23,3 +23,11 @@ def test_more_columns_than_a_store_can_name_are_refused():
                 2, BUF, _lib.DT_BF16, BUF, BUF, BUF, None, None, _lib.DT_BF16, m, n, 64, 0, BUF, 1 << 40, None, None) == -5
         # the largest number goes past that check, to the missing output
         assert _lib.lib.q8k_fp4_mm(2, BUF, BUF, BUF, BUF, BUF, BUF, None, None, _lib.DT_BF16, m, (1 << 30) - 16, 64, 0, None, None) == -1
+
+
+def test_more_columns_than_a_store_of_the_8_bit_products_can_name_are_refused():
+    """16-bit columns from 2^30 on, of rows enough for the kernel on CTA pairs (few rows have a kernel with plain stores)."""
+    for mm in (_lib.lib.q8k_q8_mm, _lib.lib.q8k_fp8_mm):
+        for m in (300, 5000):
+            assert mm(BUF, BUF, None, BUF, BUF, BUF, _lib.DT_BF16, 1, 1, m, 1 << 30, 64, 0, None, None) == -5
+            assert mm(BUF, BUF, None, BUF, BUF, BUF, _lib.DT_BF16, 1, 1, m, 0x7fffff00, 64, 1, None, None) == -5
