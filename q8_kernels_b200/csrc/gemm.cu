@@ -104,7 +104,8 @@ static int gemm_8bit(bool int8, const void* a, const void* b, const float* bias,
     Q8K_REQUIRE(aligned16(a) && aligned16(b) && aligned16(out), Q8K_ERR_INVALID_ARG,
                 "%s: a, b and out must be 16-byte aligned", op);
     Q8K_REQUIRE(out_dtype == Q8K_DT_BF16 || out_dtype == Q8K_DT_E4M3 || (out_dtype == Q8K_DT_F16 && !int8 && fuse_gelu == 0 && resid == nullptr),
-                Q8K_ERR_UNSUPPORTED, "%s: output dtype %d is not bf16 or e4m3", op, out_dtype);
+                Q8K_ERR_UNSUPPORTED, out_dtype == Q8K_DT_F16 ? "%s: output dtype %d: fp16 is for e4m3 operands without GELU and residual"
+                                                             : "%s: output dtype %d is not bf16 or e4m3", op, out_dtype);
     Q8K_REQUIRE((int64_t)bs_a * M <= 0x7fffffffLL && (int64_t)bs_b * N <= 0x7fffffffLL, Q8K_ERR_TOO_LARGE,
                 "%s: batch * rows exceeds 2^31", op);
     if (M == 0) return Q8K_OK;

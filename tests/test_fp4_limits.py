@@ -31,3 +31,16 @@ def test_more_columns_than_a_store_of_the_8_bit_products_can_name_are_refused():
         for m in (300, 5000):
             assert mm(BUF, BUF, None, BUF, BUF, BUF, _lib.DT_BF16, 1, 1, m, 1 << 30, 64, 0, None, None) == -5
             assert mm(BUF, BUF, None, BUF, BUF, BUF, _lib.DT_BF16, 1, 1, m, 0x7fffff00, 64, 1, None, None) == -5
+
+
+def test_the_message_of_a_refused_output_type():
+    """What is accepted depends on operands and epilogue: the message says on what."""
+    def message(mm, dtype, gelu):
+        assert mm(BUF, BUF, None, BUF, BUF, BUF, dtype, 1, 1, 8, 16, 64, gelu, None, None) == -2
+        return _lib.lib.q8k_last_error_detail().decode()
+
+    for mm in (_lib.lib.q8k_q8_mm, _lib.lib.q8k_fp8_mm):
+        for gelu in (0, 1):
+            assert "is not bf16 or e4m3" in message(mm, _lib.DT_F32, gelu)
+    for mm, gelu in ((_lib.lib.q8k_q8_mm, 0), (_lib.lib.q8k_q8_mm, 1), (_lib.lib.q8k_fp8_mm, 1)):
+        assert "fp16 is for e4m3 operands without GELU and residual" in message(mm, _lib.DT_F16, gelu)
