@@ -63,7 +63,7 @@ fp4_quant_kernel(const Tin* __restrict__ x, int64_t x_stride, uint8_t* __restric
                  float* __restrict__ row_scales, int64_t rows, int K, int slabs) {
     constexpr int AT_ONCE = CTA / T, STEPS = kFp4GroupRows / AT_ONCE;
     static_assert(AT_ONCE >= 1 && AT_ONCE <= kFp4GroupRows, "rows at a time");
-    __shared__ float red[CTA / 32];
+    static_assert(!NV || T == 32, "a row of nvfp4, whose absmax all of its threads need, is one warp's");
     extern __shared__ __align__(16) uint8_t scales[];          // [tiles along K][32]
     const int group = threadIdx.x / T, t = threadIdx.x % T, units = K / kFp4Unit;
     const int64_t row0 = (int64_t)(blockIdx.x >> 4) * 128 + (blockIdx.x & 15) * 2;
@@ -98,14 +98,6 @@ fp4_quant_kernel(const Tin* __restrict__ x, int64_t x_stride, uint8_t* __restric
         }
         if constexpr (NV) {
             top = warp_max<true>(top);
-            if constexpr (T > 32) {
-                const int warp = threadIdx.x >> 5;
-                if (step > 0) __syncthreads();                 // the values before have been read
-                if ((threadIdx.x & 31) == 0) red[warp] = top;
-                __syncthreads();
-#pragma unroll
-                for (int k = 0; k < T / 32; ++k) top = max_nan(top, red[group * (T / 32) + k]);
-            }
             fp4_row_factors(top, g, rs);
             if (here && t == 0) row_scales[row] = rs;
         }
