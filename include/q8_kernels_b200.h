@@ -166,7 +166,7 @@ Q8K_API int q8k_rms_norm_backward(const void* x_normed, int x_dtype, const float
  * (q8k_fp8_mm); bs_a == bs_b or one of them 1; sa [bs_a, M], sb [bs_b, N],
  * bias [N] fp32 or NULL; C [max(bs_a,bs_b), M, N] bf16 (RNE), e4m3
  * (saturating) or, of e4m3 operands without GELU, fp16 (RNE).
- * N % 16 == 0 (with 16-bit outputs of more than 128 rows below 2^30), K % 16 == 0, all pointers 16-byte aligned.
+ * N % 16 == 0 (below 2^30 with 16-bit outputs), K % 16 == 0, all pointers 16-byte aligned.
  * Replaces q8_mm / q8_mm_bias / fp8_mm / fp8_mm_bias:
  * csrc/gemm/q8_gemm_api.cpp:40-291 and the run_* launchers declared at :27-35. */
 Q8K_API int q8k_q8_mm(const void* a, const void* b, const float* bias, const float* a_scales,
@@ -379,8 +379,8 @@ Q8K_API int q8k_head_norm(const void* q, const int64_t q_strides[3], const float
                   int half_layout, void* stream);
 /* Its gradients: dq and dk from the inputs and the outputs' gradients (each with strides; a tensor with heads of 0 is left out), and the
  * weights' in fp32 [head_dim], each NULL if it is not wanted.  The sums over tokens and heads need a workspace of
- * q8k_head_norm_backward_workspace_bytes (16-byte aligned) and are taken in an order that the sizes fix: the same bits in every call
- * of the same sizes.                                                                                                             */
+ * q8k_head_norm_backward_workspace_bytes (16-byte aligned).  They are taken in an order that sizes, strides, the alignment of the tensors
+ * and the number of SMs fix, as those within a head are: equal calls give equal bits.                                             */
 Q8K_API size_t q8k_head_norm_backward_workspace_bytes(int head_dim);
 Q8K_API int q8k_head_norm_backward(const void* q, const int64_t q_strides[3], const float* q_weight, const void* q_grad, const int64_t q_grad_strides[3],
                   void* dq, const int64_t dq_strides[3], float* dq_weight, int q_heads,

@@ -8,7 +8,8 @@
 // computed here, once per token and pair (rotary.cuh), and shared by the heads through shared memory.
 //
 // What is left to save are instructions: at the copy rate an SM has some 15 for an element.  So a thread takes the same channels of
-// up to eight heads of one token: its cosines and sines come from shared memory once, and its addresses advance by the head's stride.
+// eight heads of one token, up to sixteen where that leaves fewer threads idle (launch_rotary_as), fewer in short calls: its cosines and
+// sines come from shared memory once, and its addresses advance by the head's stride.
 // CTAs of 128 threads, eight an SM: the chain from position to sine hides behind the first loads and behind other CTAs' stores, and the
 // last ones to finish are short.  Measured (bf16, CUDA graphs): 6144 tokens x 64 heads x 64 interleaved 16.3 us (0.94 of the copy rate),
 // 16384 x 40 x 128 half 53.7 us (0.95), interleaved 52.3 (0.98).  Tried, when these took 17.5 and 61.6: six CTAs without spills (17.9, 64.3), one head's loads at a

@@ -8,8 +8,11 @@ Values are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) in blocks along
 The tensor cores multiply them with their scales at four times the bf16 rate.  ``native.fp4_quant`` has the layout.  As in the 8-bit linears,
 activations are quantised per call, weights are frozen, and the activation is what has a gradient: the output's gradient is
 quantised per token and the de-quantised weight per input channel to e4m3, and the FP8 GEMM multiplies them.  (A gradient of 4 bits would lose
-an eighth of each value; the product of e4m3 takes twice the time.)  With a gradient, a fused GELU becomes a kernel of its own on the
-product rounded to bf16, which the backward pass takes again.  There are no forward-mode derivatives.
+an eighth of each value; the product of e4m3 takes twice the time.)  There are no forward-mode derivatives.
+
+With a gradient, a fused GELU becomes a kernel of its own on the product rounded to bf16, which the backward pass takes again, because the
+GELU kernels are those of the 8-bit linears, which read and write bf16 and e4m3.  So such a call has two roundings to bf16 where the call without a gradient has one to
+the output's type, and other bits: 2002 x 2048 -> 8192 is off by some 2^-7 of an element at most in the place of 2^-8 with bf16 and 2^-10.9 with fp16.  Who trains in fp16 and needs its 11 bits leaves ``fuse_gelu`` off and takes the GELU of the fp16 output.
 """
 from typing import Optional, Tuple
 
@@ -39,6 +42,7 @@ def fp4_dequantize(values: torch.Tensor, scales: Scales, out_dtype: torch.dtype 
 class FP4LinearFunc(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, b, bias, block, row, fuse_gelu, out_dtype):
+        # (bf16 with GELU: see the module's docstring)
         y = native.fp4_linear(a, b, (block, row), bias, False, torch.bfloat16 if fuse_gelu else out_dtype)
         ctx.save_for_backward(b, block, row, y if fuse_gelu else None)
         ctx.dtype = a.dtype

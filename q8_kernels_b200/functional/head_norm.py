@@ -1,8 +1,10 @@
 """Norms of queries and keys for each head, with the rotation by position in the same pass (no counterpart in the reference, which norms whole rows
 and rotates them by tables: see rms_norm.py, rope.py).
 
-``y = R(p) (x / sqrt(mean(x^2) + eps) * weight)`` over the channels of a head, in fp32 and rounded once.  The gradients are those of the formula;
-the weights' sums over tokens and heads are taken in an order that the sizes fix (the same bits in every call of the same sizes).  There are no forward-mode derivatives.
+``y = R(p) (x / sqrt(mean(x^2) + eps) * weight)`` over the channels of a head, in fp32 and rounded once; squares are fp32's, so |x| has to be below
+1e19, and without eps above 1e-19.  The gradients are those of the formula.  All sums, those of the weights' gradients over tokens and heads
+among them, are taken in an order that sizes, strides, alignment of the tensors and the number of SMs fix: equal calls give equal bits, the same values at
+other strides or an odd address may differ in the last fp32 bits.  There are no forward-mode derivatives.
 """
 from typing import Optional
 
