@@ -10,9 +10,10 @@ activations are quantised per call, weights are frozen, and the activation is wh
 quantised per token and the de-quantised weight per input channel to e4m3, and the FP8 GEMM multiplies them.  (A gradient of 4 bits would lose
 an eighth of each value; the product of e4m3 takes twice the time.)  There are no forward-mode derivatives.
 
-With a gradient, a fused GELU becomes a kernel of its own on the product rounded to bf16, which the backward pass takes again, because the
-GELU kernels are those of the 8-bit linears, which read and write bf16 and e4m3.  So such a call has two roundings to bf16 where the call without a gradient has one to
-the output's type, and other bits: 2002 x 2048 -> 8192 is off by some 2^-7 of an element at most in the place of 2^-8 with bf16 and 2^-10.9 with fp16.  Who trains in fp16 and needs its 11 bits leaves ``fuse_gelu`` off and takes the GELU of the fp16 output.
+With a gradient, a fused GELU becomes a kernel of its own on the product rounded to bf16, which the backward pass takes again, because
+the GELU kernels are those of the 8-bit linears, which read and write bf16 and e4m3.  So such a call has two roundings to bf16 where the call
+without a gradient has one to the output's type, and other bits: 2002 x 2048 -> 8192 is off by some 2^-7 of an element at most in the place of
+2^-8 with bf16 and 2^-10.9 with fp16.  Who trains in fp16 and needs its 11 bits leaves ``fuse_gelu`` off and takes the GELU of the fp16 output.
 """
 from typing import Optional, Tuple
 
